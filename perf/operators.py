@@ -257,7 +257,9 @@ def prepare(case, seed):
     else:
         for name, x in (("m", m), ("v", root)):
             x = x.view(-1, BLOCK)
-            scale = x.abs().amax(1) / 448.0
+            top = x.abs().amax(1).double().clamp(min=1e-30)
+            scale = torch.exp2(torch.ceil(torch.log2(top / 448.0))).float()
+            scale *= x.abs().amax(1) > 0
             codes = torch.where(scale[:, None] > 0, x / scale[:, None], torch.zeros_like(x))
             flat[name] = codes.clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(-1)
             flat[name + "_scale"] = scale
@@ -417,22 +419,30 @@ def _random_words(blocks, seed, step):
     return _mix(((at & WORD) * 0x9E3779B1 + _mix(key[:, None] ^ (at >> 32))) & WORD)
 
 
-def _plain_e4m3(x, bits, keep):
-    """x ([blocks, 256]) as e4m3 with a scale for each block, rounded up or down at random by 16
-    ``bits``; ``keep``: what is not zero stays so."""
+def _two_to(power):
+    return ((power + 127) << 23).view(torch.float32)
+
+
+def _plain_e4m3(x, bits, square):
+    """x ([blocks, 256]) as e4m3 numbers and a power of two for each block, rounded to one of the two
+    neighbours at random by 16 ``bits``: so that the mean is x, or with ``square`` that the mean of
+    the square is x's (and what is not zero stays so)."""
     fine = torch.isfinite(x)
     size = torch.where(fine, x.abs(), torch.zeros_like(x))
     top = size.amax(1, keepdim=True)
     some = top >= 1e-30
-    inverse = torch.where(some, 448.0 / top, torch.zeros_like(top))
-    a = (size * inverse).clamp(max=448.0)
-    large = ((a.view(torch.int32) + (bits << 4).int()) & ~0xFFFFF).view(torch.float32)
-    small = (a * 512.0 + bits.float() * 2.0**-16).floor() * 2.0**-9
-    q = torch.where(a >= 2.0**-6, large, small).clamp(max=448.0)
-    if keep:
-        q = torch.where((size > 0) & some, q.clamp(min=2.0**-9), q)
+    part, power = torch.frexp(top)  # top <= 448 scale, 448 = 0.875 2^9
+    power = torch.where(part > 0.875, power - 8, power - 9)
+    a = size * torch.where(some, _two_to(-power), torch.zeros_like(top))
+    unit = _two_to(torch.frexp(a)[1].clamp(min=-5) - 4)
+    low = (a / unit).floor() * unit
+    u = bits.float() * 2.0**-16 * unit
+    up = (a - low) * (a + low) > u * (2.0 * low + unit) if square else a - low > u
+    q = torch.where(up, low + unit, low).clamp(max=448.0)
+    if square:
+        q = torch.where(a > 0, q.clamp(min=2.0**-9), q)
     q = torch.where(fine, torch.copysign(q, x), torch.full_like(x, math.nan))
-    scale = torch.where(some, top * (1.0 / 448.0), torch.zeros_like(top))
+    scale = torch.where(some, _two_to(power), torch.zeros_like(top))
     return q.to(torch.float8_e4m3fn), scale[:, 0]
 
 
@@ -561,16 +571,19 @@ def _exact_policy(state):
             "grad": _exact_gradient(x, y, g, case["temperature"])}
 
 
-def _exact_e4m3(x, u, keep):
+def _exact_e4m3(x, u, square):
     x = x.view(-1, BLOCK)
-    top = x.abs().amax(1, keepdim=True)
-    a = torch.where(top > 0, x.abs() * (448.0 / top), torch.zeros_like(x))
-    power = torch.frexp(a)[1].clamp(min=-5).double() - 1.0  # a = f 2^power, 1 <= f < 2, or below
-    quantum = torch.exp2(power - 3.0)
-    q = (torch.floor(a / quantum + u) * quantum).clamp(max=448.0)
-    if keep:
-        q = torch.where(x.abs() > 0, q.clamp(min=2.0**-9), q)
-    return (torch.sign(x) * q).view(-1), (top / 448.0)[:, 0]
+    size = x.abs()
+    top = size.amax(1, keepdim=True)
+    scale = torch.where(top > 0, torch.exp2(torch.ceil(torch.log2(top / 448.0))), torch.zeros_like(top))
+    a = torch.where(top > 0, size / scale, torch.zeros_like(x))
+    unit = torch.exp2(torch.floor(torch.log2(a)).clamp(min=-6.0) - 3.0)
+    low = torch.floor(a / unit) * unit
+    chance = (a**2 - low**2) / ((low + unit) ** 2 - low**2) if square else (a - low) / unit
+    q = torch.where(u < chance, low + unit, low).clamp(max=448.0)
+    if square:
+        q = torch.where(a > 0, q.clamp(min=2.0**-9), q)
+    return (torch.sign(x) * q).view(-1), scale[:, 0]
 
 
 def _exact_adamw(state):
