@@ -212,6 +212,129 @@ int tiso_calib_groups(int key_dtype, const void* scores, int label_dtype, const 
 int tiso_calib_interp(int key_dtype, const void* x, int64_t m, const void* xs, const double* fit,
                       int64_t g, double* out, void* stream);
 
+/* ---- Language-model operators ----------------------------------------------------------------
+ * Losses on a model's logits and the optimizer step. None has a counterpart in the reference:
+ * additions of this library, beside the calibration of the scores that such a model answers with.
+ */
+
+/* Rows of logits: row r, 0 <= r < rows, is the `vocab` consecutive elements from
+ * data + (r / inner) * outer_stride + (r % inner) * inner_stride (strides in elements), so that
+ * [batch, length, vocab] logits cut along their length need no copy. */
+typedef struct tiso_rows {
+  const void* data;
+  int64_t rows, inner, outer_stride, inner_stride, vocab;
+} tiso_rows;
+
+/* logps[r] = log softmax(x[r] / temperature) at targets[r] (accumulation type: TISO_F64 for
+ * float64 logits, TISO_F32 otherwise); 0 where targets[r] is ignore_index (that row is not read),
+ * NaN where it is any other number outside [0, vocab). stats: NULL, or [rows][2] of the
+ * accumulation type for tiso_logprobs_grad (each row's maximum and sum of exponentials; a row that
+ * is left out has a negative sum). Needs no workspace. */
+int tiso_logprobs(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
+                  double temperature, void* logps, void* stats, void* stream);
+
+/* The gradient of sum(coef * upstream * logps) in the logits, in their type, written contiguously
+ * ([rows][vocab]): coef[r] upstream / temperature (1[v = targets[r]] - softmax(x[r] / temperature)),
+ * zeros for a row that is left out. upstream: NULL (1), or a device scalar; where it is exactly 1
+ * then nothing is written (grad must already hold the gradient for 1, as tiso_policy leaves it). */
+int tiso_logprobs_grad(int dtype, const tiso_rows* x, const int64_t* targets, double temperature,
+                       const void* stats, const void* coef, const void* upstream, void* grad,
+                       void* stream);
+
+/* Per-token inputs of the policy loss (device arrays of `rows` numbers of the accumulation type;
+ * ref_logps and weight may be NULL; weight_is_byte: weight is an array of bytes, 0 or 1). */
+typedef struct tiso_policy_args {
+  const void *old_logps, *ref_logps, *advantages, *weight;
+  int weight_is_byte;
+  double clip_low, clip_high, kl_coef;
+} tiso_policy_args;
+
+/* Workspace for tiso_policy (8-byte aligned). */
+int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes);
+
+/* The clipped policy loss and, if grad is not NULL, its gradient in the logits, in one pass. Per
+ * token: lp as of tiso_logprobs, rho = exp(lp - old), A the advantage, d = ref - lp,
+ *   l = -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)
+ * (no second term without ref_logps). out: three numbers of the accumulation type, the means
+ * sum(w q) / sum(w) of l, of exp(d) - d - 1 and of [the clip is the smaller side]; all 0 when the
+ * weights sum to 0. A token of weight 0 (or whose target is ignore_index) is left out: nothing of
+ * it is read beyond its weight and target, its logps, coef and gradient are 0. coef[r] receives
+ * d loss / d logps[r], stats what tiso_logprobs_grad needs; grad ([rows][vocab], contiguous)
+ * coef[r] / temperature (1[v = targets[r]] - softmax). Where both sides of the minimum are equal
+ * the slope is that of the unclipped one. Sums run in a fixed order. */
+int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
+                double temperature, const tiso_policy_args* args, void* logps, void* coef,
+                void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+enum tiso_preference_kind {
+  TISO_PREF_LOGISTIC = 0, /* (1 - e) log(1 + exp(-u)) + e log(1 + exp(u)), e = label_smoothing */
+  TISO_PREF_HINGE = 1,    /* max(0, 1 - u) */
+  TISO_PREF_SQUARE = 2    /* (u - 1/2)^2 / beta^2 */
+};
+
+/* A batch of preference pairs: 2 pairs sequences of token log-probabilities packed back to back,
+ * sequence k being tokens [offsets[k], offsets[k + 1]) (device int64[2 pairs + 1], non-decreasing
+ * in [0, tokens]; empty sequences allowed): first the chosen answers, then the rejected ones in
+ * the same order. logps and ref_logps: device arrays of `tokens` numbers of dtype (TISO_F32 or
+ * TISO_F64), ref_logps may be NULL (0); mask: NULL, or a byte per token, 0 where it does not count. */
+typedef struct tiso_preference_args {
+  const void *logps, *ref_logps;
+  const uint8_t* mask;
+  const int64_t* offsets;
+  int64_t tokens, pairs;
+  int kind, average; /* average: a sequence's mean over its tokens instead of their sum */
+  double beta, label_smoothing, margin;
+} tiso_preference_args;
+
+/* Workspace for tiso_preference (8-byte aligned). */
+int tiso_preference_workspace_size(int64_t pairs, size_t* bytes);
+
+/* With s_k the sum (or mean) over sequence k's counted tokens of logps - ref_logps (0 for none):
+ * *loss = the mean over pairs of the kind's l(u), u = beta (s_chosen - s_rejected) - margin;
+ * rewards[2][pairs] = beta s_k; coef[2 pairs] = d loss / d logps of each of a sequence's counted
+ * tokens. All of dtype. Sums are double, in a fixed order. */
+int tiso_preference(int dtype, const tiso_preference_args* args, void* loss, void* rewards,
+                    void* coef, void* workspace, size_t workspace_bytes, void* stream);
+
+/* grad[t] = coef of its sequence times *upstream (device scalar), 0 for tokens that do not count
+ * or lie in no sequence; grad_ref[t] = -grad[t]. Either may be NULL (not wanted). */
+int tiso_preference_grad(int dtype, const tiso_preference_args* args, const void* coef,
+                         const void* upstream, void* grad, void* grad_ref, void* stream);
+
+/* One tensor of an AdamW step: n elements each of param (changed in place), grad, exp_avg and
+ * exp_avg_sq (changed in place). With 32-bit states the last two are floats, the running means of
+ * the gradient and of its square. With 8-bit states they are e4m3 numbers standing for the running
+ * mean and for the square root of that of the square, each times its block's scale: *_scale holds a
+ * float for every 256 elements, ceil(n / 256) of them. index: the tensor's place among all of the
+ * step's (it enters the random bits of the 8-bit states). */
+typedef struct tiso_adamw_tensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  int64_t n, index;
+} tiso_adamw_tensor;
+
+typedef struct tiso_adamw_args {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step; /* from 1 */
+  uint32_t seed;
+} tiso_adamw_args;
+
+/* One AdamW step over `count` tensors (a host array, read before the call returns), with decoupled
+ * weight decay:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in float, each operation rounded on its own; p is then rounded to param_dtype (TISO_F16,
+ * TISO_BF16 or TISO_F32). grad_dtype: param_dtype or TISO_F32. state_bits: 32 or 8; 8-bit states
+ * are rounded at random (the mean of the mean, and of the square of the root, is kept), the
+ * parameters use them before they are rounded.
+ * A block's scale is the smallest power of two that brings its largest finite magnitude within
+ * e4m3's 448; an element that is not finite is held as NaN. Needs no workspace; one launch for every 480 tensors. */
+int tiso_adamw(int param_dtype, int grad_dtype, int state_bits, int64_t count,
+               const tiso_adamw_tensor* tensors, const tiso_adamw_args* args, void* stream);
+
 /* The message of the calling thread's last error ("" if none). */
 const char* tiso_last_error(void);
 

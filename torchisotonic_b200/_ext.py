@@ -27,6 +27,37 @@ ABI_VERSION = 2
 _DTYPES = {torch.float16: F16, torch.bfloat16: BF16, torch.float32: F32, torch.float64: F64}
 
 
+class Rows(ctypes.Structure):
+    """tiso_rows"""
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("inner", ctypes.c_int64),
+                ("outer_stride", ctypes.c_int64), ("inner_stride", ctypes.c_int64),
+                ("vocab", ctypes.c_int64)]
+
+
+class PolicyArgs(ctypes.Structure):
+    """tiso_policy_args"""
+    _fields_ = [("old_logps", ctypes.c_void_p), ("ref_logps", ctypes.c_void_p),
+                ("advantages", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("weight_is_byte", ctypes.c_int), ("clip_low", ctypes.c_double),
+                ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double)]
+
+
+class PreferenceArgs(ctypes.Structure):
+    """tiso_preference_args"""
+    _fields_ = [("logps", ctypes.c_void_p), ("ref_logps", ctypes.c_void_p),
+                ("mask", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("tokens", ctypes.c_int64), ("pairs", ctypes.c_int64), ("kind", ctypes.c_int),
+                ("average", ctypes.c_int), ("beta", ctypes.c_double),
+                ("label_smoothing", ctypes.c_double), ("margin", ctypes.c_double)]
+
+
+class AdamwArgs(ctypes.Structure):
+    """tiso_adamw_args"""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double),
+                ("step", ctypes.c_int64), ("seed", ctypes.c_uint32)]
+
+
 @functools.cache
 def lib() -> ctypes.CDLL:
     """libtiso.so, loaded once. Raises if it was not built."""
@@ -59,6 +90,15 @@ def lib() -> ctypes.CDLL:
     so.tiso_fit_varlen.argtypes = [i32, p, p, p, p, p, i64, i64, u32, dbl, dbl, p, p]
     so.tiso_check_weights.argtypes = [i32, p, i64, p, p]
     so.tiso_grad_varlen.argtypes = [i32, p, p, p, p, p, p, p, i64, i64, u32, dbl, dbl, p]
+    rows, policy, pref = (ctypes.POINTER(c) for c in (Rows, PolicyArgs, PreferenceArgs))
+    so.tiso_logprobs.argtypes = [i32, rows, p, i64, dbl, p, p, p]
+    so.tiso_logprobs_grad.argtypes = [i32, rows, p, dbl, p, p, p, p, p]
+    so.tiso_policy_workspace_size.argtypes = [i32, i64, ctypes.POINTER(sz)]
+    so.tiso_policy.argtypes = [i32, rows, p, i64, dbl, policy, p, p, p, p, p, p, sz, p]
+    so.tiso_preference_workspace_size.argtypes = [i64, ctypes.POINTER(sz)]
+    so.tiso_preference.argtypes = [i32, pref, p, p, p, p, sz, p]
+    so.tiso_preference_grad.argtypes = [i32, pref, p, p, p, p, p]
+    so.tiso_adamw.argtypes = [i32, i32, i32, i64, p, ctypes.POINTER(AdamwArgs), p]
     so.tiso_last_error.restype = ctypes.c_char_p
     so.tiso_abi_version.restype = i32
     for f in ("tiso_fit_workspace_size", "tiso_fit", "tiso_grad_workspace_size", "tiso_grad",
@@ -66,7 +106,10 @@ def lib() -> ctypes.CDLL:
               "tiso_segment_expand_workspace_size", "tiso_segment_expand",
               "tiso_segment_grad_workspace_size", "tiso_segment_grad_sums", "tiso_segment_grad",
               "tiso_calib_groups_workspace_size", "tiso_calib_groups", "tiso_calib_interp",
-              "tiso_fit_varlen", "tiso_grad_varlen", "tiso_check_weights"):
+              "tiso_fit_varlen", "tiso_grad_varlen", "tiso_check_weights", "tiso_logprobs",
+              "tiso_logprobs_grad", "tiso_policy_workspace_size", "tiso_policy",
+              "tiso_preference_workspace_size", "tiso_preference", "tiso_preference_grad",
+              "tiso_adamw"):
         getattr(so, f).restype = i32
     if so.tiso_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI {so.tiso_abi_version()}, expected {ABI_VERSION}")
@@ -502,3 +545,155 @@ def isotonic_grad_varlen(
                                       0.0 if y_max is None else float(y_max),
                                       torch.cuda.current_stream(g.device).cuda_stream))
     return gy, gw
+
+
+# ---------------------------------------------------------------------------------------------
+# Language-model operators
+
+PREFERENCE_KINDS = {"logistic": 0, "hinge": 1, "square": 2}
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def logits_rows(x: Tensor) -> tuple[Tensor, Rows]:
+    """``x`` ([..., vocab], CUDA) as rows of logits, and the tensor whose memory they are: x itself
+    when its last dimension is contiguous and the leading ones reduce to two strides (a contiguous
+    tensor, a cut or padded one), else a contiguous copy."""
+    if not x.is_cuda:
+        raise RuntimeError("logits must be a CUDA tensor: torchisotonic_b200 has no CPU path")
+    if x.dtype not in _DTYPES:
+        raise RuntimeError("logits must be float16, bfloat16, float32 or float64")
+    vocab = x.shape[-1]
+    if x.is_contiguous():
+        rows = x.numel() // vocab
+        return x, Rows(x.data_ptr(), rows, max(rows, 1), 0, vocab, vocab)
+    shape, stride = x.shape, x.stride()
+    if stride[-1] == 1 or vocab == 1:
+        if x.dim() == 1:
+            return x, Rows(x.data_ptr(), 1, 1, 0, 0, vocab)
+        if x.dim() == 2:
+            return x, Rows(x.data_ptr(), shape[0], max(shape[0], 1), 0, stride[0], vocab)
+        if x.dim() == 3:
+            return x, Rows(x.data_ptr(), shape[0] * shape[1], max(shape[1], 1), stride[0],
+                           stride[1], vocab)
+    return logits_rows(x.contiguous())
+
+
+def logprobs(x: Tensor, targets: Tensor, ignore_index: int, temperature: float,
+             with_stats: bool) -> tuple[Tensor, Tensor | None]:
+    """log softmax(x / temperature) at the targets (int64, contiguous, one per row of logits), in
+    the accumulation dtype and the targets' shape, and with ``with_stats`` what logprobs_grad
+    needs (each row's maximum and sum of exponentials)."""
+    x, rows = logits_rows(x)
+    dev, acc = x.device, acc_dtype(x.dtype)
+    out = torch.empty(targets.shape, dtype=acc, device=dev)
+    stats = torch.empty(2 * rows.rows, dtype=acc, device=dev) if with_stats else None
+    with _on(dev):
+        _check(lib().tiso_logprobs(_DTYPES[x.dtype], rows, targets.data_ptr(), ignore_index,
+                                   temperature, out.data_ptr(), _ptr(stats), _stream(dev)))
+    return out, stats
+
+
+def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor, coef: Tensor,
+                  upstream: Tensor | None = None, grad: Tensor | None = None) -> Tensor:
+    """The gradient of sum(coef * upstream * logprobs) in x, in its dtype and shape, contiguous.
+    ``coef``: contiguous, one per row. ``grad``: holds the gradient for upstream = 1 (left as it
+    is when upstream, a device scalar, is 1), or None for a new tensor."""
+    x, rows = logits_rows(x)
+    dev = x.device
+    if grad is None:
+        grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if upstream is not None:
+            coef, upstream = coef * upstream, None
+    with _on(dev):
+        _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
+                                        stats.data_ptr(), coef.data_ptr(), _ptr(upstream),
+                                        grad.data_ptr(), _stream(dev)))
+    return grad
+
+
+def policy(x: Tensor, targets: Tensor, ignore_index: int, temperature: float, old_logps: Tensor,
+           advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None, clip_low: float,
+           clip_high: float, kl_coef: float, with_grad: bool
+           ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor | None]:
+    """The clipped policy loss of tiso_policy: (out [3]: loss, kl, clip fraction; logps; coef;
+    stats; grad or None). The per-token tensors are contiguous, one number per row of logits, in
+    the accumulation dtype (``weight`` may be bool, ``targets`` is int64)."""
+    x, rows = logits_rows(x)
+    dev, acc = x.device, acc_dtype(x.dtype)
+    dtype, n = _DTYPES[x.dtype], rows.rows
+    logps = torch.empty(targets.shape, dtype=acc, device=dev)
+    # per row: coef, then stats; the workspace (float64) behind them
+    coef = torch.empty(n, dtype=acc, device=dev)
+    stats = torch.empty(2 * n, dtype=acc, device=dev)
+    out = torch.empty(3, dtype=acc, device=dev)
+    grad = torch.empty(x.shape, dtype=x.dtype, device=dev) if with_grad else None
+    args = PolicyArgs(old_logps.data_ptr(), _ptr(ref_logps), advantages.data_ptr(), _ptr(weight),
+                      int(weight is not None and weight.dtype == torch.bool), clip_low, clip_high,
+                      kl_coef)
+    so = lib()
+    size = ctypes.c_size_t()
+    with _on(dev):
+        _check(so.tiso_policy_workspace_size(dtype, n, ctypes.byref(size)))
+        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        _check(so.tiso_policy(dtype, rows, targets.data_ptr(), ignore_index, temperature, args,
+                              logps.data_ptr(), coef.data_ptr(), stats.data_ptr(), out.data_ptr(),
+                              _ptr(grad), ws.data_ptr(), size.value, _stream(dev)))
+    return out, logps, coef, stats, grad
+
+
+def _preference_args(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor,
+                     kind: int, average: bool, beta: float, label_smoothing: float,
+                     margin: float) -> PreferenceArgs:
+    return PreferenceArgs(logps.data_ptr(), _ptr(refs), _ptr(mask), offsets.data_ptr(),
+                          logps.numel(), (offsets.numel() - 1) // 2, kind, int(average), beta,
+                          label_smoothing, margin)
+
+
+def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor,
+               kind: int, average: bool, beta: float, label_smoothing: float,
+               margin: float) -> tuple[Tensor, Tensor, Tensor]:
+    """The preference loss of tiso_preference: (loss, rewards [2, pairs], coef [2 pairs]) from
+    contiguous 1-D logps and refs (float32 or float64), mask (bool) and offsets (int64)."""
+    args = _preference_args(logps, refs, mask, offsets, kind, average, beta, label_smoothing,
+                            margin)
+    dev, pairs = logps.device, args.pairs
+    loss = torch.empty((), dtype=logps.dtype, device=dev)
+    rewards = torch.empty(2, pairs, dtype=logps.dtype, device=dev)
+    coef = torch.empty(2 * pairs, dtype=logps.dtype, device=dev)
+    so = lib()
+    size = ctypes.c_size_t()
+    with _on(dev):
+        _check(so.tiso_preference_workspace_size(pairs, ctypes.byref(size)))
+        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+        _check(so.tiso_preference(_DTYPES[logps.dtype], args, loss.data_ptr(), rewards.data_ptr(),
+                                  coef.data_ptr(), ws.data_ptr(), size.value, _stream(dev)))
+    return loss, rewards, coef
+
+
+def preference_grad(logps: Tensor, mask: Tensor | None, offsets: Tensor, coef: Tensor,
+                    upstream: Tensor, want: bool, want_ref: bool
+                    ) -> tuple[Tensor | None, Tensor | None]:
+    """Every token's gradient in logps and in ref_logps from its sequence's coef and the loss's
+    upstream gradient (a device scalar)."""
+    args = _preference_args(logps, None, mask, offsets, 0, False, 1.0, 0.0, 0.0)
+    dev = logps.device
+    grad = torch.empty_like(logps) if want else None
+    grad_ref = torch.empty_like(logps) if want_ref else None
+    with _on(dev):
+        _check(lib().tiso_preference_grad(_DTYPES[logps.dtype], args, coef.data_ptr(),
+                                          upstream.data_ptr(), _ptr(grad), _ptr(grad_ref),
+                                          _stream(dev)))
+    return grad, grad_ref
+
+
+def adamw(device: torch.device, param_dtype: torch.dtype, grad_dtype: torch.dtype, bits: int,
+          fields: list[int], args: AdamwArgs) -> None:
+    """One tiso_adamw call: ``fields`` the tensors' tiso_adamw_tensor structures, 8 numbers each,
+    back to back (pointers of param, grad, exp_avg, exp_avg_sq and the two scales, n, index)."""
+    table = (ctypes.c_int64 * len(fields))(*fields)
+    with _on(device):
+        _check(lib().tiso_adamw(_DTYPES[param_dtype], _DTYPES[grad_dtype], bits, len(fields) // 8,
+                                ctypes.addressof(table), args, _stream(device)))

@@ -1,0 +1,197 @@
+"""AdamW over many tensors in one launch, with its moments in 32 bits or in 8 (the update that
+follows the losses of ``losses.py``; the reference has no counterpart).
+
+With 8-bit states a parameter element costs 2 bytes of optimizer state instead of 8: the running
+mean of the gradient and the square root of the running mean of its square are float8 (e4m3)
+numbers, every 256 elements sharing a power of two (a float32), rounded to one of the two
+neighbouring numbers at random, so that the means of the first moment and of the root's square stay
+right (rounded to nearest, a second moment that moves by a thousandth a step would stay where it
+is). The random bits are a function of ``seed``, the step and the element, so a run can be
+repeated.
+"""
+
+from __future__ import annotations
+
+from collections.abc import Iterable, Sequence
+from itertools import chain, repeat
+from typing import Any
+
+import torch
+from torch import Tensor
+
+from torchisotonic_b200 import _ext
+
+BLOCK = 256  # elements that share a scale
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _bits(dtype: torch.dtype) -> int:
+    if dtype == torch.float32:
+        return 32
+    if dtype == torch.float8_e4m3fn:
+        return 8
+    raise TypeError("optimizer states must be float32 or float8_e4m3fn tensors")
+
+
+def adamw_step(
+    params: Sequence[Tensor],
+    grads: Sequence[Tensor],
+    exp_avgs: Sequence[Tensor],
+    exp_avg_sqs: Sequence[Tensor],
+    *,
+    step: int,
+    lr: float = 1e-3,
+    betas: tuple[float, float] = (0.9, 0.999),
+    eps: float = 1e-8,
+    weight_decay: float = 0.01,
+    scales: tuple[Sequence[Tensor], Sequence[Tensor]] | None = None,
+    seed: int = 0,
+) -> None:
+    """One AdamW step (decoupled weight decay) over all of ``params``, in place:
+
+    ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``, ``p = p (1 - lr weight_decay) - lr / (1 -
+    b1^step) m / (sqrt(v) / sqrt(1 - b2^step) + eps)``, computed in float32.
+
+    All tensors are contiguous and on one CUDA device. ``params``: float32, bfloat16 or float16
+    (rounded to nearest after the step); ``grads``: like their parameter, or float32.
+    ``exp_avgs`` and ``exp_avg_sqs``: float32 (m and v), shaped like the parameters; or
+    float8_e4m3fn, with ``scales = (exp_avg_scales, exp_avg_sq_scales)``, a float32 tensor of
+    ceil(n / 256) numbers for every state: a state's number times its block's scale is then m, and
+    the square root of v. ``step`` counts from 1; ``seed`` enters the rounding of 8-bit states.
+    """
+    lists = [params, grads, exp_avgs, exp_avg_sqs, *(scales or ())]
+    count = len(params)
+    if scales is not None and len(scales) != 2:
+        raise ValueError("scales must be a pair of sequences")
+    if any(len(x) != count for x in lists):
+        raise ValueError("params, grads, states and scales must be of one length")
+    if step < 1:
+        raise ValueError("step must be at least 1")
+    if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+        raise ValueError("betas must be in [0, 1)")
+    if not (lr >= 0 and eps >= 0 and weight_decay >= 0):
+        raise ValueError("lr, eps and weight_decay must not be negative")
+    if count == 0:
+        return
+    for t in chain.from_iterable(lists):
+        if not isinstance(t, Tensor):
+            raise TypeError(f"params, grads, states and scales must be torch.Tensors, got "
+                            f"{type(t).__name__}")
+        if not t.is_contiguous():
+            raise ValueError("params, grads, states and scales must be contiguous")
+    if not params[0].is_cuda:
+        raise RuntimeError(
+            "torchisotonic_b200 runs on CUDA tensors only (no CPU fallback); "
+            "move params to a CUDA device"
+        )
+    device = params[0].device
+    if any(t.device != device for t in chain.from_iterable(lists)):
+        raise ValueError("params, grads, states and scales must be on one device")
+    sizes = [p.numel() for p in params]
+    if any([t.numel() for t in x] != sizes for x in lists[1:4]):
+        raise ValueError("grads and states must be shaped like their parameters")
+    bits = _bits(exp_avgs[0].dtype)
+    if any(t.dtype != exp_avgs[0].dtype for t in chain(exp_avgs, exp_avg_sqs)):
+        raise TypeError("optimizer states must be of one dtype")
+    if (bits == 8) != (scales is not None):
+        raise ValueError("scales go with float8_e4m3fn states, and only with them")
+    if scales is not None:
+        blocks = [-(-n // BLOCK) for n in sizes]
+        for x in scales:
+            if any(t.dtype != torch.float32 for t in x):
+                raise TypeError("scales must be float32 tensors")
+            if [t.numel() for t in x] != blocks:
+                raise ValueError(f"a scale tensor must hold ceil(n / {BLOCK}) numbers")
+    pointers = [[t.data_ptr() for t in x] for x in lists]
+    if scales is None:
+        pointers += [repeat(0, count), repeat(0, count)]
+    fields = zip(*pointers, sizes, range(count))
+    args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
+    by_type: dict[tuple[torch.dtype, torch.dtype], list[tuple[int, ...]]] = {}
+    for p, g, f in zip(params, grads, fields):
+        by_type.setdefault((p.dtype, g.dtype), []).append(f)
+    for pt, gt in by_type:
+        if pt not in (torch.float32, *_HALVES) or gt not in (pt, torch.float32):
+            raise TypeError("params must be float32, bfloat16 or float16, grads like their "
+                            "parameter or float32")
+    for (pt, gt), f in by_type.items():
+        _ext.adamw(device, pt, gt, bits, list(chain.from_iterable(f)), args)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s update through ``adamw_step``: every parameter group in one launch
+    for each pair of parameter and gradient types (480 tensors a launch).
+
+    ``state_bits``: 32, or 8 for float8 moments (see the module). ``seed``: of their rounding.
+    Learning rate, betas, eps and weight decay are per group. ``state_dict`` and
+    ``load_state_dict`` keep the states' types, so a run resumes exactly.
+    """
+
+    def __init__(self, params: Iterable[Any], lr: float = 1e-3,
+                 betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, *, state_bits: int = 32, seed: int = 0) -> None:
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0):
+            raise ValueError("lr, eps and weight_decay must not be negative")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("betas must be in [0, 1)")
+        super().__init__(params, {"lr": lr, "betas": betas, "eps": eps,
+                                  "weight_decay": weight_decay, "state_bits": state_bits,
+                                  "seed": seed})
+
+    def _init_state(self, p: Tensor, bits: int) -> dict[str, Any]:
+        state: dict[str, Any] = {"step": 0}
+        for name in ("exp_avg", "exp_avg_sq"):
+            if bits == 32:
+                state[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                state[name] = torch.zeros(p.shape, dtype=torch.uint8,
+                                          device=p.device).view(torch.float8_e4m3fn)
+                state[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32,
+                                                     device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure: Any = None) -> Any:
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            bits = group["state_bits"]
+            # parameters that joined later, or had no gradient in some steps, are at another step
+            at_step: dict[tuple[int, torch.device], list[Tensor]] = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                state = self.state[p]
+                if not state:
+                    state.update(self._init_state(p, bits))
+                state["step"] += 1
+                at_step.setdefault((state["step"], p.device), []).append(p)
+            for (step, _), params in at_step.items():
+                states = [self.state[p] for p in params]
+                scales = None
+                if bits == 8:
+                    scales = tuple([s[name] for s in states]
+                                   for name in ("exp_avg_scale", "exp_avg_sq_scale"))
+                adamw_step(params, [p.grad.contiguous() for p in params],
+                           [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                           step=step, lr=float(group["lr"]), betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"], scales=scales,
+                           seed=group["seed"])
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        """As torch's, but for the states' types: torch casts them to their parameter's."""
+        super().load_state_dict(state_dict)
+        saved = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = chain.from_iterable(g["params"] for g in self.param_groups)
+        for index, p in zip(saved, params):
+            for name, value in state_dict["state"].get(index, {}).items():
+                if isinstance(value, Tensor):
+                    self.state[p][name] = value.to(device=p.device, copy=True)
