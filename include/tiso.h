@@ -236,10 +236,11 @@ int tiso_logprobs(int dtype, const tiso_rows* x, const int64_t* targets, int64_t
 /* The gradient of sum(coef * upstream * logps) in the logits, in their type, written contiguously
  * ([rows][vocab]): coef[r] upstream / temperature (1[v = targets[r]] - softmax(x[r] / temperature)),
  * zeros for a row that is left out. upstream: NULL (1), or a device scalar; where it is exactly 1
- * then nothing is written (grad must already hold the gradient for 1, as tiso_policy leaves it). */
+ * then nothing is written (grad must already hold the gradient for 1, as tiso_policy leaves it).
+ * coef_dtype: the accumulation type, or TISO_F64. */
 int tiso_logprobs_grad(int dtype, const tiso_rows* x, const int64_t* targets, double temperature,
-                       const void* stats, const void* coef, const void* upstream, void* grad,
-                       void* stream);
+                       const void* stats, int coef_dtype, const void* coef,
+                       const void* upstream, void* grad, void* stream);
 
 /* Per-token inputs of the policy loss (device arrays of `rows` numbers of the accumulation type;
  * ref_logps and weight may be NULL; weight_is_byte: weight is an array of bytes, 0 or 1). */
@@ -259,11 +260,11 @@ int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes);
  * sum(w q) / sum(w) of l, of exp(d) - d - 1 and of [the clip is the smaller side]; all 0 when the
  * weights sum to 0. A token of weight 0 (or whose target is ignore_index) is left out: nothing of
  * it is read beyond its weight and target, its logps, coef and gradient are 0. coef[r] receives
- * d loss / d logps[r], stats what tiso_logprobs_grad needs; grad ([rows][vocab], contiguous)
+ * d loss / d logps[r] in double, stats what tiso_logprobs_grad needs; grad ([rows][vocab], contiguous)
  * coef[r] / temperature (1[v = targets[r]] - softmax). Where both sides of the minimum are equal
  * the slope is that of the unclipped one. Sums run in a fixed order. */
 int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
-                double temperature, const tiso_policy_args* args, void* logps, void* coef,
+                double temperature, const tiso_policy_args* args, void* logps, double* coef,
                 void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,
                 void* stream);
 

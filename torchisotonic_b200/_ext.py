@@ -92,7 +92,7 @@ def lib() -> ctypes.CDLL:
     so.tiso_grad_varlen.argtypes = [i32, p, p, p, p, p, p, p, i64, i64, u32, dbl, dbl, p]
     rows, policy, pref = (ctypes.POINTER(c) for c in (Rows, PolicyArgs, PreferenceArgs))
     so.tiso_logprobs.argtypes = [i32, rows, p, i64, dbl, p, p, p]
-    so.tiso_logprobs_grad.argtypes = [i32, rows, p, dbl, p, p, p, p, p]
+    so.tiso_logprobs_grad.argtypes = [i32, rows, p, dbl, p, i32, p, p, p, p]
     so.tiso_policy_workspace_size.argtypes = [i32, i64, ctypes.POINTER(sz)]
     so.tiso_policy.argtypes = [i32, rows, p, i64, dbl, policy, p, p, p, p, p, p, sz, p]
     so.tiso_preference_workspace_size.argtypes = [i64, ctypes.POINTER(sz)]
@@ -599,7 +599,7 @@ def logprobs(x: Tensor, targets: Tensor, ignore_index: int, temperature: float,
 def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor, coef: Tensor,
                   upstream: Tensor | None = None, grad: Tensor | None = None) -> Tensor:
     """The gradient of sum(coef * upstream * logprobs) in x, in its dtype and shape, contiguous.
-    ``coef``: contiguous, one per row. ``grad``: holds the gradient for upstream = 1 (left as it
+    ``coef``: contiguous, one per row, in the accumulation dtype or float64. ``grad``: holds the gradient for upstream = 1 (left as it
     is when upstream, a device scalar, is 1), or None for a new tensor."""
     x, rows = logits_rows(x)
     dev = x.device
@@ -609,8 +609,8 @@ def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor,
             coef, upstream = coef * upstream, None
     with _on(dev):
         _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
-                                        stats.data_ptr(), coef.data_ptr(), _ptr(upstream),
-                                        grad.data_ptr(), _stream(dev)))
+                                        stats.data_ptr(), _DTYPES[coef.dtype], coef.data_ptr(),
+                                        _ptr(upstream), grad.data_ptr(), _stream(dev)))
     return grad
 
 
@@ -625,8 +625,7 @@ def policy(x: Tensor, targets: Tensor, ignore_index: int, temperature: float, ol
     dev, acc = x.device, acc_dtype(x.dtype)
     dtype, n = _DTYPES[x.dtype], rows.rows
     logps = torch.empty(targets.shape, dtype=acc, device=dev)
-    # per row: coef, then stats; the workspace (float64) behind them
-    coef = torch.empty(n, dtype=acc, device=dev)
+    coef = torch.empty(n, dtype=torch.float64, device=dev)
     stats = torch.empty(2 * n, dtype=acc, device=dev)
     out = torch.empty(3, dtype=acc, device=dev)
     grad = torch.empty(x.shape, dtype=x.dtype, device=dev) if with_grad else None

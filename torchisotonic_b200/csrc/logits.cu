@@ -1,5 +1,6 @@
 // Operators on rows of logits (include/tiso.h: tiso_logprobs*, tiso_policy*): the log-probability
 // of one token per row and its gradient, and the clipped policy loss with its gradient.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <string>
@@ -13,7 +14,11 @@ int report_error(int code, const std::string& msg);
 
 namespace {
 
-constexpr int kThreads = 512;
+namespace cg = cooperative_groups;
+
+constexpr int kBatch = 4;       // vectors a thread loads before it uses the first
+constexpr int kRowWarps = 8;    // rows to a CTA where a warp takes a row
+constexpr int kMostRows = 1 << 28;
 
 int logits_fail(cudaError_t e, const char* what) {
   return report_error(TISO_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
@@ -22,7 +27,8 @@ int logits_fail(cudaError_t e, const char* what) {
 // Rows of logits: row r starts at x + (r / inner) * outer_stride + (r % inner) * inner_stride.
 struct Rows {
   const void* x;
-  int64_t rows, inner, outer_stride, inner_stride, vocab;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int vocab;
   const int64_t* targets;
   int64_t ignore;
 };
@@ -33,75 +39,195 @@ __device__ __forceinline__ const T* row_at(const Rows& a, int64_t r) {
          (r % a.inner) * a.inner_stride;
 }
 
-// The maximum and sum of a row, by all threads of the CTA; every thread gets them.
-template <typename T, typename A>
-__device__ Part<A> row_part(const T* x, int64_t vocab, A k) {
-  __shared__ Part<A> warp_part[kThreads / 32];
-  Part<A> p{lowest<A>(), A(0)};
-  for (int64_t v = threadIdx.x; v < vocab; v += kThreads) {
-    const A z = to_acc(x[v]);
-    const A m = max_acc(p.m, z);
-    const A base = base_of(m);
-    p.s = p.s * scaled_exp(p.m == m ? A(0) : p.m - base, k) + scaled_exp(z - base, k);
-    p.m = m;
+// Who works on a row: a warp (kThreads 32; kRowWarps rows to a CTA), a CTA, or a cluster of CTAs
+// (kThreads > 32; the row's index is the cluster's).
+template <int kThreads>
+struct Place {
+  int64_t row;
+  int rank, threads;  // this thread's and how many there are to the row
+
+  __device__ __forceinline__ Place() {
+    if constexpr (kThreads == 32) {
+      row = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+      rank = threadIdx.x & 31;
+      threads = 32;
+    } else {
+      const unsigned ctas = cg::this_cluster().num_blocks();
+      row = blockIdx.x / ctas;
+      rank = static_cast<int>(blockIdx.x % ctas) * kThreads + threadIdx.x;
+      threads = static_cast<int>(ctas) * kThreads;
+    }
   }
-  p = join_warp(p, k);
-  if ((threadIdx.x & 31) == 0) warp_part[threadIdx.x >> 5] = p;
-  __syncthreads();
-  p = warp_part[0];
-  for (int i = 1; i < kThreads / 32; ++i) p = join(p, warp_part[i], k);
-  __syncthreads();
+  __device__ __forceinline__ bool first() const { return rank == 0; }
+};
+
+// The part of a row that one thread sees: vectors rank, rank + threads, ..., and for the first
+// warp a single element each.
+template <typename T, typename A>
+__device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, int rank, int threads, A k) {
+  Part<A> p{lowest<A>(), A(0)};
+  if (rank < r.edges) {
+    const A z = to_acc(r.x[r.edge(rank)]);
+    p = {z, scaled_exp(z - base_of(z), k)};
+  }
+  for (int v = rank; v < r.vectors; v += kBatch * threads) {
+    uint4 q[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      q[i] = v + i * threads < r.vectors ? load_vector(r, v + i * threads) : no_vector<T>();
+    const A m = max_acc(p.m, vector_max<T>(q));
+    const A base = base_of(m);
+    p.s *= scaled_exp(p.m == m ? A(0) : p.m - base, k);
+    p.m = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      A x[RowView<T>::E];
+      unpack<T>(q[i], x);
+      exponentials(x, base, k);
+      p.s += total(x);
+    }
+  }
   return p;
 }
 
-// log softmax(x / t) at the target. The steps after the sum are in double: in float, rounding
-// x - m - log s near 10 would cost more than the whole sum did.
-template <typename T, typename A>
-__device__ __forceinline__ double logp_of(const T* x, int64_t vocab, int64_t target, const Part<A>& p,
-                                     double inv_temp) {
-  if (target < 0 || target >= vocab) return nan_of(0.0);
-  const double m = base_of(p.m);
-  return (static_cast<double>(to_acc(x[target])) - m) * inv_temp - log(static_cast<double>(p.s));
+// The parts of all of a row's threads joined; every thread gets the result. Called once by a CTA
+// (its shared memory is not used again), by all of its threads.
+template <int kThreads, typename A>
+__device__ __forceinline__ Part<A> join_threads(Part<A> p, A k) {
+  p = join_lanes<32>(p, k);
+  if constexpr (kThreads > 32) {
+    constexpr int kWarps = kThreads / 32, kMostCtas = 8;
+    __shared__ Part<A> of_warp[kWarps], of_cta[kMostCtas];
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) of_warp[threadIdx.x >> 5] = p;
+    __syncthreads();
+    p = join_lanes<kWarps>(of_warp[lane % kWarps], k);
+    auto cluster = cg::this_cluster();
+    const int ctas = static_cast<int>(cluster.num_blocks());
+    if (ctas > 1) {
+      if (threadIdx.x < ctas)
+        *cluster.map_shared_rank(&of_cta[cluster.block_rank()], threadIdx.x) = p;
+      cluster.sync();
+      p = {lowest<A>(), A(0)};
+      if (lane % kMostCtas < ctas) p = of_cta[lane % kMostCtas];
+      p = join_lanes<kMostCtas>(p, k);
+    }
+  }
+  return p;
 }
 
-// d/dx of c * logp(x / t): c / t (1[v = target] - softmax), c already divided by t. An index out
-// of range gives NaN throughout.
+// log softmax(x / t) at the target from its logit. The steps after the sum are in double: in float,
+// rounding x - m - log s near 10 would cost more than the whole sum did, and a policy's ratio is
+// the exponential of a difference of two such numbers.
+template <typename A>
+__device__ __forceinline__ double logp_of(A x, const Part<A>& p, double inv_temp) {
+  return (static_cast<double>(x) - static_cast<double>(base_of(p.m))) * inv_temp -
+         log(static_cast<double>(p.s));
+}
+
 template <typename T, typename A>
-__device__ void write_grad(const T* x, T* g, int64_t vocab, int64_t target, A base, A s, A c, A k) {
-  const A scale = target < 0 || target >= vocab ? nan_of(A(0)) : -c / s;
-  for (int64_t v = threadIdx.x; v < vocab; v += kThreads) {
-    A d = scaled_exp(to_acc(x[v]) - base, k) * scale;
-    if (v == target) d += c;
-    g[v] = from_acc<T>(d);
+__device__ __forceinline__ A target_logit(const T* x, int vocab, int64_t target) {
+  return target < 0 || target >= vocab ? nan_of(A(0)) : to_acc(x[target]);
+}
+
+// What a row's gradient is made of: c / t (1[v = target] - softmax), the softmax from the row's
+// base and sum, c already divided by t. A target out of range gives NaN throughout. Each product
+// and sum is rounded on its own, so that every kernel that writes it writes the same bits.
+template <typename A>
+struct Slope {
+  A base, scale, k;
+  int target;
+  double c;  // the target's own gradient, c (1 - p), is rounded once
+
+  __device__ __forceinline__ Slope(A base_, A s, double c_, A k_, int64_t target_, int vocab)
+      : base(base_), k(k_), c(c_) {
+    const bool in = target_ >= 0 && target_ < vocab;
+    target = in ? static_cast<int>(target_) : -1;
+    scale = in ? -static_cast<A>(c_) / s : nan_of(A(0));
+  }
+  __device__ __forceinline__ A at_target(A d) const {
+    return static_cast<A>(__dadd_rn(c, static_cast<double>(d)));
+  }
+  __device__ __forceinline__ A at(A x, int v) const {
+    const A d = mul_rn(scaled_exp(x - base, k), scale);
+    return v == target ? at_target(d) : d;
+  }
+};
+
+template <typename T, typename A>
+__device__ __forceinline__ uint4 slope_vector(const uint4& q, const Slope<A>& slope, int element) {
+  constexpr int E = RowView<T>::E;
+  A x[E];
+  unpack<T>(q, x);
+  exponentials(x, slope.base, slope.k);
+#pragma unroll
+  for (int j = 0; j < E; ++j) x[j] = mul_rn(x[j], slope.scale);
+  const unsigned at = static_cast<unsigned>(slope.target - element);
+  if (at < static_cast<unsigned>(E)) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (at == static_cast<unsigned>(j)) x[j] = slope.at_target(x[j]);
+  }
+  return pack<T>(x);
+}
+
+// The gradient of vectors first, first + step, ... below end, and of a single element for ranks
+// below the number of those.
+template <typename T, typename A>
+__device__ __forceinline__ void write_slope(const RowView<T>& r, int rank, int first, int step,
+                                            int end, const Slope<A>& slope) {
+  if (rank < r.edges) {
+    const int v = r.edge(rank);
+    r.g[v] = from_acc<T>(slope.at(to_acc(r.x[v]), v));
+  }
+  for (int v = first; v < end; v += kBatch * step) {
+    uint4 q[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (v + i * step < end) q[i] = load_vector(r, v + i * step);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (v + i * step < end) {
+        const int e = r.element(v + i * step);
+        store_once(r.g + e, slope_vector<T>(q[i], slope, e));
+      }
   }
 }
 
 template <typename T>
-__device__ void write_zeros(T* g, int64_t vocab) {
-  for (int64_t v = threadIdx.x; v < vocab; v += kThreads)
-    g[v] = from_acc<T>(typename AccOf<T>::type(0));
+__device__ __forceinline__ void write_zeros(const RowView<T>& r, int rank, int first, int step,
+                                            int end) {
+  if (rank < r.edges) r.g[r.edge(rank)] = from_acc<T>(typename AccOf<T>::type(0));
+  for (int v = first; v < end; v += step)
+    store_once(r.g + r.element(v), make_uint4(0, 0, 0, 0));
 }
 
 // A row that is left out (its target is the ignored index, or its weight is 0) is marked by a
 // negative sum in stats: its gradient is zeros and its logits are not read.
 constexpr int kLeftOut = -1;
 
-template <typename T, typename A>
-__global__ void __launch_bounds__(kThreads)
+template <typename T, typename A, int kThreads>
+__global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
     logprobs_kernel(Rows a, double inv_temp, A k, A* logps, A* stats) {
-  const int64_t r = blockIdx.x;
+  const Place<kThreads> place;
+  const int64_t r = place.row;
+  if (r >= a.rows) return;
   const int64_t target = a.targets[r];
   if (target == a.ignore) {
-    if (threadIdx.x == 0) {
+    if (place.first()) {
       logps[r] = A(0);
       if (stats) stats[2 * r + 1] = A(kLeftOut);
     }
     return;
   }
   const T* x = row_at<T>(a, r);
-  const Part<A> p = row_part(x, a.vocab, k);
-  if (threadIdx.x == 0) {
-    logps[r] = static_cast<A>(logp_of(x, a.vocab, target, p, inv_temp));
+  A at_target = A(0);
+  if (place.first()) at_target = target_logit<T, A>(x, a.vocab, target);
+  const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
+  const Part<A> p =
+      join_threads<kThreads>(thread_part<T, A>(view, place.rank, place.threads, k), k);
+  if (place.first()) {
+    logps[r] = static_cast<A>(logp_of(at_target, p, inv_temp));
     if (stats) {
       stats[2 * r] = base_of(p.m);
       stats[2 * r + 1] = p.s;
@@ -110,21 +236,33 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // coef: per row, d loss / d logp. upstream (may be NULL): a scalar that multiplies it, and where
-// it is 1 nothing is written.
-template <typename T, typename A>
-__global__ void __launch_bounds__(kThreads)
-    logprobs_grad_kernel(Rows a, double inv_temp, A k, const A* stats, const A* coef,
-                         const A* upstream, T* grad) {
+// it is 1 nothing is written. Work is cut into pieces of a row, `pieces` to the row, for a warp or
+// a CTA (kThreads) each.
+template <typename T, typename A, typename C, int kThreads>
+__global__ void __launch_bounds__(256)
+    logprobs_grad_kernel(Rows a, double inv_temp, A k, const A* stats, const C* coef,
+                         const A* upstream, T* grad, int pieces) {
   const A up = upstream ? *upstream : A(1);
   if (upstream && up == A(1)) return;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  constexpr int kGroups = 256 / kThreads;
+  const int rank = threadIdx.x % kThreads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kThreads;
+       i < a.rows * pieces; i += static_cast<int64_t>(gridDim.x) * kGroups) {
+    const int64_t r = i / pieces;
+    const int piece = static_cast<int>(i % pieces);
     T* g = grad + r * a.vocab;
+    const RowView<T> view(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
+    // the last piece takes what is left; the first the single elements
+    const int first = piece * kBatch * kThreads;
+    const int end = piece == pieces - 1 ? view.vectors : min(view.vectors, first + kBatch * kThreads);
+    const int edge_rank = piece == 0 ? rank : view.edges;
     const A sum = stats[2 * r + 1];
     if (sum < A(0)) {
-      write_zeros(g, a.vocab);
+      write_zeros(view, edge_rank, first + rank, kThreads, end);
     } else {
-      write_grad(row_at<T>(a, r), g, a.vocab, a.targets[r], stats[2 * r], sum,
-                 static_cast<A>(coef[r] * up * inv_temp), k);
+      const Slope<A> slope(stats[2 * r], sum, static_cast<double>(coef[r]) * up * inv_temp,
+                           k, a.targets[r], a.vocab);
+      write_slope(view, edge_rank, first + rank, kThreads, end, slope);
     }
   }
 }
@@ -141,7 +279,7 @@ struct PolicyArgs {
   int weight_kind;
   double lo, hi, kl_coef;  // lo, hi: the clip's edges 1 - clip_low and 1 + clip_high
   A* logps;           // per row
-  A* coef;            // per row, d loss / d logp
+  double* coef;       // per row, d loss / d logp
   A* stats;           // per row, maximum and sum
   A* terms;           // per row, w loss, w kl and w [clipped]
   A* out;             // loss, kl, clip fraction
@@ -183,66 +321,89 @@ __global__ void __launch_bounds__(1024) policy_total_kernel(Rows a, PolicyArgs<A
 //   rho = exp(logp - old);  loss = -min(rho A, clip(rho) A) + kl_coef kl,
 //   kl = exp(d) - d - 1, d = ref - logp;
 //   slope = -rho A where rho A <= clip(rho) A, else 0, plus kl_coef (1 - exp(d)).
-// In double: one thread a row does it, and the ratio's exponent is a difference of numbers
-// near 10 whose float rounding would be the largest error of the loss.
-template <typename A>
-__device__ void policy_token(const PolicyArgs<A>& p, int64_t r, double lp, double* loss,
-                             double* slope, double* kl, bool* clipped) {
-  const double adv = p.advantages[r];
-  const double ratio = exp(lp - static_cast<double>(p.old_logps[r]));
-  const double held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * adv;
-  const double free_side = ratio * adv;
-  *clipped = free_side > held;
-  *loss = -(free_side > held ? held : free_side);
-  *slope = free_side > held ? 0.0 : -free_side;
-  *kl = 0;
-  if (p.ref_logps) {
-    const double d = static_cast<double>(p.ref_logps[r]) - lp;
-    const double e = expm1(d);
-    *kl = e - d;
-    *loss += p.kl_coef * *kl;
-    *slope -= p.kl_coef * e;
-  }
-}
+struct Token {
+  double loss, slope, kl;
+  bool clipped;
 
-template <typename T, typename A>
-__global__ void __launch_bounds__(kThreads)
+  template <typename A>
+  __device__ __forceinline__ Token(double lp, double old, double ref, double adv,
+                                   const PolicyArgs<A>& p) {
+    const double ratio = exp(lp - old);
+    const double free_side = ratio * adv;
+    const double held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * adv;
+    clipped = free_side > held;
+    loss = -(clipped ? held : free_side);
+    slope = clipped ? 0.0 : -free_side;
+    kl = 0.0;
+    if (p.ref_logps) {
+      const double d = ref - lp;
+      const double e = expm1(d);
+      kl = e - d;
+      loss += p.kl_coef * kl;
+      slope -= p.kl_coef * e;
+    }
+  }
+};
+
+template <typename T, typename A, int kThreads>
+__global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
     policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
-  __shared__ A shared_coef;
-  const int64_t r = blockIdx.x;
-  T* g = grad + r * a.vocab;
+  const Place<kThreads> place;
+  const int64_t r = place.row;
+  if (r >= a.rows) return;
   const A w = weight_of(a, p, r);
+  const T* x = row_at<T>(a, r);
+  // without a gradient the row is cut as with one (in a buffer on a vector's boundary), so that
+  // the loss is the same bits
+  T* g = grad + r * a.vocab;
+  const RowView<T> view(x, g, reinterpret_cast<uintptr_t>(g), a.vocab);
   if (w == A(0)) {
-    if (threadIdx.x == 0) {
-      p.logps[r] = p.coef[r] = A(0);
+    if (place.first()) {
+      p.logps[r] = A(0);
+      p.coef[r] = 0;
       p.stats[2 * r + 1] = A(kLeftOut);
       p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
     }
-    if (grad) write_zeros(g, a.vocab);
+    if (grad) write_zeros(view, place.rank, place.rank, place.threads, view.vectors);
     return;
   }
-  const T* x = row_at<T>(a, r);
-  const Part<A> part = row_part(x, a.vocab, k);
   const int64_t target = a.targets[r];
-  if (threadIdx.x == 0) {
-    const double lp = logp_of(x, a.vocab, target, part, inv_temp);
-    double loss, slope, kl;
-    bool clipped;
-    policy_token(p, r, lp, &loss, &slope, &kl, &clipped);
+  // one warp of a CTA (every warp that has a row to itself) goes from the sum to the coefficient
+  const bool steps = kThreads == 32 || threadIdx.x < 32;
+  A at_target = A(0), old = A(0), adv = A(0), ref = A(0);
+  if (steps) {
+    at_target = target_logit<T, A>(x, a.vocab, target);
+    old = p.old_logps[r];
+    adv = p.advantages[r];
+    if (p.ref_logps) ref = p.ref_logps[r];
+  }
+  const Part<A> part =
+      join_threads<kThreads>(thread_part<T, A>(view, place.rank, place.threads, k), k);
+  double coef = 0;
+  if (steps) {
+    const double lp = logp_of(at_target, part, inv_temp);
+    const Token token(lp, old, ref, adv, p);
     const double total = *p.total;
-    const A coef = total == 0 ? A(0) : static_cast<A>(w * slope / total);
-    p.logps[r] = static_cast<A>(lp);
-    p.coef[r] = shared_coef = coef;
-    p.stats[2 * r] = base_of(part.m);
-    p.stats[2 * r + 1] = part.s;
-    p.terms[3 * r] = static_cast<A>(w * loss);
-    p.terms[3 * r + 1] = static_cast<A>(w * kl);
-    p.terms[3 * r + 2] = clipped ? w : A(0);
+    if (total != 0) coef = w * token.slope / total;
+    if (place.first()) {
+      p.logps[r] = static_cast<A>(lp);
+      p.coef[r] = coef;
+      p.stats[2 * r] = base_of(part.m);
+      p.stats[2 * r + 1] = part.s;
+      p.terms[3 * r] = static_cast<A>(w * token.loss);
+      p.terms[3 * r + 1] = static_cast<A>(w * token.kl);
+      p.terms[3 * r + 2] = token.clipped ? w : A(0);
+    }
   }
   if (!grad) return;
-  __syncthreads();
-  write_grad(x, g, a.vocab, target, base_of(part.m), part.s,
-             static_cast<A>(shared_coef * inv_temp), k);
+  if constexpr (kThreads > 32) {
+    __shared__ double of_warp_0;
+    if (threadIdx.x == 0) of_warp_0 = coef;
+    __syncthreads();
+    coef = of_warp_0;
+  }
+  const Slope<A> slope(base_of(part.m), part.s, coef * inv_temp, k, target, a.vocab);
+  write_slope(view, place.rank, place.rank, place.threads, view.vectors, slope);
 }
 
 // The means over the tokens, in a fixed order; 0 when the weights sum to 0.
@@ -270,15 +431,20 @@ int check_rows(int dtype, const tiso_rows* x, const int64_t* targets) {
     return report_error(TISO_ERR_ARGUMENT, "need rows >= 0, vocab >= 1 and inner >= 1");
   if (x->outer_stride < 0 || x->inner_stride < 0)
     return report_error(TISO_ERR_ARGUMENT, "strides must not be negative");
-  if (x->rows > int64_t{2147483647})
-    return report_error(TISO_ERR_ARGUMENT, "more than 2^31 - 1 rows");
+  if (x->rows > kMostRows || x->vocab > int64_t{1} << 30)
+    return report_error(TISO_ERR_ARGUMENT, "more than 2^28 rows or a vocabulary of more than 2^30");
   if (x->rows && (!x->data || !targets))
     return report_error(TISO_ERR_ARGUMENT, "logits and targets must not be NULL");
+  const int size = dtype == TISO_F64 ? 8 : dtype == TISO_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(x->data) % size)
+    return report_error(TISO_ERR_ARGUMENT, "logits must be aligned to their elements");
   return TISO_OK;
 }
 
 Rows rows_of(const tiso_rows* x, const int64_t* targets, int64_t ignore) {
-  return {x->data, x->rows, x->inner, x->outer_stride, x->inner_stride, x->vocab, targets, ignore};
+  return {x->data,         x->rows,          x->inner,
+          x->outer_stride, x->inner_stride,  static_cast<int>(x->vocab),
+          targets,         ignore};
 }
 
 // log2(e) / t for the exponentials in float, 1 / t for those in double
@@ -292,14 +458,6 @@ int launched(const char* what) {
   return e == cudaSuccess ? TISO_OK : logits_fail(e, what);
 }
 
-template <typename T>
-int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaStream_t st) {
-  using A = typename AccOf<T>::type;
-  logprobs_kernel<T, A><<<static_cast<unsigned>(a.rows), kThreads, 0, st>>>(
-      a, inv_temp, exp_factor(A(0), inv_temp), static_cast<A*>(logps), static_cast<A*>(stats));
-  return launched("logprobs_kernel launch");
-}
-
 int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess)
@@ -307,20 +465,71 @@ int sm_count() {
   return sms;
 }
 
+// A launch of a kernel over rows, `ctas` (a power of two up to 8) to the row as a cluster.
+template <typename... P, typename... Q>
+int launch_rows(void (*kernel)(P...), int64_t rows, int threads, int ctas, cudaStream_t st,
+                const char* what, Q... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(threads == 32 ? (rows + kRowWarps - 1) / kRowWarps
+                                                            : rows * ctas));
+  config.blockDim = dim3(threads == 32 ? 32 * kRowWarps : threads);
+  config.stream = st;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(threads == 32 ? 1 : ctas);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+  return e == cudaSuccess ? TISO_OK : logits_fail(e, what);
+}
+
+// Rows of at most this many vectors go to a warp each.
+constexpr int kWarpVectors = 256;
+
+// CTAs of `threads` to a row: doubled while rows are too few to fill the GPU and a CTA would have
+// more than a batch for each thread.
+int ctas_for(int64_t rows, int64_t vectors, int threads, int sms) {
+  int ctas = 1;
+  while (ctas < 8 && rows * ctas < 2 * sms && vectors > int64_t{ctas} * threads * kBatch) ctas *= 2;
+  return ctas;
+}
+
 template <typename T>
+int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  const int vectors = a.vocab / RowView<T>::E;
+  const A k = exp_factor(A(0), inv_temp);
+  if (vectors <= kWarpVectors)
+    return launch_rows(logprobs_kernel<T, A, 32>, a.rows, 32, 1, st, "logprobs_kernel launch", a,
+                       inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
+  return launch_rows(logprobs_kernel<T, A, 256>, a.rows, 256,
+                     ctas_for(a.rows, vectors, 256, sm_count()), st, "logprobs_kernel launch", a,
+                     inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
+}
+
+template <typename T, typename C>
 int run_logprobs_grad(const Rows& a, double inv_temp, const void* stats, const void* coef,
                       const void* upstream, void* grad, cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  const int64_t most = int64_t{sm_count()} * 4;
-  logprobs_grad_kernel<T, A><<<static_cast<unsigned>(a.rows < most ? a.rows : most), kThreads, 0,
-                               st>>>(a, inv_temp, exp_factor(A(0), inv_temp),
-                                     static_cast<const A*>(stats), static_cast<const A*>(coef),
-                                     static_cast<const A*>(upstream), static_cast<T*>(grad));
+  const int vectors = a.vocab / RowView<T>::E;
+  const bool by_warp = vectors <= kWarpVectors;
+  const int piece = kBatch * (by_warp ? 32 : 256);
+  const int pieces = by_warp ? 1 : (vectors + piece - 1) / piece;
+  const int64_t all = (a.rows * pieces + (by_warp ? 7 : 0)) / (by_warp ? 8 : 1);
+  // where the launch may have nothing to do (upstream is 1), no more CTAs than are resident
+  const int64_t most = upstream ? int64_t{sm_count()} * 8 : int64_t{1} << 30;
+  const unsigned grid = static_cast<unsigned>(all < most ? all : most);
+  const A k = exp_factor(A(0), inv_temp);
+  auto kernel = by_warp ? logprobs_grad_kernel<T, A, C, 32> : logprobs_grad_kernel<T, A, C, 256>;
+  kernel<<<grid, 256, 0, st>>>(a, inv_temp, k, static_cast<const A*>(stats),
+                               static_cast<const C*>(coef), static_cast<const A*>(upstream),
+                               static_cast<T*>(grad), pieces);
   return launched("logprobs_grad_kernel launch");
 }
 
 template <typename T>
-int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* logps, void* coef,
+int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* logps, double* coef,
                void* stats, void* out, void* grad, void* workspace, cudaStream_t st) {
   using A = typename AccOf<T>::type;
   PolicyArgs<A> p{};
@@ -333,15 +542,25 @@ int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* 
   p.hi = 1.0 + q->clip_high;
   p.kl_coef = q->kl_coef;
   p.logps = static_cast<A*>(logps);
-  p.coef = static_cast<A*>(coef);
+  p.coef = coef;
   p.stats = static_cast<A*>(stats);
   p.out = static_cast<A*>(out);
   p.total = static_cast<double*>(workspace);
   p.terms = reinterpret_cast<A*>(p.total + 1);
   policy_total_kernel<A><<<1, 1024, 0, st>>>(a, p);
-  if (a.rows > 0)
-    policy_kernel<T, A><<<static_cast<unsigned>(a.rows), kThreads, 0, st>>>(
-        a, p, inv_temp, exp_factor(A(0), inv_temp), static_cast<T*>(grad));
+  if (a.rows > 0) {
+    const int vectors = a.vocab / RowView<T>::E;
+    const A k = exp_factor(A(0), inv_temp);
+    T* g = static_cast<T*>(grad);
+    const int rc =
+        vectors <= kWarpVectors
+            ? launch_rows(policy_kernel<T, A, 32>, a.rows, 32, 1, st, "policy_kernel launch", a, p,
+                          inv_temp, k, g)
+            : launch_rows(policy_kernel<T, A, 256>, a.rows, 256,
+                          ctas_for(a.rows, vectors, 256, sm_count()), st, "policy_kernel launch",
+                          a, p, inv_temp, k, g);
+    if (rc) return rc;
+  }
   policy_means_kernel<A><<<1, 1024, 0, st>>>(a.rows, p);
   return launched("policy kernels launch");
 }
@@ -379,18 +598,24 @@ int tiso_logprobs(int dtype, const tiso_rows* x, const int64_t* targets, int64_t
 }
 
 int tiso_logprobs_grad(int dtype, const tiso_rows* x, const int64_t* targets, double temperature,
-                       const void* stats, const void* coef, const void* upstream, void* grad,
-                       void* stream) {
+                       const void* stats, int coef_dtype, const void* coef,
+                       const void* upstream, void* grad, void* stream) {
   const int rc = check_rows(dtype, x, targets);
   if (rc) return rc;
   if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
   if (x->rows == 0) return TISO_OK;
   if (!stats || !coef || !grad)
     return report_error(TISO_ERR_ARGUMENT, "stats, coef and grad must not be NULL");
+  if (coef_dtype != TISO_F64 && (coef_dtype != TISO_F32 || dtype == TISO_F64))
+    return report_error(TISO_ERR_ARGUMENT, "coef_dtype must be the accumulation type or TISO_F64");
   const Rows a = rows_of(x, targets, 0);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_type(dtype, [&](auto t) {
-    return run_logprobs_grad<decltype(t)>(a, 1.0 / temperature, stats, coef, upstream, grad,
-                                          static_cast<cudaStream_t>(stream));
+    using T = decltype(t);
+    if (coef_dtype == TISO_F64)
+      return run_logprobs_grad<T, double>(a, 1.0 / temperature, stats, coef, upstream, grad, st);
+    return run_logprobs_grad<T, typename AccOf<T>::type>(a, 1.0 / temperature, stats, coef,
+                                                         upstream, grad, st);
   });
 }
 
@@ -405,7 +630,7 @@ int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes) {
 }
 
 int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
-                double temperature, const tiso_policy_args* args, void* logps, void* coef,
+                double temperature, const tiso_policy_args* args, void* logps, double* coef,
                 void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,
                 void* stream) {
   int rc = check_rows(dtype, x, targets);

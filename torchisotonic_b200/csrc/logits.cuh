@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace tiso {
 
 template <typename T>
@@ -74,11 +76,17 @@ __device__ __forceinline__ float scaled_exp(float d, float k) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * k));
   return r;
 }
-__device__ __forceinline__ double scaled_exp(double d, double k) { return exp(d * k); }
+__device__ __forceinline__ double scaled_exp(double d, double k) { return exp(__dmul_rn(d, k)); }
 
 // max(a, b) with a NaN ignored: the NaN reaches the sum through its own exponential.
 __device__ __forceinline__ float max_acc(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double max_acc(double a, double b) { return fmax(a, b); }
+
+// Products and sums that are not contracted into one operation.
+__device__ __forceinline__ float mul_rn(float a, float b) { return __fmul_rn(a, b); }
+__device__ __forceinline__ double mul_rn(double a, double b) { return __dmul_rn(a, b); }
+__device__ __forceinline__ float add_rn(float a, float b) { return __fadd_rn(a, b); }
+__device__ __forceinline__ double add_rn(double a, double b) { return __dadd_rn(a, b); }
 
 // The point that exponentials are taken from: the maximum, or 0 where nothing but -infinity has
 // been seen (-infinity minus itself is NaN; every exponential is then 0).
@@ -96,15 +104,238 @@ template <typename A>
 __device__ __forceinline__ Part<A> join(const Part<A>& a, const Part<A>& b, A k) {
   const A m = max_acc(a.m, b.m);
   const A base = base_of(m);
-  // a part that holds the maximum keeps its sum as it is (its exponent is exactly 0)
-  return {m, a.s * scaled_exp(a.m == m ? A(0) : a.m - base, k) +
-                 b.s * scaled_exp(b.m == m ? A(0) : b.m - base, k)};
+  // a part that holds the maximum keeps its sum as it is (its exponent is exactly 0); no
+  // contraction, so that join(a, b) and join(b, a) are the same bits
+  return {m, add_rn(mul_rn(a.s, scaled_exp(a.m == m ? A(0) : a.m - base, k)),
+                    mul_rn(b.s, scaled_exp(b.m == m ? A(0) : b.m - base, k)))};
 }
 
-template <typename A>
-__device__ __forceinline__ Part<A> join_warp(Part<A> p, A k) {
+// ---------------------------------------------------------------------------------------------
+// A row in 16-byte vectors. Rows start anywhere (an odd vocabulary, a cut tensor), so a row is a
+// body of whole vectors and at most 4 E - 1 single elements around it (E to a vector). The body is
+// aligned for the row that is written, g; where the row read, x, is off that by `shift` elements,
+// a vector of x is put together from the two aligned ones that hold it. No load leaves the row.
+
+template <typename T>
+struct RowView {
+  static constexpr int E = 16 / sizeof(T);
+  const T* x;
+  T* g;
+  int head, vectors, edges, shift;
+
+  // `address`: the written row's; where none is written, what decides the cut
+  __device__ __forceinline__ RowView(const T* x_, T* g_, uintptr_t address, int vocab)
+      : x(x_), g(g_) {
+    head = static_cast<int>((16 - (address & 15)) & 15) / static_cast<int>(sizeof(T));
+    shift = static_cast<int>((reinterpret_cast<uintptr_t>(x_ + head) & 15) / sizeof(T));
+    if (shift > head) head += E;
+    head = min(head, vocab);
+    // with a shift, vector v also reads the aligned vector after its own
+    vectors = max(0, (vocab - head + shift) / E - (shift ? 1 : 0));
+    edges = vocab - vectors * E;
+  }
+
+  // the e-th single element's index in the row
+  __device__ __forceinline__ int edge(int e) const { return e < head ? e : vectors * E + e; }
+  __device__ __forceinline__ int element(int v) const { return head + v * E; }
+};
+
+template <int kBytes>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[8], bool on) {
+  if constexpr (kBytes >= 4) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
+    for (int i = 0; i + kBytes / 4 < 8; ++i) w[i] = on ? w[i + kBytes / 4] : w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i) w[i] = on ? __funnelshift_r(w[i], w[i + 1], 8 * kBytes) : w[i];
+  }
+}
+
+__device__ __forceinline__ uint4 load_once(const void* p) {  // read once: keeps out of L1
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 load_vector(const RowView<T>& r, int v) {
+  const T* at = r.x + r.element(v) - r.shift;
+  if (r.shift == 0) return load_once(at);
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(at));
+  const uint4 b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int bytes = r.shift * static_cast<int>(sizeof(T));
+  shift_words<8>(w, bytes & 8);
+  if constexpr (sizeof(T) <= 4) shift_words<4>(w, bytes & 4);
+  if constexpr (sizeof(T) <= 2) shift_words<2>(w, bytes & 2);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A vector of -infinity: what a thread holds where the row has no vector for it.
+template <typename T>
+__device__ __forceinline__ uint4 no_vector() {
+  if constexpr (sizeof(T) == 8) {
+    return make_uint4(0, 0xfff00000u, 0, 0xfff00000u);
+  } else {
+    const uint32_t w = std::is_same_v<T, __half>          ? 0xfc00fc00u
+                       : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u
+                                                          : 0xff800000u;
+    return make_uint4(w, w, w, w);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& q, typename AccOf<T>::type (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  } else if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]);
+  } else {
+    x[0] = __hiloint2double(static_cast<int>(w[1]), static_cast<int>(w[0]));
+    x[1] = __hiloint2double(static_cast<int>(w[3]), static_cast<int>(w[2]));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack(const typename AccOf<T>::type (&x)[16 / sizeof(T)]) {
+  uint32_t w[4];
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  } else if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[2 * i] = static_cast<uint32_t>(__double2loint(x[i]));
+      w[2 * i + 1] = static_cast<uint32_t>(__double2hiint(x[i]));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The largest element of kN vectors (a NaN is ignored; it reaches the sum).
+template <typename T, int kN>
+__device__ __forceinline__ typename AccOf<T>::type vector_max(const uint4 (&q)[kN]) {
+  using A = typename AccOf<T>::type;
+  if constexpr (sizeof(T) == 2) {
+    using H2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const uint4 none = no_vector<T>();
+    H2 m = *reinterpret_cast<const H2*>(&none.x);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const H2* h = reinterpret_cast<const H2*>(&q[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = __hmax2(m, h[j]);
+    }
+    return fmaxf(to_acc(m.x), to_acc(m.y));
+  } else {
+    A m = lowest<A>();
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      A x[16 / sizeof(T)];
+      unpack<T>(q[i], x);
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(16 / sizeof(T)); ++j) m = max_acc(m, x[j]);
+    }
+    return m;
+  }
+}
+
+// Two floats at once where the type allows it: (x - base) k, and sums.
+__device__ __forceinline__ float2 sub_mul2(float2 x, float base, float k) {
+  float2 r;
+  asm("{.reg .b64 x, b, k, d;\n\t"
+      "mov.b64 x, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %4};\n\t"
+      "mov.b64 k, {%5, %5};\n\t"
+      "add.rn.f32x2 d, x, b;\n\t"
+      "mul.rn.f32x2 d, d, k;\n\t"
+      "mov.b64 {%0, %1}, d;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(-base), "f"(k));
+  return r;
+}
+__device__ __forceinline__ float exp2_of(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// exp((x - base) / t) of a vector's elements, in place.
+template <int kE>
+__device__ __forceinline__ void exponentials(float (&x)[kE], float base, float k) {
+#pragma unroll
+  for (int j = 0; j < kE; j += 2) {
+    const float2 d = sub_mul2(make_float2(x[j], x[j + 1]), base, k);
+    x[j] = exp2_of(d.x);
+    x[j + 1] = exp2_of(d.y);
+  }
+}
+template <int kE>
+__device__ __forceinline__ void exponentials(double (&x)[kE], double base, double k) {
+#pragma unroll
+  for (int j = 0; j < kE; ++j) x[j] = exp(mul_rn(x[j] - base, k));
+}
+
+// The sum of a vector's elements.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 a, a, b;\n\t"
+      "mov.b64 {%0, %1}, a;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+template <int kE>
+__device__ __forceinline__ float total(const float (&x)[kE]) {
+  float2 s = make_float2(x[0], x[1]);
+#pragma unroll
+  for (int j = 2; j < kE; j += 2) s = add2(s, make_float2(x[j], x[j + 1]));
+  return s.x + s.y;
+}
+template <int kE>
+__device__ __forceinline__ double total(const double (&x)[kE]) {
+  return x[0] + x[1];
+}
+
+__device__ __forceinline__ void store_once(void* p, const uint4& v) {
+  __stcs(reinterpret_cast<uint4*>(p), v);
+}
+
+// The parts of kLanes neighbouring lanes joined (each lane gets the result).
+template <int kLanes, typename A>
+__device__ __forceinline__ Part<A> join_lanes(Part<A> p, A k) {
+#pragma unroll
+  for (int d = kLanes / 2; d; d >>= 1) {
     const Part<A> q{__shfl_xor_sync(0xffffffffu, p.m, d), __shfl_xor_sync(0xffffffffu, p.s, d)};
     p = join(p, q, k);
   }
