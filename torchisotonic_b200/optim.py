@@ -14,6 +14,7 @@ from __future__ import annotations
 
 from collections.abc import Iterable, Sequence
 from itertools import chain, repeat
+from operator import attrgetter
 from typing import Any
 
 import torch
@@ -22,7 +23,7 @@ from torch import Tensor
 from torchisotonic_b200 import _ext
 
 BLOCK = 256  # elements that share a scale
-_HALVES = (torch.float16, torch.bfloat16)
+_dtype = attrgetter("dtype")
 
 
 def _bits(dtype: torch.dtype) -> int:
@@ -73,49 +74,52 @@ def adamw_step(
         raise ValueError("lr, eps and weight_decay must not be negative")
     if count == 0:
         return
-    for t in chain.from_iterable(lists):
-        if not isinstance(t, Tensor):
-            raise TypeError(f"params, grads, states and scales must be torch.Tensors, got "
-                            f"{type(t).__name__}")
-        if not t.is_contiguous():
-            raise ValueError("params, grads, states and scales must be contiguous")
+    try:  # a C-level pass a check: hundreds of tensors a call
+        contiguous = all(map(Tensor.is_contiguous, chain.from_iterable(lists)))
+        devices = set(map(Tensor.get_device, chain.from_iterable(lists)))
+    except TypeError as e:
+        raise TypeError("params, grads, states and scales must be torch.Tensors") from e
+    if not contiguous:
+        raise ValueError("params, grads, states and scales must be contiguous")
     if not params[0].is_cuda:
         raise RuntimeError(
             "torchisotonic_b200 runs on CUDA tensors only (no CPU fallback); "
             "move params to a CUDA device"
         )
-    device = params[0].device
-    if any(t.device != device for t in chain.from_iterable(lists)):
+    if len(devices) != 1:
         raise ValueError("params, grads, states and scales must be on one device")
-    sizes = [p.numel() for p in params]
-    if any([t.numel() for t in x] != sizes for x in lists[1:4]):
+    sizes = list(map(Tensor.numel, params))
+    if any(list(map(Tensor.numel, x)) != sizes for x in lists[1:4]):
         raise ValueError("grads and states must be shaped like their parameters")
-    bits = _bits(exp_avgs[0].dtype)
-    if any(t.dtype != exp_avgs[0].dtype for t in chain(exp_avgs, exp_avg_sqs)):
+    param_types, grad_types, *state_types = ([*map(_dtype, x)] for x in lists)
+    bits = _bits(state_types[0][0])
+    if {*state_types[0], *state_types[1]} != {state_types[0][0]}:
         raise TypeError("optimizer states must be of one dtype")
     if (bits == 8) != (scales is not None):
         raise ValueError("scales go with float8_e4m3fn states, and only with them")
     if scales is not None:
+        if {*state_types[2], *state_types[3]} != {torch.float32}:
+            raise TypeError("scales must be float32 tensors")
         blocks = [-(-n // BLOCK) for n in sizes]
-        for x in scales:
-            if any(t.dtype != torch.float32 for t in x):
-                raise TypeError("scales must be float32 tensors")
-            if [t.numel() for t in x] != blocks:
-                raise ValueError(f"a scale tensor must hold ceil(n / {BLOCK}) numbers")
-    pointers = [[t.data_ptr() for t in x] for x in lists]
-    if scales is None:
-        pointers += [repeat(0, count), repeat(0, count)]
-    fields = zip(*pointers, sizes, range(count))
-    args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
-    by_type: dict[tuple[torch.dtype, torch.dtype], list[tuple[int, ...]]] = {}
-    for p, g, f in zip(params, grads, fields):
-        by_type.setdefault((p.dtype, g.dtype), []).append(f)
-    for pt, gt in by_type:
-        if pt not in (torch.float32, *_HALVES) or gt not in (pt, torch.float32):
+        if any(list(map(Tensor.numel, x)) != blocks for x in scales):
+            raise ValueError(f"a scale tensor must hold ceil(n / {BLOCK}) numbers")
+    types = set(zip(param_types, grad_types))
+    for pt, gt in types:
+        if pt not in (torch.float32, torch.float16, torch.bfloat16) or gt not in (pt, torch.float32):
             raise TypeError("params must be float32, bfloat16 or float16, grads like their "
                             "parameter or float32")
-    for (pt, gt), f in by_type.items():
-        _ext.adamw(device, pt, gt, bits, list(chain.from_iterable(f)), args)
+    pointers = [map(Tensor.data_ptr, x) for x in lists]
+    if scales is None:
+        pointers += [repeat(0), repeat(0)]
+    fields = zip(*pointers, sizes, range(count))
+    args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
+    if len(types) == 1:
+        _ext.adamw(params[0].device, pt, gt, bits, chain.from_iterable(fields), args)
+        return
+    tensors = list(fields)
+    for pt, gt in types:
+        its = [f for f, a, b in zip(tensors, param_types, grad_types) if a == pt and b == gt]
+        _ext.adamw(params[0].device, pt, gt, bits, chain.from_iterable(its), args)
 
 
 class AdamW(torch.optim.Optimizer):
