@@ -19,6 +19,7 @@ namespace cg = cooperative_groups;
 constexpr int kBatch = 4;       // vectors a thread loads before it uses the first
 constexpr int kRowWarps = 8;    // rows to a CTA where a warp takes a row
 constexpr int kMostRows = 1 << 28;
+constexpr int kNoEdge = 1 << 30;
 
 int logits_fail(cudaError_t e, const char* what) {
   return report_error(TISO_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
@@ -40,41 +41,51 @@ __device__ __forceinline__ const T* row_at(const Rows& a, int64_t r) {
 }
 
 // Who works on a row: a warp (kThreads 32; kRowWarps rows to a CTA), a CTA, or a cluster of CTAs
-// (kThreads > 32; the row's index is the cluster's).
+// (kThreads > 32; the row's index is the cluster's). A row's vectors are cut into tiles of kBatch
+// vectors a thread; the CTAs of a cluster take tiles in turn.
 template <int kThreads>
 struct Place {
   int64_t row;
-  int rank, threads;  // this thread's and how many there are to the row
+  int tid, cta, ctas;
 
   __device__ __forceinline__ Place() {
     if constexpr (kThreads == 32) {
       row = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
-      rank = threadIdx.x & 31;
-      threads = 32;
+      tid = threadIdx.x & 31;
+      cta = 0;
+      ctas = 1;
     } else {
-      const unsigned ctas = cg::this_cluster().num_blocks();
+      ctas = static_cast<int>(cg::this_cluster().num_blocks());
       row = blockIdx.x / ctas;
-      rank = static_cast<int>(blockIdx.x % ctas) * kThreads + threadIdx.x;
-      threads = static_cast<int>(ctas) * kThreads;
+      cta = static_cast<int>(blockIdx.x % ctas);
+      tid = threadIdx.x;
     }
   }
-  __device__ __forceinline__ bool first() const { return rank == 0; }
+  __device__ __forceinline__ bool first() const { return tid == 0 && cta == 0; }
+  // this thread's number for a row's single elements; none but the first CTA takes them
+  __device__ __forceinline__ int edge() const { return cta == 0 ? tid : kNoEdge; }
 };
 
-// The part of a row that one thread sees: vectors rank, rank + threads, ..., and for the first
-// warp a single element each.
-template <typename T, typename A>
-__device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, int rank, int threads, A k) {
+// The part of a row that a warp sees: its share of tiles cta, cta + ctas, ..., and in the row's
+// first warp a single element for each lane.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kThreads>& place, A k) {
+  constexpr int kTile = kBatch * kThreads;
   Part<A> p{lowest<A>(), A(0)};
-  if (rank < r.edges) {
-    const A z = to_acc(r.x[r.edge(rank)]);
+  if (place.edge() < r.edges) {
+    const A z = to_acc(r.x[r.edge(place.edge())]);
     p = {z, scaled_exp(z - base_of(z), k)};
   }
-  for (int v = rank; v < r.vectors; v += kBatch * threads) {
+  for (int tile = place.cta * kTile; tile < r.vectors; tile += place.ctas * kTile) {
+    const int v = tile + place.tid;
     uint4 q[kBatch];
+    if (tile + kTile <= r.vectors) {
+      load_vectors<kBatch, kThreads>(r, v, q);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      q[i] = v + i * threads < r.vectors ? load_vector(r, v + i * threads) : no_vector<T>();
+      for (int i = 0; i < kBatch; ++i)
+        q[i] = v + i * kThreads < r.vectors ? load_vector(r, v + i * kThreads) : no_vector<T>();
+    }
     const A m = max_acc(p.m, vector_max<T>(q));
     const A base = base_of(m);
     p.s *= scaled_exp(p.m == m ? A(0) : p.m - base, k);
@@ -87,14 +98,13 @@ __device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, int rank, in
       p.s += total(x);
     }
   }
-  return p;
+  return join_lanes<32>(p, k);
 }
 
-// The parts of all of a row's threads joined; every thread gets the result. Called once by a CTA
-// (its shared memory is not used again), by all of its threads.
+// The parts of all of a row's warps joined (a warp's lanes hold the same); every thread gets the
+// result. Called once by a CTA (its shared memory is not used again), by all of its threads.
 template <int kThreads, typename A>
-__device__ __forceinline__ Part<A> join_threads(Part<A> p, A k) {
-  p = join_lanes<32>(p, k);
+__device__ __forceinline__ Part<A> join_warps(Part<A> p, A k) {
   if constexpr (kThreads > 32) {
     constexpr int kWarps = kThreads / 32, kMostCtas = 8;
     __shared__ Part<A> of_warp[kWarps], of_cta[kMostCtas];
@@ -154,52 +164,69 @@ struct Slope {
   }
 };
 
+// The gradient of a vector's elements as if none was the target.
 template <typename T, typename A>
-__device__ __forceinline__ uint4 slope_vector(const uint4& q, const Slope<A>& slope, int element) {
-  constexpr int E = RowView<T>::E;
-  A x[E];
+__device__ __forceinline__ uint4 slope_vector(const uint4& q, const Slope<A>& slope) {
+  A x[RowView<T>::E];
   unpack<T>(q, x);
   exponentials(x, slope.base, slope.k);
-#pragma unroll
-  for (int j = 0; j < E; ++j) x[j] = mul_rn(x[j], slope.scale);
-  const unsigned at = static_cast<unsigned>(slope.target - element);
-  if (at < static_cast<unsigned>(E)) {
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (at == static_cast<unsigned>(j)) x[j] = slope.at_target(x[j]);
-  }
+  scale_by(x, slope.scale);
   return pack<T>(x);
 }
 
-// The gradient of vectors first, first + step, ... below end, and of a single element for ranks
-// below the number of those.
+// The target's gradient where it lies in vector v, by the thread that wrote the vector.
 template <typename T, typename A>
-__device__ __forceinline__ void write_slope(const RowView<T>& r, int rank, int first, int step,
-                                            int end, const Slope<A>& slope) {
-  if (rank < r.edges) {
-    const int v = r.edge(rank);
+__device__ __forceinline__ void write_target(const RowView<T>& r, const Slope<A>& slope, int v) {
+  const int at = slope.target - r.element(v);
+  if (at >= 0 && at < RowView<T>::E)
+    r.g[slope.target] = from_acc<T>(slope.at(to_acc(r.x[slope.target]), slope.target));
+}
+
+template <typename T, typename A>
+__device__ __forceinline__ void write_edge(const RowView<T>& r, int edge, const Slope<A>& slope) {
+  if (edge < r.edges) {
+    const int v = r.edge(edge);
     r.g[v] = from_acc<T>(slope.at(to_acc(r.x[v]), v));
   }
-  for (int v = first; v < end; v += kBatch * step) {
+}
+
+// The gradient of one tile's vectors.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void write_tile(const RowView<T>& r, int tile, int tid,
+                                           const Slope<A>& slope) {
+  constexpr int kTile = kBatch * kThreads;
+  const int v = tile + tid;
+  uint4* to = reinterpret_cast<uint4*>(r.g + r.head) + v;
+  if (tile + kTile <= r.vectors) {
     uint4 q[kBatch];
+    load_vectors<kBatch, kThreads>(r, v, q);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) store_once(to + i * kThreads, slope_vector<T>(q[i], slope));
+  } else {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      if (v + i * step < end) q[i] = load_vector(r, v + i * step);
+      if (v + i * kThreads < r.vectors)
+        store_once(to + i * kThreads, slope_vector<T>(load_vector(r, v + i * kThreads), slope));
+  }
+  // the thread whose vector holds the target
+  const int in_tile = (slope.target - r.head) / RowView<T>::E - tile;
+  if (slope.target >= r.head && in_tile >= 0 && in_tile < kTile && in_tile % kThreads == tid &&
+      tile + in_tile < r.vectors)
+    write_target(r, slope, tile + in_tile);
+}
+
+template <int kThreads, typename T>
+__device__ __forceinline__ void zero_tile(const RowView<T>& r, int tile, int tid) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (v + i * step < end) {
-        const int e = r.element(v + i * step);
-        store_once(r.g + e, slope_vector<T>(q[i], slope, e));
-      }
+  for (int i = 0; i < kBatch; ++i) {
+    const int v = tile + i * kThreads + tid;
+    if (v < r.vectors) store_once(r.g + r.element(v), make_uint4(0, 0, 0, 0));
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void write_zeros(const RowView<T>& r, int rank, int first, int step,
-                                            int end) {
-  if (rank < r.edges) r.g[r.edge(rank)] = from_acc<T>(typename AccOf<T>::type(0));
-  for (int v = first; v < end; v += step)
-    store_once(r.g + r.element(v), make_uint4(0, 0, 0, 0));
+__device__ __forceinline__ void zero_edge(const RowView<T>& r, int edge) {
+  if (edge < r.edges) r.g[r.edge(edge)] = from_acc<T>(typename AccOf<T>::type(0));
 }
 
 // A row that is left out (its target is the ignored index, or its weight is 0) is marked by a
@@ -225,7 +252,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
   if (place.first()) at_target = target_logit<T, A>(x, a.vocab, target);
   const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
   const Part<A> p =
-      join_threads<kThreads>(thread_part<T, A>(view, place.rank, place.threads, k), k);
+      join_warps<kThreads>(warp_part(view, place, k), k);
   if (place.first()) {
     logps[r] = static_cast<A>(logp_of(at_target, p, inv_temp));
     if (stats) {
@@ -236,33 +263,31 @@ __global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
 }
 
 // coef: per row, d loss / d logp. upstream (may be NULL): a scalar that multiplies it, and where
-// it is 1 nothing is written. Work is cut into pieces of a row, `pieces` to the row, for a warp or
-// a CTA (kThreads) each.
+// it is 1 nothing is written. A warp or a CTA (kThreads) takes a tile, `tiles` to the row.
 template <typename T, typename A, typename C, int kThreads>
 __global__ void __launch_bounds__(256)
     logprobs_grad_kernel(Rows a, double inv_temp, A k, const A* stats, const C* coef,
-                         const A* upstream, T* grad, int pieces) {
+                         const A* upstream, T* grad, int tiles) {
   const A up = upstream ? *upstream : A(1);
   if (upstream && up == A(1)) return;
-  constexpr int kGroups = 256 / kThreads;
-  const int rank = threadIdx.x % kThreads;
+  constexpr int kGroups = 256 / kThreads, kTile = kBatch * kThreads;
+  const int tid = threadIdx.x % kThreads;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / kThreads;
-       i < a.rows * pieces; i += static_cast<int64_t>(gridDim.x) * kGroups) {
-    const int64_t r = i / pieces;
-    const int piece = static_cast<int>(i % pieces);
+       i < a.rows * tiles; i += static_cast<int64_t>(gridDim.x) * kGroups) {
+    const int64_t r = i / tiles;
+    const int tile = static_cast<int>(i % tiles) * kTile;
     T* g = grad + r * a.vocab;
     const RowView<T> view(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
-    // the last piece takes what is left; the first the single elements
-    const int first = piece * kBatch * kThreads;
-    const int end = piece == pieces - 1 ? view.vectors : min(view.vectors, first + kBatch * kThreads);
-    const int edge_rank = piece == 0 ? rank : view.edges;
+    const int edge = tile == 0 ? tid : kNoEdge;
     const A sum = stats[2 * r + 1];
     if (sum < A(0)) {
-      write_zeros(view, edge_rank, first + rank, kThreads, end);
+      zero_edge(view, edge);
+      zero_tile<kThreads>(view, tile, tid);
     } else {
       const Slope<A> slope(stats[2 * r], sum, static_cast<double>(coef[r]) * up * inv_temp,
                            k, a.targets[r], a.vocab);
-      write_slope(view, edge_rank, first + rank, kThreads, end, slope);
+      write_edge(view, edge, slope);
+      write_tile<kThreads>(view, tile, tid, slope);
     }
   }
 }
@@ -345,56 +370,83 @@ struct Token {
   }
 };
 
+// What the policy loss needs of a token beside its row.
+template <typename A>
+struct TokenInput {
+  int64_t target;
+  A w, old, adv, ref, logit;
+
+  template <typename T>
+  __device__ __forceinline__ void read(const Rows& a, const PolicyArgs<A>& p, int64_t r, const T* x) {
+    target = a.targets[r];
+    old = p.old_logps[r];
+    adv = p.advantages[r];
+    ref = p.ref_logps ? p.ref_logps[r] : A(0);
+    logit = target_logit<T, A>(x, a.vocab, target);
+  }
+};
+
+// From a row's sum to the token's coefficient, d loss / d logp; `first` writes the token's results.
+template <typename A>
+__device__ __forceinline__ double token_coef(const PolicyArgs<A>& p, int64_t r,
+                                             const TokenInput<A>& t, const Part<A>& part,
+                                             double inv_temp, bool first) {
+  const double total = *p.total;
+  const double share = total != 0 ? t.w / total : 0.0;
+  const double lp = logp_of(t.logit, part, inv_temp);
+  const Token token(lp, t.old, t.ref, t.adv, p);
+  const double coef = total != 0 ? share * token.slope : 0.0;
+  if (first) {
+    p.logps[r] = static_cast<A>(lp);
+    p.coef[r] = coef;
+    p.stats[2 * r] = base_of(part.m);
+    p.stats[2 * r + 1] = part.s;
+    p.terms[3 * r] = static_cast<A>(t.w * token.loss);
+    p.terms[3 * r + 1] = static_cast<A>(t.w * token.kl);
+    p.terms[3 * r + 2] = token.clipped ? t.w : A(0);
+  }
+  return coef;
+}
+
+// The row's cut is as for a gradient in a buffer on a vector's boundary, also where no gradient is
+// written (grad NULL): the loss is the same bits.
+template <typename T>
+__device__ __forceinline__ RowView<T> policy_view(const Rows& a, int64_t r, T* grad) {
+  T* g = grad + r * a.vocab;
+  return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
+}
+
+// A row is read twice, for its sum and for its gradient; few enough rows are worked on at a time
+// that the second read finds them in L2.
 template <typename T, typename A, int kThreads>
 __global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
     policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+  constexpr int kTile = kBatch * kThreads;
   const Place<kThreads> place;
   const int64_t r = place.row;
   if (r >= a.rows) return;
-  const A w = weight_of(a, p, r);
-  const T* x = row_at<T>(a, r);
-  // without a gradient the row is cut as with one (in a buffer on a vector's boundary), so that
-  // the loss is the same bits
-  T* g = grad + r * a.vocab;
-  const RowView<T> view(x, g, reinterpret_cast<uintptr_t>(g), a.vocab);
-  if (w == A(0)) {
+  const RowView<T> view = policy_view(a, r, grad);
+  TokenInput<A> token;
+  token.w = weight_of(a, p, r);
+  if (token.w == A(0)) {
     if (place.first()) {
       p.logps[r] = A(0);
       p.coef[r] = 0;
       p.stats[2 * r + 1] = A(kLeftOut);
       p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
     }
-    if (grad) write_zeros(view, place.rank, place.rank, place.threads, view.vectors);
+    if (!grad) return;
+    zero_edge(view, place.edge());
+    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+      zero_tile<kThreads>(view, tile, place.tid);
     return;
   }
-  const int64_t target = a.targets[r];
-  // one warp of a CTA (every warp that has a row to itself) goes from the sum to the coefficient
-  const bool steps = kThreads == 32 || threadIdx.x < 32;
-  A at_target = A(0), old = A(0), adv = A(0), ref = A(0);
-  if (steps) {
-    at_target = target_logit<T, A>(x, a.vocab, target);
-    old = p.old_logps[r];
-    adv = p.advantages[r];
-    if (p.ref_logps) ref = p.ref_logps[r];
-  }
-  const Part<A> part =
-      join_threads<kThreads>(thread_part<T, A>(view, place.rank, place.threads, k), k);
+  token.target = a.targets[r];
+  const bool steps = kThreads == 32 || threadIdx.x < 32;  // one warp goes on from the sum
+  if (steps) token.read(a, p, r, view.x);
+  const Part<A> part = join_warps<kThreads>(warp_part(view, place, k), k);
   double coef = 0;
-  if (steps) {
-    const double lp = logp_of(at_target, part, inv_temp);
-    const Token token(lp, old, ref, adv, p);
-    const double total = *p.total;
-    if (total != 0) coef = w * token.slope / total;
-    if (place.first()) {
-      p.logps[r] = static_cast<A>(lp);
-      p.coef[r] = coef;
-      p.stats[2 * r] = base_of(part.m);
-      p.stats[2 * r + 1] = part.s;
-      p.terms[3 * r] = static_cast<A>(w * token.loss);
-      p.terms[3 * r + 1] = static_cast<A>(w * token.kl);
-      p.terms[3 * r + 2] = token.clipped ? w : A(0);
-    }
-  }
+  if (steps) coef = token_coef(p, r, token, part, inv_temp, place.first());
   if (!grad) return;
   if constexpr (kThreads > 32) {
     __shared__ double of_warp_0;
@@ -402,8 +454,10 @@ __global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
     __syncthreads();
     coef = of_warp_0;
   }
-  const Slope<A> slope(base_of(part.m), part.s, coef * inv_temp, k, target, a.vocab);
-  write_slope(view, place.rank, place.rank, place.threads, view.vectors, slope);
+  const Slope<A> slope(base_of(part.m), part.s, coef * inv_temp, k, token.target, a.vocab);
+  write_edge(view, place.edge(), slope);
+  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+    write_tile<kThreads>(view, tile, place.tid, slope);
 }
 
 // The means over the tokens, in a fixed order; 0 when the weights sum to 0.
@@ -465,18 +519,18 @@ int sm_count() {
   return sms;
 }
 
-// A launch of a kernel over rows, `ctas` (a power of two up to 8) to the row as a cluster.
+// A launch of `clusters` clusters of `ctas` CTAs (a power of two up to 8) of `threads`.
 template <typename... P, typename... Q>
-int launch_rows(void (*kernel)(P...), int64_t rows, int threads, int ctas, cudaStream_t st,
-                const char* what, Q... args) {
+int launch_clusters(void (*kernel)(P...), int64_t clusters, int ctas, int threads, size_t shared,
+                    cudaStream_t st, const char* what, Q... args) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(threads == 32 ? (rows + kRowWarps - 1) / kRowWarps
-                                                            : rows * ctas));
-  config.blockDim = dim3(threads == 32 ? 32 * kRowWarps : threads);
+  config.gridDim = dim3(static_cast<unsigned>(clusters * ctas));
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = shared;
   config.stream = st;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(threads == 32 ? 1 : ctas);
+  attribute.val.clusterDim.x = static_cast<unsigned>(ctas);
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = 1;
@@ -484,8 +538,20 @@ int launch_rows(void (*kernel)(P...), int64_t rows, int threads, int ctas, cudaS
   return e == cudaSuccess ? TISO_OK : logits_fail(e, what);
 }
 
+// A kernel over rows, a warp to each.
+template <typename... P, typename... Q>
+int launch_warps(void (*kernel)(P...), int64_t rows, cudaStream_t st, const char* what, Q... args) {
+  kernel<<<static_cast<unsigned>((rows + kRowWarps - 1) / kRowWarps), 32 * kRowWarps, 0, st>>>(
+      args...);
+  return launched(what);
+}
+
 // Rows of at most this many vectors go to a warp each.
 constexpr int kWarpVectors = 256;
+
+// Bytes of rows in work at once (3 CTAs an SM) that L2 is to hold from a row's first read to its
+// second.
+constexpr int64_t kRowsInL2 = 80 << 20;
 
 // CTAs of `threads` to a row: doubled while rows are too few to fill the GPU and a CTA would have
 // more than a batch for each thread.
@@ -501,11 +567,12 @@ int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaS
   const int vectors = a.vocab / RowView<T>::E;
   const A k = exp_factor(A(0), inv_temp);
   if (vectors <= kWarpVectors)
-    return launch_rows(logprobs_kernel<T, A, 32>, a.rows, 32, 1, st, "logprobs_kernel launch", a,
-                       inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
-  return launch_rows(logprobs_kernel<T, A, 256>, a.rows, 256,
-                     ctas_for(a.rows, vectors, 256, sm_count()), st, "logprobs_kernel launch", a,
-                     inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
+    return launch_warps(logprobs_kernel<T, A, 32>, a.rows, st, "logprobs_kernel launch", a,
+                        inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
+  return launch_clusters(logprobs_kernel<T, A, 256>, a.rows,
+                         ctas_for(a.rows, vectors, 256, sm_count()), 256, 0, st,
+                         "logprobs_kernel launch", a, inv_temp, k, static_cast<A*>(logps),
+                         static_cast<A*>(stats));
 }
 
 template <typename T, typename C>
@@ -514,9 +581,9 @@ int run_logprobs_grad(const Rows& a, double inv_temp, const void* stats, const v
   using A = typename AccOf<T>::type;
   const int vectors = a.vocab / RowView<T>::E;
   const bool by_warp = vectors <= kWarpVectors;
-  const int piece = kBatch * (by_warp ? 32 : 256);
-  const int pieces = by_warp ? 1 : (vectors + piece - 1) / piece;
-  const int64_t all = (a.rows * pieces + (by_warp ? 7 : 0)) / (by_warp ? 8 : 1);
+  const int tile = kBatch * (by_warp ? 32 : 256);
+  const int tiles = vectors > tile ? (vectors + tile - 1) / tile : 1;
+  const int64_t all = (a.rows * tiles + (by_warp ? 7 : 0)) / (by_warp ? 8 : 1);
   // where the launch may have nothing to do (upstream is 1), no more CTAs than are resident
   const int64_t most = upstream ? int64_t{sm_count()} * 8 : int64_t{1} << 30;
   const unsigned grid = static_cast<unsigned>(all < most ? all : most);
@@ -524,8 +591,24 @@ int run_logprobs_grad(const Rows& a, double inv_temp, const void* stats, const v
   auto kernel = by_warp ? logprobs_grad_kernel<T, A, C, 32> : logprobs_grad_kernel<T, A, C, 256>;
   kernel<<<grid, 256, 0, st>>>(a, inv_temp, k, static_cast<const A*>(stats),
                                static_cast<const C*>(coef), static_cast<const A*>(upstream),
-                               static_cast<T*>(grad), pieces);
+                               static_cast<T*>(grad), tiles);
   return launched("logprobs_grad_kernel launch");
+}
+
+template <typename T>
+int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, double inv_temp,
+                  T* grad, cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  const int vectors = a.vocab / RowView<T>::E;
+  const A k = exp_factor(A(0), inv_temp);
+  if (vectors <= kWarpVectors)
+    return launch_warps(policy_kernel<T, A, 32>, a.rows, st, "policy_kernel launch", a, p, inv_temp,
+                        k, grad);
+  const int sms = sm_count();
+  int ctas = ctas_for(a.rows, vectors, 512, sms);
+  while (ctas < 8 && int64_t{sms} * 3 * vectors * 16 / ctas > kRowsInL2) ctas *= 2;
+  return launch_clusters(policy_kernel<T, A, 512>, a.rows, ctas, 512, 0, st, "policy_kernel launch",
+                         a, p, inv_temp, k, grad);
 }
 
 template <typename T>
@@ -549,16 +632,7 @@ int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* 
   p.terms = reinterpret_cast<A*>(p.total + 1);
   policy_total_kernel<A><<<1, 1024, 0, st>>>(a, p);
   if (a.rows > 0) {
-    const int vectors = a.vocab / RowView<T>::E;
-    const A k = exp_factor(A(0), inv_temp);
-    T* g = static_cast<T*>(grad);
-    const int rc =
-        vectors <= kWarpVectors
-            ? launch_rows(policy_kernel<T, A, 32>, a.rows, 32, 1, st, "policy_kernel launch", a, p,
-                          inv_temp, k, g)
-            : launch_rows(policy_kernel<T, A, 256>, a.rows, 256,
-                          ctas_for(a.rows, vectors, 256, sm_count()), st, "policy_kernel launch",
-                          a, p, inv_temp, k, g);
+    const int rc = launch_policy<T>(a, p, inv_temp, static_cast<T*>(grad), st);
     if (rc) return rc;
   }
   policy_means_kernel<A><<<1, 1024, 0, st>>>(a.rows, p);

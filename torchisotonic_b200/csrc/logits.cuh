@@ -159,18 +159,32 @@ __device__ __forceinline__ uint4 load_once(const void* p) {  // read once: keeps
   return r;
 }
 
+// kN vectors of the row read, v, v + kStep, ...
+template <int kN, int kStep, typename T>
+__device__ __forceinline__ void load_vectors(const RowView<T>& r, int v, uint4 (&q)[kN]) {
+  const uint4* at = reinterpret_cast<const uint4*>(r.x + r.head - r.shift) + v;
+  if (r.shift == 0) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) q[i] = load_once(at + i * kStep);
+    return;
+  }
+  const int bytes = r.shift * static_cast<int>(sizeof(T));
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const uint4 a = __ldg(at + i * kStep), b = __ldg(at + i * kStep + 1);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    shift_words<8>(w, bytes & 8);
+    if constexpr (sizeof(T) <= 4) shift_words<4>(w, bytes & 4);
+    if constexpr (sizeof(T) <= 2) shift_words<2>(w, bytes & 2);
+    q[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ uint4 load_vector(const RowView<T>& r, int v) {
-  const T* at = r.x + r.element(v) - r.shift;
-  if (r.shift == 0) return load_once(at);
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(at));
-  const uint4 b = __ldg(reinterpret_cast<const uint4*>(at) + 1);
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  const int bytes = r.shift * static_cast<int>(sizeof(T));
-  shift_words<8>(w, bytes & 8);
-  if constexpr (sizeof(T) <= 4) shift_words<4>(w, bytes & 4);
-  if constexpr (sizeof(T) <= 2) shift_words<2>(w, bytes & 2);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  uint4 q[1];
+  load_vectors<1, 1>(r, v, q);
+  return q[0];
 }
 
 // A vector of -infinity: what a thread holds where the row has no vector for it.
@@ -267,18 +281,24 @@ __device__ __forceinline__ typename AccOf<T>::type vector_max(const uint4 (&q)[k
   }
 }
 
-// Two floats at once where the type allows it: (x - base) k, and sums.
-__device__ __forceinline__ float2 sub_mul2(float2 x, float base, float k) {
-  float2 r;
-  asm("{.reg .b64 x, b, k, d;\n\t"
-      "mov.b64 x, {%2, %3};\n\t"
-      "mov.b64 b, {%4, %4};\n\t"
-      "mov.b64 k, {%5, %5};\n\t"
-      "add.rn.f32x2 d, x, b;\n\t"
-      "mul.rn.f32x2 d, d, k;\n\t"
-      "mov.b64 {%0, %1}, d;}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(x.x), "f"(x.y), "f"(-base), "f"(k));
+// Pairs of floats in one 64-bit register, for the instructions that take two at a time.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ float exp2_of(float x) {
@@ -290,11 +310,13 @@ __device__ __forceinline__ float exp2_of(float x) {
 // exp((x - base) / t) of a vector's elements, in place.
 template <int kE>
 __device__ __forceinline__ void exponentials(float (&x)[kE], float base, float k) {
+  const Pair minus = pair_of(-base, -base), factor = pair_of(k, k);
 #pragma unroll
   for (int j = 0; j < kE; j += 2) {
-    const float2 d = sub_mul2(make_float2(x[j], x[j + 1]), base, k);
-    x[j] = exp2_of(d.x);
-    x[j + 1] = exp2_of(d.y);
+    float a, b;
+    split(mul2(add2(pair_of(x[j], x[j + 1]), minus), factor), a, b);
+    x[j] = exp2_of(a);
+    x[j + 1] = exp2_of(b);
   }
 }
 template <int kE>
@@ -303,24 +325,28 @@ __device__ __forceinline__ void exponentials(double (&x)[kE], double base, doubl
   for (int j = 0; j < kE; ++j) x[j] = exp(mul_rn(x[j] - base, k));
 }
 
-// The sum of a vector's elements.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%2, %3};\n\t"
-      "mov.b64 b, {%4, %5};\n\t"
-      "add.rn.f32x2 a, a, b;\n\t"
-      "mov.b64 {%0, %1}, a;}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
+// The elements times a number, in place.
+template <int kE>
+__device__ __forceinline__ void scale_by(float (&x)[kE], float c) {
+  const Pair factor = pair_of(c, c);
+#pragma unroll
+  for (int j = 0; j < kE; j += 2) split(mul2(pair_of(x[j], x[j + 1]), factor), x[j], x[j + 1]);
 }
 template <int kE>
-__device__ __forceinline__ float total(const float (&x)[kE]) {
-  float2 s = make_float2(x[0], x[1]);
+__device__ __forceinline__ void scale_by(double (&x)[kE], double c) {
 #pragma unroll
-  for (int j = 2; j < kE; j += 2) s = add2(s, make_float2(x[j], x[j + 1]));
-  return s.x + s.y;
+  for (int j = 0; j < kE; ++j) x[j] = mul_rn(x[j], c);
+}
+
+// The sum of a vector's elements.
+template <int kE>
+__device__ __forceinline__ float total(const float (&x)[kE]) {
+  Pair s = pair_of(x[0], x[1]);
+#pragma unroll
+  for (int j = 2; j < kE; j += 2) s = add2(s, pair_of(x[j], x[j + 1]));
+  float a, b;
+  split(s, a, b);
+  return a + b;
 }
 template <int kE>
 __device__ __forceinline__ double total(const double (&x)[kE]) {
