@@ -546,7 +546,10 @@ def test_policy_settings() -> None:
     check_policy(x, y, old, adv, weight=w, clip_high=0.28)
     check_policy(x, y, old, adv, ref_logps=ref, weight=w, kl_coef=0.0)
     check_policy(x, y, old, adv, ref_logps=ref, kl_coef=1.0, clip_low=1.0, clip_high=1e9)
-    check_policy(x[:, :-1], y[:, 1:], old[:, 1:].double(), adv[:, 1:].half().float(), weight=w[:, 1:])
+    # a cut tensor, its tokens' inputs strided and of other types
+    old1, adv1, _ = tokens_of(x[:, :-1], y[:, 1:], 2)
+    wide = torch.stack([old1.double(), adv1.double()], -1)
+    check_policy(x[:, :-1], y[:, 1:], wide[..., 0], wide[..., 1], weight=w[:, 1:])
     z = y.clone()
     z[1, :20] = 5
     check_policy(x, z, old, adv, ignore_index=5)

@@ -3,7 +3,10 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <mutex>
+#include <set>
 #include <string>
+#include <utility>
 
 #include "../../include/tiso.h"
 #include "logits.cuh"
@@ -66,17 +69,34 @@ struct Place {
   __device__ __forceinline__ int edge() const { return cta == 0 ? tid : kNoEdge; }
 };
 
-// The part of a row that a warp sees: its share of tiles cta, cta + ctas, ..., and in the row's
-// first warp a single element for each lane.
+// Adds vectors to what a thread has seen.
+template <typename T, int kN, typename A>
+__device__ __forceinline__ void add_vectors(Part<A>& p, const uint4 (&q)[kN], A k) {
+  const A m = max_acc(p.m, vector_max<T>(q));
+  const A base = base_of(m);
+  p.s *= scaled_exp(p.m == m ? A(0) : p.m - base, k);
+  p.m = m;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    A x[RowView<T>::E];
+    unpack<T>(q[i], x);
+    exponentials(x, base, k);
+    p.s += total(x);
+  }
+}
+
+// The part of a row that a thread sees: of a CTA's tiles (every ctas-th), those from vector `first`
+// on, and one of the single elements.
 template <int kThreads, typename T, typename A>
-__device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kThreads>& place, A k) {
+__device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, const Place<kThreads>& place,
+                                               int first, A k) {
   constexpr int kTile = kBatch * kThreads;
   Part<A> p{lowest<A>(), A(0)};
   if (place.edge() < r.edges) {
     const A z = to_acc(r.x[r.edge(place.edge())]);
     p = {z, scaled_exp(z - base_of(z), k)};
   }
-  for (int tile = place.cta * kTile; tile < r.vectors; tile += place.ctas * kTile) {
+  for (int tile = first; tile < r.vectors; tile += place.ctas * kTile) {
     const int v = tile + place.tid;
     uint4 q[kBatch];
     if (tile + kTile <= r.vectors) {
@@ -86,19 +106,15 @@ __device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kT
       for (int i = 0; i < kBatch; ++i)
         q[i] = v + i * kThreads < r.vectors ? load_vector(r, v + i * kThreads) : no_vector<T>();
     }
-    const A m = max_acc(p.m, vector_max<T>(q));
-    const A base = base_of(m);
-    p.s *= scaled_exp(p.m == m ? A(0) : p.m - base, k);
-    p.m = m;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      A x[RowView<T>::E];
-      unpack<T>(q[i], x);
-      exponentials(x, base, k);
-      p.s += total(x);
-    }
+    add_vectors<T>(p, q, k);
   }
-  return join_lanes<32>(p, k);
+  return p;
+}
+
+// The part of a row that a warp sees.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kThreads>& place, A k) {
+  return join_lanes<32>(thread_part(r, place, place.cta * kBatch * kThreads, k), k);
 }
 
 // The parts of all of a row's warps joined (a warp's lanes hold the same); every thread gets the
@@ -174,11 +190,14 @@ __device__ __forceinline__ uint4 slope_vector(const uint4& q, const Slope<A>& sl
   return pack<T>(x);
 }
 
-// The target's gradient where it lies in vector v, by the thread that wrote the vector.
-template <typename T, typename A>
-__device__ __forceinline__ void write_target(const RowView<T>& r, const Slope<A>& slope, int v) {
-  const int at = slope.target - r.element(v);
-  if (at >= 0 && at < RowView<T>::E)
+// The target's gradient, where the tile of kTile vectors from `tile` on has it, by the thread that
+// wrote its vector (vector v by thread v % kThreads).
+template <int kThreads, int kTile, typename T, typename A>
+__device__ __forceinline__ void write_target_of_tile(const RowView<T>& r, int tile, int tid,
+                                                     const Slope<A>& slope) {
+  const int v = (slope.target - r.head) / RowView<T>::E, in_tile = v - tile;
+  if (slope.target >= r.head && in_tile >= 0 && in_tile < kTile && in_tile % kThreads == tid &&
+      v < r.vectors)
     r.g[slope.target] = from_acc<T>(slope.at(to_acc(r.x[slope.target]), slope.target));
 }
 
@@ -208,11 +227,7 @@ __device__ __forceinline__ void write_tile(const RowView<T>& r, int tile, int ti
       if (v + i * kThreads < r.vectors)
         store_once(to + i * kThreads, slope_vector<T>(load_vector(r, v + i * kThreads), slope));
   }
-  // the thread whose vector holds the target
-  const int in_tile = (slope.target - r.head) / RowView<T>::E - tile;
-  if (slope.target >= r.head && in_tile >= 0 && in_tile < kTile && in_tile % kThreads == tid &&
-      tile + in_tile < r.vectors)
-    write_target(r, slope, tile + in_tile);
+  write_target_of_tile<kThreads, kTile>(r, tile, tid, slope);
 }
 
 template <int kThreads, typename T>
@@ -416,48 +431,130 @@ __device__ __forceinline__ RowView<T> policy_view(const Rows& a, int64_t r, T* g
   return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
 }
 
-// A row is read twice, for its sum and for its gradient; few enough rows are worked on at a time
-// that the second read finds them in L2.
-template <typename T, typename A, int kThreads>
-__global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
-    policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+// Without a row's worth of weight.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void leave_out(const PolicyArgs<A>& p, const Place<kThreads>& place,
+                                          const RowView<T>& view, bool with_grad) {
   constexpr int kTile = kBatch * kThreads;
-  const Place<kThreads> place;
+  if (place.first()) {
+    const int64_t r = place.row;
+    p.logps[r] = A(0);
+    p.coef[r] = 0;
+    p.stats[2 * r + 1] = A(kLeftOut);
+    p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
+  }
+  if (!with_grad) return;
+  zero_edge(view, place.edge());
+  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+    zero_tile<kThreads>(view, tile, place.tid);
+}
+
+// Short rows: a warp to a row, which it reads twice.
+template <typename T, typename A>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    policy_warp_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+  const Place<32> place;
   const int64_t r = place.row;
   if (r >= a.rows) return;
   const RowView<T> view = policy_view(a, r, grad);
   TokenInput<A> token;
   token.w = weight_of(a, p, r);
   if (token.w == A(0)) {
-    if (place.first()) {
-      p.logps[r] = A(0);
-      p.coef[r] = 0;
-      p.stats[2 * r + 1] = A(kLeftOut);
-      p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
-    }
-    if (!grad) return;
-    zero_edge(view, place.edge());
-    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-      zero_tile<kThreads>(view, tile, place.tid);
+    leave_out(p, place, view, grad != nullptr);
     return;
   }
-  token.target = a.targets[r];
-  const bool steps = kThreads == 32 || threadIdx.x < 32;  // one warp goes on from the sum
-  if (steps) token.read(a, p, r, view.x);
-  const Part<A> part = join_warps<kThreads>(warp_part(view, place, k), k);
-  double coef = 0;
-  if (steps) coef = token_coef(p, r, token, part, inv_temp, place.first());
+  token.read(a, p, r, view.x);
+  const Part<A> part = warp_part(view, place, k);
+  const double coef = token_coef(p, r, token, part, inv_temp, place.first());
   if (!grad) return;
-  if constexpr (kThreads > 32) {
-    __shared__ double of_warp_0;
-    if (threadIdx.x == 0) of_warp_0 = coef;
-    __syncthreads();
-    coef = of_warp_0;
-  }
   const Slope<A> slope(base_of(part.m), part.s, coef * inv_temp, k, token.target, a.vocab);
   write_edge(view, place.edge(), slope);
-  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-    write_tile<kThreads>(view, tile, place.tid, slope);
+  for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
+    write_tile<32>(view, tile, place.tid, slope);
+}
+
+// A cluster's CTAs take a row's tiles in turn, a tile kBatch vectors a thread. Whole tiles come
+// through kStages places of shared memory, each thread copying and reading its own vectors there
+// (no barrier), so that kStages tiles are in flight. The gradient takes them in the reverse order:
+// the last kStages are still there, and the others, if few enough rows are in work at a time, in
+// L2. A last tile that is not whole, and all of a row that is read and written at different
+// alignments, is loaded directly.
+constexpr int kPolicyThreads = 512, kStages = 2;
+constexpr int kPolicyTile = kBatch * kPolicyThreads;
+
+template <typename T, typename A>
+__global__ void __launch_bounds__(kPolicyThreads, 3)
+    policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+  extern __shared__ uint4 stages[];  // [kStages][kPolicyTile]
+  __shared__ double of_warp_0;
+  const Place<kPolicyThreads> place;
+  const int64_t r = place.row;
+  const RowView<T> view = policy_view(a, r, grad);
+  TokenInput<A> token;
+  token.w = weight_of(a, p, r);
+  if (token.w == A(0)) {
+    leave_out(p, place, view, grad != nullptr);
+    return;
+  }
+  // the row's whole tiles, and this CTA's: its j-th is tile cta + j ctas
+  const int whole = view.shift == 0 ? view.vectors / kPolicyTile : 0;
+  const int mine = whole > place.cta ? (whole - place.cta + place.ctas - 1) / place.ctas : 0;
+  const int stride = place.ctas * kPolicyTile;
+  const int own = place.cta * kPolicyTile + place.tid;
+  const uint4* from = reinterpret_cast<const uint4*>(view.x + view.head) + own;
+  uint4* to = reinterpret_cast<uint4*>(view.g + view.head) + own;
+  const auto copy = [&](int j) {
+    if (j >= 0 && j < mine) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        copy_async(stages + j % kStages * kPolicyTile + i * kPolicyThreads + place.tid,
+                   from + static_cast<int64_t>(j) * stride + i * kPolicyThreads);
+    }
+    close_group();
+  };
+  const auto fetch = [&](int j, uint4 (&q)[kBatch]) {
+    wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      q[i] = stages[j % kStages * kPolicyTile + i * kPolicyThreads + place.tid];
+  };
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) copy(j);
+  token.target = a.targets[r];
+  const bool steps = place.tid < 32;  // this warp goes on from the sum
+  if (steps) token.read(a, p, r, view.x);
+
+  // the tiles that are loaded directly, and the single elements
+  const int rest = whole + (place.cta - whole % place.ctas + place.ctas) % place.ctas;
+  Part<A> part = thread_part(view, place, rest * kPolicyTile, k);
+  for (int j = 0; j < mine; ++j) {
+    uint4 q[kBatch];
+    fetch(j, q);
+    copy(j + kStages);
+    add_vectors<T>(part, q, k);
+  }
+  part = join_warps<kPolicyThreads>(join_lanes<32>(part, k), k);
+  if (steps) {
+    const double coef = token_coef(p, r, token, part, inv_temp, place.first());
+    if (place.tid == 0) of_warp_0 = coef;
+  }
+  if (!grad) return;
+  __syncthreads();
+  const Slope<A> slope(base_of(part.m), part.s, of_warp_0 * inv_temp, k, token.target, a.vocab);
+  for (int j = mine - 1; j >= 0; --j) {
+    uint4 q[kBatch];
+    fetch(j, q);
+    copy(j - kStages);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      store_once(to + static_cast<int64_t>(j) * stride + i * kPolicyThreads,
+                 slope_vector<T>(q[i], slope));
+    write_target_of_tile<kPolicyThreads, kPolicyTile>(view, own - place.tid + j * stride, place.tid,
+                                                      slope);
+  }
+  write_edge(view, place.edge(), slope);
+  for (int tile = rest * kPolicyTile; tile < view.vectors; tile += stride)
+    write_tile<kPolicyThreads>(view, tile, place.tid, slope);
 }
 
 // The means over the tokens, in a fixed order; 0 when the weights sum to 0.
@@ -517,6 +614,23 @@ int sm_count() {
   if (cudaGetDevice(&dev) == cudaSuccess)
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   return sms;
+}
+
+// Allows a kernel more than 48 KB of dynamic shared memory: once per kernel and device.
+int allow_shared(const void* kernel, size_t bytes) {
+  static std::mutex mutex;
+  static std::set<std::pair<const void*, int>> done;
+  if (bytes <= 48 * 1024) return TISO_OK;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return logits_fail(e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mutex);
+  if (done.count({kernel, dev})) return TISO_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(bytes));
+  if (e != cudaSuccess) return logits_fail(e, "cudaFuncSetAttribute");
+  done.insert({kernel, dev});
+  return TISO_OK;
 }
 
 // A launch of `clusters` clusters of `ctas` CTAs (a power of two up to 8) of `threads`.
@@ -602,13 +716,17 @@ int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, d
   const int vectors = a.vocab / RowView<T>::E;
   const A k = exp_factor(A(0), inv_temp);
   if (vectors <= kWarpVectors)
-    return launch_warps(policy_kernel<T, A, 32>, a.rows, st, "policy_kernel launch", a, p, inv_temp,
-                        k, grad);
+    return launch_warps(policy_warp_kernel<T, A>, a.rows, st, "policy_warp_kernel launch", a, p,
+                        inv_temp, k, grad);
   const int sms = sm_count();
-  int ctas = ctas_for(a.rows, vectors, 512, sms);
+  int ctas = ctas_for(a.rows, vectors, kPolicyThreads, sms);
   while (ctas < 8 && int64_t{sms} * 3 * vectors * 16 / ctas > kRowsInL2) ctas *= 2;
-  return launch_clusters(policy_kernel<T, A, 512>, a.rows, ctas, 512, 0, st, "policy_kernel launch",
-                         a, p, inv_temp, k, grad);
+  constexpr size_t kShared = size_t{kStages} * kPolicyTile * 16;
+  const auto kernel = policy_kernel<T, A>;
+  const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kShared);
+  if (rc) return rc;
+  return launch_clusters(kernel, a.rows, ctas, kPolicyThreads, kShared, st,
+                         "policy_kernel launch", a, p, inv_temp, k, grad);
 }
 
 template <typename T>

@@ -357,6 +357,20 @@ __device__ __forceinline__ void store_once(void* p, const uint4& v) {
   __stcs(reinterpret_cast<uint4*>(p), v);
 }
 
+// Copies of 16 bytes to shared memory that a thread starts, closes a group of, and waits for until
+// no more than kOpen groups are open.
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from)
+               : "memory");
+}
+__device__ __forceinline__ void close_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kOpen>
+__device__ __forceinline__ void wait_groups() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kOpen) : "memory");
+}
+
 // The parts of kLanes neighbouring lanes joined (each lane gets the result).
 template <int kLanes, typename A>
 __device__ __forceinline__ Part<A> join_lanes(Part<A> p, A k) {
