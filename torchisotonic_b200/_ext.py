@@ -560,6 +560,14 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+@functools.lru_cache(maxsize=256)
+def _size(query_name: str, *args: int) -> int:
+    """A workspace query's answer."""
+    size = ctypes.c_size_t(0)
+    _check(getattr(lib(), query_name)(*args, ctypes.byref(size)))
+    return size.value
+
+
 def logits_rows(x: Tensor) -> tuple[Tensor, Rows]:
     """``x`` ([..., vocab], CUDA) as rows of logits, and the tensor whose memory they are: x itself
     when its last dimension is contiguous and the leading ones reduce to two strides (a contiguous
@@ -568,17 +576,18 @@ def logits_rows(x: Tensor) -> tuple[Tensor, Rows]:
         raise RuntimeError("logits must be a CUDA tensor: torchisotonic_b200 has no CPU path")
     if x.dtype not in _DTYPES:
         raise RuntimeError("logits must be float16, bfloat16, float32 or float64")
-    vocab = x.shape[-1]
+    shape = x.shape
+    vocab = shape[-1]
     if x.is_contiguous():
         rows = x.numel() // vocab
         return x, Rows(x.data_ptr(), rows, max(rows, 1), 0, vocab, vocab)
-    shape, stride = x.shape, x.stride()
+    stride = x.stride()
     if stride[-1] == 1 or vocab == 1:
-        if x.dim() == 1:
+        if len(shape) == 1:
             return x, Rows(x.data_ptr(), 1, 1, 0, 0, vocab)
-        if x.dim() == 2:
+        if len(shape) == 2:
             return x, Rows(x.data_ptr(), shape[0], max(shape[0], 1), 0, stride[0], vocab)
-        if x.dim() == 3:
+        if len(shape) == 3:
             return x, Rows(x.data_ptr(), shape[0] * shape[1], max(shape[1], 1), stride[0],
                            stride[1], vocab)
     return logits_rows(x.contiguous())
@@ -591,66 +600,77 @@ def logprobs(x: Tensor, targets: Tensor, ignore_index: int, temperature: float,
     needs (each row's maximum and sum of exponentials)."""
     x, rows = logits_rows(x)
     dev, acc = x.device, acc_dtype(x.dtype)
-    out = torch.empty(targets.shape, dtype=acc, device=dev)
-    stats = torch.empty(2 * rows.rows, dtype=acc, device=dev) if with_stats else None
+    out = x.new_empty(targets.shape, dtype=acc)
+    stats = x.new_empty(2 * rows.rows, dtype=acc) if with_stats else None
     with _on(dev):
         _check(lib().tiso_logprobs(_DTYPES[x.dtype], rows, targets.data_ptr(), ignore_index,
                                    temperature, out.data_ptr(), _ptr(stats), _stream(dev)))
     return out, stats
 
 
-def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor, coef: Tensor,
-                  upstream: Tensor | None = None, grad: Tensor | None = None) -> Tensor:
-    """The gradient of sum(coef * upstream * logprobs) in x, in its dtype and shape, contiguous.
-    ``coef``: contiguous, one per row, in the accumulation dtype or float64. ``grad``: holds the gradient for upstream = 1 (left as it
-    is when upstream, a device scalar, is 1), or None for a new tensor."""
+def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor,
+                  coef: Tensor) -> Tensor:
+    """The gradient of sum(coef * logprobs) in x, in its dtype and shape, contiguous. ``coef``:
+    contiguous, one per row, in the accumulation dtype."""
     x, rows = logits_rows(x)
     dev = x.device
-    if grad is None:
-        grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if upstream is not None:
-            coef, upstream = coef * upstream, None
+    grad = torch.empty_like(x, memory_format=torch.contiguous_format)
     with _on(dev):
         _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
                                         stats.data_ptr(), _DTYPES[coef.dtype], coef.data_ptr(),
-                                        _ptr(upstream), grad.data_ptr(), _stream(dev)))
+                                        None, grad.data_ptr(), _stream(dev)))
     return grad
 
 
 def policy(x: Tensor, targets: Tensor, ignore_index: int, temperature: float, old_logps: Tensor,
            advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None, clip_low: float,
            clip_high: float, kl_coef: float, with_grad: bool
-           ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor | None]:
-    """The clipped policy loss of tiso_policy: (out [3]: loss, kl, clip fraction; logps; coef;
-    stats; grad or None). The per-token tensors are contiguous, one number per row of logits, in
-    the accumulation dtype (``weight`` may be bool, ``targets`` is int64)."""
+           ) -> tuple[tuple[Tensor, ...], Tensor, Tensor, Tensor | None]:
+    """The clipped policy loss of tiso_policy: ((loss, kl, clip fraction), logps, what
+    policy_grad needs, grad or None). The per-token tensors are contiguous, one number per row of
+    logits, in the accumulation dtype (``weight`` may be bool, ``targets`` is int64)."""
     x, rows = logits_rows(x)
     dev, acc = x.device, acc_dtype(x.dtype)
     dtype, n = _DTYPES[x.dtype], rows.rows
-    logps = torch.empty(targets.shape, dtype=acc, device=dev)
-    coef = torch.empty(n, dtype=torch.float64, device=dev)
-    stats = torch.empty(2 * n, dtype=acc, device=dev)
-    out = torch.empty(3, dtype=acc, device=dev)
-    grad = torch.empty(x.shape, dtype=x.dtype, device=dev) if with_grad else None
+    logps = x.new_empty(targets.shape, dtype=acc)
+    out = x.new_empty(3, dtype=acc)
+    grad = torch.empty_like(x, memory_format=torch.contiguous_format) if with_grad else None
     args = PolicyArgs(old_logps.data_ptr(), _ptr(ref_logps), advantages.data_ptr(), _ptr(weight),
                       int(weight is not None and weight.dtype == torch.bool), clip_low, clip_high,
                       kl_coef)
-    so = lib()
-    size = ctypes.c_size_t()
+    size = _size("tiso_policy_workspace_size", dtype, n)
+    # n numbers coef, up to 2 n stats, the workspace: one allocation
+    kept = x.new_empty(3 * n + -(-size // 8), dtype=torch.float64)
+    at = kept.data_ptr()
     with _on(dev):
-        _check(so.tiso_policy_workspace_size(dtype, n, ctypes.byref(size)))
-        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        _check(so.tiso_policy(dtype, rows, targets.data_ptr(), ignore_index, temperature, args,
-                              logps.data_ptr(), coef.data_ptr(), stats.data_ptr(), out.data_ptr(),
-                              _ptr(grad), ws.data_ptr(), size.value, _stream(dev)))
-    return out, logps, coef, stats, grad
+        _check(lib().tiso_policy(dtype, rows, targets.data_ptr(), ignore_index, temperature, args,
+                                 logps.data_ptr(), at, at + 8 * n, out.data_ptr(), _ptr(grad),
+                                 at + 24 * n, size, _stream(dev)))
+    return out.unbind(), logps, kept, grad
+
+
+def policy_grad(x: Tensor, targets: Tensor, temperature: float, kept: Tensor, upstream: Tensor,
+                grad: Tensor | None) -> Tensor:
+    """The policy loss's gradient in x times ``upstream`` (a scalar tensor). ``grad``: what policy
+    wrote, the gradient for upstream = 1, overwritten unless it is; or None for a new tensor."""
+    x, rows = logits_rows(x)
+    dev, n = x.device, rows.rows
+    coef, once = kept, upstream
+    if grad is None:
+        grad = torch.empty_like(x, memory_format=torch.contiguous_format)
+        coef, once = kept[:n] * upstream, None
+    with _on(dev):
+        _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
+                                        kept.data_ptr() + 8 * n, F64, coef.data_ptr(), _ptr(once),
+                                        grad.data_ptr(), _stream(dev)))
+    return grad
 
 
 def _preference_args(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor,
                      kind: int, average: bool, beta: float, label_smoothing: float,
                      margin: float) -> PreferenceArgs:
     return PreferenceArgs(logps.data_ptr(), _ptr(refs), _ptr(mask), offsets.data_ptr(),
-                          logps.numel(), (offsets.numel() - 1) // 2, kind, int(average), beta,
+                          logps.numel(), (offsets.numel() - 1) // 2, kind, average, beta,
                           label_smoothing, margin)
 
 
@@ -662,16 +682,17 @@ def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets:
     args = _preference_args(logps, refs, mask, offsets, kind, average, beta, label_smoothing,
                             margin)
     dev, pairs = logps.device, args.pairs
-    loss = torch.empty((), dtype=logps.dtype, device=dev)
-    rewards = torch.empty(2, pairs, dtype=logps.dtype, device=dev)
-    coef = torch.empty(2 * pairs, dtype=logps.dtype, device=dev)
-    so = lib()
-    size = ctypes.c_size_t()
+    loss = logps.new_empty(())
+    rewards = logps.new_empty((2, pairs))
+    # coef and, behind it, the workspace: one allocation
+    size = _size("tiso_preference_workspace_size", pairs)
+    each = logps.element_size()
+    first = -(-2 * pairs * each // 8) * 8
+    coef = logps.new_empty((first + size) // each)
     with _on(dev):
-        _check(so.tiso_preference_workspace_size(pairs, ctypes.byref(size)))
-        ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        _check(so.tiso_preference(_DTYPES[logps.dtype], args, loss.data_ptr(), rewards.data_ptr(),
-                                  coef.data_ptr(), ws.data_ptr(), size.value, _stream(dev)))
+        _check(lib().tiso_preference(_DTYPES[logps.dtype], args, loss.data_ptr(),
+                                     rewards.data_ptr(), coef.data_ptr(), coef.data_ptr() + first,
+                                     size, _stream(dev)))
     return loss, rewards, coef
 
 

@@ -26,6 +26,10 @@ def _need_cuda(t: Tensor, name: str) -> None:
         )
 
 
+def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
 def _check_logits(logits: Tensor, targets: Tensor, temperature: float) -> None:
     if not isinstance(logits, Tensor) or not isinstance(targets, Tensor):
         raise TypeError("logits and targets must be torch.Tensors")
@@ -75,7 +79,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     read in place.
     """
     _check_logits(logits, targets, temperature)
-    targets = targets.to(torch.int64).contiguous()
+    targets = _as(targets, torch.int64)
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogprobs.apply(logits, targets, float(temperature), int(ignore_index))
     return _ext.logprobs(logits, targets, int(ignore_index), float(temperature), False)[0]
@@ -84,7 +88,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, logps: Tensor, refs: Tensor | None, mask: Tensor | None,
-                offsets: Tensor, *settings: Any) -> tuple[Tensor, Tensor]:
+                offsets: Tensor, settings: tuple[Any, ...]) -> tuple[Tensor, Tensor]:
         loss, rewards, coef = _ext.preference(logps, refs, mask, offsets, *settings)
         ctx.save_for_backward(logps, mask, offsets, coef)
         ctx.mark_non_differentiable(rewards)
@@ -94,12 +98,12 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: Tensor | None, _: Any) -> tuple[Tensor | None, ...]:
-        logps, mask, offsets, coef = ctx.saved_tensors
-        none = (None,) * 7
         if grad is None:
-            return (None, None, *none)
+            return None, None, None, None, None
         want, want_ref = ctx.needs_input_grad[:2]
-        return (*_ext.preference_grad(logps, mask, offsets, coef, grad, want, want_ref), *none)
+        logps, mask, offsets, coef = ctx.saved_tensors
+        return (*_ext.preference_grad(logps, mask, offsets, coef, grad, want, want_ref), None,
+                None, None)
 
 
 def preference_loss(
@@ -156,7 +160,7 @@ def preference_loss(
             raise TypeError("ref_logps must be a floating-point torch.Tensor")
         if ref_logps.shape != logps.shape or ref_logps.device != dev:
             raise ValueError("ref_logps must be shaped like logps and on its device")
-        ref_logps = ref_logps.to(dtype).contiguous()
+        ref_logps = _as(ref_logps, dtype)
     if mask is not None:
         if not isinstance(mask, Tensor) or mask.dtype != torch.bool:
             raise TypeError("mask must be a bool torch.Tensor")
@@ -165,9 +169,11 @@ def preference_loss(
         mask = mask.contiguous()
     if offsets.device != dev:
         raise ValueError("offsets must be on logps' device")
-    return _Preference.apply(logps.to(dtype).contiguous(), ref_logps, mask,
-                             offsets.to(torch.int64).contiguous(), _ext.PREFERENCE_KINDS[kind],
-                             bool(average), float(beta), float(label_smoothing), float(margin))
+    loss, rewards = _Preference.apply(
+        _as(logps, dtype), ref_logps, mask, _as(offsets, torch.int64),
+        (_ext.PREFERENCE_KINDS[kind], bool(average), float(beta), float(label_smoothing),
+         float(margin)))
+    return loss, rewards
 
 
 class PolicyLoss(NamedTuple):
@@ -181,30 +187,27 @@ class PolicyLoss(NamedTuple):
 
 class _Policy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, logits: Tensor, targets: Tensor, ignore_index: int, temperature: float,
-                *settings: Any) -> tuple[Tensor, Tensor, Tensor]:
-        out, logps, coef, stats, grad = _ext.policy(logits, targets, ignore_index, temperature,
-                                                    *settings, True)
-        ctx.save_for_backward(logits, targets, coef, stats)
+    def forward(ctx: Any, logits: Tensor, targets: Tensor, temperature: float,
+                run: Any) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+        (loss, kl, clip_fraction), logps, kept, grad = run(True)
+        ctx.save_for_backward(logits, targets, kept)
         ctx.temperature = temperature
         ctx.grad = grad
-        loss, rest = out[0], out[1:]
-        ctx.mark_non_differentiable(rest, logps)
+        ctx.mark_non_differentiable(logps, kl, clip_fraction)
         ctx.set_materialize_grads(False)
-        return loss, rest, logps
+        return loss, logps, kl, clip_fraction
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, up: Tensor | None, *_: Any) -> tuple[Tensor | None, ...]:
-        none = (None,) * 10
         if up is None:
-            return (None, *none)
-        logits, targets, coef, stats = ctx.saved_tensors
+            return None, None, None, None
+        logits, targets, kept = ctx.saved_tensors
         # the gradient for an upstream gradient of 1, written with the loss, is given away the
         # first time (the kernel rewrites it unless upstream is 1); later calls write a new one
         grad, ctx.grad = ctx.grad, None
-        return (_ext.logprobs_grad(logits, targets, ctx.temperature, stats, coef, up, grad),
-                *none)
+        return (_ext.policy_grad(logits, targets, ctx.temperature, kept, up, grad), None, None,
+                None)
 
 
 def policy_loss(
@@ -241,28 +244,30 @@ def policy_loss(
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError("clip_low and clip_high must not be negative")
     _check_logits(logits, targets, temperature)
-    acc = _ext.acc_dtype(logits.dtype)
-    tokens = {"old_logps": old_logps, "advantages": advantages, "ref_logps": ref_logps,
-              "weight": weight}
-    for name, t in tokens.items():
-        if t is None and name in ("ref_logps", "weight"):
-            continue
+    acc, shape, device = _ext.acc_dtype(logits.dtype), targets.shape, logits.device
+
+    def constant(name: str, t: Tensor | None) -> Tensor:
         if not isinstance(t, Tensor) or t.is_complex():
             raise TypeError(f"{name} must be a real torch.Tensor")
-        if t.shape != targets.shape or t.device != logits.device:
+        if t.shape != shape or t.device != device:
             raise ValueError(f"{name} must be shaped like targets and on logits' device")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} is a constant of the loss: detach it")
-        if not (name == "weight" and t.dtype == torch.bool):
-            t = t.to(acc)
-        tokens[name] = t.contiguous()
-    settings = (int(ignore_index), float(temperature), tokens["old_logps"], tokens["advantages"],
-                tokens["ref_logps"], tokens["weight"], float(clip_low), float(clip_high),
-                float(kl_coef))
-    targets = targets.to(torch.int64).contiguous()
+        return _as(t, torch.bool if name == "weight" and t.dtype == torch.bool else acc)
+
+    old_logps = constant("old_logps", old_logps)
+    advantages = constant("advantages", advantages)
+    ref_logps = None if ref_logps is None else constant("ref_logps", ref_logps)
+    weight = None if weight is None else constant("weight", weight)
+    targets = _as(targets, torch.int64)
+    temperature = float(temperature)
+
+    def run(with_grad: bool) -> tuple[tuple[Tensor, ...], Tensor, Tensor, Tensor | None]:
+        return _ext.policy(logits.detach(), targets, int(ignore_index), temperature, old_logps,
+                           advantages, ref_logps, weight, float(clip_low), float(clip_high),
+                           float(kl_coef), with_grad)
+
     if logits.requires_grad and torch.is_grad_enabled():
-        loss, rest, logps = _Policy.apply(logits, targets, *settings)
-    else:
-        out, logps, *_ = _ext.policy(logits, targets, *settings, False)
-        loss, rest = out[0], out[1:]
-    return PolicyLoss(loss, logps, rest[0], rest[1])
+        return PolicyLoss(*_Policy.apply(logits, targets, temperature, run))
+    (loss, kl, clip_fraction), logps, _, _ = run(False)
+    return PolicyLoss(loss, logps, kl, clip_fraction)
