@@ -64,7 +64,7 @@ def adamw_step(
     count = len(params)
     if scales is not None and len(scales) != 2:
         raise ValueError("scales must be a pair of sequences")
-    if any(len(x) != count for x in lists):
+    if {*map(len, lists)} != {count}:
         raise ValueError("params, grads, states and scales must be of one length")
     if step < 1:
         raise ValueError("step must be at least 1")
@@ -74,9 +74,12 @@ def adamw_step(
         raise ValueError("lr, eps and weight_decay must not be negative")
     if count == 0:
         return
-    try:  # a C-level pass a check: hundreds of tensors a call
-        contiguous = all(map(Tensor.is_contiguous, chain.from_iterable(lists)))
-        devices = set(map(Tensor.get_device, chain.from_iterable(lists)))
+    # a C-level pass over the lists for each check: hundreds of tensors a call
+    tensors = [*chain.from_iterable(lists)]
+    try:
+        contiguous = all(map(Tensor.is_contiguous, tensors))
+        devices = {*map(Tensor.get_device, tensors)}
+        sizes = [*map(Tensor.numel, tensors)]
     except TypeError as e:
         raise TypeError("params, grads, states and scales must be torch.Tensors") from e
     if not contiguous:
@@ -88,38 +91,37 @@ def adamw_step(
         )
     if len(devices) != 1:
         raise ValueError("params, grads, states and scales must be on one device")
-    sizes = list(map(Tensor.numel, params))
-    if any(list(map(Tensor.numel, x)) != sizes for x in lists[1:4]):
+    if sizes[:4 * count] != sizes[:count] * 4:
         raise ValueError("grads and states must be shaped like their parameters")
-    param_types, grad_types, *state_types = ([*map(_dtype, x)] for x in lists)
-    bits = _bits(state_types[0][0])
-    if {*state_types[0], *state_types[1]} != {state_types[0][0]}:
+    types = [*map(_dtype, tensors)]
+    bits = _bits(types[2 * count])
+    if {*types[2 * count:4 * count]} != {types[2 * count]}:
         raise TypeError("optimizer states must be of one dtype")
     if (bits == 8) != (scales is not None):
         raise ValueError("scales go with float8_e4m3fn states, and only with them")
-    if scales is not None:
-        if {*state_types[2], *state_types[3]} != {torch.float32}:
+    if bits == 8:
+        if {*types[4 * count:]} != {torch.float32}:
             raise TypeError("scales must be float32 tensors")
-        blocks = [-(-n // BLOCK) for n in sizes]
-        if any(list(map(Tensor.numel, x)) != blocks for x in scales):
+        if sizes[4 * count:] != [-(-n // BLOCK) for n in sizes[:count]] * 2:
             raise ValueError(f"a scale tensor must hold ceil(n / {BLOCK}) numbers")
-    types = set(zip(param_types, grad_types))
-    for pt, gt in types:
+    kinds = [*zip(types[:count], types[count:2 * count])]
+    for pt, gt in {*kinds}:
         if pt not in (torch.float32, torch.float16, torch.bfloat16) or gt not in (pt, torch.float32):
             raise TypeError("params must be float32, bfloat16 or float16, grads like their "
                             "parameter or float32")
-    pointers = [map(Tensor.data_ptr, x) for x in lists]
-    if scales is None:
-        pointers += [repeat(0), repeat(0)]
-    fields = zip(*pointers, sizes, range(count))
+    at = [*map(Tensor.data_ptr, tensors)]
+    none = (repeat(0), repeat(0))
+    fields = zip(at[:count], at[count:2 * count], at[2 * count:3 * count],
+                 at[3 * count:4 * count], *((at[4 * count:5 * count], at[5 * count:])
+                                            if bits == 8 else none), sizes[:count], range(count))
     args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
-    if len(types) == 1:
-        _ext.adamw(params[0].device, pt, gt, bits, chain.from_iterable(fields), args)
+    if kinds.count(kinds[0]) == count:
+        _ext.adamw(params[0].device, *kinds[0], bits, chain.from_iterable(fields), args)
         return
-    tensors = list(fields)
-    for pt, gt in types:
-        its = [f for f, a, b in zip(tensors, param_types, grad_types) if a == pt and b == gt]
-        _ext.adamw(params[0].device, pt, gt, bits, chain.from_iterable(its), args)
+    rows = [*fields]
+    for kind in {*kinds}:
+        its = [f for f, k in zip(rows, kinds) if k == kind]
+        _ext.adamw(params[0].device, *kind, bits, chain.from_iterable(its), args)
 
 
 class AdamW(torch.optim.Optimizer):
