@@ -15,7 +15,7 @@ import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
-from torchisotonic_b200 import _ext
+from torchisotonic_b200 import _ext, ops
 
 
 def _need_cuda(t: Tensor, name: str) -> None:
@@ -80,6 +80,8 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     """
     _check_logits(logits, targets, temperature)
     targets = _as(targets, torch.int64)
+    if torch.compiler.is_compiling():  # traced: the operators, which the compiler keeps whole
+        return ops.token_logprobs(logits, targets, float(temperature), int(ignore_index))[0]
     if logits.requires_grad and torch.is_grad_enabled():
         return _TokenLogprobs.apply(logits, targets, float(temperature), int(ignore_index))
     return _ext.logprobs(logits, targets, int(ignore_index), float(temperature), False)[0]
@@ -169,10 +171,13 @@ def preference_loss(
         mask = mask.contiguous()
     if offsets.device != dev:
         raise ValueError("offsets must be on logps' device")
-    loss, rewards = _Preference.apply(
-        _as(logps, dtype), ref_logps, mask, _as(offsets, torch.int64),
-        (_ext.PREFERENCE_KINDS[kind], bool(average), float(beta), float(label_smoothing),
-         float(margin)))
+    settings = (_ext.PREFERENCE_KINDS[kind], bool(average), float(beta), float(label_smoothing),
+                float(margin))
+    logps, offsets = _as(logps, dtype), _as(offsets, torch.int64)
+    if torch.compiler.is_compiling():
+        loss, rewards, _ = ops.preference(logps, ref_logps, mask, offsets, *settings)
+        return loss, rewards.detach()
+    loss, rewards = _Preference.apply(logps, ref_logps, mask, offsets, settings)
     return loss, rewards
 
 
@@ -262,10 +267,16 @@ def policy_loss(
     targets = _as(targets, torch.int64)
     temperature = float(temperature)
 
+    settings = (old_logps, advantages, ref_logps, weight, float(clip_low), float(clip_high),
+                float(kl_coef))
+    if torch.compiler.is_compiling():
+        out, logps, _ = ops.policy(logits, targets, int(ignore_index), temperature, *settings)
+        rest = out.detach()
+        return PolicyLoss(out[0], logps.detach(), rest[1], rest[2])
+
     def run(with_grad: bool) -> tuple[tuple[Tensor, ...], Tensor, Tensor, Tensor | None]:
-        return _ext.policy(logits.detach(), targets, int(ignore_index), temperature, old_logps,
-                           advantages, ref_logps, weight, float(clip_low), float(clip_high),
-                           float(kl_coef), with_grad)
+        return _ext.policy(logits.detach(), targets, int(ignore_index), temperature, *settings,
+                           with_grad)
 
     if logits.requires_grad and torch.is_grad_enabled():
         return PolicyLoss(*_Policy.apply(logits, targets, temperature, run))

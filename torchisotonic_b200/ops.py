@@ -20,6 +20,11 @@ Two more carry what this library folds into its kernels, and are what ``isotonic
   float? y_min, float? y_max) -> (Tensor, Tensor)``: d/dy and d/dw (empty when not wanted),
   the clamp's inclusive mask applied.
 
+The losses of ``losses.py`` have theirs, which the public functions run under ``torch.compile``:
+``token_logprobs``, ``preference`` and ``policy``, each with its ``_grad``. (``policy`` leaves the
+gradient to ``policy_grad``, which reads the logits again; the eager function writes it with the
+loss.)
+
 ``fit`` has its autograd registered (the reference's _Isotonic, src/torchisotonic/_api.py:73-97)
 and every operator a fake (meta) implementation, so ``torch.compile`` traces through them
 without a graph break. There is no CPU kernel: CUDA tensors only.
@@ -134,3 +139,133 @@ def _fit_backward(ctx, grad_out: Tensor, _grad_starts: Tensor):
 
 
 torch.library.register_autograd(f"{_NS}::fit", _fit_backward, setup_context=_fit_setup)
+
+
+# ---------------------------------------------------------------------------------------------
+# The losses
+
+
+@torch.library.custom_op(f"{_NS}::token_logprobs", mutates_args=())
+def token_logprobs(logits: Tensor, targets: Tensor, temperature: float,
+                   ignore_index: int) -> tuple[Tensor, Tensor]:
+    out, stats = _ext.logprobs(logits, targets.contiguous(), ignore_index, temperature, True)
+    assert stats is not None
+    return out, stats
+
+
+@token_logprobs.register_fake
+def _(logits, targets, temperature, ignore_index):
+    acc = _acc(logits.dtype)
+    return (logits.new_empty(targets.shape, dtype=acc),
+            logits.new_empty((2 * targets.numel(),), dtype=acc))
+
+
+@torch.library.custom_op(f"{_NS}::token_logprobs_grad", mutates_args=())
+def token_logprobs_grad(logits: Tensor, targets: Tensor, temperature: float, stats: Tensor,
+                        coef: Tensor) -> Tensor:
+    return _ext.logprobs_grad(logits, targets.contiguous(), temperature, stats, coef.contiguous())
+
+
+@token_logprobs_grad.register_fake
+def _(logits, targets, temperature, stats, coef):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _token_logprobs_setup(ctx, inputs, output) -> None:
+    logits, targets, ctx.temperature, _ = inputs
+    ctx.save_for_backward(logits, targets, output[1])
+
+
+def _token_logprobs_backward(ctx, grad: Tensor, _grad_stats: Tensor):
+    logits, targets, stats = ctx.saved_tensors
+    return (token_logprobs_grad(logits, targets, ctx.temperature, stats, grad), None, None, None)
+
+
+torch.library.register_autograd(f"{_NS}::token_logprobs", _token_logprobs_backward,
+                                setup_context=_token_logprobs_setup)
+
+
+@torch.library.custom_op(f"{_NS}::preference", mutates_args=())
+def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor, kind: int,
+               average: bool, beta: float, label_smoothing: float,
+               margin: float) -> tuple[Tensor, Tensor, Tensor]:
+    loss, rewards, coef = _ext.preference(logps, refs, mask, offsets, kind, average, beta,
+                                          label_smoothing, margin)
+    return loss, rewards, coef[:rewards.numel()].clone()
+
+
+@preference.register_fake
+def _(logps, refs, mask, offsets, kind, average, beta, label_smoothing, margin):
+    pairs = (offsets.numel() - 1) // 2
+    return (logps.new_empty(()), logps.new_empty((2, pairs)), logps.new_empty((2 * pairs,)))
+
+
+@torch.library.custom_op(f"{_NS}::preference_grad", mutates_args=())
+def preference_grad(logps: Tensor, mask: Tensor | None, offsets: Tensor, coef: Tensor,
+                    upstream: Tensor) -> Tensor:
+    grad, _ = _ext.preference_grad(logps, mask, offsets, coef, upstream, True, False)
+    assert grad is not None
+    return grad
+
+
+@preference_grad.register_fake
+def _(logps, mask, offsets, coef, upstream):
+    return torch.empty_like(logps)
+
+
+def _preference_setup(ctx, inputs, output) -> None:
+    logps, _, mask, offsets = inputs[:4]
+    ctx.save_for_backward(logps, mask, offsets, output[2])
+
+
+def _preference_backward(ctx, grad: Tensor, _grad_rewards: Tensor, _grad_coef: Tensor):
+    logps, mask, offsets, coef = ctx.saved_tensors
+    g = preference_grad(logps, mask, offsets, coef, grad)
+    want, want_ref = ctx.needs_input_grad[:2]
+    return (g if want else None, -g if want_ref else None, *(None,) * 7)
+
+
+torch.library.register_autograd(f"{_NS}::preference", _preference_backward,
+                                setup_context=_preference_setup)
+
+
+@torch.library.custom_op(f"{_NS}::policy", mutates_args=())
+def policy(logits: Tensor, targets: Tensor, ignore_index: int, temperature: float,
+           old_logps: Tensor, advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None,
+           clip_low: float, clip_high: float, kl_coef: float) -> tuple[Tensor, Tensor, Tensor]:
+    out, logps, kept, _ = _ext.policy(logits, targets, ignore_index, temperature, old_logps,
+                                      advantages, ref_logps, weight, clip_low, clip_high, kl_coef,
+                                      False)
+    return torch.stack(out), logps, kept[:3 * targets.numel()].clone()
+
+
+@policy.register_fake
+def _(logits, targets, ignore_index, temperature, old_logps, advantages, ref_logps, weight,
+      clip_low, clip_high, kl_coef):
+    acc = _acc(logits.dtype)
+    return (logits.new_empty((3,), dtype=acc), logits.new_empty(targets.shape, dtype=acc),
+            logits.new_empty((3 * targets.numel(),), dtype=torch.float64))
+
+
+@torch.library.custom_op(f"{_NS}::policy_grad", mutates_args=())
+def policy_grad(logits: Tensor, targets: Tensor, temperature: float, kept: Tensor,
+                upstream: Tensor) -> Tensor:
+    return _ext.policy_grad(logits, targets, temperature, kept, upstream, None)
+
+
+@policy_grad.register_fake
+def _(logits, targets, temperature, kept, upstream):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _policy_setup(ctx, inputs, output) -> None:
+    logits, targets, _, ctx.temperature = inputs[:4]
+    ctx.save_for_backward(logits, targets, output[2])
+
+
+def _policy_backward(ctx, grad: Tensor, _grad_logps: Tensor, _grad_kept: Tensor):
+    logits, targets, kept = ctx.saved_tensors
+    return (policy_grad(logits, targets, ctx.temperature, kept, grad[0]), *(None,) * 10)
+
+
+torch.library.register_autograd(f"{_NS}::policy", _policy_backward, setup_context=_policy_setup)
