@@ -94,7 +94,7 @@ def main(argv: list[str] | None = None) -> dict[str, Any]:
         opt.zero_grad()
         loss.backward()
         opt.step()
-        out["loss"].append(float(loss))
+        out["loss"].append(float(loss.detach()))
 
     # margins of held-out pairs, shown in either order: the curve from a margin to the probability
     # that the first answer shown is the better one
