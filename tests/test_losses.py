@@ -734,6 +734,8 @@ def test_abi_refusals() -> None:
     assert so.tiso_logprobs(2, _ext.Rows(None, 0, 1, 0, 8, 8), None, -100, 1.0, None, None, None) == 0
     assert so.tiso_logprobs_grad(2, rows, p, 1.0, None, 2, p, None, p, None) == 1
     assert so.tiso_logprobs_grad(3, rows, p, 1.0, p, 2, p, None, p, None) == 1
+    assert so.tiso_logprobs_grad(2, rows, p, 1.0, p, 2, p, None, ctypes.c_void_p(18), None) == 1
+    assert b"aligned" in so.tiso_last_error()
     args = _ext.PolicyArgs(16, None, 16, None, 0, 0.2, 0.2, 0.0)
     size = ctypes.c_size_t()
     assert so.tiso_policy_workspace_size(2, 4, ctypes.byref(size)) == 0 and size.value > 0

@@ -334,6 +334,17 @@ def test_optimizer_groups_and_missing_gradients() -> None:
 
 
 @pytest.mark.gpu
+def test_a_step_counts_as_a_change_in_place() -> None:
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    q = (p * p).sum()  # keeps p for its gradient
+    version = p._version
+    ti.adamw_step([p], [torch.ones_like(p)], [torch.zeros_like(p)], [torch.zeros_like(p)], step=1)
+    assert p._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        q.backward()
+
+
+@pytest.mark.gpu
 def test_step_on_another_stream() -> None:
     a = tensors([(5000,)], torch.float32, torch.float32, 32)
     b = copy.deepcopy(a)
@@ -413,6 +424,9 @@ def test_abi_refusals() -> None:
     assert so.tiso_adamw(2, 2, 32, 1, None, good, None) == 1
     assert so.tiso_adamw(2, 2, 32, 1, at, _ext.AdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.01, 0, 0), None) == 1
     assert b"step" in so.tiso_last_error()
+    off = (ctypes.c_int64 * 8)(18, 16, 16, 16, 0, 0, 4, 0)
+    assert so.tiso_adamw(2, 2, 32, 1, ctypes.addressof(off), good, None) == 1
+    assert b"aligned" in so.tiso_last_error()
     assert so.tiso_adamw(2, 2, 32, 0, None, good, None) == 0
     empty = (ctypes.c_int64 * 8)(0, 0, 0, 0, 0, 0, 0, 0)
     assert so.tiso_adamw(2, 2, 32, 1, ctypes.addressof(empty), good, None) == 0

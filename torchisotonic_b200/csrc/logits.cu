@@ -8,12 +8,10 @@
 #include <string>
 #include <utility>
 
-#include "../../include/tiso.h"
+#include "entry.cuh"
 #include "logits.cuh"
 
 namespace tiso {
-
-int report_error(int code, const std::string& msg);
 
 namespace {
 
@@ -574,7 +572,8 @@ __global__ void __launch_bounds__(1024) policy_means_kernel(int64_t rows, Policy
 // ---------------------------------------------------------------------------------------------
 // Host side
 
-int check_rows(int dtype, const tiso_rows* x, const int64_t* targets) {
+// grad: NULL, or the gradient that the call writes
+int check_rows(int dtype, const tiso_rows* x, const int64_t* targets, const void* grad) {
   if (dtype < TISO_F16 || dtype > TISO_F64)
     return report_error(TISO_ERR_ARGUMENT, "dtype must be a tiso_dtype");
   if (!x) return report_error(TISO_ERR_ARGUMENT, "rows is NULL");
@@ -587,8 +586,8 @@ int check_rows(int dtype, const tiso_rows* x, const int64_t* targets) {
   if (x->rows && (!x->data || !targets))
     return report_error(TISO_ERR_ARGUMENT, "logits and targets must not be NULL");
   const int size = dtype == TISO_F64 ? 8 : dtype == TISO_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(x->data) % size)
-    return report_error(TISO_ERR_ARGUMENT, "logits must be aligned to their elements");
+  if ((reinterpret_cast<uintptr_t>(x->data) | reinterpret_cast<uintptr_t>(grad)) % size)
+    return report_error(TISO_ERR_ARGUMENT, "logits and grad must be aligned to their elements");
   return TISO_OK;
 }
 
@@ -777,74 +776,82 @@ extern "C" {
 
 int tiso_logprobs(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
                   double temperature, void* logps, void* stats, void* stream) {
-  const int rc = check_rows(dtype, x, targets);
-  if (rc) return rc;
-  if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
-  if (x->rows == 0) return TISO_OK;
-  if (!logps) return report_error(TISO_ERR_ARGUMENT, "logps must not be NULL");
-  const Rows a = rows_of(x, targets, ignore_index);
-  return by_type(dtype, [&](auto t) {
-    return run_logprobs<decltype(t)>(a, 1.0 / temperature, logps, stats,
-                                     static_cast<cudaStream_t>(stream));
+  return guarded([&]() -> int {
+    const int rc = check_rows(dtype, x, targets, nullptr);
+    if (rc) return rc;
+    if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
+    if (x->rows == 0) return TISO_OK;
+    if (!logps) return report_error(TISO_ERR_ARGUMENT, "logps must not be NULL");
+    const Rows a = rows_of(x, targets, ignore_index);
+    return by_type(dtype, [&](auto t) {
+      return run_logprobs<decltype(t)>(a, 1.0 / temperature, logps, stats,
+                                       static_cast<cudaStream_t>(stream));
+    });
   });
 }
 
 int tiso_logprobs_grad(int dtype, const tiso_rows* x, const int64_t* targets, double temperature,
                        const void* stats, int coef_dtype, const void* coef,
                        const void* upstream, void* grad, void* stream) {
-  const int rc = check_rows(dtype, x, targets);
-  if (rc) return rc;
-  if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
-  if (x->rows == 0) return TISO_OK;
-  if (!stats || !coef || !grad)
-    return report_error(TISO_ERR_ARGUMENT, "stats, coef and grad must not be NULL");
-  if (coef_dtype != TISO_F64 && (coef_dtype != TISO_F32 || dtype == TISO_F64))
-    return report_error(TISO_ERR_ARGUMENT, "coef_dtype must be the accumulation type or TISO_F64");
-  const Rows a = rows_of(x, targets, 0);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (coef_dtype == TISO_F64)
-      return run_logprobs_grad<T, double>(a, 1.0 / temperature, stats, coef, upstream, grad, st);
-    return run_logprobs_grad<T, typename AccOf<T>::type>(a, 1.0 / temperature, stats, coef,
-                                                         upstream, grad, st);
+  return guarded([&]() -> int {
+    const int rc = check_rows(dtype, x, targets, grad);
+    if (rc) return rc;
+    if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
+    if (x->rows == 0) return TISO_OK;
+    if (!stats || !coef || !grad)
+      return report_error(TISO_ERR_ARGUMENT, "stats, coef and grad must not be NULL");
+    if (coef_dtype != TISO_F64 && (coef_dtype != TISO_F32 || dtype == TISO_F64))
+      return report_error(TISO_ERR_ARGUMENT, "coef_dtype must be the accumulation type or TISO_F64");
+    const Rows a = rows_of(x, targets, 0);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return by_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      if (coef_dtype == TISO_F64)
+        return run_logprobs_grad<T, double>(a, 1.0 / temperature, stats, coef, upstream, grad, st);
+      return run_logprobs_grad<T, typename AccOf<T>::type>(a, 1.0 / temperature, stats, coef,
+                                                           upstream, grad, st);
+    });
   });
 }
 
 int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes) {
-  if (!bytes) return report_error(TISO_ERR_ARGUMENT, "bytes is NULL");
-  *bytes = 0;
-  if (dtype < TISO_F16 || dtype > TISO_F64)
-    return report_error(TISO_ERR_ARGUMENT, "dtype must be a tiso_dtype");
-  if (rows < 0) return report_error(TISO_ERR_ARGUMENT, "need rows >= 0");
-  *bytes = 8 + static_cast<size_t>(rows) * 3 * (dtype == TISO_F64 ? 8 : 4);
-  return TISO_OK;
+  return guarded([&]() -> int {
+    if (!bytes) return report_error(TISO_ERR_ARGUMENT, "bytes is NULL");
+    *bytes = 0;
+    if (dtype < TISO_F16 || dtype > TISO_F64)
+      return report_error(TISO_ERR_ARGUMENT, "dtype must be a tiso_dtype");
+    if (rows < 0) return report_error(TISO_ERR_ARGUMENT, "need rows >= 0");
+    *bytes = 8 + static_cast<size_t>(rows) * 3 * (dtype == TISO_F64 ? 8 : 4);
+    return TISO_OK;
+  });
 }
 
 int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
                 double temperature, const tiso_policy_args* args, void* logps, double* coef,
                 void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,
                 void* stream) {
-  int rc = check_rows(dtype, x, targets);
-  if (rc) return rc;
-  if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
-  if (!args) return report_error(TISO_ERR_ARGUMENT, "args is NULL");
-  if (!(args->clip_low >= 0 && args->clip_high >= 0))
-    return report_error(TISO_ERR_ARGUMENT, "clip_low and clip_high must not be negative");
-  if (x->rows && (!args->old_logps || !args->advantages || !logps || !coef || !stats))
-    return report_error(TISO_ERR_ARGUMENT,
-                        "old_logps, advantages, logps, coef and stats must not be NULL");
-  if (!out) return report_error(TISO_ERR_ARGUMENT, "out must not be NULL");
-  size_t need = 0;
-  rc = tiso_policy_workspace_size(dtype, x->rows, &need);
-  if (rc) return rc;
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
-    return report_error(TISO_ERR_WORKSPACE,
-                        "workspace missing, unaligned or smaller than tiso_policy_workspace_size");
-  const Rows a = rows_of(x, targets, ignore_index);
-  return by_type(dtype, [&](auto t) {
-    return run_policy<decltype(t)>(a, args, 1.0 / temperature, logps, coef, stats, out, grad,
-                                   workspace, static_cast<cudaStream_t>(stream));
+  return guarded([&]() -> int {
+    int rc = check_rows(dtype, x, targets, grad);
+    if (rc) return rc;
+    if (!(temperature > 0)) return report_error(TISO_ERR_ARGUMENT, "temperature must be > 0");
+    if (!args) return report_error(TISO_ERR_ARGUMENT, "args is NULL");
+    if (!(args->clip_low >= 0 && args->clip_high >= 0))
+      return report_error(TISO_ERR_ARGUMENT, "clip_low and clip_high must not be negative");
+    if (x->rows && (!args->old_logps || !args->advantages || !logps || !coef || !stats))
+      return report_error(TISO_ERR_ARGUMENT,
+                          "old_logps, advantages, logps, coef and stats must not be NULL");
+    if (!out) return report_error(TISO_ERR_ARGUMENT, "out must not be NULL");
+    size_t need = 0;
+    rc = tiso_policy_workspace_size(dtype, x->rows, &need);
+    if (rc) return rc;
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 7))
+      return report_error(TISO_ERR_WORKSPACE,
+                          "workspace missing, unaligned or smaller than tiso_policy_workspace_size");
+    const Rows a = rows_of(x, targets, ignore_index);
+    return by_type(dtype, [&](auto t) {
+      return run_policy<decltype(t)>(a, args, 1.0 / temperature, logps, coef, stats, out, grad,
+                                     workspace, static_cast<cudaStream_t>(stream));
+    });
   });
 }
 

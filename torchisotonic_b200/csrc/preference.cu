@@ -10,11 +10,9 @@
 
 #include <string>
 
-#include "../../include/tiso.h"
+#include "entry.cuh"
 
 namespace tiso {
-
-int report_error(int code, const std::string& msg);
 
 namespace {
 
@@ -187,8 +185,8 @@ int check_preference(int dtype, const tiso_preference_args* q) {
   if (dtype != TISO_F32 && dtype != TISO_F64)
     return report_error(TISO_ERR_ARGUMENT, "dtype must be TISO_F32 or TISO_F64");
   if (!q) return report_error(TISO_ERR_ARGUMENT, "args is NULL");
-  if (q->pairs < 1 || q->pairs > int64_t{1} << 30)
-    return report_error(TISO_ERR_ARGUMENT, "pairs must be in [1, 2^30]");
+  if (q->pairs < 1 || q->pairs > int64_t{1} << 28)
+    return report_error(TISO_ERR_ARGUMENT, "pairs must be in [1, 2^28]");
   if (q->tokens < 0 || q->tokens > int64_t{1} << 38)
     return report_error(TISO_ERR_ARGUMENT, "tokens must be in [0, 2^38]");
   if (!q->offsets || (q->tokens && !q->logps))
@@ -209,40 +207,46 @@ using namespace tiso;
 extern "C" {
 
 int tiso_preference_workspace_size(int64_t pairs, size_t* bytes) {
-  if (!bytes) return report_error(TISO_ERR_ARGUMENT, "bytes is NULL");
-  *bytes = 0;
-  if (pairs < 1 || pairs > int64_t{1} << 30)
-    return report_error(TISO_ERR_ARGUMENT, "pairs must be in [1, 2^30]");
-  *bytes = static_cast<size_t>(pairs) * 4 * sizeof(double);
-  return TISO_OK;
+  return guarded([&]() -> int {
+    if (!bytes) return report_error(TISO_ERR_ARGUMENT, "bytes is NULL");
+    *bytes = 0;
+    if (pairs < 1 || pairs > int64_t{1} << 28)
+      return report_error(TISO_ERR_ARGUMENT, "pairs must be in [1, 2^28]");
+    *bytes = static_cast<size_t>(pairs) * 4 * sizeof(double);
+    return TISO_OK;
+  });
 }
 
 int tiso_preference(int dtype, const tiso_preference_args* args, void* loss, void* rewards,
                     void* coef, void* workspace, size_t workspace_bytes, void* stream) {
-  const int rc = check_preference(dtype, args);
-  if (rc) return rc;
-  if (!loss || !rewards || !coef)
-    return report_error(TISO_ERR_ARGUMENT, "loss, rewards and coef must not be NULL");
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7) ||
-      workspace_bytes < static_cast<size_t>(args->pairs) * 4 * sizeof(double))
-    return report_error(TISO_ERR_WORKSPACE, "workspace missing, unaligned or smaller than "
-                                            "tiso_preference_workspace_size");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == TISO_F32 ? run_preference<float>(args, loss, rewards, coef, workspace, st)
-                           : run_preference<double>(args, loss, rewards, coef, workspace, st);
+  return guarded([&]() -> int {
+    const int rc = check_preference(dtype, args);
+    if (rc) return rc;
+    if (!loss || !rewards || !coef)
+      return report_error(TISO_ERR_ARGUMENT, "loss, rewards and coef must not be NULL");
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7) ||
+        workspace_bytes < static_cast<size_t>(args->pairs) * 4 * sizeof(double))
+      return report_error(TISO_ERR_WORKSPACE, "workspace missing, unaligned or smaller than "
+                                              "tiso_preference_workspace_size");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == TISO_F32 ? run_preference<float>(args, loss, rewards, coef, workspace, st)
+                             : run_preference<double>(args, loss, rewards, coef, workspace, st);
+  });
 }
 
 int tiso_preference_grad(int dtype, const tiso_preference_args* args, const void* coef,
                          const void* upstream, void* grad, void* grad_ref, void* stream) {
-  const int rc = check_preference(dtype, args);
-  if (rc) return rc;
-  if (!coef || !upstream)
-    return report_error(TISO_ERR_ARGUMENT, "coef and upstream must not be NULL");
-  if (args->tokens == 0 || (!grad && !grad_ref)) return TISO_OK;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == TISO_F32
-             ? run_preference_grad<float>(args, coef, upstream, grad, grad_ref, st)
-             : run_preference_grad<double>(args, coef, upstream, grad, grad_ref, st);
+  return guarded([&]() -> int {
+    const int rc = check_preference(dtype, args);
+    if (rc) return rc;
+    if (!coef || !upstream)
+      return report_error(TISO_ERR_ARGUMENT, "coef and upstream must not be NULL");
+    if (args->tokens == 0 || (!grad && !grad_ref)) return TISO_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == TISO_F32
+               ? run_preference_grad<float>(args, coef, upstream, grad, grad_ref, st)
+               : run_preference_grad<double>(args, coef, upstream, grad, grad_ref, st);
+  });
 }
 
 }  // extern "C"

@@ -114,6 +114,8 @@ def adamw_step(
     fields = zip(at[:count], at[count:2 * count], at[2 * count:3 * count],
                  at[3 * count:4 * count], *((at[4 * count:5 * count], at[5 * count:])
                                             if bits == 8 else none), sizes[:count], range(count))
+    # autograd's check of saved tensors sees the change
+    torch.autograd.graph.increment_version(tensors[:count] + tensors[2 * count:])
     args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
     if kinds.count(kinds[0]) == count:
         _ext.adamw(params[0].device, *kinds[0], bits, chain.from_iterable(fields), args)
