@@ -37,8 +37,9 @@ struct Rows {
 
 template <typename T>
 __device__ __forceinline__ const T* row_at(const Rows& a, int64_t r) {
-  return static_cast<const T*>(a.x) + (r / a.inner) * a.outer_stride +
-         (r % a.inner) * a.inner_stride;
+  const T* x = static_cast<const T*>(a.x);
+  if (r < a.inner) return x + r * a.inner_stride;  // one stride: no division
+  return x + (r / a.inner) * a.outer_stride + (r % a.inner) * a.inner_stride;
 }
 
 // Who works on a row: a warp (kThreads 32; kRowWarps rows to a CTA), a CTA, or a cluster of CTAs
@@ -326,11 +327,14 @@ struct PolicyArgs {
 
 template <typename A>
 __device__ __forceinline__ A weight_of(const Rows& a, const PolicyArgs<A>& p, int64_t r) {
-  if (a.targets[r] == a.ignore) return A(0);
-  if (p.weight_kind == kNoWeight) return A(1);
-  if (p.weight_kind == kByteWeight)
-    return static_cast<const uint8_t*>(p.weight)[r] ? A(1) : A(0);
-  return static_cast<const A*>(p.weight)[r];
+  const int64_t target = a.targets[r];  // both loads in flight together
+  A w = A(1);
+  if (p.weight_kind == kByteWeight) {
+    w = static_cast<const uint8_t*>(p.weight)[r] ? A(1) : A(0);
+  } else if (p.weight_kind == kAccWeight) {
+    w = static_cast<const A*>(p.weight)[r];
+  }
+  return target == a.ignore ? A(0) : w;
 }
 
 // The sum of v over the CTA in a fixed order (thread 0 has it).
@@ -355,71 +359,76 @@ __global__ void __launch_bounds__(1024) policy_total_kernel(Rows a, PolicyArgs<A
   if (threadIdx.x == 0) *p.total = sum;
 }
 
-// The loss of one token and its slope d loss / d logp (both without the token's weight):
-//   rho = exp(logp - old);  loss = -min(rho A, clip(rho) A) + kl_coef kl,
-//   kl = exp(d) - d - 1, d = ref - logp;
-//   slope = -rho A where rho A <= clip(rho) A, else 0, plus kl_coef (1 - exp(d)).
-struct Token {
-  double loss, slope, kl;
-  bool clipped;
-
-  template <typename A>
-  __device__ __forceinline__ Token(double lp, double old, double ref, double adv,
-                                   const PolicyArgs<A>& p) {
-    const double ratio = exp(lp - old);
-    const double free_side = ratio * adv;
-    const double held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * adv;
-    clipped = free_side > held;
-    loss = -(clipped ? held : free_side);
-    slope = clipped ? 0.0 : -free_side;
-    kl = 0.0;
-    if (p.ref_logps) {
-      const double d = ref - lp;
-      const double e = expm1(d);
-      kl = e - d;
-      loss += p.kl_coef * kl;
-      slope -= p.kl_coef * e;
-    }
-  }
-};
-
 // What the policy loss needs of a token beside its row.
 template <typename A>
 struct TokenInput {
   int64_t target;
   A w, old, adv, ref, logit;
+  double total;  // of the weights
 
-  template <typename T>
-  __device__ __forceinline__ void read(const Rows& a, const PolicyArgs<A>& p, int64_t r, const T* x) {
+  __device__ __forceinline__ void read(const Rows& a, const PolicyArgs<A>& p, int64_t r,
+                                       A logit_) {
     target = a.targets[r];
     old = p.old_logps[r];
     adv = p.advantages[r];
     ref = p.ref_logps ? p.ref_logps[r] : A(0);
-    logit = target_logit<T, A>(x, a.vocab, target);
+    logit = logit_;
+    total = *p.total;
   }
 };
 
-// From a row's sum to the token's coefficient, d loss / d logp; `first` writes the token's results.
+// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest).
+__device__ __forceinline__ float exp_as(float, double d) {
+  const float hi = static_cast<float>(d);
+  const float lo = static_cast<double>(hi) == d ? 0.0f : static_cast<float>(d - hi);
+  const float e = expf(hi);
+  return __fmaf_rn(e, lo, e);
+}
+__device__ __forceinline__ double exp_as(double, double d) { return exp(d); }
+
+// A token's loss and its slope d loss / d logp (both without the token's weight):
+//   rho = exp(logp - old);  loss = -min(rho A, clip(rho) A) + kl_coef kl,
+//   kl = exp(d) - d - 1, d = ref - logp;
+//   slope = -rho A where rho A <= clip(rho) A, else 0, plus kl_coef (1 - exp(d)).
+// With t = (x - base) / temperature at the target and s the row's sum, logp = t - log s, so that
+// rho = exp(t - old) / s and exp(d) = exp(ref - t) s: the slope, which a row's gradient waits for,
+// needs no logarithm. t is in double: rounding it near 10 would be the largest error of all.
 template <typename A>
-__device__ __forceinline__ double token_coef(const PolicyArgs<A>& p, int64_t r,
-                                             const TokenInput<A>& t, const Part<A>& part,
-                                             double inv_temp, bool first) {
-  const double total = *p.total;
-  const double share = total != 0 ? t.w / total : 0.0;
-  const double lp = logp_of(t.logit, part, inv_temp);
-  const Token token(lp, t.old, t.ref, t.adv, p);
-  const double coef = total != 0 ? share * token.slope : 0.0;
-  if (first) {
+struct Token {
+  double t, ratio, free_side, held;
+  double coef;  // d loss / d logp with the weight's share
+
+  __device__ __forceinline__ Token(const PolicyArgs<A>& p, const TokenInput<A>& in,
+                                   const Part<A>& part, double inv_temp) {
+    t = (static_cast<double>(in.logit) - static_cast<double>(base_of(part.m))) * inv_temp;
+    ratio = exp_as(A(0), t - static_cast<double>(in.old)) / part.s;
+    free_side = ratio * static_cast<double>(in.adv);
+    held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * static_cast<double>(in.adv);
+    double slope = free_side > held ? 0.0 : -free_side;
+    if (p.ref_logps)
+      slope += p.kl_coef * (1.0 - static_cast<double>(
+                                      exp_as(A(0), static_cast<double>(in.ref) - t) * part.s));
+    coef = in.total != 0 ? static_cast<double>(in.w) / in.total * slope : 0.0;
+  }
+
+  __device__ __forceinline__ void write(const PolicyArgs<A>& p, int64_t r, const TokenInput<A>& in,
+                                        const Part<A>& part) const {
+    const double lp = t - log(static_cast<double>(part.s));
+    double loss = -(free_side > held ? held : free_side), kl = 0.0;
+    if (p.ref_logps) {
+      const double d = static_cast<double>(in.ref) - lp;
+      kl = expm1(d) - d;
+      loss += p.kl_coef * kl;
+    }
     p.logps[r] = static_cast<A>(lp);
     p.coef[r] = coef;
     p.stats[2 * r] = base_of(part.m);
     p.stats[2 * r + 1] = part.s;
-    p.terms[3 * r] = static_cast<A>(t.w * token.loss);
-    p.terms[3 * r + 1] = static_cast<A>(t.w * token.kl);
-    p.terms[3 * r + 2] = token.clipped ? t.w : A(0);
+    p.terms[3 * r] = static_cast<A>(in.w * loss);
+    p.terms[3 * r + 1] = static_cast<A>(in.w * kl);
+    p.terms[3 * r + 2] = free_side > held ? in.w : A(0);
   }
-  return coef;
-}
+};
 
 // The row's cut is as for a gradient in a buffer on a vector's boundary, also where no gradient is
 // written (grad NULL): the loss is the same bits.
@@ -461,11 +470,12 @@ __global__ void __launch_bounds__(32 * kRowWarps)
     leave_out(p, place, view, grad != nullptr);
     return;
   }
-  token.read(a, p, r, view.x);
+  token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
   const Part<A> part = warp_part(view, place, k);
-  const double coef = token_coef(p, r, token, part, inv_temp, place.first());
+  const Token<A> result(p, token, part, inv_temp);
+  if (place.first()) result.write(p, r, token, part);
   if (!grad) return;
-  const Slope<A> slope(base_of(part.m), part.s, coef * inv_temp, k, token.target, a.vocab);
+  const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
   write_edge(view, place.edge(), slope);
   for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
     write_tile<32>(view, tile, place.tid, slope);
@@ -484,13 +494,12 @@ template <typename T, typename A>
 __global__ void __launch_bounds__(kPolicyThreads, 3)
     policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
   extern __shared__ uint4 stages[];  // [kStages][kPolicyTile]
-  __shared__ double of_warp_0;
+  __shared__ TokenInput<A> token;    // read after the join's barrier
   const Place<kPolicyThreads> place;
   const int64_t r = place.row;
   const RowView<T> view = policy_view(a, r, grad);
-  TokenInput<A> token;
-  token.w = weight_of(a, p, r);
-  if (token.w == A(0)) {
+  const A w = weight_of(a, p, r);
+  if (w == A(0)) {
     leave_out(p, place, view, grad != nullptr);
     return;
   }
@@ -518,9 +527,10 @@ __global__ void __launch_bounds__(kPolicyThreads, 3)
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) copy(j);
-  token.target = a.targets[r];
-  const bool steps = place.tid < 32;  // this warp goes on from the sum
-  if (steps) token.read(a, p, r, view.x);
+  if (place.tid == 0) {
+    token.w = w;
+    token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
+  }
 
   // the tiles that are loaded directly, and the single elements
   const int rest = whole + (place.cta - whole % place.ctas + place.ctas) % place.ctas;
@@ -532,13 +542,11 @@ __global__ void __launch_bounds__(kPolicyThreads, 3)
     add_vectors<T>(part, q, k);
   }
   part = join_warps<kPolicyThreads>(join_lanes<32>(part, k), k);
-  if (steps) {
-    const double coef = token_coef(p, r, token, part, inv_temp, place.first());
-    if (place.tid == 0) of_warp_0 = coef;
-  }
+  // every warp takes the few steps to the coefficient by itself: one more barrier takes longer
+  const Token<A> result(p, token, part, inv_temp);
+  if (place.first()) result.write(p, r, token, part);
   if (!grad) return;
-  __syncthreads();
-  const Slope<A> slope(base_of(part.m), part.s, of_warp_0 * inv_temp, k, token.target, a.vocab);
+  const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
   for (int j = mine - 1; j >= 0; --j) {
     uint4 q[kBatch];
     fetch(j, q);

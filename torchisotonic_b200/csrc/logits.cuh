@@ -100,16 +100,6 @@ struct Part {
   A m, s;
 };
 
-template <typename A>
-__device__ __forceinline__ Part<A> join(const Part<A>& a, const Part<A>& b, A k) {
-  const A m = max_acc(a.m, b.m);
-  const A base = base_of(m);
-  // a part that holds the maximum keeps its sum as it is (its exponent is exactly 0); no
-  // contraction, so that join(a, b) and join(b, a) are the same bits
-  return {m, add_rn(mul_rn(a.s, scaled_exp(a.m == m ? A(0) : a.m - base, k)),
-                    mul_rn(b.s, scaled_exp(b.m == m ? A(0) : b.m - base, k)))};
-}
-
 // ---------------------------------------------------------------------------------------------
 // A row in 16-byte vectors. Rows start anywhere (an odd vocabulary, a cut tensor), so a row is a
 // body of whole vectors and at most 4 E - 1 single elements around it (E to a vector). The body is
@@ -371,15 +361,35 @@ __device__ __forceinline__ void wait_groups() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kOpen) : "memory");
 }
 
-// The parts of kLanes neighbouring lanes joined (each lane gets the result).
-template <int kLanes, typename A>
-__device__ __forceinline__ Part<A> join_lanes(Part<A> p, A k) {
+// The parts of kLanes neighbouring lanes joined: the same bits in each of them (sums pair by pair
+// do not depend on the order of the two).
+template <int kLanes>
+__device__ __forceinline__ float max_of_lanes(float m) {
+  if constexpr (kLanes == 32) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(m));
+    return r;
+  } else {
 #pragma unroll
-  for (int d = kLanes / 2; d; d >>= 1) {
-    const Part<A> q{__shfl_xor_sync(0xffffffffu, p.m, d), __shfl_xor_sync(0xffffffffu, p.s, d)};
-    p = join(p, q, k);
+    for (int d = kLanes / 2; d; d >>= 1) m = max_acc(m, __shfl_xor_sync(0xffffffffu, m, d));
+    return m;
   }
-  return p;
+}
+template <int kLanes>
+__device__ __forceinline__ double max_of_lanes(double m) {
+#pragma unroll
+  for (int d = kLanes / 2; d; d >>= 1) m = max_acc(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+
+template <int kLanes, typename A>
+__device__ __forceinline__ Part<A> join_lanes(const Part<A>& p, A k) {
+  const A m = max_of_lanes<kLanes>(p.m);
+  // a part that holds the maximum keeps its sum as it is
+  A s = p.m == m ? p.s : mul_rn(p.s, scaled_exp(p.m - base_of(m), k));
+#pragma unroll
+  for (int d = kLanes / 2; d; d >>= 1) s = add_rn(s, __shfl_xor_sync(0xffffffffu, s, d));
+  return {m, s};
 }
 
 }  // namespace tiso
