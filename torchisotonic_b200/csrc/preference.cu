@@ -6,6 +6,7 @@
 //   u_i = beta (s_i - s_{P+i}) - margin,  loss = mean of l(u_i),
 //   d loss / d logp_t = +-beta l'(u) / P (1 / count with `average`), + for chosen.
 // Sums are double, in a fixed order.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <string>
@@ -13,10 +14,11 @@
 #include "entry.cuh"
 
 namespace tiso {
-
 namespace {
 
-constexpr int kThreads = 256;
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256, kManyThreads = 1024;
 
 template <typename A>
 struct PrefArgs {
@@ -46,22 +48,55 @@ __device__ double block_sum(double v, double* shared) {
   return v;
 }
 
-// A CTA per sequence: the sum and number of its unmasked tokens. A masked token is not used in
-// any way (its value may be NaN).
-template <typename A>
-__global__ void __launch_bounds__(kThreads) pref_sum_kernel(PrefArgs<A> a) {
-  __shared__ double shared[32];
-  const int64_t k = blockIdx.x;
+// A cluster of CTAs (one, where there are many sequences) to a sequence: the sum and number of its
+// unmasked tokens. A masked token is read but not used in any way (its value may be NaN).
+template <typename A, int kT>
+__global__ void __launch_bounds__(kT) pref_sum_kernel(PrefArgs<A> a) {
+  constexpr int kAhead = 4, kMostCtas = 8;
+  __shared__ double shared[32], sums[kMostCtas], counts[kMostCtas];
+  auto cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int64_t k = blockIdx.x / ctas;
   const int64_t begin = cut(a.offsets[k], 0, a.tokens);
   const int64_t end = cut(a.offsets[k + 1], begin, a.tokens);
+  const int64_t step = static_cast<int64_t>(ctas) * kT;
   double sum = 0, count = 0;
-  for (int64_t t = begin + threadIdx.x; t < end; t += kThreads) {
-    if (a.mask && !a.mask[t]) continue;
-    sum += static_cast<double>(a.logps[t]) - (a.refs ? static_cast<double>(a.refs[t]) : 0.0);
-    count += 1;
+  for (int64_t t = begin + rank * kT + threadIdx.x; t < end; t += kAhead * step) {
+    A x[kAhead], ref[kAhead];
+    bool used[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t u = t + i * step;
+      used[i] = u < end;
+      x[i] = ref[i] = A(0);
+      if (u < end) {
+        if (a.mask) used[i] = a.mask[u] != 0;
+        x[i] = a.logps[u];
+        if (a.refs) ref[i] = a.refs[u];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      sum += used[i] ? static_cast<double>(x[i]) - static_cast<double>(ref[i]) : 0.0;
+      count += used[i] ? 1.0 : 0.0;
+    }
   }
   sum = block_sum(sum, shared);
   count = block_sum(count, shared);
+  if (ctas > 1) {
+    if (threadIdx.x == 0) {
+      *cluster.map_shared_rank(&sums[rank], 0) = sum;
+      *cluster.map_shared_rank(&counts[rank], 0) = count;
+    }
+    cluster.sync();
+    if (rank != 0) return;
+    sum = count = 0;
+    for (int i = 0; i < ctas; ++i) {
+      sum += sums[i];
+      count += counts[i];
+    }
+  }
   if (threadIdx.x == 0) {
     a.sums[k] = sum;
     a.counts[k] = count;
@@ -115,28 +150,50 @@ __global__ void __launch_bounds__(kThreads) pref_pair_kernel(PrefArgs<A> a) {
   if (threadIdx.x == 0) *a.loss = static_cast<A>(total / static_cast<double>(a.pairs));
 }
 
-// A token's sequence by a binary search: the last k with offsets[k] <= t. Tokens of no sequence
-// and masked ones get 0.
+// A thread takes 4 tokens in a row: the first one's sequence by a binary search (the last k with
+// offsets[k] <= t), the others' from there on. Tokens of no sequence and masked ones get 0.
+constexpr int kEach = 4;
+
 template <typename A>
 __global__ void __launch_bounds__(kThreads)
     pref_grad_kernel(const uint8_t* mask, const int64_t* offsets, int64_t tokens, int64_t sequences,
-                     const A* coef, const A* upstream, A* grad, A* grad_ref) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (t >= tokens) return;
-  int64_t lo = 0, hi = sequences + 1;  // offsets[lo - 1] <= t < offsets[hi], as if -inf and inf
+                     const A* coef, const A* upstream, A* grad, A* grad_ref, bool aligned) {
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * kEach;
+  if (first >= tokens) return;
+  const A up = *upstream;
+  int64_t lo = 0, hi = sequences + 1;  // offsets[lo - 1] <= first < offsets[hi], as if -inf and inf
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if (offsets[mid] <= t) {
+    if (offsets[mid] <= first) {
       lo = mid + 1;
     } else {
       hi = mid;
     }
   }
-  const int64_t k = lo - 1;
-  A g = A(0);
-  if (k >= 0 && k < sequences && (!mask || mask[t])) g = coef[k] * *upstream;
-  if (grad) grad[t] = g;
-  if (grad_ref) grad_ref[t] = -g;
+  A g[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t t = first + i;
+    g[i] = A(0);
+    if (t < tokens) {
+      while (lo <= sequences && offsets[lo] <= t) ++lo;
+      if (lo > 0 && lo <= sequences && (!mask || mask[t])) g[i] = coef[lo - 1] * up;
+    }
+  }
+  struct alignas(kEach * sizeof(A) < 16 ? kEach * sizeof(A) : 16) Four {
+    A x[kEach];
+  };
+  if (aligned && first + kEach <= tokens) {
+    if (grad) *reinterpret_cast<Four*>(grad + first) = Four{{g[0], g[1], g[2], g[3]}};
+    if (grad_ref) *reinterpret_cast<Four*>(grad_ref + first) = Four{{-g[0], -g[1], -g[2], -g[3]}};
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (first + i >= tokens) break;
+      if (grad) grad[first + i] = g[i];
+      if (grad_ref) grad_ref[first + i] = -g[i];
+    }
+  }
 }
 
 int pref_launched(const char* what) {
@@ -166,7 +223,31 @@ int run_preference(const tiso_preference_args* q, void* loss, void* rewards, voi
   a.loss = static_cast<A*>(loss);
   a.rewards = static_cast<A*>(rewards);
   a.coef = static_cast<A*>(coef);
-  pref_sum_kernel<A><<<static_cast<unsigned>(2 * q->pairs), kThreads, 0, st>>>(a);
+  // more CTAs, then larger ones, to a sequence while there are few of them and each has over 4096
+  // tokens to read (two answers of 670,000 tokens: 1028 us with one CTA of 256 threads each, 102 with
+  // 8 of them, 36 with 8 of 1024)
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int ctas = 1;
+  while (ctas < 8 && 2 * q->pairs * ctas < 2 * sms && q->tokens > 2 * q->pairs * ctas * 4096)
+    ctas *= 2;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(2 * q->pairs * ctas));
+  const bool many = ctas == 8 && q->tokens > 2 * q->pairs * ctas * 4096;
+  config.blockDim = dim3(many ? kManyThreads : kThreads);
+  config.stream = st;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(
+      &config, many ? pref_sum_kernel<A, kManyThreads> : pref_sum_kernel<A, kThreads>, a);
+  if (e != cudaSuccess)
+    return report_error(TISO_ERR_CUDA,
+                        std::string("pref_sum_kernel launch: ") + cudaGetErrorString(e));
   pref_pair_kernel<A><<<1, kThreads, 0, st>>>(a);
   return pref_launched("preference kernels launch");
 }
@@ -174,10 +255,12 @@ int run_preference(const tiso_preference_args* q, void* loss, void* rewards, voi
 template <typename A>
 int run_preference_grad(const tiso_preference_args* q, const void* coef, const void* upstream,
                         void* grad, void* grad_ref, cudaStream_t st) {
-  pref_grad_kernel<A><<<static_cast<unsigned>((q->tokens + kThreads - 1) / kThreads), kThreads, 0,
-                        st>>>(q->mask, q->offsets, q->tokens, 2 * q->pairs,
-                              static_cast<const A*>(coef), static_cast<const A*>(upstream),
-                              static_cast<A*>(grad), static_cast<A*>(grad_ref));
+  const int64_t ctas = (q->tokens + kThreads * kEach - 1) / (kThreads * kEach);
+  const bool aligned =
+      ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(grad_ref)) & 15) == 0;
+  pref_grad_kernel<A><<<static_cast<unsigned>(ctas), kThreads, 0, st>>>(
+      q->mask, q->offsets, q->tokens, 2 * q->pairs, static_cast<const A*>(coef),
+      static_cast<const A*>(upstream), static_cast<A*>(grad), static_cast<A*>(grad_ref), aligned);
   return pref_launched("pref_grad_kernel launch");
 }
 
