@@ -13,8 +13,6 @@ import contextlib
 import ctypes
 import functools
 import threading
-from array import array
-from collections.abc import Iterable
 from pathlib import Path
 
 import torch
@@ -552,171 +550,20 @@ def isotonic_grad_varlen(
 # ---------------------------------------------------------------------------------------------
 # Language-model operators
 
+NATIVE_PATH = Path(__file__).resolve().parent / "_native.so"
 PREFERENCE_KINDS = {"logistic": 0, "hinge": 1, "square": 2}
 
 
-def _stream(device: torch.device) -> int:
-    # the handle alone: building torch.cuda.current_stream's object takes 2 us
-    return torch._C._cuda_getCurrentRawStream(device.index)
+@functools.cache
+def native():
+    """The extension module over the same library that the losses and the optimizer step are called
+    through (csrc/native.cpp), loaded once. Raises if it was not built."""
+    if not NATIVE_PATH.exists():
+        raise RuntimeError(
+            f"{NATIVE_PATH} is missing: build it with `python -m torchisotonic_b200.build` "
+            "(torchisotonic_b200 has no CPU fallback)"
+        )
+    lib()
+    from torchisotonic_b200 import _native
 
-
-@functools.lru_cache(maxsize=256)
-def _size(query_name: str, *args: int) -> int:
-    """A workspace query's answer."""
-    size = ctypes.c_size_t(0)
-    _check(getattr(lib(), query_name)(*args, ctypes.byref(size)))
-    return size.value
-
-
-def logits_rows(x: Tensor) -> tuple[Tensor, Rows]:
-    """``x`` ([..., vocab], CUDA) as rows of logits, and the tensor whose memory they are: x itself
-    when its last dimension is contiguous and the leading ones reduce to two strides (a contiguous
-    tensor, a cut or padded one), else a contiguous copy."""
-    if not x.is_cuda:
-        raise RuntimeError("logits must be a CUDA tensor: torchisotonic_b200 has no CPU path")
-    if x.dtype not in _DTYPES:
-        raise RuntimeError("logits must be float16, bfloat16, float32 or float64")
-    shape = x.shape
-    vocab = shape[-1]
-    if x.is_contiguous():
-        rows = x.numel() // vocab
-        return x, Rows(x.data_ptr(), rows, max(rows, 1), 0, vocab, vocab)
-    stride = x.stride()
-    if stride[-1] == 1 or vocab == 1:
-        if len(shape) == 1:
-            return x, Rows(x.data_ptr(), 1, 1, 0, 0, vocab)
-        if len(shape) == 2:
-            return x, Rows(x.data_ptr(), shape[0], max(shape[0], 1), 0, stride[0], vocab)
-        if len(shape) == 3:
-            return x, Rows(x.data_ptr(), shape[0] * shape[1], max(shape[1], 1), stride[0],
-                           stride[1], vocab)
-    return logits_rows(x.contiguous())
-
-
-def logprobs(x: Tensor, targets: Tensor, ignore_index: int, temperature: float,
-             with_stats: bool) -> tuple[Tensor, Tensor | None]:
-    """log softmax(x / temperature) at the targets (int64, contiguous, one per row of logits), in
-    the accumulation dtype and the targets' shape, and with ``with_stats`` what logprobs_grad
-    needs (each row's maximum and sum of exponentials)."""
-    x, rows = logits_rows(x)
-    dev, acc = x.device, acc_dtype(x.dtype)
-    out = x.new_empty(targets.shape, dtype=acc)
-    stats = x.new_empty(2 * rows.rows, dtype=acc) if with_stats else None
-    with _on(dev):
-        _check(lib().tiso_logprobs(_DTYPES[x.dtype], rows, targets.data_ptr(), ignore_index,
-                                   temperature, out.data_ptr(), _ptr(stats), _stream(dev)))
-    return out, stats
-
-
-def logprobs_grad(x: Tensor, targets: Tensor, temperature: float, stats: Tensor,
-                  coef: Tensor) -> Tensor:
-    """The gradient of sum(coef * logprobs) in x, in its dtype and shape, contiguous. ``coef``:
-    contiguous, one per row, in the accumulation dtype."""
-    x, rows = logits_rows(x)
-    dev = x.device
-    grad = torch.empty_like(x, memory_format=torch.contiguous_format)
-    with _on(dev):
-        _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
-                                        stats.data_ptr(), _DTYPES[coef.dtype], coef.data_ptr(),
-                                        None, grad.data_ptr(), _stream(dev)))
-    return grad
-
-
-def policy(x: Tensor, targets: Tensor, ignore_index: int, temperature: float, old_logps: Tensor,
-           advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None, clip_low: float,
-           clip_high: float, kl_coef: float, with_grad: bool
-           ) -> tuple[tuple[Tensor, ...], Tensor, Tensor, Tensor | None]:
-    """The clipped policy loss of tiso_policy: ((loss, kl, clip fraction), logps, what
-    policy_grad needs, grad or None). The per-token tensors are contiguous, one number per row of
-    logits, in the accumulation dtype (``weight`` may be bool, ``targets`` is int64)."""
-    x, rows = logits_rows(x)
-    dev, acc = x.device, acc_dtype(x.dtype)
-    dtype, n = _DTYPES[x.dtype], rows.rows
-    logps = x.new_empty(targets.shape, dtype=acc)
-    out = x.new_empty(3, dtype=acc)
-    grad = torch.empty_like(x, memory_format=torch.contiguous_format) if with_grad else None
-    args = PolicyArgs(old_logps.data_ptr(), _ptr(ref_logps), advantages.data_ptr(), _ptr(weight),
-                      int(weight is not None and weight.dtype == torch.bool), clip_low, clip_high,
-                      kl_coef)
-    size = _size("tiso_policy_workspace_size", dtype, n)
-    # n numbers coef, up to 2 n stats, the workspace: one allocation
-    kept = x.new_empty(3 * n + -(-size // 8), dtype=torch.float64)
-    at = kept.data_ptr()
-    with _on(dev):
-        _check(lib().tiso_policy(dtype, rows, targets.data_ptr(), ignore_index, temperature, args,
-                                 logps.data_ptr(), at, at + 8 * n, out.data_ptr(), _ptr(grad),
-                                 at + 24 * n, size, _stream(dev)))
-    return out.unbind(), logps, kept, grad
-
-
-def policy_grad(x: Tensor, targets: Tensor, temperature: float, kept: Tensor, upstream: Tensor,
-                grad: Tensor | None) -> Tensor:
-    """The policy loss's gradient in x times ``upstream`` (a scalar tensor). ``grad``: what policy
-    wrote, the gradient for upstream = 1, overwritten unless it is; or None for a new tensor."""
-    x, rows = logits_rows(x)
-    dev, n = x.device, rows.rows
-    coef, once = kept, upstream
-    if grad is None:
-        grad = torch.empty_like(x, memory_format=torch.contiguous_format)
-        coef, once = kept[:n] * upstream, None
-    with _on(dev):
-        _check(lib().tiso_logprobs_grad(_DTYPES[x.dtype], rows, targets.data_ptr(), temperature,
-                                        kept.data_ptr() + 8 * n, F64, coef.data_ptr(), _ptr(once),
-                                        grad.data_ptr(), _stream(dev)))
-    return grad
-
-
-def _preference_args(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor,
-                     kind: int, average: bool, beta: float, label_smoothing: float,
-                     margin: float) -> PreferenceArgs:
-    return PreferenceArgs(logps.data_ptr(), _ptr(refs), _ptr(mask), offsets.data_ptr(),
-                          logps.numel(), (offsets.numel() - 1) // 2, kind, average, beta,
-                          label_smoothing, margin)
-
-
-def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor,
-               kind: int, average: bool, beta: float, label_smoothing: float,
-               margin: float) -> tuple[Tensor, Tensor, Tensor]:
-    """The preference loss of tiso_preference: (loss, rewards [2, pairs], coef [2 pairs]) from
-    contiguous 1-D logps and refs (float32 or float64), mask (bool) and offsets (int64)."""
-    args = _preference_args(logps, refs, mask, offsets, kind, average, beta, label_smoothing,
-                            margin)
-    dev, pairs = logps.device, args.pairs
-    loss = logps.new_empty(())
-    rewards = logps.new_empty((2, pairs))
-    # coef and, behind it, the workspace: one allocation
-    size = _size("tiso_preference_workspace_size", pairs)
-    each = logps.element_size()
-    first = -(-2 * pairs * each // 8) * 8
-    coef = logps.new_empty((first + size) // each)
-    with _on(dev):
-        _check(lib().tiso_preference(_DTYPES[logps.dtype], args, loss.data_ptr(),
-                                     rewards.data_ptr(), coef.data_ptr(), coef.data_ptr() + first,
-                                     size, _stream(dev)))
-    return loss, rewards, coef
-
-
-def preference_grad(logps: Tensor, mask: Tensor | None, offsets: Tensor, coef: Tensor,
-                    upstream: Tensor, want: bool, want_ref: bool
-                    ) -> tuple[Tensor | None, Tensor | None]:
-    """Every token's gradient in logps and in ref_logps from its sequence's coef and the loss's
-    upstream gradient (a device scalar)."""
-    args = _preference_args(logps, None, mask, offsets, 0, False, 1.0, 0.0, 0.0)
-    dev = logps.device
-    grad = torch.empty_like(logps) if want else None
-    grad_ref = torch.empty_like(logps) if want_ref else None
-    with _on(dev):
-        _check(lib().tiso_preference_grad(_DTYPES[logps.dtype], args, coef.data_ptr(),
-                                          upstream.data_ptr(), _ptr(grad), _ptr(grad_ref),
-                                          _stream(dev)))
-    return grad, grad_ref
-
-
-def adamw(device: torch.device, param_dtype: torch.dtype, grad_dtype: torch.dtype, bits: int,
-          fields: Iterable[int], args: AdamwArgs) -> None:
-    """One tiso_adamw call: ``fields`` the tensors' tiso_adamw_tensor structures, 8 numbers each,
-    back to back (pointers of param, grad, exp_avg, exp_avg_sq and the two scales, n, index)."""
-    table = array("q", fields)
-    with _on(device):
-        _check(lib().tiso_adamw(_DTYPES[param_dtype], _DTYPES[grad_dtype], bits, len(table) // 8,
-                                table.buffer_info()[0], args, _stream(device)))
+    return _native

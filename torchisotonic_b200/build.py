@@ -1,4 +1,6 @@
-"""Builds torchisotonic_b200/libtiso.so: the CUDA kernels behind include/tiso.h, for sm_100a.
+"""Builds torchisotonic_b200/libtiso.so: the CUDA kernels behind include/tiso.h, for sm_100a; and
+torchisotonic_b200/_native.so, the extension module over it that the losses and the optimizer step
+are called through.
 
     python -m torchisotonic_b200.build [--verbose]
 
@@ -11,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,6 +21,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtiso.so"
 SOURCES = [CSRC / f for f in ("tiso.cu", "calib.cu", "logits.cu", "preference.cu", "adamw.cu")]
+NATIVE, NATIVE_SOURCE = PKG / "_native.so", CSRC / "native.cpp"
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "tiso.h"]
 
 NVCC_FLAGS = [
@@ -35,22 +39,38 @@ def nvcc() -> str:
     return str(path) if path.exists() else (shutil.which("nvcc") or "nvcc")
 
 
-def stale() -> bool:
-    if not LIB.exists():
-        return True
-    built = LIB.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in DEPS)
+def stale(built: Path = LIB, deps: list[Path] = DEPS) -> bool:
+    return not built.exists() or any(p.stat().st_mtime > built.stat().st_mtime for p in deps)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not stale():
-        return LIB
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []),
-           "-o", str(tmp), *map(str, SOURCES), "-lcudart"]
-    subprocess.run(cmd, check=True, cwd=str(ROOT))
-    tmp.replace(LIB)
+    if force or stale():
+        tmp = LIB.with_suffix(".so.tmp")
+        cmd = [nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []),
+               "-o", str(tmp), *map(str, SOURCES), "-lcudart"]
+        subprocess.run(cmd, check=True, cwd=str(ROOT))
+        tmp.replace(LIB)
+    build_native(force)
     return LIB
+
+
+def build_native(force: bool = False) -> Path:
+    """The extension module, against this interpreter's torch; it finds libtiso.so beside itself."""
+    if not force and not stale(NATIVE, [NATIVE_SOURCE, ROOT / "include" / "tiso.h"]):
+        return NATIVE
+    from torch.utils import cpp_extension
+
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    includes = [*cpp_extension.include_paths(), f"{cuda}/include", sysconfig.get_path("include")]
+    tmp = NATIVE.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           *(f"-I{p}" for p in includes), str(NATIVE_SOURCE), "-o", str(tmp),
+           *(f"-L{p}" for p in cpp_extension.library_paths()), f"-L{PKG}",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-l:libtiso.so",
+           "-Wl,-rpath,$ORIGIN"]
+    subprocess.run(cmd, check=True, cwd=str(ROOT))
+    tmp.replace(NATIVE)
+    return NATIVE
 
 
 if __name__ == "__main__":

@@ -9,11 +9,10 @@ tensors only, float16 and bfloat16 computed in float32, float64 kept, rows packe
 
 from __future__ import annotations
 
-from typing import Any, NamedTuple
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from torchisotonic_b200 import _ext, ops
 
@@ -49,23 +48,6 @@ def _check_logits(logits: Tensor, targets: Tensor, temperature: float) -> None:
         raise ValueError("targets must be on logits' device")
 
 
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, logits: Tensor, targets: Tensor, temperature: float,
-                ignore_index: int) -> Tensor:
-        out, stats = _ext.logprobs(logits, targets, ignore_index, temperature, True)
-        ctx.save_for_backward(logits, targets, stats)
-        ctx.temperature = temperature
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad: Tensor) -> tuple[Tensor | None, ...]:
-        logits, targets, stats = ctx.saved_tensors
-        return (_ext.logprobs_grad(logits, targets, ctx.temperature, stats, grad.contiguous()),
-                None, None, None)
-
-
 def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
                    ignore_index: int = -100) -> Tensor:
     """Log-probability of one token per row: ``log softmax(logits / temperature)`` ([..., vocab],
@@ -82,30 +64,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     targets = _as(targets, torch.int64)
     if torch.compiler.is_compiling():  # traced: the operators, which the compiler keeps whole
         return ops.token_logprobs(logits, targets, float(temperature), int(ignore_index))[0]
-    if logits.requires_grad and torch.is_grad_enabled():
-        return _TokenLogprobs.apply(logits, targets, float(temperature), int(ignore_index))
-    return _ext.logprobs(logits, targets, int(ignore_index), float(temperature), False)[0]
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, logps: Tensor, refs: Tensor | None, mask: Tensor | None,
-                offsets: Tensor, settings: tuple[Any, ...]) -> tuple[Tensor, Tensor]:
-        loss, rewards, coef = _ext.preference(logps, refs, mask, offsets, *settings)
-        ctx.save_for_backward(logps, mask, offsets, coef)
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad: Tensor | None, _: Any) -> tuple[Tensor | None, ...]:
-        if grad is None:
-            return None, None, None, None, None
-        want, want_ref = ctx.needs_input_grad[:2]
-        logps, mask, offsets, coef = ctx.saved_tensors
-        return (*_ext.preference_grad(logps, mask, offsets, coef, grad, want, want_ref), None,
-                None, None)
+    return _ext.native().token_logprobs(logits, targets, float(temperature), int(ignore_index))
 
 
 def preference_loss(
@@ -177,8 +136,7 @@ def preference_loss(
     if torch.compiler.is_compiling():
         loss, rewards, _ = ops.preference(logps, ref_logps, mask, offsets, *settings)
         return loss, rewards.detach()
-    loss, rewards = _Preference.apply(logps, ref_logps, mask, offsets, settings)
-    return loss, rewards
+    return _ext.native().preference_loss(logps, ref_logps, mask, offsets, *settings)
 
 
 class PolicyLoss(NamedTuple):
@@ -188,31 +146,6 @@ class PolicyLoss(NamedTuple):
     logps: Tensor
     kl: Tensor
     clip_fraction: Tensor
-
-
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, logits: Tensor, targets: Tensor, temperature: float,
-                run: Any) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-        (loss, kl, clip_fraction), logps, kept, grad = run(True)
-        ctx.save_for_backward(logits, targets, kept)
-        ctx.temperature = temperature
-        ctx.grad = grad
-        ctx.mark_non_differentiable(logps, kl, clip_fraction)
-        ctx.set_materialize_grads(False)
-        return loss, logps, kl, clip_fraction
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, up: Tensor | None, *_: Any) -> tuple[Tensor | None, ...]:
-        if up is None:
-            return None, None, None, None
-        logits, targets, kept = ctx.saved_tensors
-        # the gradient for an upstream gradient of 1, written with the loss, is given away the
-        # first time (the kernel rewrites it unless upstream is 1); later calls write a new one
-        grad, ctx.grad = ctx.grad, None
-        return (_ext.policy_grad(logits, targets, ctx.temperature, kept, up, grad), None, None,
-                None)
 
 
 def policy_loss(
@@ -274,11 +207,5 @@ def policy_loss(
         rest = out.detach()
         return PolicyLoss(out[0], logps.detach(), rest[1], rest[2])
 
-    def run(with_grad: bool) -> tuple[tuple[Tensor, ...], Tensor, Tensor, Tensor | None]:
-        return _ext.policy(logits.detach(), targets, int(ignore_index), temperature, *settings,
-                           with_grad)
-
-    if logits.requires_grad and torch.is_grad_enabled():
-        return PolicyLoss(*_Policy.apply(logits, targets, temperature, run))
-    (loss, kl, clip_fraction), logps, _, _ = run(False)
-    return PolicyLoss(loss, logps, kl, clip_fraction)
+    return PolicyLoss(*_ext.native().policy_loss(logits, targets, int(ignore_index), temperature,
+                                                 *settings))

@@ -148,9 +148,7 @@ torch.library.register_autograd(f"{_NS}::fit", _fit_backward, setup_context=_fit
 @torch.library.custom_op(f"{_NS}::token_logprobs", mutates_args=())
 def token_logprobs(logits: Tensor, targets: Tensor, temperature: float,
                    ignore_index: int) -> tuple[Tensor, Tensor]:
-    out, stats = _ext.logprobs(logits, targets.contiguous(), ignore_index, temperature, True)
-    assert stats is not None
-    return out, stats
+    return _ext.native().logprobs(logits, targets.contiguous(), temperature, ignore_index, True)
 
 
 @token_logprobs.register_fake
@@ -163,7 +161,8 @@ def _(logits, targets, temperature, ignore_index):
 @torch.library.custom_op(f"{_NS}::token_logprobs_grad", mutates_args=())
 def token_logprobs_grad(logits: Tensor, targets: Tensor, temperature: float, stats: Tensor,
                         coef: Tensor) -> Tensor:
-    return _ext.logprobs_grad(logits, targets.contiguous(), temperature, stats, coef.contiguous())
+    return _ext.native().logprobs_grad(logits, targets.contiguous(), temperature, stats,
+                                       coef.contiguous())
 
 
 @token_logprobs_grad.register_fake
@@ -189,8 +188,8 @@ torch.library.register_autograd(f"{_NS}::token_logprobs", _token_logprobs_backwa
 def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor, kind: int,
                average: bool, beta: float, label_smoothing: float,
                margin: float) -> tuple[Tensor, Tensor, Tensor]:
-    loss, rewards, coef = _ext.preference(logps, refs, mask, offsets, kind, average, beta,
-                                          label_smoothing, margin)
+    loss, rewards, coef = _ext.native().preference(logps, refs, mask, offsets, kind, average,
+                                                   beta, label_smoothing, margin)
     return loss, rewards, coef[:rewards.numel()].clone()
 
 
@@ -203,9 +202,7 @@ def _(logps, refs, mask, offsets, kind, average, beta, label_smoothing, margin):
 @torch.library.custom_op(f"{_NS}::preference_grad", mutates_args=())
 def preference_grad(logps: Tensor, mask: Tensor | None, offsets: Tensor, coef: Tensor,
                     upstream: Tensor) -> Tensor:
-    grad, _ = _ext.preference_grad(logps, mask, offsets, coef, upstream, True, False)
-    assert grad is not None
-    return grad
+    return _ext.native().preference_grad(logps, mask, offsets, coef, upstream, True, False)[0]
 
 
 @preference_grad.register_fake
@@ -229,14 +226,20 @@ torch.library.register_autograd(f"{_NS}::preference", _preference_backward,
                                 setup_context=_preference_setup)
 
 
+def _kept(logits: Tensor, targets: Tensor) -> int:
+    """float64 numbers of what policy_grad needs: a coefficient, a maximum and a sum for each token
+    (the last two in the accumulation dtype)."""
+    return targets.numel() * (3 if _acc(logits.dtype) == torch.float64 else 2)
+
+
 @torch.library.custom_op(f"{_NS}::policy", mutates_args=())
 def policy(logits: Tensor, targets: Tensor, ignore_index: int, temperature: float,
            old_logps: Tensor, advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None,
            clip_low: float, clip_high: float, kl_coef: float) -> tuple[Tensor, Tensor, Tensor]:
-    out, logps, kept, _ = _ext.policy(logits, targets, ignore_index, temperature, old_logps,
-                                      advantages, ref_logps, weight, clip_low, clip_high, kl_coef,
-                                      False)
-    return torch.stack(out), logps, kept[:3 * targets.numel()].clone()
+    out, logps, kept = _ext.native().policy(logits, targets, ignore_index, temperature, old_logps,
+                                            advantages, ref_logps, weight, clip_low, clip_high,
+                                            kl_coef)
+    return out, logps, kept[:_kept(logits, targets)].clone()
 
 
 @policy.register_fake
@@ -244,13 +247,13 @@ def _(logits, targets, ignore_index, temperature, old_logps, advantages, ref_log
       clip_low, clip_high, kl_coef):
     acc = _acc(logits.dtype)
     return (logits.new_empty((3,), dtype=acc), logits.new_empty(targets.shape, dtype=acc),
-            logits.new_empty((3 * targets.numel(),), dtype=torch.float64))
+            logits.new_empty((_kept(logits, targets),), dtype=torch.float64))
 
 
 @torch.library.custom_op(f"{_NS}::policy_grad", mutates_args=())
 def policy_grad(logits: Tensor, targets: Tensor, temperature: float, kept: Tensor,
                 upstream: Tensor) -> Tensor:
-    return _ext.policy_grad(logits, targets, temperature, kept, upstream, None)
+    return _ext.native().policy_grad(logits, targets, temperature, kept, upstream)
 
 
 @policy_grad.register_fake

@@ -13,8 +13,7 @@ repeated.
 from __future__ import annotations
 
 from collections.abc import Iterable, Sequence
-from itertools import chain, repeat
-from operator import attrgetter
+from itertools import chain
 from typing import Any
 
 import torch
@@ -23,17 +22,6 @@ from torch import Tensor
 from torchisotonic_b200 import _ext
 
 BLOCK = 256  # elements that share a scale
-_dtype = attrgetter("dtype")
-
-
-def _bits(dtype: torch.dtype) -> int:
-    if dtype == torch.float32:
-        return 32
-    if dtype == torch.float8_e4m3fn:
-        return 8
-    raise TypeError("optimizer states must be float32 or float8_e4m3fn tensors")
-
-
 def adamw_step(
     params: Sequence[Tensor],
     grads: Sequence[Tensor],
@@ -60,70 +48,17 @@ def adamw_step(
     ceil(n / 256) numbers for every state: a state's number times its block's scale is then m, and
     the square root of v. ``step`` counts from 1; ``seed`` enters the rounding of 8-bit states.
     """
-    lists = [params, grads, exp_avgs, exp_avg_sqs, *(scales or ())]
-    count = len(params)
     if scales is not None and len(scales) != 2:
         raise ValueError("scales must be a pair of sequences")
-    if {*map(len, lists)} != {count}:
-        raise ValueError("params, grads, states and scales must be of one length")
     if step < 1:
         raise ValueError("step must be at least 1")
     if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
         raise ValueError("betas must be in [0, 1)")
     if not (lr >= 0 and eps >= 0 and weight_decay >= 0):
         raise ValueError("lr, eps and weight_decay must not be negative")
-    if count == 0:
-        return
-    # a C-level pass over the lists for each check: hundreds of tensors a call
-    tensors = [*chain.from_iterable(lists)]
-    try:
-        contiguous = all(map(Tensor.is_contiguous, tensors))
-        devices = {*map(Tensor.get_device, tensors)}
-        sizes = [*map(Tensor.numel, tensors)]
-    except TypeError as e:
-        raise TypeError("params, grads, states and scales must be torch.Tensors") from e
-    if not contiguous:
-        raise ValueError("params, grads, states and scales must be contiguous")
-    if not params[0].is_cuda:
-        raise RuntimeError(
-            "torchisotonic_b200 runs on CUDA tensors only (no CPU fallback); "
-            "move params to a CUDA device"
-        )
-    if len(devices) != 1:
-        raise ValueError("params, grads, states and scales must be on one device")
-    if sizes[:4 * count] != sizes[:count] * 4:
-        raise ValueError("grads and states must be shaped like their parameters")
-    types = [*map(_dtype, tensors)]
-    bits = _bits(types[2 * count])
-    if {*types[2 * count:4 * count]} != {types[2 * count]}:
-        raise TypeError("optimizer states must be of one dtype")
-    if (bits == 8) != (scales is not None):
-        raise ValueError("scales go with float8_e4m3fn states, and only with them")
-    if bits == 8:
-        if {*types[4 * count:]} != {torch.float32}:
-            raise TypeError("scales must be float32 tensors")
-        if sizes[4 * count:] != [-(-n // BLOCK) for n in sizes[:count]] * 2:
-            raise ValueError(f"a scale tensor must hold ceil(n / {BLOCK}) numbers")
-    kinds = [*zip(types[:count], types[count:2 * count])]
-    for pt, gt in {*kinds}:
-        if pt not in (torch.float32, torch.float16, torch.bfloat16) or gt not in (pt, torch.float32):
-            raise TypeError("params must be float32, bfloat16 or float16, grads like their "
-                            "parameter or float32")
-    at = [*map(Tensor.data_ptr, tensors)]
-    none = (repeat(0), repeat(0))
-    fields = zip(at[:count], at[count:2 * count], at[2 * count:3 * count],
-                 at[3 * count:4 * count], *((at[4 * count:5 * count], at[5 * count:])
-                                            if bits == 8 else none), sizes[:count], range(count))
-    # autograd's check of saved tensors sees the change
-    torch.autograd.graph.increment_version(tensors[:count] + tensors[2 * count:])
-    args = _ext.AdamwArgs(lr, betas[0], betas[1], eps, weight_decay, step, seed & 0xFFFFFFFF)
-    if kinds.count(kinds[0]) == count:
-        _ext.adamw(params[0].device, *kinds[0], bits, chain.from_iterable(fields), args)
-        return
-    rows = [*fields]
-    for kind in {*kinds}:
-        its = [f for f, k in zip(rows, kinds) if k == kind]
-        _ext.adamw(params[0].device, *kind, bits, chain.from_iterable(its), args)
+    # the lists are checked there: hundreds of tensors a call
+    _ext.native().adamw([params, grads, exp_avgs, exp_avg_sqs, *(scales or ())], step, lr, betas[0],
+                        betas[1], eps, weight_decay, seed & 0xFFFFFFFF)
 
 
 class AdamW(torch.optim.Optimizer):
