@@ -1,5 +1,7 @@
 """Batched isotonic regression for PyTorch on NVIDIA B200 (sm_100a): a drop-in for
-``torchisotonic.isotonic`` over hand-written CUDA kernels behind a C ABI (include/tiso.h)."""
+``torchisotonic.isotonic`` over hand-written CUDA kernels behind a C ABI (include/tiso.h); and the
+losses and the optimizer step of a language model whose answers it calibrates (losses.py,
+optim.py)."""
 
 from torchisotonic_b200._api import isotonic, isotonic_varlen
 from torchisotonic_b200.calibration import calibrate, fit_calibration
