@@ -332,6 +332,7 @@ struct PolicyArgs {
   A* terms;           // per row, w loss, w kl and w [clipped]
   A* out;             // loss, kl, clip fraction
   double* total;      // sum of the weights
+  unsigned* done;     // rows whose results are written
 };
 
 template <typename A>
@@ -358,14 +359,44 @@ __device__ double block_sum(double v, double* shared) {
   return v;
 }
 
+// The sum of the weights, ahead of the rows. The rows' kernel starts meanwhile (a programmatic
+// launch): what it needs of this one it reads after waiting for it.
 template <typename A>
 __global__ void __launch_bounds__(1024) policy_total_kernel(Rows a, PolicyArgs<A> p) {
+  cudaTriggerProgrammaticLaunchCompletion();
   __shared__ double shared[32];
   double sum = 0;
   for (int64_t r = threadIdx.x; r < a.rows; r += blockDim.x)
     sum += static_cast<double>(weight_of(a, p, r));
   sum = block_sum(sum, shared);
-  if (threadIdx.x == 0) *p.total = sum;
+  if (threadIdx.x == 0) {
+    *p.total = sum;
+    *p.done = 0;
+    if (a.rows == 0) p.out[0] = p.out[1] = p.out[2] = A(0);
+  }
+}
+
+// Called by the one thread that has written a row's results: whether it was the last row.
+template <typename A>
+__device__ __forceinline__ bool last_row(const PolicyArgs<A>& p, int64_t rows) {
+  __threadfence();
+  return atomicAdd(p.done, 1u) == static_cast<unsigned>(rows - 1);
+}
+
+// The means over the tokens by the CTA that wrote the last row's results: in a fixed order whichever
+// it is; 0 when the weights sum to 0.
+template <typename A>
+__device__ void write_means(const PolicyArgs<A>& p, int64_t rows) {
+  __shared__ double shared[32];
+  __threadfence();
+  double s[3] = {0, 0, 0};
+  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
+    for (int j = 0; j < 3; ++j) s[j] += static_cast<double>(__ldcg(p.terms + 3 * i + j));
+  const double total = *p.total;
+  for (int j = 0; j < 3; ++j) {
+    const double v = block_sum(s[j], shared);
+    if (threadIdx.x == 0) p.out[j] = total == 0 ? A(0) : static_cast<A>(v / total);
+  }
 }
 
 // What the policy loss needs of a token beside its row.
@@ -382,6 +413,7 @@ struct TokenInput {
     adv = p.advantages[r];
     ref = p.ref_logps ? p.ref_logps[r] : A(0);
     logit = logit_;
+    cudaGridDependencySynchronize();  // the total's kernel is done
     total = *p.total;
   }
 };
@@ -447,47 +479,59 @@ __device__ __forceinline__ RowView<T> policy_view(const Rows& a, int64_t r, T* g
   return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
 }
 
-// A row that is left out.
+// A row that is left out; whether it was the last one.
 template <int kThreads, typename T, typename A>
-__device__ __forceinline__ void leave_out(const PolicyArgs<A>& p, const Place<kThreads>& place,
-                                          const RowView<T>& view, bool with_grad) {
+__device__ __forceinline__ bool leave_out(const PolicyArgs<A>& p, const Place<kThreads>& place,
+                                          const RowView<T>& view, int64_t rows, bool with_grad) {
   constexpr int kTile = kBatch * kThreads;
+  bool last = false;
   if (place.first()) {
     const int64_t r = place.row;
     p.logps[r] = A(0);
     p.coef[r] = 0;
     p.stats[2 * r + 1] = A(kLeftOut);
     p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
+    cudaGridDependencySynchronize();
+    last = last_row(p, rows);
   }
-  if (!with_grad) return;
+  if (!with_grad) return last;
   zero_edge(view, place.edge());
   for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
     zero_tile<kThreads>(view, tile, place.tid);
+  return last;
 }
 
 // Short rows: a warp to a row, which it reads twice.
 template <typename T, typename A>
-__global__ void __launch_bounds__(32 * kRowWarps)
-    policy_warp_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+__device__ __forceinline__ bool policy_warp(const Rows& a, const PolicyArgs<A>& p, double inv_temp,
+                                            A k, T* grad) {
   const Place<32> place;
   const int64_t r = place.row;
-  if (r >= a.rows) return;
+  if (r >= a.rows) return false;
   const RowView<T> view = policy_view(a, r, grad);
   TokenInput<A> token;
   token.w = weight_of(a, p, r);
-  if (token.w == A(0)) {
-    leave_out(p, place, view, grad != nullptr);
-    return;
-  }
+  if (token.w == A(0)) return leave_out(p, place, view, a.rows, grad != nullptr);
   token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
   const Part<A> part = warp_part(view, place, k);
   const Token<A> result(p, token, part, inv_temp);
-  if (place.first()) result.write(p, r, token, part);
-  if (!grad) return;
+  bool last = false;
+  if (place.first()) {
+    result.write(p, r, token, part);
+    last = last_row(p, a.rows);
+  }
+  if (!grad) return last;
   const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
   write_edge(view, place.edge(), slope);
   for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
     write_tile<32>(view, tile, place.tid, slope);
+  return last;
+}
+
+template <typename T, typename A>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    policy_warp_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+  if (__syncthreads_or(policy_warp(a, p, inv_temp, k, grad))) write_means(p, a.rows);
 }
 
 // Loss and gradient in one launch: the row's sum, the token's coefficient, then the row's gradient
@@ -506,8 +550,8 @@ constexpr int kPolicyThreads = 512, kStages = 2;
 constexpr int kPolicyTile = kBatch * kPolicyThreads;
 
 template <typename T, typename A>
-__global__ void __launch_bounds__(kPolicyThreads, 3)
-    policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+__device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p, double inv_temp,
+                                           A k, T* grad, bool& last) {
   extern __shared__ uint4 stages[];  // [kStages][kPolicyTile]
   __shared__ TokenInput<A> token;    // read after the join's barrier
   const Place<kPolicyThreads> place;
@@ -515,7 +559,7 @@ __global__ void __launch_bounds__(kPolicyThreads, 3)
   const RowView<T> view = policy_view(a, r, grad);
   const A w = weight_of(a, p, r);
   if (w == A(0)) {
-    leave_out(p, place, view, grad != nullptr);
+    if (leave_out(p, place, view, a.rows, grad != nullptr)) last = true;
     return;
   }
   // the row's whole tiles, and this CTA's: its j-th is tile cta + j ctas
@@ -559,7 +603,10 @@ __global__ void __launch_bounds__(kPolicyThreads, 3)
   part = join_warps<kPolicyThreads>(join_lanes<32>(part, k), k);
   // every warp takes the few steps to the coefficient by itself: one more barrier takes longer
   const Token<A> result(p, token, part, inv_temp);
-  if (place.first()) result.write(p, r, token, part);
+  if (place.first()) {
+    result.write(p, r, token, part);
+    last = last_row(p, a.rows);
+  }
   if (!grad) return;
   const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
   for (int j = mine - 1; j >= 0; --j) {
@@ -578,19 +625,16 @@ __global__ void __launch_bounds__(kPolicyThreads, 3)
     write_tile<kPolicyThreads>(view, tile, place.tid, slope);
 }
 
-// The means over the tokens, in a fixed order; 0 when the weights sum to 0.
-template <typename A>
-__global__ void __launch_bounds__(1024) policy_means_kernel(int64_t rows, PolicyArgs<A> p) {
-  __shared__ double shared[32];
-  double s[3] = {0, 0, 0};
-  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x)
-    for (int j = 0; j < 3; ++j) s[j] += static_cast<double>(p.terms[3 * r + j]);
-  const double total = *p.total;
-  for (int j = 0; j < 3; ++j) {
-    const double v = block_sum(s[j], shared);
-    if (threadIdx.x == 0) p.out[j] = total == 0 ? A(0) : static_cast<A>(v / total);
-  }
+template <typename T, typename A>
+__global__ void __launch_bounds__(kPolicyThreads, 3)
+    policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
+  __shared__ bool last;  // written by thread 0 alone
+  if (threadIdx.x == 0) last = false;
+  policy_row(a, p, inv_temp, k, grad, last);
+  __syncthreads();
+  if (last) write_means(p, a.rows);
 }
+
 
 // ---------------------------------------------------------------------------------------------
 // Host side
@@ -655,21 +699,24 @@ int allow_shared(const void* kernel, size_t bytes) {
   return TISO_OK;
 }
 
-// A launch of `clusters` clusters of `ctas` CTAs (a power of two up to 8) of `threads`.
+// A launch of `clusters` clusters of `ctas` CTAs (a power of two up to 8) of `threads`. early: it may
+// start before the kernel ahead of it in the stream is done, and waits for it itself.
 template <typename... P, typename... Q>
 int launch_clusters(void (*kernel)(P...), int64_t clusters, int ctas, int threads, size_t shared,
-                    cudaStream_t st, const char* what, Q... args) {
+                    bool early, cudaStream_t st, const char* what, Q... args) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(static_cast<unsigned>(clusters * ctas));
   config.blockDim = dim3(static_cast<unsigned>(threads));
   config.dynamicSmemBytes = shared;
   config.stream = st;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(ctas);
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-  config.attrs = &attribute;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = early ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
   return e == cudaSuccess ? TISO_OK : logits_fail(e, what);
 }
@@ -707,7 +754,7 @@ int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaS
     return launch_warps(logprobs_kernel<T, A, 32>, a.rows, st, "logprobs_kernel launch", a,
                         inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
   return launch_clusters(logprobs_kernel<T, A, 256>, a.rows,
-                         ctas_for(a.rows, vectors, 256, sm_count()), 256, 0, st,
+                         ctas_for(a.rows, vectors, 256, sm_count()), 256, 0, false, st,
                          "logprobs_kernel launch", a, inv_temp, k, static_cast<A*>(logps),
                          static_cast<A*>(stats));
 }
@@ -739,8 +786,9 @@ int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, d
   const int vectors = a.vocab / RowView<T>::E;
   const A k = exp_factor(A(0), inv_temp);
   if (vectors <= kWarpVectors)
-    return launch_warps(policy_warp_kernel<T, A>, a.rows, st, "policy_warp_kernel launch", a, p,
-                        inv_temp, k, grad);
+    return launch_clusters(policy_warp_kernel<T, A>, (a.rows + kRowWarps - 1) / kRowWarps, 1,
+                           32 * kRowWarps, 0, true, st, "policy_warp_kernel launch", a, p, inv_temp,
+                           k, grad);
   const int sms = sm_count();
   int ctas = ctas_for(a.rows, vectors, kPolicyThreads, sms);
   while (ctas < 8 && int64_t{sms} * 3 * vectors * 16 / ctas > kRowsInL2) ctas *= 2;
@@ -748,7 +796,7 @@ int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, d
   const auto kernel = policy_kernel<T, A>;
   const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kShared);
   if (rc) return rc;
-  return launch_clusters(kernel, a.rows, ctas, kPolicyThreads, kShared, st,
+  return launch_clusters(kernel, a.rows, ctas, kPolicyThreads, kShared, true, st,
                          "policy_kernel launch", a, p, inv_temp, k, grad);
 }
 
@@ -770,14 +818,12 @@ int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* 
   p.stats = static_cast<A*>(stats);
   p.out = static_cast<A*>(out);
   p.total = static_cast<double*>(workspace);
-  p.terms = reinterpret_cast<A*>(p.total + 1);
+  p.done = reinterpret_cast<unsigned*>(p.total + 1);
+  p.terms = reinterpret_cast<A*>(p.total + 2);
   policy_total_kernel<A><<<1, 1024, 0, st>>>(a, p);
-  if (a.rows > 0) {
-    const int rc = launch_policy<T>(a, p, inv_temp, static_cast<T*>(grad), st);
-    if (rc) return rc;
-  }
-  policy_means_kernel<A><<<1, 1024, 0, st>>>(a.rows, p);
-  return launched("policy kernels launch");
+  const int rc = launched("policy_total_kernel launch");
+  if (rc || a.rows == 0) return rc;
+  return launch_policy<T>(a, p, inv_temp, static_cast<T*>(grad), st);
 }
 
 // fn(T{}) with T the element type of dtype
@@ -845,7 +891,7 @@ int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes) {
     if (dtype < TISO_F16 || dtype > TISO_F64)
       return report_error(TISO_ERR_ARGUMENT, "dtype must be a tiso_dtype");
     if (rows < 0) return report_error(TISO_ERR_ARGUMENT, "need rows >= 0");
-    *bytes = 8 + static_cast<size_t>(rows) * 3 * (dtype == TISO_F64 ? 8 : 4);
+    *bytes = 16 + static_cast<size_t>(rows) * 3 * (dtype == TISO_F64 ? 8 : 4);
     return TISO_OK;
   });
 }
