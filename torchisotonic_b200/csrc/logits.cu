@@ -546,15 +546,16 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 // the last kStages are still there, and the others, if few enough rows are in work at a time, in
 // L2. A last tile that is not whole, and all of a row that is read and written at different
 // alignments, is loaded directly.
-constexpr int kPolicyThreads = 512, kStages = 2;
-constexpr int kPolicyTile = kBatch * kPolicyThreads;
+constexpr int kStages = 2;
+constexpr int kSmThreads = 1536;  // resident at 40 registers a thread
 
-template <typename T, typename A>
+template <int kThreads, typename T, typename A>
 __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p, double inv_temp,
                                            A k, T* grad, bool& last) {
-  extern __shared__ uint4 stages[];  // [kStages][kPolicyTile]
+  constexpr int kTile = kBatch * kThreads;
+  extern __shared__ uint4 stages[];  // [kStages][kTile]
   __shared__ TokenInput<A> token;    // read after the join's barrier
-  const Place<kPolicyThreads> place;
+  const Place<kThreads> place;
   const int64_t r = place.row;
   const RowView<T> view = policy_view(a, r, grad);
   const A w = weight_of(a, p, r);
@@ -563,18 +564,18 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     return;
   }
   // the row's whole tiles, and this CTA's: its j-th is tile cta + j ctas
-  const int whole = view.shift == 0 ? view.vectors / kPolicyTile : 0;
+  const int whole = view.shift == 0 ? view.vectors / kTile : 0;
   const int mine = whole > place.cta ? (whole - place.cta + place.ctas - 1) / place.ctas : 0;
-  const int stride = place.ctas * kPolicyTile;
-  const int own = place.cta * kPolicyTile + place.tid;
+  const int stride = place.ctas * kTile;
+  const int own = place.cta * kTile + place.tid;
   const uint4* from = reinterpret_cast<const uint4*>(view.x + view.head) + own;
   uint4* to = reinterpret_cast<uint4*>(view.g + view.head) + own;
   const auto copy = [&](int j) {
     if (j >= 0 && j < mine) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
-        copy_async(stages + j % kStages * kPolicyTile + i * kPolicyThreads + place.tid,
-                   from + static_cast<int64_t>(j) * stride + i * kPolicyThreads);
+        copy_async(stages + j % kStages * kTile + i * kThreads + place.tid,
+                   from + static_cast<int64_t>(j) * stride + i * kThreads);
     }
     close_group();
   };
@@ -582,7 +583,7 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      q[i] = stages[j % kStages * kPolicyTile + i * kPolicyThreads + place.tid];
+      q[i] = stages[j % kStages * kTile + i * kThreads + place.tid];
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) copy(j);
@@ -593,14 +594,14 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
 
   // the tiles that are loaded directly, and the single elements
   const int rest = whole + (place.cta - whole % place.ctas + place.ctas) % place.ctas;
-  Part<A> part = thread_part(view, place, rest * kPolicyTile, k);
+  Part<A> part = thread_part(view, place, rest * kTile, k);
   for (int j = 0; j < mine; ++j) {
     uint4 q[kBatch];
     fetch(j, q);
     copy(j + kStages);
     add_vectors<T>(part, q, k);
   }
-  part = join_warps<kPolicyThreads>(join_lanes<32>(part, k), k);
+  part = join_warps<kThreads>(join_lanes<32>(part, k), k);
   // every warp takes the few steps to the coefficient by itself: one more barrier takes longer
   const Token<A> result(p, token, part, inv_temp);
   if (place.first()) {
@@ -615,22 +616,22 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     copy(j - kStages);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      store_once(to + static_cast<int64_t>(j) * stride + i * kPolicyThreads,
+      store_once(to + static_cast<int64_t>(j) * stride + i * kThreads,
                  slope_vector<T>(q[i], slope));
-    write_target_of_tile<kPolicyThreads, kPolicyTile>(view, own - place.tid + j * stride, place.tid,
+    write_target_of_tile<kThreads, kTile>(view, own - place.tid + j * stride, place.tid,
                                                       slope);
   }
   write_edge(view, place.edge(), slope);
-  for (int tile = rest * kPolicyTile; tile < view.vectors; tile += stride)
-    write_tile<kPolicyThreads>(view, tile, place.tid, slope);
+  for (int tile = rest * kTile; tile < view.vectors; tile += stride)
+    write_tile<kThreads>(view, tile, place.tid, slope);
 }
 
-template <typename T, typename A>
-__global__ void __launch_bounds__(kPolicyThreads, 3)
+template <typename T, typename A, int kThreads>
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
     policy_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
   __shared__ bool last;  // written by thread 0 alone
   if (threadIdx.x == 0) last = false;
-  policy_row(a, p, inv_temp, k, grad, last);
+  policy_row<kThreads>(a, p, inv_temp, k, grad, last);
   __syncthreads();
   if (last) write_means(p, a.rows);
 }
@@ -729,10 +730,17 @@ int launch_warps(void (*kernel)(P...), int64_t rows, cudaStream_t st, const char
   return launched(what);
 }
 
-// Rows of at most this many vectors go to a warp each (8176 x 777 float: 14 us, 67 with a CTA each).
+// Rows of at most kWarpVectors vectors go to a warp each; of up to `most` of them where there are
+// enough rows to fill the GPU with warps. A CTA's start and join cost as much as some 1000 vectors:
+// 97656 x 4096 bf16, log-probabilities 133 us by warps and 342 by CTAs of 256 threads, their gradient
+// 272 and 358, the policy loss 421 and 779; 976 x 8192: 11.2 and 10.2 us.
 constexpr int kWarpVectors = 256;
 
-// Bytes of rows in work at once (3 CTAs an SM) that L2 is to hold from a row's first read to its
+bool by_warps(int64_t rows, int64_t vectors, int64_t most, int sms) {
+  return vectors <= kWarpVectors || (vectors <= most && rows >= int64_t{16} * sms);
+}
+
+// Bytes of rows in work at once that L2 is to hold from a row's first read to its
 // second. Rows of 256 KB: one CTA to a row (116 MB) reads 1.8 GB where two (58 MB) read 1.06 and
 // four 0.95 (0.94 is each byte once); two are fastest (828, 874 and 931 us with 2, 1 and 4).
 constexpr int64_t kRowsInL2 = 80 << 20;
@@ -750,11 +758,12 @@ int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaS
   using A = typename AccOf<T>::type;
   const int vectors = a.vocab / RowView<T>::E;
   const A k = exp_factor(A(0), inv_temp);
-  if (vectors <= kWarpVectors)
+  const int sms = sm_count();
+  if (by_warps(a.rows, vectors, 2048, sms))  // 24414 x 16384 bf16: 125 us, by CTAs 140
     return launch_warps(logprobs_kernel<T, A, 32>, a.rows, st, "logprobs_kernel launch", a,
                         inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
   return launch_clusters(logprobs_kernel<T, A, 256>, a.rows,
-                         ctas_for(a.rows, vectors, 256, sm_count()), 256, 0, false, st,
+                         ctas_for(a.rows, vectors, 256, sms), 256, 0, false, st,
                          "logprobs_kernel launch", a, inv_temp, k, static_cast<A*>(logps),
                          static_cast<A*>(stats));
 }
@@ -764,12 +773,13 @@ int run_logprobs_grad(const Rows& a, double inv_temp, const void* stats, const v
                       const void* upstream, void* grad, cudaStream_t st) {
   using A = typename AccOf<T>::type;
   const int vectors = a.vocab / RowView<T>::E;
-  const bool by_warp = vectors <= kWarpVectors;
+  const int sms = sm_count();
+  const bool by_warp = by_warps(a.rows, vectors, 768, sms);  // 48828 x 8192: 262 us, by CTAs 250
   const int tile = kBatch * (by_warp ? 32 : 256);
   const int tiles = vectors > tile ? (vectors + tile - 1) / tile : 1;
   const int64_t all = (a.rows * tiles + (by_warp ? 7 : 0)) / (by_warp ? 8 : 1);
   // where the launch may have nothing to do (upstream is 1), no more CTAs than are resident
-  const int64_t most = upstream ? int64_t{sm_count()} * 8 : int64_t{1} << 30;
+  const int64_t most = upstream ? int64_t{sms} * 8 : int64_t{1} << 30;
   const unsigned grid = static_cast<unsigned>(all < most ? all : most);
   const A k = exp_factor(A(0), inv_temp);
   auto kernel = by_warp ? logprobs_grad_kernel<T, A, C, 32> : logprobs_grad_kernel<T, A, C, 256>;
@@ -779,25 +789,41 @@ int run_logprobs_grad(const Rows& a, double inv_temp, const void* stats, const v
   return launched("logprobs_grad_kernel launch");
 }
 
+template <typename T, int kThreads>
+int launch_policy_rows(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, double inv_temp,
+                       T* grad, int sms, cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  constexpr size_t kShared = size_t{kStages} * kBatch * kThreads * 16;
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  int ctas = ctas_for(a.rows, vectors, kThreads, sms);
+  while (ctas < 8 && int64_t{sms} * (kSmThreads / kThreads) * vectors * 16 / ctas > kRowsInL2)
+    ctas *= 2;
+  const auto kernel = policy_kernel<T, A, kThreads>;
+  const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kShared);
+  if (rc) return rc;
+  return launch_clusters(kernel, a.rows, ctas, kThreads, kShared, true, st, "policy_kernel launch",
+                         a, p, inv_temp, exp_factor(A(0), inv_temp), grad);
+}
+
+// By warps, or in CTAs of the more threads the longer the row: smaller ones have more rows in work,
+// which hides a row's start and join, larger ones less of both. 800 MB of bf16 logits, us with 128,
+// 256 and 512 threads (a warp): 8192 to the row 394, 449, 765 (392), 16384: 308, 320, 435 (382),
+// 32000: 331, 312, 390, 50021: 351, 318, 320, 65536: 304, 304, 280, 131072: 302, 306, 290. Rows whose
+// tiles are not whole lose more with 512 (100003: 314 with 256, 333 with 512).
 template <typename T>
 int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, double inv_temp,
                   T* grad, cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  const int vectors = a.vocab / RowView<T>::E;
-  const A k = exp_factor(A(0), inv_temp);
-  if (vectors <= kWarpVectors)
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  const int sms = sm_count();
+  if (by_warps(a.rows, vectors, 768, sms))
     return launch_clusters(policy_warp_kernel<T, A>, (a.rows + kRowWarps - 1) / kRowWarps, 1,
                            32 * kRowWarps, 0, true, st, "policy_warp_kernel launch", a, p, inv_temp,
-                           k, grad);
-  const int sms = sm_count();
-  int ctas = ctas_for(a.rows, vectors, kPolicyThreads, sms);
-  while (ctas < 8 && int64_t{sms} * 3 * vectors * 16 / ctas > kRowsInL2) ctas *= 2;
-  constexpr size_t kShared = size_t{kStages} * kPolicyTile * 16;
-  const auto kernel = policy_kernel<T, A>;
-  const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kShared);
-  if (rc) return rc;
-  return launch_clusters(kernel, a.rows, ctas, kPolicyThreads, kShared, true, st,
-                         "policy_kernel launch", a, p, inv_temp, k, grad);
+                           exp_factor(A(0), inv_temp), grad);
+  if (vectors <= 2560) return launch_policy_rows<T, 128>(a, p, inv_temp, grad, sms, st);
+  if (vectors >= 8192 && vectors % (kBatch * 512) == 0)
+    return launch_policy_rows<T, 512>(a, p, inv_temp, grad, sms, st);
+  return launch_policy_rows<T, 256>(a, p, inv_temp, grad, sms, st);
 }
 
 template <typename T>
