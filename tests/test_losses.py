@@ -537,6 +537,17 @@ def test_policy_rows(rows: int, vocab: int, dtype: torch.dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 40), (torch.float64, 2100)])
+def test_policy_many_rows(vocab: int, dtype: torch.dtype) -> None:
+    # enough of them that a cluster sums their weights
+    x, y, _ = logits_of((8200 + vocab, vocab), dtype, seed=vocab)
+    old, adv, ref = tokens_of(x, y, vocab)
+    w = torch.rand(x.shape[0], device="cuda", dtype=dtype)
+    w[w < 0.4] = 0.0
+    check_policy(x, y, old, adv, ref_logps=ref, weight=w, kl_coef=0.1)
+
+
+@pytest.mark.gpu
 def test_policy_settings() -> None:
     x, y, _ = logits_of((4, 50, 301), torch.float32)
     old, adv, ref = tokens_of(x, y, 1)

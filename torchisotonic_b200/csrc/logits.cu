@@ -92,11 +92,9 @@ template <int kThreads, typename T, typename A>
 __device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, const Place<kThreads>& place,
                                                int first, A k) {
   constexpr int kTile = kBatch * kThreads;
+  // loaded ahead of the vectors, used behind them
+  const A edge = place.edge() < r.edges ? to_acc(r.x[r.edge(place.edge())]) : lowest<A>();
   Part<A> p{lowest<A>(), A(0)};
-  if (place.edge() < r.edges) {
-    const A z = to_acc(r.x[r.edge(place.edge())]);
-    p = {z, scaled_exp(z - base_of(z), k)};
-  }
   for (int tile = first; tile < r.vectors; tile += place.ctas * kTile) {
     const int v = tile + place.tid;
     uint4 q[kBatch];
@@ -109,6 +107,9 @@ __device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, const Place<
     }
     add_vectors<T>(p, q, k);
   }
+  const A m = max_acc(p.m, edge), base = base_of(m);
+  p.s = (p.m == m ? p.s : p.s * scaled_exp(p.m - base, k)) + scaled_exp(edge - base, k);
+  p.m = m;
   return p;
 }
 
@@ -118,8 +119,15 @@ __device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kT
   return join_lanes<32>(thread_part(r, place, place.cta * kBatch * kThreads, k), k);
 }
 
+// The CTAs of a cluster write to one another's shared memory once, at their joins. Before that each
+// has to have started: says that this one has.
+__device__ __forceinline__ void cluster_started(int ctas) {
+  if (ctas > 1) cg::this_cluster().barrier_arrive();
+}
+
 // The parts of all of a row's warps joined (a warp's lanes hold the same); every thread gets the
-// result. Called once by a CTA (its shared memory is not used again), by all of its threads.
+// result. Called once by a CTA (its shared memory is not used again), by all of its threads, after
+// cluster_started.
 template <int kThreads, typename A>
 __device__ __forceinline__ Part<A> join_warps(Part<A> p, A k) {
   if constexpr (kThreads > 32) {
@@ -132,6 +140,7 @@ __device__ __forceinline__ Part<A> join_warps(Part<A> p, A k) {
     auto cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks());
     if (ctas > 1) {
+      cluster.barrier_wait();
       if (threadIdx.x < ctas)
         *cluster.map_shared_rank(&of_cta[cluster.block_rank()], threadIdx.x) = p;
       cluster.sync();
@@ -249,35 +258,71 @@ __device__ __forceinline__ void zero_edge(const RowView<T>& r, int edge) {
 // negative sum in stats: its gradient is zeros and its logits are not read.
 constexpr int kLeftOut = -1;
 
+template <typename A>
+__device__ __forceinline__ void write_logp(int64_t r, A logit, const Part<A>& p, double inv_temp,
+                                           A* logps, A* stats) {
+  logps[r] = static_cast<A>(logp_of(logit, p, inv_temp));
+  if (stats) {
+    stats[2 * r] = base_of(p.m);
+    stats[2 * r + 1] = p.s;
+  }
+}
+
+template <typename A>
+__device__ __forceinline__ void write_ignored(int64_t r, A* logps, A* stats) {
+  logps[r] = A(0);
+  if (stats) stats[2 * r + 1] = A(kLeftOut);
+}
+
 // logps[r] = (x[r, y] - m) / t - log s, m and s the row's maximum and sum of exponentials. One pass:
 // a thread keeps its own maximum and sum, rescaled once for every four vectors, the row's are
 // joined at its end. Bound by memory: 4096 x 131072 in 150 us (0.97 GB read, 99 % of the copy
 // bandwidth), 4 x 1023 x 50021 in 78 us (80 %: a CTA's start and join are a larger part of a row of
-// 100 KB). Rows of up to 256 vectors take a warp each, others a CTA, or for few rows a cluster.
+// 100 KB). A row takes a CTA, or where rows are few a cluster.
 template <typename T, typename A, int kThreads>
-__global__ void __launch_bounds__(kThreads == 32 ? 32 * kRowWarps : kThreads)
+__global__ void __launch_bounds__(kThreads)
     logprobs_kernel(Rows a, double inv_temp, A k, A* logps, A* stats) {
   const Place<kThreads> place;
-  const int64_t r = place.row;
-  if (r >= a.rows) return;
-  const int64_t target = a.targets[r];
+  const int64_t r = place.row, target = a.targets[r];
   if (target == a.ignore) {
-    if (place.first()) {
-      logps[r] = A(0);
-      if (stats) stats[2 * r + 1] = A(kLeftOut);
-    }
+    if (place.first()) write_ignored(r, logps, stats);
     return;
   }
+  cluster_started(place.ctas);
   const T* x = row_at<T>(a, r);
   A at_target = A(0);
   if (place.first()) at_target = target_logit<T, A>(x, a.vocab, target);
   const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
   const Part<A> p = join_warps<kThreads>(warp_part(view, place, k), k);
-  if (place.first()) {
-    logps[r] = static_cast<A>(logp_of(at_target, p, inv_temp));
-    if (stats) {
-      stats[2 * r] = base_of(p.m);
-      stats[2 * r + 1] = p.s;
+  if (place.first()) write_logp(r, at_target, p, inv_temp, logps, stats);
+}
+
+// A warp to a row; the steps after the sums by a lane for each of the CTA's rows.
+template <typename T, typename A>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    logprobs_warp_kernel(Rows a, double inv_temp, A k, A* logps, A* stats) {
+  __shared__ Part<A> parts[kRowWarps];
+  __shared__ A logits[kRowWarps];
+  __shared__ bool read[kRowWarps];
+  const Place<32> place;
+  const int64_t r = place.row;
+  const int warp = threadIdx.x / 32;
+  const int64_t target = r < a.rows ? a.targets[r] : a.ignore;
+  if (place.tid == 0) read[warp] = target != a.ignore;
+  if (target != a.ignore) {
+    const T* x = row_at<T>(a, r);
+    if (place.tid == 0) logits[warp] = target_logit<T, A>(x, a.vocab, target);
+    const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
+    const Part<A> p = warp_part(view, place, k);
+    if (place.tid == 0) parts[warp] = p;
+  }
+  __syncthreads();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowWarps + threadIdx.x;
+  if (threadIdx.x < kRowWarps && row < a.rows) {
+    if (read[threadIdx.x]) {
+      write_logp(row, logits[threadIdx.x], parts[threadIdx.x], inv_temp, logps, stats);
+    } else {
+      write_ignored(row, logps, stats);
     }
   }
 }
@@ -329,10 +374,10 @@ struct PolicyArgs {
   A* logps;           // per row
   double* coef;       // per row, d loss / d logp
   A* stats;           // per row, maximum and sum
-  A* terms;           // per row, w loss, w kl and w [clipped]
+  A* terms;           // per unit (a row, or a CTA's rows), w loss, w kl and w [clipped]
   A* out;             // loss, kl, clip fraction
   double* total;      // sum of the weights
-  unsigned* done;     // rows whose results are written
+  unsigned* done;     // units whose results are written
 };
 
 template <typename A>
@@ -359,40 +404,75 @@ __device__ double block_sum(double v, double* shared) {
   return v;
 }
 
-// The sum of the weights, ahead of the rows. The rows' kernel starts meanwhile (a programmatic
-// launch): what it needs of this one it reads after waiting for it.
+// The sum of the weights, by a CTA, or a cluster of them where there are many rows, ahead of the
+// rows. The rows' kernel starts meanwhile (a programmatic launch): what it needs of this one it reads
+// after waiting for it.
+constexpr int kTotalThreads = 1024, kTotalCtas = 8;
+
 template <typename A>
-__global__ void __launch_bounds__(1024) policy_total_kernel(Rows a, PolicyArgs<A> p) {
+__global__ void __launch_bounds__(kTotalThreads) policy_total_kernel(Rows a, PolicyArgs<A> p) {
   cudaTriggerProgrammaticLaunchCompletion();
-  __shared__ double shared[32];
+  constexpr int kAhead = 4;
+  __shared__ double shared[32], sums[kTotalCtas];
+  auto cluster = cg::this_cluster();
+  cluster_started(gridDim.x);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTotalThreads;
   double sum = 0;
-  for (int64_t r = threadIdx.x; r < a.rows; r += blockDim.x)
-    sum += static_cast<double>(weight_of(a, p, r));
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kTotalThreads + threadIdx.x; r < a.rows;
+       r += kAhead * step) {
+    A w[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      w[i] = r + i * step < a.rows ? weight_of(a, p, r + i * step) : A(0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) sum += static_cast<double>(w[i]);
+  }
   sum = block_sum(sum, shared);
-  if (threadIdx.x == 0) {
+  if (gridDim.x > 1) {
+    cluster.barrier_wait();
+    if (threadIdx.x == 0) *cluster.map_shared_rank(&sums[blockIdx.x], 0) = sum;
+    cluster.sync();
+    sum = 0;
+    for (unsigned i = 0; i < gridDim.x; ++i) sum += sums[i];  // the first CTA's are the sums
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
     *p.total = sum;
     *p.done = 0;
     if (a.rows == 0) p.out[0] = p.out[1] = p.out[2] = A(0);
   }
 }
 
-// Called by the one thread that has written a row's results: whether it was the last row.
+// Called by one thread of each unit (a row, or a CTA's rows) once its results are written: whether it
+// was the last of them.
 template <typename A>
-__device__ __forceinline__ bool last_row(const PolicyArgs<A>& p, int64_t rows) {
+__device__ __forceinline__ bool last_unit(const PolicyArgs<A>& p, int64_t units) {
   __threadfence();
-  return atomicAdd(p.done, 1u) == static_cast<unsigned>(rows - 1);
+  return atomicAdd(p.done, 1u) == static_cast<unsigned>(units - 1);
 }
 
-// The means over the tokens by the CTA that wrote the last row's results: in a fixed order whichever
-// it is; 0 when the weights sum to 0.
+// The means over the tokens by the CTA of the last unit: in a fixed order whichever it is; 0 when the
+// weights sum to 0.
 template <typename A>
-__device__ void write_means(const PolicyArgs<A>& p, int64_t rows) {
+__device__ void write_means(const PolicyArgs<A>& p, int64_t units) {
+  constexpr int kAhead = 4;
   __shared__ double shared[32];
   __threadfence();
   double s[3] = {0, 0, 0};
-  for (int64_t i = threadIdx.x; i < rows; i += blockDim.x)
-    for (int j = 0; j < 3; ++j) s[j] += static_cast<double>(__ldcg(p.terms + 3 * i + j));
+  const int64_t step = blockDim.x;
+  for (int64_t u = threadIdx.x; u < units; u += kAhead * step) {
+    A q[kAhead][3];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        q[i][j] = u + i * step < units ? __ldcg(p.terms + 3 * (u + i * step) + j) : A(0);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) s[j] += static_cast<double>(q[i][j]);
+  }
   const double total = *p.total;
+#pragma unroll
   for (int j = 0; j < 3; ++j) {
     const double v = block_sum(s[j], shared);
     if (threadIdx.x == 0) p.out[j] = total == 0 ? A(0) : static_cast<A>(v / total);
@@ -452,8 +532,9 @@ struct Token {
     coef = in.total != 0 ? static_cast<double>(in.w) / in.total * slope : 0.0;
   }
 
+  // the row's results, and in `terms` what the means sum
   __device__ __forceinline__ void write(const PolicyArgs<A>& p, int64_t r, const TokenInput<A>& in,
-                                        const Part<A>& part) const {
+                                        const Part<A>& part, A (&terms)[3]) const {
     const double lp = t - log(static_cast<double>(part.s));
     double loss = -(free_side > held ? held : free_side), kl = 0.0;
     if (p.ref_logps) {
@@ -465,11 +546,18 @@ struct Token {
     p.coef[r] = coef;
     p.stats[2 * r] = base_of(part.m);
     p.stats[2 * r + 1] = part.s;
-    p.terms[3 * r] = static_cast<A>(in.w * loss);
-    p.terms[3 * r + 1] = static_cast<A>(in.w * kl);
-    p.terms[3 * r + 2] = free_side > held ? in.w : A(0);
+    terms[0] = static_cast<A>(in.w * loss);
+    terms[1] = static_cast<A>(in.w * kl);
+    terms[2] = free_side > held ? in.w : A(0);
   }
 };
+
+template <typename A>
+__device__ __forceinline__ void write_terms(const PolicyArgs<A>& p, int64_t unit,
+                                            const A (&terms)[3]) {
+#pragma unroll
+  for (int j = 0; j < 3; ++j) p.terms[3 * unit + j] = terms[j];
+}
 
 // The row's cut is as for a gradient in a buffer on a vector's boundary, also where no gradient is
 // written (grad NULL): the loss is the same bits.
@@ -479,59 +567,81 @@ __device__ __forceinline__ RowView<T> policy_view(const Rows& a, int64_t r, T* g
   return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
 }
 
-// A row that is left out; whether it was the last one.
-template <int kThreads, typename T, typename A>
-__device__ __forceinline__ bool leave_out(const PolicyArgs<A>& p, const Place<kThreads>& place,
-                                          const RowView<T>& view, int64_t rows, bool with_grad) {
-  constexpr int kTile = kBatch * kThreads;
-  bool last = false;
-  if (place.first()) {
-    const int64_t r = place.row;
-    p.logps[r] = A(0);
-    p.coef[r] = 0;
-    p.stats[2 * r + 1] = A(kLeftOut);
-    p.terms[3 * r] = p.terms[3 * r + 1] = p.terms[3 * r + 2] = A(0);
-    cudaGridDependencySynchronize();
-    last = last_row(p, rows);
-  }
-  if (!with_grad) return last;
-  zero_edge(view, place.edge());
-  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-    zero_tile<kThreads>(view, tile, place.tid);
-  return last;
+template <typename A>
+__device__ __forceinline__ void write_left_out(const PolicyArgs<A>& p, int64_t r) {
+  p.logps[r] = A(0);
+  p.coef[r] = 0;
+  p.stats[2 * r + 1] = A(kLeftOut);
 }
 
-// Short rows: a warp to a row, which it reads twice.
-template <typename T, typename A>
-__device__ __forceinline__ bool policy_warp(const Rows& a, const PolicyArgs<A>& p, double inv_temp,
-                                            A k, T* grad) {
-  const Place<32> place;
-  const int64_t r = place.row;
-  if (r >= a.rows) return false;
-  const RowView<T> view = policy_view(a, r, grad);
-  TokenInput<A> token;
-  token.w = weight_of(a, p, r);
-  if (token.w == A(0)) return leave_out(p, place, view, a.rows, grad != nullptr);
-  token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
-  const Part<A> part = warp_part(view, place, k);
-  const Token<A> result(p, token, part, inv_temp);
-  bool last = false;
-  if (place.first()) {
-    result.write(p, r, token, part);
-    last = last_row(p, a.rows);
-  }
-  if (!grad) return last;
-  const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
-  write_edge(view, place.edge(), slope);
-  for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
-    write_tile<32>(view, tile, place.tid, slope);
-  return last;
-}
-
+// Short rows: a warp to a row, which it reads twice; the tokens' steps between by a lane for each of
+// the CTA's rows (by every warp for its own row they cost as much as 2000 logits).
 template <typename T, typename A>
 __global__ void __launch_bounds__(32 * kRowWarps)
     policy_warp_kernel(Rows a, PolicyArgs<A> p, double inv_temp, A k, T* grad) {
-  if (__syncthreads_or(policy_warp(a, p, inv_temp, k, grad))) write_means(p, a.rows);
+  __shared__ Part<A> parts[kRowWarps];
+  __shared__ TokenInput<A> tokens[kRowWarps];  // of weight 0: a row that is left out, or none
+  __shared__ double coefs[kRowWarps];
+  __shared__ bool last;
+  const Place<32> place;
+  const int64_t r = place.row, first_row = static_cast<int64_t>(blockIdx.x) * kRowWarps;
+  const int warp = threadIdx.x / 32;
+  const bool is_row = r < a.rows;
+  const RowView<T> view = policy_view(a, is_row ? r : first_row, grad);
+  const A w = is_row ? weight_of(a, p, r) : A(0);
+  if (w != A(0)) {
+    TokenInput<A> token;
+    if (place.tid == 0)  // in flight with the row's own loads
+      token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
+    const Part<A> part = warp_part(view, place, k);
+    if (place.tid == 0) {
+      token.w = w;
+      tokens[warp] = token;
+      parts[warp] = part;
+    }
+  } else if (place.tid == 0) {
+    tokens[warp].w = w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int64_t row = first_row + threadIdx.x;
+    A terms[3] = {};
+    if (threadIdx.x < kRowWarps && row < a.rows) {
+      const TokenInput<A>& token = tokens[threadIdx.x];
+      if (token.w != A(0)) {
+        const Token<A> result(p, token, parts[threadIdx.x], inv_temp);
+        result.write(p, row, token, parts[threadIdx.x], terms);
+        coefs[threadIdx.x] = result.coef;
+      } else {
+        write_left_out(p, row);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+#pragma unroll
+      for (int d = kRowWarps / 2; d; d >>= 1) terms[j] += __shfl_xor_sync(0xffffffffu, terms[j], d);
+    if (threadIdx.x == 0) write_terms(p, blockIdx.x, terms);
+  }
+  __syncthreads();
+  if (grad && is_row) {
+    if (w != A(0)) {
+      const Slope<A> slope(base_of(parts[warp].m), parts[warp].s, coefs[warp] * inv_temp, k,
+                           tokens[warp].target, a.vocab);
+      write_edge(view, place.edge(), slope);
+      for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
+        write_tile<32>(view, tile, place.tid, slope);
+    } else {
+      zero_edge(view, place.edge());
+      for (int tile = 0; tile < view.vectors; tile += kBatch * 32)
+        zero_tile<32>(view, tile, place.tid);
+    }
+  }
+  if (threadIdx.x == 0) {
+    cudaGridDependencySynchronize();
+    last = last_unit(p, gridDim.x);
+  }
+  __syncthreads();
+  if (last) write_means(p, gridDim.x);
 }
 
 // Loss and gradient in one launch: the row's sum, the token's coefficient, then the row's gradient
@@ -560,9 +670,19 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   const RowView<T> view = policy_view(a, r, grad);
   const A w = weight_of(a, p, r);
   if (w == A(0)) {
-    if (leave_out(p, place, view, a.rows, grad != nullptr)) last = true;
+    if (place.first()) {
+      write_left_out(p, r);
+      write_terms(p, r, {A(0), A(0), A(0)});
+      cudaGridDependencySynchronize();
+      last = last_unit(p, a.rows);
+    }
+    if (!grad) return;
+    zero_edge(view, place.edge());
+    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+      zero_tile<kThreads>(view, tile, place.tid);
     return;
   }
+  cluster_started(place.ctas);
   // the row's whole tiles, and this CTA's: its j-th is tile cta + j ctas
   const int whole = view.shift == 0 ? view.vectors / kTile : 0;
   const int mine = whole > place.cta ? (whole - place.cta + place.ctas - 1) / place.ctas : 0;
@@ -605,8 +725,10 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   // every warp takes the few steps to the coefficient by itself: one more barrier takes longer
   const Token<A> result(p, token, part, inv_temp);
   if (place.first()) {
-    result.write(p, r, token, part);
-    last = last_row(p, a.rows);
+    A terms[3];
+    result.write(p, r, token, part, terms);
+    write_terms(p, r, terms);
+    last = last_unit(p, a.rows);
   }
   if (!grad) return;
   const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
@@ -635,7 +757,6 @@ __global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
   __syncthreads();
   if (last) write_means(p, a.rows);
 }
-
 
 // ---------------------------------------------------------------------------------------------
 // Host side
@@ -760,8 +881,8 @@ int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaS
   const A k = exp_factor(A(0), inv_temp);
   const int sms = sm_count();
   if (by_warps(a.rows, vectors, 2048, sms))  // 24414 x 16384 bf16: 125 us, by CTAs 140
-    return launch_warps(logprobs_kernel<T, A, 32>, a.rows, st, "logprobs_kernel launch", a,
-                        inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
+    return launch_warps(logprobs_warp_kernel<T, A>, a.rows, st, "logprobs_warp_kernel launch",
+                        a, inv_temp, k, static_cast<A*>(logps), static_cast<A*>(stats));
   return launch_clusters(logprobs_kernel<T, A, 256>, a.rows,
                          ctas_for(a.rows, vectors, 256, sms), 256, 0, false, st,
                          "logprobs_kernel launch", a, inv_temp, k, static_cast<A*>(logps),
@@ -846,8 +967,10 @@ int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* 
   p.total = static_cast<double*>(workspace);
   p.done = reinterpret_cast<unsigned*>(p.total + 1);
   p.terms = reinterpret_cast<A*>(p.total + 2);
-  policy_total_kernel<A><<<1, 1024, 0, st>>>(a, p);
-  const int rc = launched("policy_total_kernel launch");
+  // 8192 rows: 7 us by one CTA
+  const int ctas = a.rows > 8 * kTotalThreads ? kTotalCtas : 1;
+  const int rc = launch_clusters(policy_total_kernel<A>, 1, ctas, kTotalThreads, 0, false, st,
+                                 "policy_total_kernel launch", a, p);
   if (rc || a.rows == 0) return rc;
   return launch_policy<T>(a, p, inv_temp, static_cast<T*>(grad), st);
 }
