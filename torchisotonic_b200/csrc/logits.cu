@@ -650,12 +650,13 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 // unit is busy 58 % of the time, and what is missing are the joins between a row's two passes (of a
 // CTA's 20 us about 5), which two other CTAs of the SM fill in part.
 //
-// A cluster's CTAs take a row's tiles in turn, a tile kBatch vectors a thread. Whole tiles come
-// through kStages places of shared memory, each thread copying and reading its own vectors there
-// (no barrier), so that kStages tiles are in flight. The gradient takes them in the reverse order:
-// the last kStages are still there, and the others, if few enough rows are in work at a time, in
-// L2. A last tile that is not whole, and all of a row that is read and written at different
-// alignments, is loaded directly.
+// A cluster's CTAs take a row's tiles in turn, a tile kBatch vectors a thread. Tiles come through
+// kStages places of shared memory, each thread copying and reading its own vectors there (no
+// barrier), so that kStages tiles are in flight. The gradient takes them in the reverse order: the
+// last kStages are still there, and the others, if few enough rows are in work at a time, in L2.
+// A last tile that is cut goes this way too: loaded directly it is waited for twice (32000 to the
+// row: 306 us for 800 MB of bf16 logits, 320 with it loaded). The tiles of a row that is read and
+// written at different alignments are loaded directly, from two vectors each.
 constexpr int kStages = 2;
 constexpr int kSmThreads = 1536;  // resident at 40 registers a thread
 
@@ -683,19 +684,25 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     return;
   }
   cluster_started(place.ctas);
-  // the row's whole tiles, and this CTA's: its j-th is tile cta + j ctas
-  const int whole = view.shift == 0 ? view.vectors / kTile : 0;
-  const int mine = whole > place.cta ? (whole - place.cta + place.ctas - 1) / place.ctas : 0;
+  // this CTA's tiles that go through shared memory: its j-th is tile cta + j ctas; the row's last
+  // tile may be cut
+  const int staged = view.shift == 0 ? view.vectors : 0;
+  const int tiles = (staged + kTile - 1) / kTile;
+  const int mine = tiles > place.cta ? (tiles - place.cta + place.ctas - 1) / place.ctas : 0;
+  const bool cut = staged % kTile != 0 && (tiles - 1) % place.ctas == place.cta;
+  const int whole = mine - cut;
   const int stride = place.ctas * kTile;
   const int own = place.cta * kTile + place.tid;
   const uint4* from = reinterpret_cast<const uint4*>(view.x + view.head) + own;
   uint4* to = reinterpret_cast<uint4*>(view.g + view.head) + own;
+  const auto has = [&](int i) { return own + whole * stride + i * kThreads < staged; };  // if cut
   const auto copy = [&](int j) {
     if (j >= 0 && j < mine) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
-        copy_async(stages + j % kStages * kTile + i * kThreads + place.tid,
-                   from + static_cast<int64_t>(j) * stride + i * kThreads);
+        if (j < whole || has(i))
+          copy_async(stages + j % kStages * kTile + i * kThreads + place.tid,
+                     from + static_cast<int64_t>(j) * stride + i * kThreads);
     }
     close_group();
   };
@@ -713,13 +720,21 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   }
 
   // the tiles that are loaded directly, and the single elements
-  const int rest = whole + (place.cta - whole % place.ctas + place.ctas) % place.ctas;
-  Part<A> part = thread_part(view, place, rest * kTile, k);
-  for (int j = 0; j < mine; ++j) {
+  Part<A> part = thread_part(view, place, staged ? staged : place.cta * kTile, k);
+  for (int j = 0; j < whole; ++j) {
     uint4 q[kBatch];
     fetch(j, q);
     copy(j + kStages);
     add_vectors<T>(part, q, k);
+  }
+  if (cut) {
+    uint4 q[kBatch];
+    fetch(whole, q);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (!has(i)) q[i] = no_vector<T>();
+    add_vectors<T>(part, q, k);
+    close_group();
   }
   part = join_warps<kThreads>(join_lanes<32>(part, k), k);
   // every warp takes the few steps to the coefficient by itself: one more barrier takes longer
@@ -732,7 +747,21 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   }
   if (!grad) return;
   const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
-  for (int j = mine - 1; j >= 0; --j) {
+  const auto write_target = [&](int j) {
+    write_target_of_tile<kThreads, kTile>(view, own - place.tid + j * stride, place.tid, slope);
+  };
+  if (cut) {
+    uint4 q[kBatch];
+    fetch(whole, q);
+    copy(whole - kStages);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (has(i))
+        store_once(to + static_cast<int64_t>(whole) * stride + i * kThreads,
+                   slope_vector<T>(q[i], slope));
+    write_target(whole);
+  }
+  for (int j = whole - 1; j >= 0; --j) {
     uint4 q[kBatch];
     fetch(j, q);
     copy(j - kStages);
@@ -740,12 +769,12 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     for (int i = 0; i < kBatch; ++i)
       store_once(to + static_cast<int64_t>(j) * stride + i * kThreads,
                  slope_vector<T>(q[i], slope));
-    write_target_of_tile<kThreads, kTile>(view, own - place.tid + j * stride, place.tid,
-                                                      slope);
+    write_target(j);
   }
   write_edge(view, place.edge(), slope);
-  for (int tile = rest * kTile; tile < view.vectors; tile += stride)
-    write_tile<kThreads>(view, tile, place.tid, slope);
+  if (staged == 0)
+    for (int tile = place.cta * kTile; tile < view.vectors; tile += stride)
+      write_tile<kThreads>(view, tile, place.tid, slope);
 }
 
 template <typename T, typename A, int kThreads>
@@ -853,8 +882,8 @@ int launch_warps(void (*kernel)(P...), int64_t rows, cudaStream_t st, const char
 
 // Rows of at most kWarpVectors vectors go to a warp each; of up to `most` of them where there are
 // enough rows to fill the GPU with warps. A CTA's start and join cost as much as some 1000 vectors:
-// 97656 x 4096 bf16, log-probabilities 133 us by warps and 342 by CTAs of 256 threads, their gradient
-// 272 and 358, the policy loss 421 and 779; 976 x 8192: 11.2 and 10.2 us.
+// 97656 x 4096 bf16, log-probabilities 126 us by warps and 342 by CTAs of 256 threads, their gradient
+// 272 and 358, the policy loss 380 and 779; 976 x 8192: 11.2 and 10.2 us.
 constexpr int kWarpVectors = 256;
 
 bool by_warps(int64_t rows, int64_t vectors, int64_t most, int sms) {
@@ -927,17 +956,18 @@ int launch_policy_rows(const Rows& a, const PolicyArgs<typename AccOf<T>::type>&
 }
 
 // By warps, or in CTAs of the more threads the longer the row: smaller ones have more rows in work,
-// which hides a row's start and join, larger ones less of both. 800 MB of bf16 logits, us with 128,
-// 256 and 512 threads (a warp): 8192 to the row 394, 449, 765 (392), 16384: 308, 320, 435 (382),
-// 32000: 331, 312, 390, 50021: 351, 318, 320, 65536: 304, 304, 280, 131072: 302, 306, 290. Rows whose
-// tiles are not whole lose more with 512 (100003: 314 with 256, 333 with 512).
+// which hides a row's start and join, larger ones less of both. 800 MB of bf16 logits, us: 8192 to
+// the row by warps 374, by 128 threads 431; 10000: 394, 449; 12000: 394, 403; 16384: 374, 331. By
+// 128, 256 and 512 threads 16384: 308, 320, 435, 32000: 331, 312, 390, 50021: 351, 318, 320, 65536:
+// 304, 304, 280, 131072: 302, 306, 290. Rows whose last tile is cut lose more with 512 (100003: 314
+// with 256, 333 with 512).
 template <typename T>
 int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, double inv_temp,
                   T* grad, cudaStream_t st) {
   using A = typename AccOf<T>::type;
   const int64_t vectors = a.vocab / RowView<T>::E;
   const int sms = sm_count();
-  if (by_warps(a.rows, vectors, 768, sms))
+  if (by_warps(a.rows, vectors, 1536, sms))
     return launch_clusters(policy_warp_kernel<T, A>, (a.rows + kRowWarps - 1) / kRowWarps, 1,
                            32 * kRowWarps, 0, true, st, "policy_warp_kernel launch", a, p, inv_temp,
                            exp_factor(A(0), inv_temp), grad);
