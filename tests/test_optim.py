@@ -334,6 +334,55 @@ def test_optimizer_groups_and_missing_gradients() -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_parameters_in_other_layouts(bits: int) -> None:
+    # stepped as their contiguous copies would be, bit for bit; what lies between is not touched
+    torch.manual_seed(0)
+    held = torch.randn(40, 1000, device="cuda")
+    before = held.clone()
+    params = [held.t()[:, :17], held[20:, 1::3], torch.randn(3, 5, device="cuda").expand(1, 3, 5)]
+    params = [p.detach().requires_grad_() for p in params]
+    copies = [p.detach().contiguous().clone().requires_grad_() for p in params]
+    a, b = (ti.AdamW(ps, lr=0.1, state_bits=bits) for ps in (params, copies))
+    for _ in range(3):
+        for p, c in zip(params, copies):
+            c.grad = torch.randn_like(c)
+            p.grad = c.grad.clone()
+        a.step()
+        b.step()
+    for p, c in zip(params, copies):
+        assert torch.equal(p, c)
+    assert torch.equal(held[17:20], before[17:20])
+    assert torch.equal(held[20:, ::3], before[20:, ::3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_optimizer_takes_over_a_state_of_torch(dtype: torch.dtype) -> None:
+    p = torch.randn(300, device="cuda", dtype=dtype).requires_grad_()
+    theirs = torch.optim.AdamW([p], lr=0.01)
+    for _ in range(3):
+        p.grad = torch.randn_like(p)
+        theirs.step()
+    ours = ti.AdamW([p], lr=0.5)
+    ours.load_state_dict(theirs.state_dict())
+    state, was = ours.state[p], theirs.state[p]
+    assert state["step"] == 3 and ours.param_groups[0]["lr"] == 0.01
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert state[name].dtype == torch.float32
+        assert torch.equal(state[name], was[name].float())
+    want = [p.detach().clone()], [state["exp_avg"].clone()], [state["exp_avg_sq"].clone()]
+    p.grad = torch.randn_like(p)
+    ti.adamw_step(want[0], [p.grad], want[1], want[2], step=4, lr=0.01)
+    ours.step()
+    assert torch.equal(p, want[0][0])
+    bad = theirs.state_dict()
+    bad["param_groups"][0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        ours.load_state_dict(bad)
+
+
+@pytest.mark.gpu
 def test_a_step_counts_as_a_change_in_place() -> None:
     p = torch.nn.Parameter(torch.ones(5, device="cuda"))
     q = (p * p).sum()  # keeps p for its gradient

@@ -66,7 +66,8 @@ class AdamW(torch.optim.Optimizer):
     for each pair of parameter and gradient types (480 tensors a launch).
 
     ``state_bits``: 32, or 8 for float8 moments (see the module). ``seed``: of their rounding.
-    Learning rate, betas, eps and weight decay are per group. ``state_dict`` and
+    Learning rate, betas, eps and weight decay are per group. A parameter that is not contiguous is
+    stepped as a contiguous copy, written back. ``state_dict`` and
     ``load_state_dict`` keep the states' types, so a run resumes exactly.
     """
 
@@ -121,20 +122,39 @@ class AdamW(torch.optim.Optimizer):
                 if bits == 8:
                     scales = tuple([s[name] for s in states]
                                    for name in ("exp_avg_scale", "exp_avg_sq_scale"))
-                adamw_step(params, [p.grad.contiguous() for p in params],
+                values = [p if p.is_contiguous() else p.contiguous() for p in params]
+                adamw_step(values, [p.grad.contiguous() for p in params],
                            [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                            step=step, lr=float(group["lr"]), betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"], scales=scales,
                            seed=group["seed"])
+                for p, value in zip(params, values):
+                    if value is not p:
+                        p.copy_(value)
         return loss
+
+    def __setstate__(self, state: dict[str, Any]) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
+            group.setdefault("seed", 0)
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
-        """As torch's, but for the states' types: torch casts them to their parameter's."""
+        """As torch's, but for the states' types: torch casts them to their parameter's. Also takes
+        a state of ``torch.optim.AdamW`` (the moments become float32), without its ``amsgrad`` and
+        ``maximize``."""
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("AdamW has no amsgrad and no maximize")
         super().load_state_dict(state_dict)
         saved = chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = chain.from_iterable(g["params"] for g in self.param_groups)
         for index, p in zip(saved, params):
             for name, value in state_dict["state"].get(index, {}).items():
-                if isinstance(value, Tensor):
-                    self.state[p][name] = value.to(device=p.device, copy=True)
+                if name == "step":
+                    self.state[p][name] = int(value)
+                elif isinstance(value, Tensor):
+                    kept = value.dtype in (torch.float32, torch.float8_e4m3fn)
+                    self.state[p][name] = value.to(
+                        p.device, value.dtype if kept else torch.float32, copy=True,
+                        memory_format=torch.contiguous_format)
