@@ -5,7 +5,9 @@
 // time, 54 of them for an autograd function that does nothing; most of the rest was the interpreter,
 // in the forward and, after a hand-over of its lock, in the autograd engine's thread.
 //
-// Arguments come checked by losses.py; those of adamw, lists of tensors, are checked here.
+// The losses take their arguments as they are given and answer None where one of them is to be
+// converted or refused, which losses.py does (checked there first, a call took 2 to 6 us more);
+// adamw's, lists of tensors, are checked here.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -57,6 +59,25 @@ Tensor empty(const Tensor& like, at::IntArrayRef sizes, ScalarType type) {
 
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+
+// A Python object's tensor, or NULL for another object.
+const Tensor* tensor_in(py::handle h) {
+  return THPVariable_Check(h.ptr()) ? &THPVariable_Unpack(h.ptr()) : nullptr;
+}
+
+// Whether a tensor needs no conversion: of this type, contiguous, and where and of the sizes that go
+// with the others.
+bool ready(const Tensor* t, ScalarType type, at::IntArrayRef sizes, at::Device device) {
+  return t && t->scalar_type() == type && t->device() == device && t->sizes() == sizes &&
+         t->is_contiguous();
+}
+
+bool ready_logits(const Tensor* x, const Tensor* targets, double temperature) {
+  if (!x || !x->is_cuda() || x->dim() < 1 || x->size(-1) < 1 || !(temperature > 0)) return false;
+  const ScalarType type = x->scalar_type();
+  return (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat || type == at::kDouble) &&
+         ready(targets, at::kLong, x->sizes().slice(0, x->dim() - 1), x->device());
 }
 
 // x ([..., vocab]) as rows of logits, and the tensor whose memory they are: x itself when its last
@@ -133,11 +154,13 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
   }
 };
 
-Tensor token_logprobs(const Tensor& x, const Tensor& targets, double temperature,
-                      int64_t ignore_index) {
-  if (x.requires_grad() && at::GradMode::is_enabled())
-    return Logprobs::apply(x, targets, temperature, ignore_index);
-  return std::get<0>(logprobs(x, targets, temperature, ignore_index, false));
+std::optional<Tensor> token_logprobs(py::handle logits, py::handle y, double temperature,
+                                     int64_t ignore_index) {
+  const Tensor *x = tensor_in(logits), *targets = tensor_in(y);
+  if (!ready_logits(x, targets, temperature)) return std::nullopt;
+  if (x->requires_grad() && at::GradMode::is_enabled())
+    return Logprobs::apply(*x, *targets, temperature, ignore_index);
+  return std::get<0>(logprobs(*x, *targets, temperature, ignore_index, false));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -225,19 +248,40 @@ struct Preference : torch::autograd::Function<Preference> {
   }
 };
 
-std::tuple<Tensor, Tensor> preference_loss(const Tensor& logps, const std::optional<Tensor>& refs,
-                                           const std::optional<Tensor>& mask, const Tensor& offsets,
-                                           int64_t kind, bool average, double beta,
-                                           double label_smoothing, double margin) {
+std::optional<std::tuple<Tensor, Tensor>> preference_loss(py::handle of_logps, py::handle of_refs,
+                                                          py::handle of_mask, py::handle of_offsets,
+                                                          int64_t kind, bool average, double beta,
+                                                          double label_smoothing, double margin) {
+  const Tensor *logps = tensor_in(of_logps), *offsets = tensor_in(of_offsets);
+  if (!logps || !logps->is_cuda() || logps->dim() != 1 || !offsets || offsets->dim() != 1 ||
+      offsets->numel() < 3 || offsets->numel() % 2 == 0)
+    return std::nullopt;
+  const ScalarType type = logps->scalar_type();
+  const at::Device device = logps->device();
+  if (kind < 0 || !(beta > 0) || !(label_smoothing >= 0 && label_smoothing < 0.5) ||
+      (type != at::kFloat && type != at::kDouble) || !ready(logps, type, logps->sizes(), device) ||
+      !ready(offsets, at::kLong, offsets->sizes(), device))
+    return std::nullopt;
+  std::optional<Tensor> refs, mask;
+  if (!of_refs.is_none()) {
+    const Tensor* t = tensor_in(of_refs);
+    if (!ready(t, type, logps->sizes(), device)) return std::nullopt;
+    refs = *t;
+  }
+  if (!of_mask.is_none()) {
+    const Tensor* t = tensor_in(of_mask);
+    if (!ready(t, at::kBool, logps->sizes(), device)) return std::nullopt;
+    mask = *t;
+  }
   if (at::GradMode::is_enabled() &&
-      (logps.requires_grad() || (refs.has_value() && refs->requires_grad()))) {
-    const variable_list out = Preference::apply(logps, refs, mask, offsets, kind, average, beta,
+      (logps->requires_grad() || (refs.has_value() && refs->requires_grad()))) {
+    const variable_list out = Preference::apply(*logps, refs, mask, *offsets, kind, average, beta,
                                                 label_smoothing, margin);
-    return {out[0], out[1]};
+    return std::make_tuple(out[0], out[1]);
   }
   auto [loss, rewards, coef] =
-      Preference::run(logps, refs, mask, offsets, kind, average, beta, label_smoothing, margin);
-  return {loss, rewards};
+      Preference::run(*logps, refs, mask, *offsets, kind, average, beta, label_smoothing, margin);
+  return std::make_tuple(loss, rewards);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -336,19 +380,43 @@ struct Policy : torch::autograd::Function<Policy> {
   }
 };
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(
-    const Tensor& x, const Tensor& targets, int64_t ignore_index, double temperature,
-    const Tensor& old_logps, const Tensor& advantages, const std::optional<Tensor>& ref_logps,
-    const std::optional<Tensor>& weight, double clip_low, double clip_high, double kl_coef) {
-  const PolicySettings s{targets,      old_logps,   advantages, ref_logps, weight,
-                         ignore_index, temperature, clip_low,   clip_high, kl_coef};
-  if (x.requires_grad() && at::GradMode::is_enabled()) {
-    const variable_list out = Policy::apply(x, s);
-    return {out[0], out[3], out[1], out[2]};
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> policy_loss(
+    py::handle logits, py::handle y, int64_t ignore_index, double temperature, py::handle old_logps,
+    py::handle advantages, py::handle ref_logps, py::handle weight, double clip_low,
+    double clip_high, double kl_coef) {
+  const Tensor *x = tensor_in(logits), *targets = tensor_in(y);
+  if (!ready_logits(x, targets, temperature) || !(clip_low >= 0 && clip_high >= 0))
+    return std::nullopt;
+  const bool grad_mode = at::GradMode::is_enabled();
+  const auto constant = [&](py::handle h, bool may_be_bool) -> const Tensor* {
+    const Tensor* t = tensor_in(h);
+    const bool is_bool = may_be_bool && t && t->scalar_type() == at::kBool;
+    return ready(t, is_bool ? at::kBool : acc_of(*x), targets->sizes(), x->device()) &&
+                   !(grad_mode && t->requires_grad())
+               ? t
+               : nullptr;
+  };
+  const Tensor *old = constant(old_logps, false), *adv = constant(advantages, false);
+  if (!old || !adv) return std::nullopt;
+  PolicySettings s{*targets,     *old,        *adv,     std::nullopt, std::nullopt,
+                   ignore_index, temperature, clip_low, clip_high,    kl_coef};
+  if (!ref_logps.is_none()) {
+    const Tensor* t = constant(ref_logps, false);
+    if (!t) return std::nullopt;
+    s.ref_logps = *t;
   }
-  const PolicyResult r = policy(x, s, false);
+  if (!weight.is_none()) {
+    const Tensor* t = constant(weight, true);
+    if (!t) return std::nullopt;
+    s.weight = *t;
+  }
+  if (x->requires_grad() && grad_mode) {
+    const variable_list out = Policy::apply(*x, s);
+    return std::make_tuple(out[0], out[3], out[1], out[2]);
+  }
+  const PolicyResult r = policy(*x, s, false);
   const auto out = r.out.unbind();
-  return {out[0], r.logps, out[1], out[2]};
+  return std::make_tuple(out[0], r.logps, out[1], out[2]);
 }
 
 // ---------------------------------------------------------------------------------------------

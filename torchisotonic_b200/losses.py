@@ -60,11 +60,17 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     A cut along the length (``logits[:, :-1]``) or a padded vocabulary (``logits[..., :v]``) is
     read in place.
     """
+    traced = torch.compiler.is_compiling()
+    settings = float(temperature), int(ignore_index)
+    if not traced:
+        got = _ext.native().token_logprobs(logits, targets, *settings)
+        if got is not None:
+            return got
     _check_logits(logits, targets, temperature)
     targets = _as(targets, torch.int64)
-    if torch.compiler.is_compiling():  # traced: the operators, which the compiler keeps whole
-        return ops.token_logprobs(logits, targets, float(temperature), int(ignore_index))[0]
-    return _ext.native().token_logprobs(logits, targets, float(temperature), int(ignore_index))
+    if traced:  # the operators, which the compiler keeps whole
+        return ops.token_logprobs(logits, targets, *settings)[0]
+    return _ext.native().token_logprobs(logits, targets, *settings)
 
 
 def preference_loss(
@@ -97,6 +103,13 @@ def preference_loss(
     gradient: ``rewards[0] - rewards[1]`` are the margins that a calibration curve is fitted on.
     float32 (float64 for float64 logps); sums are float64 in a fixed order.
     """
+    traced = torch.compiler.is_compiling()
+    settings = (_ext.PREFERENCE_KINDS.get(kind, -1), bool(average), float(beta),
+                float(label_smoothing), float(margin))
+    if not traced:
+        got = _ext.native().preference_loss(logps, ref_logps, mask, offsets, *settings)
+        if got is not None:
+            return got
     if not isinstance(logps, Tensor) or not isinstance(offsets, Tensor):
         raise TypeError("logps and offsets must be torch.Tensors")
     if not logps.is_floating_point():
@@ -130,10 +143,8 @@ def preference_loss(
         mask = mask.contiguous()
     if offsets.device != dev:
         raise ValueError("offsets must be on logps' device")
-    settings = (_ext.PREFERENCE_KINDS[kind], bool(average), float(beta), float(label_smoothing),
-                float(margin))
     logps, offsets = _as(logps, dtype), _as(offsets, torch.int64)
-    if torch.compiler.is_compiling():
+    if traced:
         loss, rewards, _ = ops.preference(logps, ref_logps, mask, offsets, *settings)
         return loss, rewards.detach()
     return _ext.native().preference_loss(logps, ref_logps, mask, offsets, *settings)
@@ -179,6 +190,14 @@ def policy_loss(
     ``logits`` alone; the tokens' log-probabilities (0 where left out); the weighted means of
     ``exp(d) - d - 1`` and of where the clip holds. float32 (float64 for float64 logits).
     """
+    traced = torch.compiler.is_compiling()
+    rows = int(ignore_index), float(temperature)
+    clip = float(clip_low), float(clip_high), float(kl_coef)
+    if not traced:
+        got = _ext.native().policy_loss(logits, targets, *rows, old_logps, advantages, ref_logps,
+                                        weight, *clip)
+        if got is not None:
+            return PolicyLoss(*got)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError("clip_low and clip_high must not be negative")
     _check_logits(logits, targets, temperature)
@@ -198,14 +217,9 @@ def policy_loss(
     ref_logps = None if ref_logps is None else constant("ref_logps", ref_logps)
     weight = None if weight is None else constant("weight", weight)
     targets = _as(targets, torch.int64)
-    temperature = float(temperature)
-
-    settings = (old_logps, advantages, ref_logps, weight, float(clip_low), float(clip_high),
-                float(kl_coef))
-    if torch.compiler.is_compiling():
-        out, logps, _ = ops.policy(logits, targets, int(ignore_index), temperature, *settings)
+    constants = old_logps, advantages, ref_logps, weight
+    if traced:
+        out, logps, _ = ops.policy(logits, targets, *rows, *constants, *clip)
         rest = out.detach()
         return PolicyLoss(out[0], logps.detach(), rest[1], rest[2])
-
-    return PolicyLoss(*_ext.native().policy_loss(logits, targets, int(ignore_index), temperature,
-                                                 *settings))
+    return PolicyLoss(*_ext.native().policy_loss(logits, targets, *rows, *constants, *clip))
