@@ -120,9 +120,12 @@ __device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kT
 }
 
 // The CTAs of a cluster write to one another's shared memory once, at their joins. Before that each
-// has to have started: says that this one has.
+// has to have started: says that this one has (and nothing about memory: relaxed).
 __device__ __forceinline__ void cluster_started(int ctas) {
-  if (ctas > 1) cg::this_cluster().barrier_arrive();
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_start() {
+  asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
 // The parts of all of a row's warps joined (a warp's lanes hold the same); every thread gets the
@@ -140,7 +143,7 @@ __device__ __forceinline__ Part<A> join_warps(Part<A> p, A k) {
     auto cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks());
     if (ctas > 1) {
-      cluster.barrier_wait();
+      wait_for_start();
       if (threadIdx.x < ctas)
         *cluster.map_shared_rank(&of_cta[cluster.block_rank()], threadIdx.x) = p;
       cluster.sync();
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kTotalThreads) policy_total_kernel(Rows a, Pol
   }
   sum = block_sum(sum, shared);
   if (gridDim.x > 1) {
-    cluster.barrier_wait();
+    wait_for_start();
     if (threadIdx.x == 0) *cluster.map_shared_rank(&sums[blockIdx.x], 0) = sum;
     cluster.sync();
     sum = 0;
@@ -645,10 +648,10 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 }
 
 // Loss and gradient in one launch: the row's sum, the token's coefficient, then the row's gradient
-// from a second read that does not reach memory. 8192 x 131072, a tenth of them left out, in 780 us:
-// 4.4 GB of DRAM traffic, 8 % over each byte once, at 86 % of the copy bandwidth; the exponential
-// unit is busy 58 % of the time, and what is missing are the joins between a row's two passes (of a
-// CTA's 20 us about 5), which two other CTAs of the SM fill in part.
+// from a second read that does not reach memory. 4000 x 131072, a tenth of them left out, in 376 us:
+// 2.07 GB of DRAM traffic, 5 % over each byte once, at 84 % of the copy bandwidth; 8192 rows in 850 to
+// 880 us. The exponential unit is busy 63 % of the time, and what is missing are the joins between a
+// row's two passes (of a CTA's 20 us about 5), which two other CTAs of the SM fill in part.
 //
 // A cluster's CTAs take a row's tiles in turn, a tile kBatch vectors a thread. Tiles come through
 // kStages places of shared memory, each thread copying and reading its own vectors there (no
@@ -697,12 +700,16 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   uint4* to = reinterpret_cast<uint4*>(view.g + view.head) + own;
   const auto has = [&](int i) { return own + whole * stride + i * kThreads < staged; };  // if cut
   const auto copy = [&](int j) {
-    if (j >= 0 && j < mine) {
+    uint4* at = stages + static_cast<unsigned>(j) % kStages * kTile + place.tid;
+    if (j >= 0 && j < whole) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
-        if (j < whole || has(i))
-          copy_async(stages + j % kStages * kTile + i * kThreads + place.tid,
-                     from + static_cast<int64_t>(j) * stride + i * kThreads);
+        copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
+    } else if (cut && j == whole) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (has(i))
+          copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
     }
     close_group();
   };
@@ -710,7 +717,7 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      q[i] = stages[j % kStages * kTile + i * kThreads + place.tid];
+      q[i] = stages[static_cast<unsigned>(j) % kStages * kTile + i * kThreads + place.tid];
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) copy(j);
