@@ -12,6 +12,8 @@ come the roundings of the outputs to their types. float64: the same with 2^-53.
 from __future__ import annotations
 
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -430,6 +432,29 @@ def test_preference_strided_and_shared() -> None:
     w = torch.tensor(-0.7, dtype=torch.float64, requires_grad=True)
     (gw,) = torch.autograd.grad(plain_preference(w.expand(220), None, offsets, beta=0.01)[0], w)
     check(g, gw, 0.0, 220 * 2.0**-22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[400_000, 0], [1, 400_000], [0, 1, 300_000, 0],
+                                     [90_001, 1, 0, 5, 70_000, 2048]], ids=str)
+def test_preference_long_answers_beside_short_ones(lengths) -> None:
+    # several CTAs to an answer, of which most have no token where the answer is short
+    for average in (False, True):
+        check_preference(*sequences(lengths, seed=len(lengths)), average=average, beta=0.01)
+
+
+def test_remote_shared_memory_is_written_after_its_cluster_has_started() -> None:
+    # a CTA that has not started has no shared memory to write to
+    sources = sorted((Path(_ext.__file__).parent / "csrc").glob("*.cu*"))
+    found = 0
+    for source in sources:
+        for body in re.split(r"\n}\n", source.read_text()):  # a function each
+            write = body.find("map_shared_rank")
+            if write < 0:
+                continue
+            found += 1
+            assert 0 <= body.find("wait_for_start()") < write, source.name
+    assert found == 3
 
 
 # ---------------------------------------------------------------------------------------------

@@ -11,6 +11,7 @@
 #include <string>
 #include <utility>
 
+#include "cta.cuh"
 #include "entry.cuh"
 #include "logits.cuh"
 
@@ -117,15 +118,6 @@ __device__ __forceinline__ Part<A> thread_part(const RowView<T>& r, const Place<
 template <int kThreads, typename T, typename A>
 __device__ __forceinline__ Part<A> warp_part(const RowView<T>& r, const Place<kThreads>& place, A k) {
   return join_lanes<32>(thread_part(r, place, place.cta * kBatch * kThreads, k), k);
-}
-
-// The CTAs of a cluster write to one another's shared memory once, at their joins. Before that each
-// has to have started: says that this one has (and nothing about memory: relaxed).
-__device__ __forceinline__ void cluster_started(int ctas) {
-  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
-}
-__device__ __forceinline__ void wait_for_start() {
-  asm volatile("barrier.cluster.wait;" ::: "memory");
 }
 
 // The parts of all of a row's warps joined (a warp's lanes hold the same); every thread gets the
@@ -393,18 +385,6 @@ __device__ __forceinline__ A weight_of(const Rows& a, const PolicyArgs<A>& p, in
     w = static_cast<const A*>(p.weight)[r];
   }
   return target == a.ignore ? A(0) : w;
-}
-
-// The sum of v over the CTA in a fixed order (thread 0 has it).
-__device__ double block_sum(double v, double* shared) {
-  for (int d = 16; d; d >>= 1) v += __shfl_down_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = threadIdx.x < blockDim.x / 32 ? shared[threadIdx.x] : 0.0;
-  if (threadIdx.x < 32)
-    for (int d = 16; d; d >>= 1) v += __shfl_down_sync(0xffffffffu, v, d);
-  __syncthreads();
-  return v;
 }
 
 // The sum of the weights, by a CTA, or a cluster of them where there are many rows, ahead of the

@@ -16,6 +16,7 @@
 
 #include <string>
 
+#include "cta.cuh"
 #include "entry.cuh"
 
 namespace tiso {
@@ -42,17 +43,6 @@ __device__ __forceinline__ int64_t cut(int64_t v, int64_t lo, int64_t hi) {
   return v < lo ? lo : v > hi ? hi : v;
 }
 
-__device__ double block_sum(double v, double* shared) {
-  for (int d = 16; d; d >>= 1) v += __shfl_down_sync(0xffffffffu, v, d);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = threadIdx.x < blockDim.x / 32 ? shared[threadIdx.x] : 0.0;
-  if (threadIdx.x < 32)
-    for (int d = 16; d; d >>= 1) v += __shfl_down_sync(0xffffffffu, v, d);
-  __syncthreads();
-  return v;
-}
-
 // A cluster of CTAs (one, where there are many sequences) to a sequence: the sum and number of its
 // unmasked tokens. A masked token is read but not used in any way (its value may be NaN).
 template <typename A, int kT>
@@ -62,6 +52,7 @@ __global__ void __launch_bounds__(kT) pref_sum_kernel(PrefArgs<A> a) {
   auto cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
+  cluster_started(ctas);
   const int64_t k = blockIdx.x / ctas;
   const int64_t begin = cut(a.offsets[k], 0, a.tokens);
   const int64_t end = cut(a.offsets[k + 1], begin, a.tokens);
@@ -90,6 +81,7 @@ __global__ void __launch_bounds__(kT) pref_sum_kernel(PrefArgs<A> a) {
   sum = block_sum(sum, shared);
   count = block_sum(count, shared);
   if (ctas > 1) {
+    wait_for_start();
     if (threadIdx.x == 0) {
       *cluster.map_shared_rank(&sums[rank], 0) = sum;
       *cluster.map_shared_rank(&counts[rank], 0) = count;
