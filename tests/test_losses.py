@@ -651,6 +651,88 @@ def test_policy_not_finite() -> None:
     assert got.loss.isnan() and got.logps.isnan().tolist() == [False, False, True] + [False] * 3
 
 
+FAR = [95.0, 1e4, math.inf]  # beyond float's exponential (88.7), double's (709.8), and any
+
+
+def far_tokens(vocab, dtype):
+    """Six rows; the third is the one whose old or reference log-probability a test moves."""
+    x, y, _ = logits_of((6, vocab), dtype, seed=vocab)
+    old, adv, ref = tokens_of(x, y, vocab)
+    lp = plain_logprobs(x, y).to(old.dtype)
+    others = torch.arange(6, device="cuda") != 2
+    return x, y, old, adv, ref, lp, others
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("vocab", [40, 5000, 70001])
+def test_policy_ratio_of_any_size(vocab: int, dtype: torch.dtype, far: float) -> None:
+    # A token that the old policy all but excluded. With a positive advantage the clip holds: the
+    # loss is -(1 + clip_high) A, the slope 0. With a negative one nothing does: the loss is rho |A|,
+    # infinite where its type has no room for it; the other rows' gradients are not touched.
+    x, y, old, adv, _, lp, others = far_tokens(vocab, dtype)
+    acc, e = old.dtype, lp_atol(dtype, vocab)
+    old[2] = lp[2] - far
+    for a in (1.5, -1.5):
+        adv[2] = a
+        leaf = x.detach().requires_grad_()
+        got = ti.policy_loss(leaf, y, old, adv)
+        (gx,) = torch.autograd.grad(got.loss, leaf)
+        p = torch.softmax(x.double(), -1)
+        rho = torch.exp(plain_logprobs(x, y) - old.double())
+        free, held = rho * adv.double(), rho.clamp(0.8, 1.2) * adv.double()
+        slope = torch.where(free > held, torch.zeros_like(rho), -free) / 6
+        want = -torch.minimum(free, held).mean()
+        gw = slope[:, None] * (torch.nn.functional.one_hot(y, vocab) - p)
+        check(got.logps, plain_logprobs(x, y), e, 2 * unit(dtype))
+        check(got.clip_fraction, (free > held).double().mean(), 0.0, 8 * unit(dtype))
+        rows = others if a < 0 else slice(None)
+        if not torch.isfinite(gw[2].to(acc)).all():
+            assert gx[2, y[2]] == math.inf
+        check(gx[rows], gw[rows], 80 / 6 * (e + unit(dtype) * (80 + vocab / 256)),
+              HALF_ULP[dtype] * 1.01)
+        # rho |A| is off by its exponent's error, which is that of lp
+        check(got.loss, want.to(acc), 40 * e, (2 * e + 8 * unit(dtype)) if a < 0 else 8 * unit(dtype))
+        if a > 0:
+            assert (gx[2] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("vocab", [40, 5000, 70001])
+def test_policy_reference_of_any_size(vocab: int, dtype: torch.dtype, far: float) -> None:
+    # a token that the reference all but excludes costs its distance, one that only the policy
+    # excludes has no bound: infinite, not NaN, and not in the other rows
+    x, y, old, adv, ref, lp, others = far_tokens(vocab, dtype)
+    acc, e = old.dtype, lp_atol(dtype, vocab)
+    plain = plain_logprobs(x, y)
+    p = torch.softmax(x.double(), -1)
+    rho = torch.exp(plain - old.double())
+    free, held = rho * adv.double(), rho.clamp(0.8, 1.2) * adv.double()
+    for moved in (-far, far if far < math.inf else 1e300):
+        if moved > torch.finfo(acc).max:
+            continue
+        ref[2] = lp[2] + moved
+        leaf = x.detach().requires_grad_()
+        got = ti.policy_loss(leaf, y, old, adv, ref_logps=ref, kl_coef=0.1)
+        (gx,) = torch.autograd.grad(got.loss, leaf)
+        d = ref.double() - plain
+        kl = torch.expm1(d) - d
+        slope = (torch.where(free > held, torch.zeros_like(rho), -free) - 0.1 * torch.expm1(d)) / 6
+        gw = slope[:, None] * (torch.nn.functional.one_hot(y, vocab) - p)
+        rows = others if moved > 0 else slice(None)
+        if not torch.isfinite(gw[2].to(acc)).all():
+            assert gx[2, y[2]] == -math.inf
+        check(gx[rows], gw[rows], 80 / 6 * (e + unit(dtype) * (80 + vocab / 256)),
+              HALF_ULP[dtype] * 1.01)
+        rtol = 2 * e + 8 * unit(dtype)
+        check(got.kl, kl.mean().to(acc), 40 * e, rtol)
+        check(got.loss, (0.1 * kl - torch.minimum(free, held)).mean().to(acc), 40 * e, rtol)
+        check(got.logps, plain, e, 2 * unit(dtype))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 9), (3, 1100)])
 def test_policy_gradcheck(shape) -> None:

@@ -176,8 +176,9 @@ struct Slope {
     target = in ? static_cast<int>(target_) : -1;
     scale = in ? -static_cast<A>(c_) / s : nan_of(A(0));
   }
+  // (a coefficient that the type has no room for is infinite in its own direction)
   __device__ __forceinline__ A at_target(A d) const {
-    return static_cast<A>(__dadd_rn(c, static_cast<double>(d)));
+    return static_cast<A>(isinf(d) ? c : __dadd_rn(c, static_cast<double>(d)));
   }
   __device__ __forceinline__ A at(A x, int v) const {
     const A d = mul_rn(scaled_exp(x - base, k), scale);
@@ -481,7 +482,8 @@ struct TokenInput {
   }
 };
 
-// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest).
+// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest;
+// for |d| < kFar).
 __device__ __forceinline__ float exp_as(float, double d) {
   const float hi = static_cast<float>(d);
   const float lo = static_cast<double>(hi) == d ? 0.0f : static_cast<float>(d - hi);
@@ -489,6 +491,21 @@ __device__ __forceinline__ float exp_as(float, double d) {
   return __fmaf_rn(e, lo, e);
 }
 __device__ __forceinline__ double exp_as(double, double d) { return exp(d); }
+
+// exp(d) / s and exp(d) s, s a row's sum (up to 2^30). Beyond e^+-60 float has no room for them, nor
+// for exp(d) on the way: a token that the old policy all but excluded has a ratio of any size, which
+// the clip then cuts.
+constexpr double kFar = 60.0;
+template <typename A>
+__device__ __forceinline__ double exp_over(double d, A s) {
+  if (fabs(d) < kFar) return exp_as(A(0), d) / s;
+  return exp(d - log(static_cast<double>(s)));
+}
+template <typename A>
+__device__ __forceinline__ double exp_times(double d, A s) {
+  if (fabs(d) < kFar) return exp_as(A(0), d) * s;
+  return exp(d + log(static_cast<double>(s)));
+}
 
 // A token's loss and its slope d loss / d logp (both without the token's weight):
 //   rho = exp(logp - old);  loss = -min(rho A, clip(rho) A) + kl_coef kl,
@@ -505,13 +522,12 @@ struct Token {
   __device__ __forceinline__ Token(const PolicyArgs<A>& p, const TokenInput<A>& in,
                                    const Part<A>& part, double inv_temp) {
     t = (static_cast<double>(in.logit) - static_cast<double>(base_of(part.m))) * inv_temp;
-    ratio = exp_as(A(0), t - static_cast<double>(in.old)) / part.s;
+    ratio = exp_over(t - static_cast<double>(in.old), part.s);
     free_side = ratio * static_cast<double>(in.adv);
     held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * static_cast<double>(in.adv);
     double slope = free_side > held ? 0.0 : -free_side;
     if (p.ref_logps)
-      slope += p.kl_coef * (1.0 - static_cast<double>(
-                                      exp_as(A(0), static_cast<double>(in.ref) - t) * part.s));
+      slope += p.kl_coef * (1.0 - exp_times(static_cast<double>(in.ref) - t, part.s));
     coef = in.total != 0 ? static_cast<double>(in.w) / in.total * slope : 0.0;
   }
 
