@@ -262,7 +262,8 @@ int tiso_policy_workspace_size(int dtype, int64_t rows, size_t* bytes);
  * it is read beyond its weight and target, its logps, coef and gradient are 0. coef[r] receives
  * d loss / d logps[r] in double, stats what tiso_logprobs_grad needs; grad ([rows][vocab], contiguous)
  * coef[r] / temperature (1[v = targets[r]] - softmax). Where both sides of the minimum are equal
- * the slope is that of the unclipped one. Sums run in a fixed order. */
+ * the slope is that of the unclipped one. A factor of 0 (A, kl_coef) leaves its term out, whatever
+ * overflows in the other one. Sums run in a fixed order. */
 int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
                 double temperature, const tiso_policy_args* args, void* logps, double* coef,
                 void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,

@@ -734,6 +734,43 @@ def test_policy_reference_of_any_size(vocab: int, dtype: torch.dtype, far: float
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64])
+@pytest.mark.parametrize("vocab", [40, 5000, 70001])
+def test_policy_terms_with_a_factor_of_zero(vocab: int, dtype: torch.dtype, far: float) -> None:
+    x, y, old, adv, ref, lp, others = far_tokens(vocab, dtype)
+    e = lp_atol(dtype, vocab)
+
+    def run(old, adv, x=x, **settings):
+        leaf = x.detach().requires_grad_()
+        got = ti.policy_loss(leaf, y, old, adv, **settings)
+        return (got, *torch.autograd.grad(got.loss, leaf))
+
+    # no advantage: neither loss nor gradient, however large the ratio
+    far_old, no_adv = old.clone(), adv.clone()
+    far_old[2], no_adv[2] = lp[2] - far, 0.0
+    got, gx = run(far_old, no_adv)
+    want, gw = run(old, no_adv)
+    assert torch.equal(got.loss, want.loss) and torch.equal(got.clip_fraction, want.clip_fraction)
+    assert torch.equal(gx, gw) and (gx[2] == 0).all()
+    # the KL term only watched: it is not in the loss, however large
+    want, gw = run(old, adv)
+    far_ref = ref.clone()
+    far_ref[2] = lp[2] + min(far, 1e30)
+    got, gx = run(old, adv, ref_logps=far_ref)
+    assert torch.equal(got.loss, want.loss) and torch.equal(gx, gw)
+    d = far_ref.double() - plain_logprobs(x, y)
+    check(got.kl, (torch.expm1(d) - d).mean().to(old.dtype), 40 * e, 2 * e + 8 * unit(dtype))
+    # a target that the policy excludes: its ratio is 0, its distance to the reference infinite
+    masked = x.clone()
+    masked[2, y[2]] = -math.inf
+    want, gw = run(old, adv, masked)
+    got, gx = run(old, adv, masked, ref_logps=ref)
+    assert torch.isfinite(got.loss) and torch.equal(got.loss, want.loss) and torch.equal(gx, gw)
+    assert got.kl == math.inf
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 9), (3, 1100)])
 def test_policy_gradcheck(shape) -> None:
     x, y, _ = logits_of(shape, torch.float64, scale=1.0)

@@ -523,10 +523,11 @@ struct Token {
                                    const Part<A>& part, double inv_temp) {
     t = (static_cast<double>(in.logit) - static_cast<double>(base_of(part.m))) * inv_temp;
     ratio = exp_over(t - static_cast<double>(in.old), part.s);
-    free_side = ratio * static_cast<double>(in.adv);
+    // a factor of 0 leaves its term out, whatever overflowed in the other one
+    free_side = in.adv == A(0) && isinf(ratio) ? 0.0 : ratio * static_cast<double>(in.adv);
     held = (ratio < p.lo ? p.lo : ratio > p.hi ? p.hi : ratio) * static_cast<double>(in.adv);
     double slope = free_side > held ? 0.0 : -free_side;
-    if (p.ref_logps)
+    if (p.ref_logps && p.kl_coef != 0)
       slope += p.kl_coef * (1.0 - exp_times(static_cast<double>(in.ref) - t, part.s));
     coef = in.total != 0 ? static_cast<double>(in.w) / in.total * slope : 0.0;
   }
@@ -538,8 +539,8 @@ struct Token {
     double loss = -(free_side > held ? held : free_side), kl = 0.0;
     if (p.ref_logps) {
       const double d = static_cast<double>(in.ref) - lp;
-      kl = expm1(d) - d;
-      loss += p.kl_coef * kl;
+      kl = isinf(d) ? static_cast<double>(INFINITY) : expm1(d) - d;
+      if (p.kl_coef != 0) loss += p.kl_coef * kl;
     }
     p.logps[r] = static_cast<A>(lp);
     p.coef[r] = coef;

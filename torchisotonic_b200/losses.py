@@ -184,7 +184,8 @@ def policy_loss(
     ``logits``: [..., vocab]; every other tensor has the targets' shape [...]. ``weight``: numbers,
     or a bool mask; None for 1. A token of weight 0 (or with target ``ignore_index``) is left out:
     nothing else of it is read, its gradient is 0. Where both sides of the minimum are equal the
-    gradient is the unclipped side's.
+    gradient is the unclipped side's. A ratio or a ``kl_coef`` term beyond the type's range is
+    infinite; a factor of 0 (the advantage, ``kl_coef``) leaves its term out also there.
 
     Returns ``PolicyLoss(loss, logps, kl, clip_fraction)``: the loss, differentiable (once) in
     ``logits`` alone; the tokens' log-probabilities (0 where left out); the weighted means of
