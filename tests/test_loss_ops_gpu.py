@@ -42,6 +42,72 @@ def test_opcheck() -> None:
     torch.library.opcheck(ops.policy, (leaf, y, -100, 0.9, old, adv, ref, None, 0.2, 0.2, 0.1))
 
 
+def good():
+    """Arguments that every operator takes."""
+    x, y, old, adv, ref = inputs()
+    stats = ops.token_logprobs(x, y, 1.0, -100)[1]
+    kept = ops.policy(x, y, -100, 1.0, old, adv, None, None, 0.2, 0.2, 0.0)[2]
+    lp, off, one = old.flatten(), offsets()[:5], torch.ones((), device="cuda")
+    coef = ops.preference(lp, None, None, off, 0, False, 0.1, 0.0, 0.0)[2]
+    return {
+        ops.token_logprobs: [x, y, 0.9, -100],
+        ops.token_logprobs_grad: [x, y, 0.9, stats, adv],
+        ops.preference: [lp, ref.flatten(), lp > -6, off, 0, True, 0.1, 0.1, 0.0],
+        ops.preference_grad: [lp, lp > -6, off, coef, one],
+        ops.policy: [x, y, -100, 0.9, old, adv, ref, adv.abs(), 0.2, 0.2, 0.1],
+        ops.policy_grad: [x, y, 0.9, kept, one],
+    }
+
+
+def test_operators_take_strided_tensors() -> None:
+    for op, args in good().items():
+        want = op(*args)
+        spread = [torch.stack([a, a], -1)[..., 0] if isinstance(a, torch.Tensor) and a.dim() else a
+                  for a in args]
+        got = op(*spread)
+        for a, b in zip(got, want) if isinstance(want, tuple) else [(got, want)]:
+            assert torch.equal(a, b)
+
+
+def test_operators_refuse_what_they_would_misread() -> None:
+    def short(t):
+        return t[..., :-1] if t.dim() else torch.ones(2, device="cuda", dtype=t.dtype)
+
+    def longer(t):
+        return torch.cat([t, t], -1) if t.dim() else torch.ones(2, device="cuda", dtype=t.dtype)
+
+    def other_type(t):
+        if t.dtype == torch.float32:
+            return t.half() if t.shape != (6, 10, 501) else t.int()
+        return t.float() if t.dtype in (torch.int64, torch.float64) else t.to(torch.uint8)
+
+    for op, args in good().items():
+        op(*args)
+        first_is_logits = args[0].dim() == 3
+        for i, a in enumerate(args):
+            if not isinstance(a, torch.Tensor):
+                continue
+            bad = [(other_type(a), TypeError), (a.cpu(), (ValueError, RuntimeError))]
+            if not (i == 0 and first_is_logits):  # another vocabulary is another call
+                bad += [(short(a), ValueError), (longer(a), ValueError)]
+            for b, error in bad:
+                with pytest.raises(error):
+                    op(*args[:i], b, *args[i + 1:])
+        if first_is_logits:
+            for x in (args[0][..., :0], args[0][0], args[0][0, 0, 0]):
+                with pytest.raises(ValueError):
+                    op(x, *args[1:])
+    # settings
+    x, y, old, adv, _ = inputs()
+    with pytest.raises(RuntimeError, match="temperature"):
+        ops.token_logprobs(x, y, 0.0, -100)
+    with pytest.raises(RuntimeError, match="clip_low"):
+        ops.policy(x, y, -100, 1.0, old, adv, None, None, -0.1, 0.2, 0.0)
+    for kind, beta, smoothing in ((3, 0.1, 0.0), (0, 0.0, 0.0), (0, 0.1, 0.5)):
+        with pytest.raises(RuntimeError, match="kind|beta|label_smoothing"):
+            ops.preference(old.flatten(), None, None, offsets(), kind, False, beta, smoothing, 0.0)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_compile_fullgraph(dtype: torch.dtype) -> None:
     torch._dynamo.reset()

@@ -19,7 +19,7 @@ import pytest
 import torch
 
 import torchisotonic_b200 as ti
-from torchisotonic_b200 import _ext
+from torchisotonic_b200 import _ext, ops
 
 HALF_ULP = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24,
             torch.float64: 2.0**-53}
@@ -870,6 +870,23 @@ def test_refusals() -> None:
     (g,) = torch.autograd.grad(ti.token_logprobs(leaf, y).sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):  # differentiable once
         g.sum().backward()
+
+
+def test_operator_refusals_without_a_gpu() -> None:
+    x, y, t = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    off = torch.tensor([0, 1, 3])
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.token_logprobs(x, y, 1.0, -100)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.token_logprobs_grad(x, y, 1.0, torch.zeros(6), t)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.policy(x, y, -100, 1.0, t, t, None, None, 0.2, 0.2, 0.0)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.policy_grad(x, y, 1.0, torch.zeros(6, dtype=torch.float64), t[0])
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.preference(t, None, None, off, 0, False, 0.1, 0.0, 0.0)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ops.preference_grad(t, None, off, t[:2], t[0])
 
 
 def test_abi_refusals() -> None:

@@ -102,6 +102,59 @@ struct Logits {
   }
 };
 
+// The steps that the torch.library operators call take tensors as a caller of those operators gives
+// them: refused here, by what each has to be.
+[[noreturn]] void refuse(const std::string& what) { throw py::value_error(what); }
+
+void need_cuda(const Tensor& t, const char* name) {
+  if (!t.is_cuda())
+    throw std::runtime_error(
+        std::string("torchisotonic_b200 runs on CUDA tensors only (no CPU fallback); move ") + name +
+        " to a CUDA device");
+}
+
+void need(const Tensor& t, const char* name, ScalarType type, at::IntArrayRef sizes,
+          const Tensor& beside) {
+  if (t.scalar_type() != type)
+    throw py::type_error(std::string(name) + " must be of dtype " + c10::toString(type));
+  if (!ready(&t, type, sizes, beside.device())) {
+    std::string text;
+    for (const int64_t n : sizes) text += (text.empty() ? "" : ", ") + std::to_string(n);
+    refuse(std::string(name) + " must be contiguous, of sizes [" + text +
+           "] and on the first argument's device");
+  }
+}
+
+void need(const std::optional<Tensor>& t, const char* name, ScalarType type,
+          at::IntArrayRef sizes, const Tensor& beside) {
+  if (t) need(*t, name, type, sizes, beside);
+}
+
+// An upstream gradient: one number, where the loss is.
+void need_scalar(const Tensor& t, ScalarType type, const Tensor& beside) {
+  need(t, "upstream", type, t.numel() == 1 ? t.sizes() : at::IntArrayRef(), beside);
+}
+
+void need_logits(const Tensor& x, const Tensor& targets) {
+  need_cuda(x, "logits");
+  if (!x.is_floating_point() || x.element_size() == 1)
+    throw py::type_error("logits must be float16, bfloat16, float32 or float64");
+  if (x.dim() < 1 || x.size(-1) < 1)
+    refuse("logits must have a last dimension of at least one element");
+  need(targets, "targets", at::kLong, x.sizes().slice(0, x.dim() - 1), x);
+}
+
+void need_answers(const Tensor& logps, const std::optional<Tensor>& mask, const Tensor& offsets) {
+  need_cuda(logps, "logps");
+  if (logps.scalar_type() != at::kFloat && logps.scalar_type() != at::kDouble)
+    throw py::type_error("logps must be float32 or float64");
+  if (logps.dim() != 1 || !logps.is_contiguous()) refuse("logps must be contiguous and 1-D");
+  need(mask, "mask", at::kBool, logps.sizes(), logps);
+  if (offsets.dim() != 1 || offsets.numel() < 3 || offsets.numel() % 2 == 0)
+    refuse("offsets must be 1-D with 2 * pairs + 1 entries, pairs >= 1");
+  need(offsets, "offsets", at::kLong, offsets.sizes(), logps);
+}
+
 // A gradient under create_graph: what depends on it raises when it is differentiated.
 Tensor once(const Tensor& grad) {
   if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
@@ -529,14 +582,44 @@ PYBIND11_MODULE(_native, m) {
   m.def("policy_loss", &policy_loss);
   m.def("adamw", &adamw);
   // the steps alone, for the torch.library operators
-  m.def("logprobs", &logprobs);
-  m.def("logprobs_grad", &logprobs_grad);
-  m.def("preference", &Preference::run);
-  m.def("preference_grad", &Preference::run_grad);
+  m.def("logprobs", [](const Tensor& x, const Tensor& targets, double temperature,
+                       int64_t ignore_index) {
+    need_logits(x, targets);
+    return logprobs(x, targets, temperature, ignore_index, true);
+  });
+  m.def("logprobs_grad", [](const Tensor& x, const Tensor& targets, double temperature,
+                            const Tensor& stats, const Tensor& coef) {
+    need_logits(x, targets);
+    need(stats, "stats", acc_of(x), {2 * targets.numel()}, x);
+    need(coef, "coef", coef.scalar_type() == at::kDouble ? at::kDouble : acc_of(x), targets.sizes(),
+         x);
+    return logprobs_grad(x, targets, temperature, stats, coef);
+  });
+  m.def("preference", [](const Tensor& logps, const std::optional<Tensor>& refs,
+                         const std::optional<Tensor>& mask, const Tensor& offsets, int64_t kind,
+                         bool average, double beta, double label_smoothing, double margin) {
+    need_answers(logps, mask, offsets);
+    need(refs, "refs", logps.scalar_type(), logps.sizes(), logps);
+    return Preference::run(logps, refs, mask, offsets, kind, average, beta, label_smoothing, margin);
+  });
+  m.def("preference_grad", [](const Tensor& logps, const std::optional<Tensor>& mask,
+                              const Tensor& offsets, const Tensor& coef, const Tensor& upstream) {
+    need_answers(logps, mask, offsets);
+    need(coef, "coef", logps.scalar_type(), {offsets.numel() - 1}, logps);
+    need_scalar(upstream, logps.scalar_type(), logps);
+    return std::get<0>(Preference::run_grad(logps, mask, offsets, coef, upstream, true, false));
+  });
   m.def("policy", [](const Tensor& x, const Tensor& targets, int64_t ignore_index,
                      double temperature, const Tensor& old_logps, const Tensor& advantages,
                      const std::optional<Tensor>& ref_logps, const std::optional<Tensor>& weight,
                      double clip_low, double clip_high, double kl_coef) {
+    need_logits(x, targets);
+    const ScalarType acc = acc_of(x);
+    need(old_logps, "old_logps", acc, targets.sizes(), x);
+    need(advantages, "advantages", acc, targets.sizes(), x);
+    need(ref_logps, "ref_logps", acc, targets.sizes(), x);
+    need(weight, "weight", weight && weight->scalar_type() == at::kBool ? at::kBool : acc,
+         targets.sizes(), x);
     const PolicyResult r = policy(x, {targets, old_logps, advantages, ref_logps, weight,
                                       ignore_index, temperature, clip_low, clip_high, kl_coef},
                                   false);
@@ -544,6 +627,9 @@ PYBIND11_MODULE(_native, m) {
   });
   m.def("policy_grad", [](const Tensor& x, const Tensor& targets, double temperature,
                           const Tensor& kept, const Tensor& upstream) {
+    need_logits(x, targets);
+    need(kept, "kept", at::kDouble, {targets.numel() * (acc_of(x) == at::kDouble ? 3 : 2)}, x);
+    need_scalar(upstream, acc_of(x), x);
     return policy_grad(x, targets, temperature, kept, upstream, Tensor());
   });
 }

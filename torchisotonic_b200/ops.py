@@ -142,13 +142,17 @@ torch.library.register_autograd(f"{_NS}::fit", _fit_backward, setup_context=_fit
 
 
 # ---------------------------------------------------------------------------------------------
-# The losses
+# The losses (sizes, types and devices are checked in csrc/native.cpp)
+
+
+def _dense(t: Tensor | None) -> Tensor | None:
+    return None if t is None else t.contiguous()
 
 
 @torch.library.custom_op(f"{_NS}::token_logprobs", mutates_args=())
 def token_logprobs(logits: Tensor, targets: Tensor, temperature: float,
                    ignore_index: int) -> tuple[Tensor, Tensor]:
-    return _ext.native().logprobs(logits, targets.contiguous(), temperature, ignore_index, True)
+    return _ext.native().logprobs(logits, targets.contiguous(), temperature, ignore_index)
 
 
 @token_logprobs.register_fake
@@ -161,7 +165,7 @@ def _(logits, targets, temperature, ignore_index):
 @torch.library.custom_op(f"{_NS}::token_logprobs_grad", mutates_args=())
 def token_logprobs_grad(logits: Tensor, targets: Tensor, temperature: float, stats: Tensor,
                         coef: Tensor) -> Tensor:
-    return _ext.native().logprobs_grad(logits, targets.contiguous(), temperature, stats,
+    return _ext.native().logprobs_grad(logits, targets.contiguous(), temperature, _dense(stats),
                                        coef.contiguous())
 
 
@@ -188,8 +192,9 @@ torch.library.register_autograd(f"{_NS}::token_logprobs", _token_logprobs_backwa
 def preference(logps: Tensor, refs: Tensor | None, mask: Tensor | None, offsets: Tensor, kind: int,
                average: bool, beta: float, label_smoothing: float,
                margin: float) -> tuple[Tensor, Tensor, Tensor]:
-    loss, rewards, coef = _ext.native().preference(logps, refs, mask, offsets, kind, average,
-                                                   beta, label_smoothing, margin)
+    loss, rewards, coef = _ext.native().preference(_dense(logps), _dense(refs), _dense(mask),
+                                                   _dense(offsets), kind, average, beta,
+                                                   label_smoothing, margin)
     return loss, rewards, coef[:rewards.numel()].clone()
 
 
@@ -202,12 +207,13 @@ def _(logps, refs, mask, offsets, kind, average, beta, label_smoothing, margin):
 @torch.library.custom_op(f"{_NS}::preference_grad", mutates_args=())
 def preference_grad(logps: Tensor, mask: Tensor | None, offsets: Tensor, coef: Tensor,
                     upstream: Tensor) -> Tensor:
-    return _ext.native().preference_grad(logps, mask, offsets, coef, upstream, True, False)[0]
+    return _ext.native().preference_grad(_dense(logps), _dense(mask), _dense(offsets), _dense(coef),
+                                         upstream)
 
 
 @preference_grad.register_fake
 def _(logps, mask, offsets, coef, upstream):
-    return torch.empty_like(logps)
+    return torch.empty_like(logps, memory_format=torch.contiguous_format)
 
 
 def _preference_setup(ctx, inputs, output) -> None:
@@ -236,8 +242,9 @@ def _kept(logits: Tensor, targets: Tensor) -> int:
 def policy(logits: Tensor, targets: Tensor, ignore_index: int, temperature: float,
            old_logps: Tensor, advantages: Tensor, ref_logps: Tensor | None, weight: Tensor | None,
            clip_low: float, clip_high: float, kl_coef: float) -> tuple[Tensor, Tensor, Tensor]:
-    out, logps, kept = _ext.native().policy(logits, targets, ignore_index, temperature, old_logps,
-                                            advantages, ref_logps, weight, clip_low, clip_high,
+    out, logps, kept = _ext.native().policy(logits, _dense(targets), ignore_index, temperature,
+                                            _dense(old_logps), _dense(advantages),
+                                            _dense(ref_logps), _dense(weight), clip_low, clip_high,
                                             kl_coef)
     return out, logps, kept[:_kept(logits, targets)].clone()
 
@@ -253,7 +260,7 @@ def _(logits, targets, ignore_index, temperature, old_logps, advantages, ref_log
 @torch.library.custom_op(f"{_NS}::policy_grad", mutates_args=())
 def policy_grad(logits: Tensor, targets: Tensor, temperature: float, kept: Tensor,
                 upstream: Tensor) -> Tensor:
-    return _ext.native().policy_grad(logits, targets, temperature, kept, upstream)
+    return _ext.native().policy_grad(logits, _dense(targets), temperature, _dense(kept), upstream)
 
 
 @policy_grad.register_fake
