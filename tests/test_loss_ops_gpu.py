@@ -136,6 +136,26 @@ def test_compile_fullgraph(dtype: torch.dtype) -> None:
                 assert torch.equal(u, v)
 
 
+def test_compiled_losses_change_in_place() -> None:
+    torch._dynamo.reset()
+    x, y, old, adv, _ = inputs()
+
+    def policy(x):
+        return ti.policy_loss(x, y, old, adv).loss
+
+    def preference(x):
+        return ti.preference_loss(ti.token_logprobs(x, y).flatten(), None, offsets()[:5])[0]
+
+    for f in (policy, preference):
+        for g in (f, torch.compile(f, fullgraph=True)):
+            a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+            loss = g(a)
+            loss /= 4
+            loss.backward()
+            (f(b) / 4).backward()
+            assert torch.equal(a.grad, b.grad)
+
+
 def test_training_example() -> None:
     sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
     import preference_training

@@ -771,6 +771,40 @@ def test_policy_terms_with_a_factor_of_zero(vocab: int, dtype: torch.dtype, far:
 
 
 @pytest.mark.gpu
+def test_policy_loss_changes_in_place() -> None:
+    # as a training loop does: divided by the accumulated steps, another term added
+    x, y, _ = logits_of((40, 2003), torch.float32)
+    old, adv, ref = tokens_of(x, y, 1)
+    leaf = x.requires_grad_()
+
+    def grad(change):
+        got = ti.policy_loss(leaf, y, old, adv, ref_logps=ref, kl_coef=0.1)
+        was = [t.detach().clone() for t in got]
+        loss = change(got.loss)
+        for a, b in zip(got[1:], was[1:]):
+            assert torch.equal(a, b)  # the other results stay as they were
+        return loss.detach(), *torch.autograd.grad(loss, leaf)
+
+    def divided(loss):
+        loss /= 4
+        return loss
+
+    def added(loss):
+        loss += leaf.square().mean()
+        return loss
+
+    for a, b in ((divided, lambda loss: loss / 4), (added, lambda loss: loss + leaf.square().mean())):
+        for u, v in zip(grad(a), grad(b)):
+            assert torch.equal(u, v)
+    with torch.no_grad():
+        got = ti.policy_loss(x, y, old, adv)
+    want = got.loss.clone() * 2
+    got.loss.mul_(2)
+    got.kl.add_(1)
+    assert got.loss == want and got.clip_fraction <= 1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 9), (3, 1100)])
 def test_policy_gradcheck(shape) -> None:
     x, y, _ = logits_of(shape, torch.float64, scale=1.0)

@@ -379,6 +379,13 @@ PolicyResult policy(const Tensor& x, const PolicySettings& s, bool with_grad) {
   return r;
 }
 
+// Loss, kl and clip fraction as tensors of their own: parts of `out` that autograd does not take for
+// views, whose change in place (loss /= n) it would refuse.
+variable_list parts(const Tensor& out) {
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return {out.select(0, 0), out.select(0, 1), out.select(0, 2)};
+}
+
 // The gradient in x times upstream. grad: what policy wrote, the gradient for upstream 1, overwritten
 // unless it is; or undefined, for a new tensor.
 Tensor policy_grad(const Tensor& x, const Tensor& targets, double temperature, const Tensor& kept,
@@ -405,7 +412,7 @@ struct Policy : torch::autograd::Function<Policy> {
     ctx->save_for_backward({x, s.targets, r.kept});
     ctx->saved_data["temperature"] = s.temperature;
     ctx->saved_data["grad"] = r.grad;
-    variable_list out = r.out.unbind();
+    variable_list out = parts(r.out);
     out.push_back(r.logps);
     ctx->mark_non_differentiable({out[1], out[2], out[3]});
     ctx->set_materialize_grads(false);
@@ -468,7 +475,7 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> policy_loss(
     return std::make_tuple(out[0], out[3], out[1], out[2]);
   }
   const PolicyResult r = policy(*x, s, false);
-  const auto out = r.out.unbind();
+  const variable_list out = parts(r.out);
   return std::make_tuple(out[0], r.logps, out[1], out[2]);
 }
 
