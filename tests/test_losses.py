@@ -906,6 +906,41 @@ def test_refusals() -> None:
         g.sum().backward()
 
 
+@pytest.mark.gpu
+def test_forward_mode_is_refused() -> None:
+    # a tangent would be lost; also where an argument is converted first, and by the operators
+    fw = torch.autograd.forward_ad
+    x, y, _ = logits_of((4, 33), torch.float32)
+    old, adv, ref = tokens_of(x, y, 1)
+    off = torch.tensor([0, 2, 4], device="cuda")
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t.clone(), torch.ones_like(t))
+
+        calls = [
+            lambda: ti.token_logprobs(dual(x), y),
+            lambda: ti.token_logprobs(dual(x), y.int()),
+            lambda: ti.preference_loss(dual(old), None, off),
+            lambda: ti.preference_loss(old, dual(ref), off),
+            lambda: ti.preference_loss(dual(old.half()), None, off),
+            lambda: ti.policy_loss(dual(x), y, old, adv),
+            lambda: ti.policy_loss(x, y, dual(old), adv),
+            lambda: ti.policy_loss(x, y, old, dual(adv.double())),
+            lambda: ti.policy_loss(x, y, old, adv, ref_logps=dual(ref)),
+            lambda: ti.policy_loss(x, y, old, adv, weight=dual(ref)),
+            lambda: ops.token_logprobs(dual(x), y, 1.0, -100),
+            lambda: ops.preference(dual(old), None, None, off, 0, False, 0.1, 0.0, 0.0),
+            lambda: ops.policy(x, y, -100, 1.0, old, dual(adv), None, None, 0.2, 0.2, 0.0),
+        ]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ti.token_logprobs(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), y)
+        ti.token_logprobs(x, y)  # one that has none passes
+
+
+
 def test_operator_refusals_without_a_gpu() -> None:
     x, y, t = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
     off = torch.tensor([0, 1, 3])

@@ -73,6 +73,17 @@ bool ready(const Tensor* t, ScalarType type, at::IntArrayRef sizes, at::Device d
          t->is_contiguous();
 }
 
+// Refuses tensors with a tangent: the result would be without one, and nothing would tell.
+void need_no_tangent(const Tensor& t) {
+  if (!t._fw_grad(0).defined()) return;
+  PyErr_SetString(PyExc_NotImplementedError,
+                  "torchisotonic_b200's losses have no forward-mode derivative");
+  throw py::error_already_set();
+}
+void need_no_tangent(const std::optional<Tensor>& t) {
+  if (t) need_no_tangent(*t);
+}
+
 bool ready_logits(const Tensor* x, const Tensor* targets, double temperature) {
   if (!x || !x->is_cuda() || x->dim() < 1 || x->size(-1) < 1 || !(temperature > 0)) return false;
   const ScalarType type = x->scalar_type();
@@ -115,6 +126,7 @@ void need_cuda(const Tensor& t, const char* name) {
 
 void need(const Tensor& t, const char* name, ScalarType type, at::IntArrayRef sizes,
           const Tensor& beside) {
+  need_no_tangent(t);
   if (t.scalar_type() != type)
     throw py::type_error(std::string(name) + " must be of dtype " + c10::toString(type));
   if (!ready(&t, type, sizes, beside.device())) {
@@ -137,6 +149,7 @@ void need_scalar(const Tensor& t, ScalarType type, const Tensor& beside) {
 
 void need_logits(const Tensor& x, const Tensor& targets) {
   need_cuda(x, "logits");
+  need_no_tangent(x);
   if (!x.is_floating_point() || x.element_size() == 1)
     throw py::type_error("logits must be float16, bfloat16, float32 or float64");
   if (x.dim() < 1 || x.size(-1) < 1)
@@ -146,6 +159,7 @@ void need_logits(const Tensor& x, const Tensor& targets) {
 
 void need_answers(const Tensor& logps, const std::optional<Tensor>& mask, const Tensor& offsets) {
   need_cuda(logps, "logps");
+  need_no_tangent(logps);
   if (logps.scalar_type() != at::kFloat && logps.scalar_type() != at::kDouble)
     throw py::type_error("logps must be float32 or float64");
   if (logps.dim() != 1 || !logps.is_contiguous()) refuse("logps must be contiguous and 1-D");
@@ -211,6 +225,7 @@ std::optional<Tensor> token_logprobs(py::handle logits, py::handle y, double tem
                                      int64_t ignore_index) {
   const Tensor *x = tensor_in(logits), *targets = tensor_in(y);
   if (!ready_logits(x, targets, temperature)) return std::nullopt;
+  need_no_tangent(*x);
   if (x->requires_grad() && at::GradMode::is_enabled())
     return Logprobs::apply(*x, *targets, temperature, ignore_index);
   return std::get<0>(logprobs(*x, *targets, temperature, ignore_index, false));
@@ -326,6 +341,8 @@ std::optional<std::tuple<Tensor, Tensor>> preference_loss(py::handle of_logps, p
     if (!ready(t, at::kBool, logps->sizes(), device)) return std::nullopt;
     mask = *t;
   }
+  need_no_tangent(*logps);
+  need_no_tangent(refs);
   if (at::GradMode::is_enabled() &&
       (logps->requires_grad() || (refs.has_value() && refs->requires_grad()))) {
     const variable_list out = Preference::apply(*logps, refs, mask, *offsets, kind, average, beta,
@@ -470,6 +487,9 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> policy_loss(
     if (!t) return std::nullopt;
     s.weight = *t;
   }
+  for (const Tensor* t : {x, old, adv}) need_no_tangent(*t);
+  need_no_tangent(s.ref_logps);
+  need_no_tangent(s.weight);
   if (x->requires_grad() && grad_mode) {
     const variable_list out = Policy::apply(*x, s);
     return std::make_tuple(out[0], out[3], out[1], out[2]);
