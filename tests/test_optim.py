@@ -406,6 +406,34 @@ def test_step_on_another_stream() -> None:
     assert torch.equal(a[0][0], b[0][0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_capture_of_a_step_is_refused(bits: int) -> None:
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = ti.AdamW([p], lr=0.1, weight_decay=0.0, state_bits=bits)
+    p.grad = torch.ones_like(p)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured in a CUDA graph"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert not opt.state and (p == 1).all()
+    opt.step()  # the next one is the first
+    assert opt.state[p]["step"] == 1
+    torch.testing.assert_close(p.detach(), torch.full_like(p, 0.9), rtol=1e-5, atol=0)
+
+
+def test_capture_of_a_step_is_refused_without_a_gpu(monkeypatch) -> None:
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    opt = ti.AdamW([p])
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="captured in a CUDA graph"):
+        opt.step(lambda: pytest.fail("nothing of a refused step runs"))
+    assert not opt.state
+
+
 # ---------------------------------------------------------------------------------------------
 # Refusals
 

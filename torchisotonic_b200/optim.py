@@ -22,6 +22,8 @@ from torch import Tensor
 from torchisotonic_b200 import _ext
 
 BLOCK = 256  # elements that share a scale
+
+
 def adamw_step(
     params: Sequence[Tensor],
     grads: Sequence[Tensor],
@@ -46,7 +48,8 @@ def adamw_step(
     ``exp_avgs`` and ``exp_avg_sqs``: float32 (m and v), shaped like the parameters; or
     float8_e4m3fn, with ``scales = (exp_avg_scales, exp_avg_sq_scales)``, a float32 tensor of
     ceil(n / 256) numbers for every state: a state's number times its block's scale is then m, and
-    the square root of v. ``step`` counts from 1; ``seed`` enters the rounding of 8-bit states.
+    the square root of v. ``step`` counts from 1; ``seed`` enters the rounding of 8-bit states. Both
+    are numbers of this call: captured in a CUDA graph, a replay repeats them.
     """
     if scales is not None and len(scales) != 2:
         raise ValueError("scales must be a pair of sequences")
@@ -68,7 +71,8 @@ class AdamW(torch.optim.Optimizer):
     ``state_bits``: 32, or 8 for float8 moments (see the module). ``seed``: of their rounding.
     Learning rate, betas, eps and weight decay are per group. A parameter that is not contiguous is
     stepped as a contiguous copy, written back. ``state_dict`` and
-    ``load_state_dict`` keep the states' types, so a run resumes exactly.
+    ``load_state_dict`` keep the states' types, so a run resumes exactly. A step counts on the host:
+    capturing one in a CUDA graph raises.
     """
 
     def __init__(self, params: Iterable[Any], lr: float = 1e-3,
@@ -98,6 +102,11 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure: Any = None) -> Any:
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(
+                "AdamW.step cannot be captured in a CUDA graph: a replay would repeat this step's "
+                "number, bias corrections and random rounding"
+            )
         loss = None
         if closure is not None:
             with torch.enable_grad():
