@@ -407,6 +407,44 @@ def test_step_on_another_stream() -> None:
 
 
 @pytest.mark.gpu
+def test_no_two_parameters_are_rounded_alike() -> None:
+    # equal parameters with equal gradients, a group each: other random bits, so of 4096 numbers
+    # between two neighbours many go the other way. A parameter's own do not depend on whether
+    # another one has a gradient.
+    grad = torch.randn(4096, generator=torch.Generator().manual_seed(0)).cuda()
+
+    def codes(groups, without=()):
+        params = [torch.nn.Parameter(torch.zeros(4096, device="cuda")) for _ in range(3)]
+        opt = ti.AdamW([{"params": [params[k] for k in g]} for g in groups], state_bits=8, seed=3)
+        for k, p in enumerate(params):
+            p.grad = None if k in without else grad.clone()
+        opt.step()
+        return {k: opt.state[p]["exp_avg"].view(torch.uint8).clone() for k, p in enumerate(params)
+                if k not in without}
+
+    together = codes([[0, 1, 2]])
+    apart = codes([[0], [1], [2]])
+    for a, b in ((0, 1), (0, 2), (1, 2)):
+        assert int((apart[a] != apart[b]).sum()) > 500
+    for k in range(3):  # the place over all groups counts
+        assert torch.equal(apart[k], together[k])
+    for groups in ([[0, 1, 2]], [[0], [1, 2]]):
+        some = codes(groups, without=(0, 1))
+        assert torch.equal(some[2], together[2])
+
+
+@pytest.mark.gpu
+def test_indices_enter_the_rounding() -> None:
+    params, grads, ms, vs, scales = tensors([(300,), (1000,)], torch.float32, torch.float32, 8)
+    want = [plain_step(params[k], grads[k], ms[k], vs[k], 3, place, 5, torch.float32,
+                       (scales[0][k], scales[1][k]), **SETTINGS) for k, place in enumerate((9, 2))]
+    ti.adamw_step(params, grads, ms, vs, step=3, seed=5, scales=scales, indices=[9, 2], **SETTINGS)
+    for k in range(2):
+        for x, y in zip((params[k], ms[k], vs[k]), want[k]):
+            assert torch.equal(x.float(), y.to(x.dtype).float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [32, 8])
 def test_capture_of_a_step_is_refused(bits: int) -> None:
     p = torch.nn.Parameter(torch.ones(300, device="cuda"))
@@ -507,3 +545,14 @@ def test_abi_refusals() -> None:
     assert so.tiso_adamw(2, 2, 32, 0, None, good, None) == 0
     empty = (ctypes.c_int64 * 8)(0, 0, 0, 0, 0, 0, 0, 0)
     assert so.tiso_adamw(2, 2, 32, 1, ctypes.addressof(empty), good, None) == 0
+
+
+def test_indices_go_with_params() -> None:
+    x = [torch.zeros(4)]
+    for bad in ([1, 2], [0, 1, 2]):
+        with pytest.raises(ValueError, match="as many as params"):
+            ti.adamw_step(x, x, x, x, step=1, indices=bad)
+    with pytest.raises(TypeError):
+        ti.adamw_step(x, x, x, x, step=1, indices=["a"])  # type: ignore[list-item]
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        ti.adamw_step(x, x, x, x, step=1, indices=[5])

@@ -522,8 +522,9 @@ struct Tensors {
   }
 };
 
+// indices: the tensors' places among all of the step's; empty for those in the lists.
 void adamw(const py::list& lists, int64_t step, double lr, double beta1, double beta2, double eps,
-           double weight_decay, uint32_t seed) {
+           double weight_decay, uint32_t seed, const std::vector<int64_t>& indices) {
   std::vector<Tensors> held;
   std::vector<std::vector<const Tensor*>> all;
   for (const py::handle& list : lists) {
@@ -534,6 +535,8 @@ void adamw(const py::list& lists, int64_t step, double lr, double beta1, double 
   for (const auto& list : all)
     if (list.size() != count)
       throw py::value_error("params, grads, states and scales must be of one length");
+  if (!indices.empty() && indices.size() != count)
+    throw py::value_error("indices must be as many as params");
   if (count == 0) return;
   const at::Device device = all[0][0]->device();
   for (const auto& list : all)
@@ -590,7 +593,7 @@ void adamw(const py::list& lists, int64_t step, double lr, double beta1, double 
       table.push_back({all[0][i]->data_ptr(), all[1][i]->data_ptr(), all[2][i]->data_ptr(),
                        all[3][i]->data_ptr(), small ? all[4][i]->data_ptr<float>() : nullptr,
                        small ? all[5][i]->data_ptr<float>() : nullptr, all[0][i]->numel(),
-                       static_cast<int64_t>(i)});
+                       indices.empty() ? static_cast<int64_t>(i) : indices[i]});
     }
     check(tiso_adamw(dtype_of(p), dtype_of(g), small ? 8 : 32, static_cast<int64_t>(table.size()),
                      table.data(), &args, stream_of(*all[0][0])));

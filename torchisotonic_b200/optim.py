@@ -37,6 +37,7 @@ def adamw_step(
     weight_decay: float = 0.01,
     scales: tuple[Sequence[Tensor], Sequence[Tensor]] | None = None,
     seed: int = 0,
+    indices: Sequence[int] | None = None,
 ) -> None:
     """One AdamW step (decoupled weight decay) over all of ``params``, in place:
 
@@ -49,7 +50,9 @@ def adamw_step(
     float8_e4m3fn, with ``scales = (exp_avg_scales, exp_avg_sq_scales)``, a float32 tensor of
     ceil(n / 256) numbers for every state: a state's number times its block's scale is then m, and
     the square root of v. ``step`` counts from 1; ``seed`` enters the rounding of 8-bit states. Both
-    are numbers of this call: captured in a CUDA graph, a replay repeats them.
+    are numbers of this call: captured in a CUDA graph, a replay repeats them. ``indices``: where a
+    step takes several calls, each tensor's place among all of the step's (an integer for every
+    parameter; its place in the list if None), so that no two are rounded by the same random bits.
     """
     if scales is not None and len(scales) != 2:
         raise ValueError("scales must be a pair of sequences")
@@ -61,7 +64,8 @@ def adamw_step(
         raise ValueError("lr, eps and weight_decay must not be negative")
     # the lists are checked there: hundreds of tensors a call
     _ext.native().adamw([params, grads, exp_avgs, exp_avg_sqs, *(scales or ())], step, lr, betas[0],
-                        betas[1], eps, weight_decay, seed & 0xFFFFFFFF)
+                        betas[1], eps, weight_decay, seed & 0xFFFFFFFF,
+                        () if indices is None else indices)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -111,11 +115,12 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        first = 0  # of the group's parameters among all
         for group in self.param_groups:
             bits = group["state_bits"]
             # parameters that joined later, or had no gradient in some steps, are at another step
-            at_step: dict[tuple[int, torch.device], list[Tensor]] = {}
-            for p in group["params"]:
+            at_step: dict[tuple[int, torch.device], list[tuple[int, Tensor]]] = {}
+            for index, p in enumerate(group["params"], first):
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
@@ -124,8 +129,10 @@ class AdamW(torch.optim.Optimizer):
                 if not state:
                     state.update(self._init_state(p, bits))
                 state["step"] += 1
-                at_step.setdefault((state["step"], p.device), []).append(p)
-            for (step, _), params in at_step.items():
+                at_step.setdefault((state["step"], p.device), []).append((index, p))
+            first += len(group["params"])
+            for (step, _), stepped in at_step.items():
+                indices, params = zip(*stepped)
                 states = [self.state[p] for p in params]
                 scales = None
                 if bits == 8:
@@ -136,7 +143,7 @@ class AdamW(torch.optim.Optimizer):
                            [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                            step=step, lr=float(group["lr"]), betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"], scales=scales,
-                           seed=group["seed"])
+                           seed=group["seed"], indices=indices if bits == 8 else None)
                 for p, value in zip(params, values):
                     if value is not p:
                         p.copy_(value)
