@@ -556,3 +556,26 @@ def test_indices_go_with_params() -> None:
         ti.adamw_step(x, x, x, x, step=1, indices=["a"])  # type: ignore[list-item]
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         ti.adamw_step(x, x, x, x, step=1, indices=[5])
+
+
+def test_a_refused_step_does_not_count() -> None:
+    # a caller that catches the error goes on at the step's right number
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    opt = ti.AdamW([p])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            opt.step()
+        assert opt.state[p]["step"] == 0
+
+
+@pytest.mark.gpu
+def test_a_refused_step_does_not_count_in_its_group_alone() -> None:
+    a = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    b = torch.nn.Parameter(torch.ones(3, device="cuda", dtype=torch.float64))
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt = ti.AdamW([{"params": [a]}, {"params": [b]}], lr=0.1, weight_decay=0.0)
+    with pytest.raises(TypeError, match="params must be"):
+        opt.step()
+    assert opt.state[a]["step"] == 1 and opt.state[b]["step"] == 0
+    assert (a < 1).all() and (b == 1).all()

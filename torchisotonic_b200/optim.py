@@ -128,8 +128,7 @@ class AdamW(torch.optim.Optimizer):
                 state = self.state[p]
                 if not state:
                     state.update(self._init_state(p, bits))
-                state["step"] += 1
-                at_step.setdefault((state["step"], p.device), []).append((index, p))
+                at_step.setdefault((state["step"] + 1, p.device), []).append((index, p))
             first += len(group["params"])
             for (step, _), stepped in at_step.items():
                 indices, params = zip(*stepped)
@@ -144,7 +143,8 @@ class AdamW(torch.optim.Optimizer):
                            step=step, lr=float(group["lr"]), betas=group["betas"],
                            eps=group["eps"], weight_decay=group["weight_decay"], scales=scales,
                            seed=group["seed"], indices=indices if bits == 8 else None)
-                for p, value in zip(params, values):
+                for p, state, value in zip(params, states, values):
+                    state["step"] = step  # a step that is refused does not count
                     if value is not p:
                         p.copy_(value)
         return loss
