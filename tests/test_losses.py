@@ -392,6 +392,21 @@ def test_preference_extremes() -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("u", [-40.0, -25.0, 0.0, 3.0, 20.0, 30.0, 40.0, 80.0])
+def test_preference_slope_far_from_the_decision(u: float, dtype: torch.dtype) -> None:
+    # -1 / (1 + exp(u)), to the type's precision however small: a dozen roundings in double, then one
+    off = torch.tensor([0, 1, 2], device="cuda")
+    x = torch.tensor([u, 0.0], device="cuda", dtype=dtype, requires_grad=True)
+    for e in (0.0, 0.125):
+        loss, _ = ti.preference_loss(x, None, off, beta=1.0, label_smoothing=e)
+        (g,) = torch.autograd.grad(loss, x)
+        slope = e / (1 + math.exp(-u)) - (1 - e) / (1 + math.exp(u))
+        want = torch.tensor([slope, -slope], dtype=torch.float64)
+        check(g, want, 0.0, unit(dtype) + 12 * 2.0**-53)
+
+
+@pytest.mark.gpu
 def test_preference_tokens_of_no_answer() -> None:
     # offsets that start late and end early: the tokens outside get no gradient
     logps, refs, _, _ = sequences([100])

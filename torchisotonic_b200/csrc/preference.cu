@@ -110,7 +110,10 @@ __device__ void pair_loss(int kind, double u, double smoothing, double beta, dou
   if (kind == TISO_PREF_LOGISTIC) {
     *loss = (1 - smoothing) * softplus_neg(u);
     if (smoothing != 0) *loss += smoothing * softplus_neg(-u);  // an infinite u stays out of it
-    *slope = 1 / (1 + exp(-u)) - (1 - smoothing);
+    // e / (1 + exp(-u)) - (1 - e) / (1 + exp(u)): a difference from 1 would leave nothing of the slope
+    // of a pair that is far on the right side
+    const double z = exp(-fabs(u)), near = 1 / (1 + z), far = z / (1 + z);
+    *slope = smoothing * (u < 0 ? far : near) - (1 - smoothing) * (u < 0 ? near : far);
   } else if (kind == TISO_PREF_HINGE) {
     *loss = u < 1 ? 1 - u : u >= 1 ? 0.0 : u;  // NaN stays
     *slope = u < 1 ? -1.0 : u >= 1 ? 0.0 : u;
