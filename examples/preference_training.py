@@ -60,7 +60,7 @@ def pair_batch(pairs: int, gen: torch.Generator) -> torch.Tensor:
 
 def scores(policy: Policy, tokens: torch.Tensor) -> torch.Tensor:
     """Token log-probabilities of every sequence, packed back to back. (The logits are cut along
-    their length, without a copy.)"""
+    their length, in the forward without a copy.)"""
     return ti.token_logprobs(policy(tokens)[:, :-1], tokens[:, 1:]).flatten()
 
 

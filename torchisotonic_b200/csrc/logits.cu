@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 
 // Loss and gradient in one launch: the row's sum, the token's coefficient, then the row's gradient
 // from a second read that does not reach memory. 4000 x 131072, a tenth of them left out, in 376 us:
-// 2.07 GB of DRAM traffic, 5 % over each byte once, at 84 % of the copy bandwidth; 8192 rows in 850 to
+// 2.04 GB of DRAM traffic, 3 % over each byte once, at 83 % of the copy bandwidth; 8192 rows in 840 to
 // 880 us. The exponential unit is busy 63 % of the time, and what is missing are the joins between a
 // row's two passes (of a CTA's 20 us about 5), which two other CTAs of the SM fill in part.
 //
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 // row: 306 us for 800 MB of bf16 logits, 320 with it loaded). The tiles of a row that is read and
 // written at different alignments are loaded directly, from two vectors each.
 constexpr int kStages = 2;
-constexpr int kSmThreads = 1536;  // resident at 40 registers a thread
+constexpr int kSmThreads = 1536;  // resident at 40 registers a thread (spills: double 96 bytes, 16-bit types 8)
 
 template <int kThreads, typename T, typename A>
 __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p, double inv_temp,
@@ -961,10 +961,10 @@ int launch_policy_rows(const Rows& a, const PolicyArgs<typename AccOf<T>::type>&
 
 // By warps, or in CTAs of the more threads the longer the row: smaller ones have more rows in work,
 // which hides a row's start and join, larger ones less of both. 800 MB of bf16 logits, us: 8192 to
-// the row by warps 374, by 128 threads 431; 10000: 394, 449; 12000: 394, 403; 16384: 374, 331. By
-// 128, 256 and 512 threads 16384: 308, 320, 435, 32000: 331, 312, 390, 50021: 351, 318, 320, 65536:
-// 304, 304, 280, 131072: 302, 306, 290. Rows whose last tile is cut lose more with 512 (100003: 314
-// with 256, 333 with 512).
+// the row by warps 374, by 128 threads 415; 10000: 394, 435; 12000: 394, 391; 16384: 375, 312. By
+// 128, 256 and 512 threads 16384: 312, 314, 431, 32000: 312, 294, 333, 50021: 347, 314, 323, 65536:
+// 303, 303, 277, 131072: 297, 302, 290. Rows whose last tile is cut lose more with 512 (100003: 311
+// with 256, 337 with 512).
 template <typename T>
 int launch_policy(const Rows& a, const PolicyArgs<typename AccOf<T>::type>& p, double inv_temp,
                   T* grad, cudaStream_t st) {

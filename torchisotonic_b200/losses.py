@@ -58,7 +58,8 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     not read; any other target outside ``[0, vocab)`` gives NaN. Logits may be -inf or the type's
     lowest value (a masked vocabulary); a row with nothing but -inf, or with NaN or +inf, gives NaN.
     A cut along the length (``logits[:, :-1]``) or a padded vocabulary (``logits[..., :v]``) is
-    read in place.
+    read in place; in the backward the cut's own gradient is torch's, which fills a tensor of the
+    whole logits' size and copies this one's gradient into it.
     """
     traced = torch.compiler.is_compiling()
     settings = float(temperature), int(ignore_index)
@@ -186,6 +187,9 @@ def policy_loss(
     nothing else of it is read, its gradient is 0. Where both sides of the minimum are equal the
     gradient is the unclipped side's. A ratio or a ``kl_coef`` term beyond the type's range is
     infinite; a factor of 0 (the advantage, ``kl_coef``) leaves its term out also there.
+
+    The gradient is written with the loss, for an upstream gradient of exactly 1; any other one
+    (``loss / n``, a scaled loss) takes another pass over the logits in the backward.
 
     Returns ``PolicyLoss(loss, logps, kl, clip_fraction)``: the loss, differentiable (once) in
     ``logits`` alone; the tokens' log-probabilities (0 where left out); the weighted means of
