@@ -579,3 +579,10 @@ def test_a_refused_step_does_not_count_in_its_group_alone() -> None:
         opt.step()
     assert opt.state[a]["step"] == 1 and opt.state[b]["step"] == 0
     assert (a < 1).all() and (b == 1).all()
+
+
+def test_no_indices_for_some_params_are_refused() -> None:
+    x = [torch.zeros(4)]
+    with pytest.raises(ValueError, match="as many as params"):
+        ti.adamw_step(x, x, x, x, step=1, indices=[])
+    ti.adamw_step([], [], [], [], step=1, indices=[])

@@ -62,6 +62,8 @@ def adamw_step(
         raise ValueError("betas must be in [0, 1)")
     if not (lr >= 0 and eps >= 0 and weight_decay >= 0):
         raise ValueError("lr, eps and weight_decay must not be negative")
+    if indices is not None and len(indices) != len(params):
+        raise ValueError("indices must be as many as params")
     # the lists are checked there: hundreds of tensors a call
     _ext.native().adamw([params, grads, exp_avgs, exp_avg_sqs, *(scales or ())], step, lr, betas[0],
                         betas[1], eps, weight_decay, seed & 0xFFFFFFFF,
