@@ -10,10 +10,12 @@ nvcc compiles for the B200 (compute_100a / sm_100a) only; no JIT build at import
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,13 +23,14 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtiso.so"
 SOURCES = [CSRC / f for f in ("tiso.cu", "calib.cu", "logits.cu", "preference.cu", "adamw.cu")]
+OBJECTS = PKG / "_build"
 NATIVE, NATIVE_SOURCE = PKG / "_native.so", CSRC / "native.cpp"
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "tiso.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
     "-Xptxas", "-warn-spills",
 ]
@@ -43,12 +46,38 @@ def stale(built: Path = LIB, deps: list[Path] = DEPS) -> bool:
     return not built.exists() or any(p.stat().st_mtime > built.stat().st_mtime for p in deps)
 
 
+def includes_of(source: Path) -> set[Path]:
+    """The repository's headers that a source includes, directly or not."""
+    found: set[Path] = set()
+    todo = [source]
+    while todo:
+        at = todo.pop()
+        for name in re.findall(r'^#include "([^"]+)"', at.read_text(), re.M):
+            path = (at.parent / name).resolve()
+            if path not in found:
+                found.add(path)
+                todo.append(path)
+    return found
+
+
+def compile_source(source: Path, force: bool, verbose: bool) -> Path:
+    made = OBJECTS / f"{source.stem}.o"
+    if force or stale(made, [source, *includes_of(source)]):
+        tmp = made.with_suffix(".o.tmp")
+        subprocess.run([nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-c",
+                        "-o", str(tmp), str(source)], check=True, cwd=str(ROOT))
+        tmp.replace(made)
+    return made
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     if force or stale():
+        OBJECTS.mkdir(exist_ok=True)
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            objects = list(pool.map(lambda s: compile_source(s, force, verbose), SOURCES))
         tmp = LIB.with_suffix(".so.tmp")
-        cmd = [nvcc(), *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []),
-               "-o", str(tmp), *map(str, SOURCES), "-lcudart"]
-        subprocess.run(cmd, check=True, cwd=str(ROOT))
+        subprocess.run([nvcc(), *NVCC_FLAGS[:2], "-shared", "-o", str(tmp), *map(str, objects),
+                        "-lcudart"], check=True, cwd=str(ROOT))
         tmp.replace(LIB)
     build_native(force)
     return LIB
