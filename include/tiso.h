@@ -269,6 +269,69 @@ int tiso_policy(int dtype, const tiso_rows* x, const int64_t* targets, int64_t i
                 void* stats, void* out, void* grad, void* workspace, size_t workspace_bytes,
                 void* stream);
 
+/* A token's scores from its row of logits: logps (where targets is not NULL) as of tiso_logprobs;
+ * entropy[r] = -sum p log p of p = softmax(x[r] / temperature); and the `top` largest logits of the row
+ * (0 <= top <= 128, at most the vocabulary), largest first, equal ones by their index (-0 equals 0, NaN
+ * counts as -infinity): top_ids[r][top] and their log-probabilities top_logps[r][top]. Numbers of the
+ * accumulation type. A row whose target is ignore_index is not read: 0, 0, ids ignore_index with
+ * log-probabilities 0. A row with NaN or +infinity, or with nothing but -infinity, has NaN numbers;
+ * one whose target is out of range a NaN logp. stats: NULL, or [rows][3] of the accumulation type for
+ * tiso_scores_grad. Needs no workspace. */
+int tiso_scores(int dtype, const tiso_rows* x, const int64_t* targets, int64_t ignore_index,
+                double temperature, int64_t top, void* logps, void* entropy, void* top_logps,
+                int64_t* top_ids, void* stats, void* stream);
+
+/* The gradient of sum(coef_logp * logps + coef_entropy * entropy) in the logits, in their type, written
+ * contiguously: (c (1[v = y] - p_v) - h p_v (log p_v + entropy)) / temperature; zeros for a row that
+ * was left out, NaN for one whose target is out of range. Either coefficient may be NULL (0; without
+ * targets coef_logp is). */
+int tiso_scores_grad(int dtype, const tiso_rows* x, const int64_t* targets, double temperature,
+                     const void* stats, const void* coef_logp, const void* coef_entropy, void* grad,
+                     void* stream);
+
+enum tiso_distill_kind {
+  TISO_DISTILL_FORWARD = 0, /* sum Q log(Q / P) */
+  TISO_DISTILL_REVERSE = 1, /* sum P log(P / Q) */
+  TISO_DISTILL_JENSEN = 2   /* mix sum Q log(Q / M) + (1 - mix) sum P log(P / M), M = mix Q + (1 - mix) P */
+};
+
+/* A teacher's top lists: for each row of the student's logits `top` entries (1 to 128) of a token's id
+ * and the teacher's log-probability of it ([rows][top], contiguous; logps of the accumulation type).
+ * weight as in tiso_policy_args. drop: the teacher's probabilities are renormalised over the list. */
+typedef struct tiso_distill_args {
+  const int64_t* ids;
+  const void *logps, *weight;
+  int64_t top;
+  int weight_is_byte, kind, drop;
+  double mix, upstream;
+} tiso_distill_args;
+
+/* Workspace for tiso_distill (8-byte aligned). */
+int tiso_distill_workspace_size(int dtype, int64_t rows, size_t* bytes);
+
+/* The distillation loss and, if grad is not NULL, its gradient in the student's logits, in one pass. The
+ * student's probabilities P (softmax(x / temperature)) and the teacher's Q are compared over the listed
+ * tokens and the rest as one: P_rest the sum of the others' p, Q_rest = max(0, 1 - sum Q) (0 with drop,
+ * and where the whole vocabulary is listed; at least 2^-24 in TISO_DISTILL_REVERSE, which drop does not
+ * go with). An entry whose id is ignore_index is left out; a token listed more than once has the sum
+ * of its probabilities; an id out of range makes its row NaN. divergence[r] = the row's D; out: one
+ * number, sum(w D) / sum(w), 0 when the weights sum to 0. A row of weight 0, or whose first entry is
+ * ignore_index, is left out: nothing else of it is read, its divergence and gradient are 0. grad
+ * ([rows][vocab], contiguous): upstream dloss/dx, where f = dD/dP: w / sum(w) p_v (f - sum P f) /
+ * temperature. coef ([rows] doubles), stats ([rows][2]) and listed ([rows][top], both of the
+ * accumulation type): NULL, or what tiso_distill_grad needs. Sums run in a fixed order. */
+int tiso_distill(int dtype, const tiso_rows* x, int64_t ignore_index, double temperature,
+                 const tiso_distill_args* args, void* divergence, double* coef, void* stats,
+                 void* listed, void* out, void* grad, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* The gradient for *upstream (a device scalar of the accumulation type), from what tiso_distill left;
+ * where *upstream equals `expected` nothing is written (grad must already hold that gradient). */
+int tiso_distill_grad(int dtype, const tiso_rows* x, int64_t ignore_index, double temperature,
+                      const int64_t* ids, int64_t top, const double* coef, const void* stats,
+                      const void* listed, double expected, const void* upstream, void* grad,
+                      void* stream);
+
 enum tiso_preference_kind {
   TISO_PREF_LOGISTIC = 0, /* (1 - e) log(1 + exp(-u)) + e log(1 + exp(u)), e = label_smoothing */
   TISO_PREF_HINGE = 1,    /* max(0, 1 - u) */

@@ -51,6 +51,13 @@ class PreferenceArgs(ctypes.Structure):
                 ("label_smoothing", ctypes.c_double), ("margin", ctypes.c_double)]
 
 
+class DistillArgs(ctypes.Structure):
+    """tiso_distill_args"""
+    _fields_ = [("ids", ctypes.c_void_p), ("logps", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("top", ctypes.c_int64), ("weight_is_byte", ctypes.c_int), ("kind", ctypes.c_int),
+                ("drop", ctypes.c_int), ("mix", ctypes.c_double), ("upstream", ctypes.c_double)]
+
+
 class AdamwArgs(ctypes.Structure):
     """tiso_adamw_args"""
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
@@ -98,6 +105,12 @@ def lib() -> ctypes.CDLL:
     so.tiso_preference_workspace_size.argtypes = [i64, ctypes.POINTER(sz)]
     so.tiso_preference.argtypes = [i32, pref, p, p, p, p, sz, p]
     so.tiso_preference_grad.argtypes = [i32, pref, p, p, p, p, p]
+    distill = ctypes.POINTER(DistillArgs)
+    so.tiso_scores.argtypes = [i32, rows, p, i64, dbl, i64, p, p, p, p, p, p]
+    so.tiso_scores_grad.argtypes = [i32, rows, p, dbl, p, p, p, p, p]
+    so.tiso_distill_workspace_size.argtypes = [i32, i64, ctypes.POINTER(sz)]
+    so.tiso_distill.argtypes = [i32, rows, i64, dbl, distill, p, p, p, p, p, p, p, sz, p]
+    so.tiso_distill_grad.argtypes = [i32, rows, i64, dbl, p, i64, p, p, p, dbl, p, p, p]
     so.tiso_adamw.argtypes = [i32, i32, i32, i64, p, ctypes.POINTER(AdamwArgs), p]
     so.tiso_last_error.restype = ctypes.c_char_p
     so.tiso_abi_version.restype = i32
@@ -109,7 +122,8 @@ def lib() -> ctypes.CDLL:
               "tiso_fit_varlen", "tiso_grad_varlen", "tiso_check_weights", "tiso_logprobs",
               "tiso_logprobs_grad", "tiso_policy_workspace_size", "tiso_policy",
               "tiso_preference_workspace_size", "tiso_preference", "tiso_preference_grad",
-              "tiso_adamw"):
+              "tiso_scores", "tiso_scores_grad", "tiso_distill_workspace_size", "tiso_distill",
+              "tiso_distill_grad", "tiso_adamw"):
         getattr(so, f).restype = i32
     if so.tiso_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH} has ABI {so.tiso_abi_version()}, expected {ABI_VERSION}")
@@ -552,6 +566,8 @@ def isotonic_grad_varlen(
 
 NATIVE_PATH = Path(__file__).resolve().parent / "_native.so"
 PREFERENCE_KINDS = {"logistic": 0, "hinge": 1, "square": 2}
+DISTILLATION_KINDS = {"forward": 0, "reverse": 1, "jensen": 2}
+MOST_LISTED = 128  # top alternatives, entries of a teacher's list
 
 
 @functools.cache

@@ -22,7 +22,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtiso.so"
-SOURCES = [CSRC / f for f in ("tiso.cu", "calib.cu", "logits.cu", "preference.cu", "adamw.cu")]
+SOURCES = [CSRC / f for f in ("tiso.cu", "calib.cu", "logits.cu", "preference.cu", "adamw.cu",
+                              "scores.cu", "distill.cu")]
 OBJECTS = PKG / "_build"
 NATIVE, NATIVE_SOURCE = PKG / "_native.so", CSRC / "native.cpp"
 DEPS = SOURCES + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "tiso.h"]

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <cstdint>
+#include <limits>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -84,10 +85,14 @@ void need_no_tangent(const std::optional<Tensor>& t) {
   if (t) need_no_tangent(*t);
 }
 
-bool ready_logits(const Tensor* x, const Tensor* targets, double temperature) {
+bool ready_rows(const Tensor* x, double temperature) {
   if (!x || !x->is_cuda() || x->dim() < 1 || x->size(-1) < 1 || !(temperature > 0)) return false;
   const ScalarType type = x->scalar_type();
-  return (type == at::kHalf || type == at::kBFloat16 || type == at::kFloat || type == at::kDouble) &&
+  return type == at::kHalf || type == at::kBFloat16 || type == at::kFloat || type == at::kDouble;
+}
+
+bool ready_logits(const Tensor* x, const Tensor* targets, double temperature) {
+  return ready_rows(x, temperature) &&
          ready(targets, at::kLong, x->sizes().slice(0, x->dim() - 1), x->device());
 }
 
@@ -147,14 +152,24 @@ void need_scalar(const Tensor& t, ScalarType type, const Tensor& beside) {
   need(t, "upstream", type, t.numel() == 1 ? t.sizes() : at::IntArrayRef(), beside);
 }
 
-void need_logits(const Tensor& x, const Tensor& targets) {
+void need_rows(const Tensor& x) {
   need_cuda(x, "logits");
   need_no_tangent(x);
   if (!x.is_floating_point() || x.element_size() == 1)
     throw py::type_error("logits must be float16, bfloat16, float32 or float64");
   if (x.dim() < 1 || x.size(-1) < 1)
     refuse("logits must have a last dimension of at least one element");
+}
+
+void need_logits(const Tensor& x, const Tensor& targets) {
+  need_rows(x);
   need(targets, "targets", at::kLong, x.sizes().slice(0, x.dim() - 1), x);
+}
+
+void need_list(const Tensor& x, const Tensor& ids) {
+  if (ids.dim() != x.dim() || ids.sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1))
+    refuse("ids must have logits' leading dimensions and one of entries");
+  need(ids, "ids", at::kLong, ids.sizes(), x);
 }
 
 void need_answers(const Tensor& logps, const std::optional<Tensor>& mask, const Tensor& offsets) {
@@ -500,6 +515,239 @@ std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> policy_loss(
 }
 
 // ---------------------------------------------------------------------------------------------
+// A token's scores
+
+struct ScoresResult {
+  Tensor logps, entropy, top_logps, top_ids, stats;  // logps: undefined without targets
+};
+
+ScoresResult scores(const Tensor& x, const std::optional<Tensor>& targets, int64_t top,
+                    double temperature, int64_t ignore_index, bool with_stats) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Logits logits(x);
+  const ScalarType acc = acc_of(x);
+  const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
+  c10::SmallVector<int64_t, 8> lists(shape.begin(), shape.end());
+  lists.push_back(top);
+  ScoresResult r;
+  if (targets) r.logps = empty(x, shape, acc);
+  r.entropy = empty(x, shape, acc);
+  r.top_logps = empty(x, lists, acc);
+  r.top_ids = empty(x, lists, at::kLong);
+  if (with_stats) r.stats = empty(x, {3 * logits.rows.rows}, acc);
+  check(tiso_scores(dtype_of(x.scalar_type()), &logits.rows,
+                    targets ? targets->data_ptr<int64_t>() : nullptr, ignore_index, temperature, top,
+                    targets ? data(r.logps) : nullptr, data(r.entropy), data(r.top_logps),
+                    r.top_ids.data_ptr<int64_t>(), with_stats ? data(r.stats) : nullptr,
+                    stream_of(x)));
+  return r;
+}
+
+// coef_logp, coef_entropy: contiguous, or undefined
+Tensor scores_grad(const Tensor& x, const std::optional<Tensor>& targets, double temperature,
+                   const Tensor& stats, const Tensor& coef_logp, const Tensor& coef_entropy) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Logits logits(x);
+  Tensor grad = empty(x, x.sizes(), x.scalar_type());
+  check(tiso_scores_grad(dtype_of(x.scalar_type()), &logits.rows,
+                         targets ? targets->data_ptr<int64_t>() : nullptr, temperature, data(stats),
+                         coef_logp.defined() ? data(coef_logp) : nullptr,
+                         coef_entropy.defined() ? data(coef_entropy) : nullptr, data(grad),
+                         stream_of(x)));
+  return grad;
+}
+
+struct Scores : torch::autograd::Function<Scores> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x,
+                               const std::optional<Tensor>& targets, int64_t top, double temperature,
+                               int64_t ignore_index) {
+    ScoresResult r = scores(x, targets, top, temperature, ignore_index, true);
+    ctx->save_for_backward({x, targets.value_or(Tensor()), r.stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->mark_non_differentiable({r.top_logps, r.top_ids});
+    ctx->set_materialize_grads(false);
+    variable_list out{r.entropy, r.top_logps, r.top_ids};
+    if (targets) out.push_back(r.logps);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(5);
+    const Tensor coef_entropy = grads[0].defined() ? grads[0].contiguous() : Tensor();
+    const Tensor coef_logp =
+        grads.size() > 3 && grads[3].defined() ? grads[3].contiguous() : Tensor();
+    if (!coef_entropy.defined() && !coef_logp.defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const auto targets = saved[1].defined() ? std::optional<Tensor>(saved[1]) : std::nullopt;
+    out[0] = once(scores_grad(saved[0], targets, ctx->saved_data["temperature"].toDouble(), saved[2],
+                              coef_logp, coef_entropy));
+    return out;
+  }
+};
+
+constexpr int64_t kMostListed = 128;
+
+std::optional<std::tuple<std::optional<Tensor>, Tensor, Tensor, Tensor>> token_scores(
+    py::handle logits, py::handle y, int64_t top, double temperature, int64_t ignore_index) {
+  const Tensor* x = tensor_in(logits);
+  if (!ready_rows(x, temperature) || top < 0 || top > kMostListed || top > x->size(-1))
+    return std::nullopt;
+  std::optional<Tensor> targets;
+  if (!y.is_none()) {
+    const Tensor* t = tensor_in(y);
+    if (!ready(t, at::kLong, x->sizes().slice(0, x->dim() - 1), x->device())) return std::nullopt;
+    targets = *t;
+  }
+  need_no_tangent(*x);
+  if (x->requires_grad() && at::GradMode::is_enabled()) {
+    const variable_list out = Scores::apply(*x, targets, top, temperature, ignore_index);
+    return std::make_tuple(targets ? std::optional<Tensor>(out[3]) : std::nullopt, out[0], out[1],
+                           out[2]);
+  }
+  const ScoresResult r = scores(*x, targets, top, temperature, ignore_index, false);
+  return std::make_tuple(targets ? std::optional<Tensor>(r.logps) : std::nullopt, r.entropy,
+                         r.top_logps, r.top_ids);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Distillation
+
+struct DistillSettings {
+  Tensor ids, logps;
+  std::optional<Tensor> weight;
+  int64_t kind;
+  bool drop;
+  double mix, temperature, upstream;
+  int64_t ignore_index;
+};
+
+struct DistillResult {
+  Tensor loss, divergence, kept, grad;
+};
+
+// kept: for a gradient n numbers coef, 2 n stats and n top listed (in doubles' places), then the
+// workspace (one allocation, in double).
+int64_t kept_of(int64_t n, int64_t top, ScalarType acc) {
+  return acc == at::kDouble ? n * (3 + top) : n + (n * (2 + top) + 1) / 2;
+}
+
+DistillResult distill(const Tensor& x, const DistillSettings& s, bool with_kept, bool with_grad) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Logits logits(x);
+  const ScalarType acc = acc_of(x);
+  const int dtype = dtype_of(x.scalar_type());
+  const int64_t n = logits.rows.rows, top = s.ids.size(-1);
+  tiso_distill_args args{};
+  args.ids = s.ids.data_ptr<int64_t>();
+  args.logps = data(s.logps);
+  args.weight = data(s.weight);
+  args.weight_is_byte = s.weight && s.weight->scalar_type() == at::kBool;
+  args.top = top;
+  args.kind = static_cast<int>(s.kind);
+  args.drop = s.drop;
+  args.mix = s.mix;
+  args.upstream = s.upstream;
+  size_t bytes = 0;
+  check(tiso_distill_workspace_size(dtype, n, &bytes));
+  const int64_t behind = with_kept ? kept_of(n, top, acc) : 0;
+  DistillResult r{empty(x, {}, acc), empty(x, x.sizes().slice(0, x.dim() - 1), acc),
+                  empty(x, {behind + static_cast<int64_t>((bytes + 7) / 8)}, at::kDouble), Tensor()};
+  if (with_grad) r.grad = empty(x, x.sizes(), x.scalar_type());
+  double* at = r.kept.data_ptr<double>();
+  char* stats = reinterpret_cast<char*>(at + n);
+  const int64_t each = acc == at::kDouble ? 8 : 4;
+  check(tiso_distill(dtype, &logits.rows, s.ignore_index, s.temperature, &args, data(r.divergence),
+                     with_kept ? at : nullptr, with_kept ? stats : nullptr,
+                     with_kept ? stats + 2 * n * each : nullptr, data(r.loss),
+                     with_grad ? data(r.grad) : nullptr, at + behind, bytes, stream_of(x)));
+  return r;
+}
+
+// The gradient times upstream. grad: what distill wrote for `expected`, overwritten unless upstream is
+// that; or undefined, for a new tensor.
+Tensor distill_grad(const Tensor& x, const Tensor& ids, double temperature, int64_t ignore_index,
+                    const Tensor& kept, double expected, const Tensor& upstream, Tensor grad) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const Logits logits(x);
+  const int64_t n = logits.rows.rows, top = ids.size(-1);
+  if (!grad.defined()) {
+    grad = empty(x, x.sizes(), x.scalar_type());
+    expected = std::numeric_limits<double>::quiet_NaN();
+  }
+  const double* at = kept.data_ptr<double>();
+  const char* stats = reinterpret_cast<const char*>(at + n);
+  check(tiso_distill_grad(dtype_of(x.scalar_type()), &logits.rows, ignore_index, temperature,
+                          ids.data_ptr<int64_t>(), top, at, stats,
+                          stats + 2 * n * (acc_of(x) == at::kDouble ? 8 : 4), expected,
+                          data(upstream), data(grad), stream_of(x)));
+  return grad;
+}
+
+struct Distill : torch::autograd::Function<Distill> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const DistillSettings& s) {
+    DistillResult r = distill(x, s, true, true);
+    ctx->save_for_backward({x, s.ids, r.kept});
+    ctx->saved_data["temperature"] = s.temperature;
+    ctx->saved_data["ignore_index"] = s.ignore_index;
+    ctx->saved_data["upstream"] = s.upstream;
+    ctx->saved_data["grad"] = r.grad;
+    ctx->mark_non_differentiable({r.divergence});
+    ctx->set_materialize_grads(false);
+    return {r.loss, r.divergence};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    // as of the policy loss: the gradient written with the loss is given away the first time
+    Tensor ready;
+    const auto at = ctx->saved_data.find("grad");
+    if (at != ctx->saved_data.end()) {
+      ready = at->second.toTensor();
+      ctx->saved_data.erase(at);
+    }
+    return {once(distill_grad(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(),
+                              ctx->saved_data["ignore_index"].toInt(), saved[2],
+                              ctx->saved_data["upstream"].toDouble(), grads[0], ready)),
+            Tensor()};
+  }
+};
+
+std::optional<std::tuple<Tensor, Tensor>> distillation_loss(
+    py::handle logits, py::handle of_ids, py::handle of_logps, py::handle of_weight, int64_t kind,
+    bool drop, double mix, double temperature, double upstream, int64_t ignore_index) {
+  const Tensor *x = tensor_in(logits), *ids = tensor_in(of_ids), *logps = tensor_in(of_logps);
+  if (!ready_rows(x, temperature) || !ids || ids->dim() != x->dim() || kind < 0 ||
+      !(mix > 0 && mix < 1) || (kind == TISO_DISTILL_REVERSE && drop))
+    return std::nullopt;
+  const at::IntArrayRef shape = x->sizes().slice(0, x->dim() - 1);
+  const at::Device device = x->device();
+  if (ids->sizes().slice(0, x->dim() - 1) != shape || ids->size(-1) < 1 ||
+      ids->size(-1) > kMostListed || !ready(ids, at::kLong, ids->sizes(), device) ||
+      !ready(logps, acc_of(*x), ids->sizes(), device))
+    return std::nullopt;
+  const bool grad_mode = at::GradMode::is_enabled();
+  if (grad_mode && logps->requires_grad()) return std::nullopt;
+  DistillSettings s{*ids, *logps, std::nullopt, kind, drop, mix, temperature, upstream, ignore_index};
+  if (!of_weight.is_none()) {
+    const Tensor* t = tensor_in(of_weight);
+    if (!t || !ready(t, t->scalar_type() == at::kBool ? at::kBool : acc_of(*x), shape, device) ||
+        (grad_mode && t->requires_grad()))
+      return std::nullopt;
+    s.weight = *t;
+  }
+  need_no_tangent(*x);
+  need_no_tangent(*logps);
+  need_no_tangent(s.weight);
+  if (x->requires_grad() && grad_mode) {
+    const variable_list out = Distill::apply(*x, s);
+    return std::make_tuple(out[0], out[1]);
+  }
+  const DistillResult r = distill(*x, s, false, false);
+  return std::make_tuple(r.loss, r.divergence);
+}
+
+// ---------------------------------------------------------------------------------------------
 // AdamW
 
 // The tensors of a sequence, and what keeps them alive.
@@ -610,6 +858,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("token_logprobs", &token_logprobs);
   m.def("preference_loss", &preference_loss);
   m.def("policy_loss", &policy_loss);
+  m.def("token_scores", &token_scores);
+  m.def("distillation_loss", &distillation_loss);
   m.def("adamw", &adamw);
   // the steps alone, for the torch.library operators
   m.def("logprobs", [](const Tensor& x, const Tensor& targets, double temperature,
@@ -661,5 +911,44 @@ PYBIND11_MODULE(_native, m) {
     need(kept, "kept", at::kDouble, {targets.numel() * (acc_of(x) == at::kDouble ? 3 : 2)}, x);
     need_scalar(upstream, acc_of(x), x);
     return policy_grad(x, targets, temperature, kept, upstream, Tensor());
+  });
+  m.def("scores", [](const Tensor& x, const std::optional<Tensor>& targets, int64_t top,
+                     double temperature, int64_t ignore_index) {
+    need_rows(x);
+    need(targets, "targets", at::kLong, x.sizes().slice(0, x.dim() - 1), x);
+    const ScoresResult r = scores(x, targets, top, temperature, ignore_index, true);
+    return std::make_tuple(targets ? r.logps : empty(x, {0}, acc_of(x)), r.entropy, r.top_logps,
+                           r.top_ids, r.stats);
+  });
+  m.def("scores_grad", [](const Tensor& x, const std::optional<Tensor>& targets, double temperature,
+                          const Tensor& stats, const std::optional<Tensor>& coef_logp,
+                          const Tensor& coef_entropy) {
+    need_rows(x);
+    const at::IntArrayRef shape = x.sizes().slice(0, x.dim() - 1);
+    need(targets, "targets", at::kLong, shape, x);
+    need(stats, "stats", acc_of(x), {3 * (x.numel() / x.size(-1))}, x);
+    need(coef_logp, "coef_logp", acc_of(x), shape, x);
+    need(coef_entropy, "coef_entropy", acc_of(x), shape, x);
+    return scores_grad(x, targets, temperature, stats, coef_logp.value_or(Tensor()), coef_entropy);
+  });
+  m.def("distill", [](const Tensor& x, const Tensor& ids, const Tensor& logps,
+                      const std::optional<Tensor>& weight, int64_t kind, bool drop, double mix,
+                      double temperature, int64_t ignore_index) {
+    need_rows(x);
+    need_list(x, ids);
+    need(logps, "logps", acc_of(x), ids.sizes(), x);
+    need(weight, "weight", weight && weight->scalar_type() == at::kBool ? at::kBool : acc_of(x),
+         x.sizes().slice(0, x.dim() - 1), x);
+    const DistillResult r = distill(
+        x, {ids, logps, weight, kind, drop, mix, temperature, 1.0, ignore_index}, true, false);
+    return std::make_tuple(r.loss, r.divergence, r.kept);
+  });
+  m.def("distill_grad", [](const Tensor& x, const Tensor& ids, double temperature,
+                           int64_t ignore_index, const Tensor& kept, const Tensor& upstream) {
+    need_rows(x);
+    need_list(x, ids);
+    need(kept, "kept", at::kDouble, {kept_of(x.numel() / x.size(-1), ids.size(-1), acc_of(x))}, x);
+    need_scalar(upstream, acc_of(x), x);
+    return distill_grad(x, ids, temperature, ignore_index, kept, 0.0, upstream, Tensor());
   });
 }

@@ -1,7 +1,9 @@
 """Losses that a language model is trained on, in front of the calibration of its answers: token
-log-probabilities, the preference loss over paired log ratios, and the clipped policy loss with a
-KL term, each forward and backward in this library's kernels. The margins that a preference-trained
-model gives held-out pairs are what ``fit_calibration`` turns into probabilities.
+log-probabilities, a token's scores (with the entropy and the top alternatives), the preference loss
+over paired log ratios, the clipped policy loss with a KL term, and the distillation from a
+teacher's top lists, each forward and backward in this library's kernels. The margins that a
+preference-trained model gives held-out pairs, and the probability of a token's best alternative,
+are what ``fit_calibration`` turns into probabilities.
 
 The reference has no such operators; the conventions are those of the rest of this package: CUDA
 tensors only, float16 and bfloat16 computed in float32, float64 kept, rows packed with offsets.
@@ -27,6 +29,17 @@ def _need_cuda(t: Tensor, name: str) -> None:
 
 def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _check_rows(logits: Tensor, temperature: float) -> None:
+    if not isinstance(logits, Tensor):
+        raise TypeError("logits must be a torch.Tensor")
+    if not logits.is_floating_point() or logits.dtype not in _ext._DTYPES:
+        raise TypeError("logits must be float16, bfloat16, float32 or float64")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must have a last dimension of at least one element")
+    if not temperature > 0:
+        raise ValueError("temperature must be > 0")
 
 
 def _check_logits(logits: Tensor, targets: Tensor, temperature: float) -> None:
@@ -72,6 +85,61 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, temperature: float = 1.0,
     if traced:  # the operators, which the compiler keeps whole
         return ops.token_logprobs(logits, targets, *settings)[0]
     return _ext.native().token_logprobs(logits, targets, *settings)
+
+
+class TokenScores(NamedTuple):
+    """What ``token_scores`` returns; ``logps`` and ``entropy`` have gradients."""
+
+    logps: Tensor | None
+    entropy: Tensor
+    top_logps: Tensor
+    top_ids: Tensor
+
+
+def token_scores(logits: Tensor, targets: Tensor | None = None, *, top: int = 0,
+                 temperature: float = 1.0, ignore_index: int = -100) -> TokenScores:
+    """A token's scores in one pass over its logits: its log-probability, the entropy of the
+    distribution it was drawn from, and the likeliest alternatives.
+
+    ``logits``: [..., vocab], CUDA, read in place where ``token_logprobs`` does; ``targets``: [...],
+    integers, or None where no token is given; ``top``: how many alternatives, 0 to 128 (at most
+    the vocabulary). With ``p = softmax(logits / temperature)`` returns ``TokenScores(logps, entropy,
+    top_logps, top_ids)``:
+
+    * ``logps`` [...]: ``log p`` at the target (None without targets);
+    * ``entropy`` [...]: ``-sum p log p``, in nats (tokens of probability 0 add nothing);
+    * ``top_ids``, ``top_logps`` [..., top]: the largest logits' tokens, largest first, equal ones by
+      their id (NaN stands with -inf), and their log-probabilities: the lists that
+      ``distillation_loss`` takes from a teacher.
+
+    ``logps`` and ``entropy`` are differentiable (once) in ``logits``, the alternatives are not.
+    float32 (float64 for float64 logits), ids int64.
+
+    Where a target is ``ignore_index`` the row is not read: log-probability, entropy and gradient
+    are 0, its ids ``ignore_index`` and their log-probabilities 0. Any other target outside ``[0,
+    vocab)`` gives a NaN log-probability and gradient. A row with nothing but -inf, or with NaN or
+    +inf, gives NaN numbers.
+    """
+    traced = torch.compiler.is_compiling()
+    if isinstance(top, bool) or not isinstance(top, int):
+        raise TypeError("top must be an int")
+    settings = float(temperature), int(ignore_index)
+    if not traced:
+        got = _ext.native().token_scores(logits, targets, max(-1, min(top, 1 << 20)), *settings)
+        if got is not None:
+            return TokenScores(*got)
+    _check_rows(logits, temperature)
+    if not 0 <= top <= min(_ext.MOST_LISTED, logits.shape[-1]):
+        raise ValueError(f"top must be from 0 to {_ext.MOST_LISTED} and to the vocabulary, got {top}")
+    if targets is None:
+        _need_cuda(logits, "logits")
+    else:
+        _check_logits(logits, targets, temperature)
+        targets = _as(targets, torch.int64)
+    if traced:
+        logps, *rest, _ = ops.token_scores(logits, targets, top, *settings)
+        return TokenScores(None if targets is None else logps, *rest)
+    return TokenScores(*_ext.native().token_scores(logits, targets, top, *settings))
 
 
 def preference_loss(
@@ -228,3 +296,111 @@ def policy_loss(
         rest = out.detach()
         return PolicyLoss(out[0], logps.detach(), rest[1], rest[2])
     return PolicyLoss(*_ext.native().policy_loss(logits, targets, *rows, *constants, *clip))
+
+
+class DistillationLoss(NamedTuple):
+    """What ``distillation_loss`` returns; only ``loss`` has a gradient."""
+
+    loss: Tensor
+    divergence: Tensor
+
+
+def distillation_loss(
+    logits: Tensor,
+    teacher_ids: Tensor,
+    teacher_logps: Tensor,
+    *,
+    kind: str = "forward",
+    rest: str = "bucket",
+    mix: float = 0.5,
+    weight: Tensor | None = None,
+    temperature: float = 1.0,
+    ignore_index: int = -100,
+    upstream: float = 1.0,
+) -> DistillationLoss:
+    """Divergence of a student from a teacher whose likeliest tokens are known, from the student's
+    logits, with its gradient in one pass over them.
+
+    ``logits``: [..., vocab], CUDA; ``teacher_ids``, ``teacher_logps``: [..., k], 1 to 128 entries, the
+    teacher's top tokens and their log-probabilities, taken at the student's ``temperature``
+    (``token_scores(teacher_logits, top=k, temperature=temperature)``). An entry whose id is
+    ``ignore_index`` is left out; a list may come in any order, and a token listed twice has the sum
+    of its probabilities.
+
+    Student (``P``, ``softmax(logits / temperature)``) and teacher (``Q``) are compared over the listed
+    tokens and all others as one: with ``rest="bucket"`` the others' ``P`` is their sum and their
+    ``Q`` is ``max(0, 1 - sum Q)`` (0 where the whole vocabulary is listed); with ``rest="drop"`` the
+    teacher's probabilities are renormalised over the list and the others' ``Q`` is 0. By ``kind``:
+
+    * "forward": ``sum Q log(Q / P)``, infinite where a token of the teacher's has ``P = 0``;
+    * "reverse": ``sum P log(P / Q)``, the others' ``Q`` at least ``2^-24`` (only with "bucket");
+    * "jensen": ``mix sum Q log(Q / M) + (1 - mix) sum P log(P / M)``, ``M = mix Q + (1 - mix) P``, 0 <
+      mix < 1.
+
+    The loss is ``sum(weight D) / sum(weight)`` (0 if the weights sum to 0), without the factor
+    ``temperature^2`` that some put in front. ``weight``: [...], numbers or a bool mask; None for 1.
+    A token of weight 0, or whose list begins with ``ignore_index``, is left out: nothing else of it
+    is read, its divergence and gradient are 0. An id outside ``[0, vocab)``, and a row of logits
+    with nothing but -inf or with NaN or +inf, make that token NaN. Logits of -inf have no
+    gradient, unless they are listed.
+
+    The gradient is written with the loss, for an upstream gradient of exactly ``upstream`` (give a
+    loss scale, or 1 / the number of micro-batches); any other one takes another pass over the
+    logits in the backward.
+
+    Returns ``DistillationLoss(loss, divergence)``: the loss, differentiable (once) in ``logits``
+    alone, and every token's ``D`` [...]. float32 (float64 for float64 logits).
+    """
+    traced = torch.compiler.is_compiling()
+    number = _ext.DISTILLATION_KINDS.get(kind, -1)
+    settings = float(mix), float(temperature)
+    if not traced and rest in ("bucket", "drop"):
+        got = _ext.native().distillation_loss(logits, teacher_ids, teacher_logps, weight, number,
+                                              rest == "drop", *settings, float(upstream),
+                                              int(ignore_index))
+        if got is not None:
+            return DistillationLoss(*got)
+    if number < 0:
+        raise ValueError(f"kind must be one of {', '.join(_ext.DISTILLATION_KINDS)}, got {kind!r}")
+    if rest not in ("bucket", "drop"):
+        raise ValueError(f"rest must be bucket or drop, got {rest!r}")
+    if kind == "reverse" and rest == "drop":
+        raise ValueError("the reverse divergence has no value without the rest")
+    if not 0 < mix < 1:
+        raise ValueError("mix must be between 0 and 1")
+    _check_rows(logits, temperature)
+    if not isinstance(teacher_ids, Tensor) or not isinstance(teacher_logps, Tensor):
+        raise TypeError("teacher_ids and teacher_logps must be torch.Tensors")
+    if (teacher_ids.is_floating_point() or teacher_ids.is_complex()
+            or teacher_ids.dtype == torch.bool):
+        raise TypeError("teacher_ids must be an integer tensor")
+    if not teacher_logps.is_floating_point():
+        raise TypeError("teacher_logps must be a floating-point tensor")
+    if teacher_ids.dim() != logits.dim() or teacher_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"teacher_ids of shape {tuple(teacher_ids.shape)} do not fit logits of shape "
+                         f"{tuple(logits.shape)}")
+    if not 1 <= teacher_ids.shape[-1] <= _ext.MOST_LISTED:
+        raise ValueError(f"a list must have 1 to {_ext.MOST_LISTED} entries")
+    if teacher_logps.shape != teacher_ids.shape:
+        raise ValueError("teacher_logps must be shaped like teacher_ids")
+    _need_cuda(logits, "logits")
+    if teacher_ids.device != logits.device or teacher_logps.device != logits.device:
+        raise ValueError("teacher_ids and teacher_logps must be on logits' device")
+    acc = _ext.acc_dtype(logits.dtype)
+    if weight is not None:
+        if not isinstance(weight, Tensor) or weight.is_complex():
+            raise TypeError("weight must be a real torch.Tensor")
+        if weight.shape != logits.shape[:-1] or weight.device != logits.device:
+            raise ValueError("weight must have logits' leading dimensions and be on their device")
+    for name, t in (("teacher_logps", teacher_logps), ("weight", weight)):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} is a constant of the loss: detach it")
+    if weight is not None:
+        weight = _as(weight, torch.bool if weight.dtype == torch.bool else acc)
+    lists = _as(teacher_ids, torch.int64), _as(teacher_logps, acc), weight
+    if traced:
+        loss, divergence, _ = ops.distillation(logits, *lists, number, rest == "drop", *settings,
+                                               int(ignore_index))
+        return DistillationLoss(loss, divergence)
+    return DistillationLoss(*_ext.native().distillation_loss(
+        logits, *lists, number, rest == "drop", *settings, float(upstream), int(ignore_index)))

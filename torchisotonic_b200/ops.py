@@ -21,9 +21,9 @@ Two more carry what this library folds into its kernels, and are what ``isotonic
   the clamp's inclusive mask applied.
 
 The losses of ``losses.py`` have theirs, which the public functions run under ``torch.compile``:
-``token_logprobs``, ``preference`` and ``policy``, each with its ``_grad``. (``policy`` leaves the
-gradient to ``policy_grad``, which reads the logits again; the eager function writes it with the
-loss.)
+``token_logprobs``, ``token_scores``, ``preference``, ``policy`` and ``distillation``, each with its
+``_grad``. (``policy`` and ``distillation`` leave the gradient to their ``_grad``, which reads the
+logits again; the eager functions write it with the loss.)
 
 ``fit`` has its autograd registered (the reference's _Isotonic, src/torchisotonic/_api.py:73-97)
 and every operator a fake (meta) implementation, so ``torch.compile`` traces through them
@@ -279,3 +279,98 @@ def _policy_backward(ctx, grad: Tensor, _grad_logps: Tensor, _grad_kept: Tensor)
 
 
 torch.library.register_autograd(f"{_NS}::policy", _policy_backward, setup_context=_policy_setup)
+
+
+@torch.library.custom_op(f"{_NS}::token_scores", mutates_args=())
+def token_scores(logits: Tensor, targets: Tensor | None, top: int, temperature: float,
+                 ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    return _ext.native().scores(logits, _dense(targets), top, temperature, ignore_index)
+
+
+@token_scores.register_fake
+def _(logits, targets, top, temperature, ignore_index):
+    acc, shape = _acc(logits.dtype), logits.shape[:-1]
+    return (logits.new_empty((0,) if targets is None else shape, dtype=acc),
+            logits.new_empty(shape, dtype=acc), logits.new_empty((*shape, top), dtype=acc),
+            logits.new_empty((*shape, top), dtype=torch.int64),
+            logits.new_empty((3 * (logits.numel() // logits.shape[-1]),), dtype=acc))
+
+
+@torch.library.custom_op(f"{_NS}::token_scores_grad", mutates_args=())
+def token_scores_grad(logits: Tensor, targets: Tensor | None, temperature: float, stats: Tensor,
+                      coef_logp: Tensor | None, coef_entropy: Tensor) -> Tensor:
+    return _ext.native().scores_grad(logits, _dense(targets), temperature, _dense(stats),
+                                     _dense(coef_logp), _dense(coef_entropy))
+
+
+@token_scores_grad.register_fake
+def _(logits, targets, temperature, stats, coef_logp, coef_entropy):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _token_scores_setup(ctx, inputs, output) -> None:
+    logits, targets, _, ctx.temperature, _ = inputs
+    ctx.save_for_backward(logits, targets, output[4])
+    ctx.mark_non_differentiable(output[2], output[3])
+
+
+def _token_scores_backward(ctx, grad: Tensor, grad_entropy: Tensor, *_):
+    logits, targets, stats = ctx.saved_tensors
+    return (token_scores_grad(logits, targets, ctx.temperature, stats,
+                              None if targets is None else grad, grad_entropy), *(None,) * 4)
+
+
+torch.library.register_autograd(f"{_NS}::token_scores", _token_scores_backward,
+                                setup_context=_token_scores_setup)
+
+
+def _kept_of_lists(logits: Tensor, ids: Tensor) -> int:
+    """float64 numbers of what distillation_grad needs: for each token a coefficient, two numbers
+    and one for each entry (in the accumulation dtype)."""
+    n, numbers = logits.numel() // logits.shape[-1], 2 + ids.shape[-1]
+    return n * (1 + numbers) if _acc(logits.dtype) == torch.float64 else n + (n * numbers + 1) // 2
+
+
+@torch.library.custom_op(f"{_NS}::distillation", mutates_args=())
+def distillation(logits: Tensor, teacher_ids: Tensor, teacher_logps: Tensor, weight: Tensor | None,
+                 kind: int, drop: bool, mix: float, temperature: float,
+                 ignore_index: int) -> tuple[Tensor, Tensor, Tensor]:
+    loss, divergence, kept = _ext.native().distill(
+        logits, _dense(teacher_ids), _dense(teacher_logps), _dense(weight), kind, drop, mix,
+        temperature, ignore_index)
+    return loss, divergence, kept[:_kept_of_lists(logits, teacher_ids)].clone()
+
+
+@distillation.register_fake
+def _(logits, teacher_ids, teacher_logps, weight, kind, drop, mix, temperature, ignore_index):
+    acc = _acc(logits.dtype)
+    return (logits.new_empty((), dtype=acc), logits.new_empty(logits.shape[:-1], dtype=acc),
+            logits.new_empty((_kept_of_lists(logits, teacher_ids),), dtype=torch.float64))
+
+
+@torch.library.custom_op(f"{_NS}::distillation_grad", mutates_args=())
+def distillation_grad(logits: Tensor, teacher_ids: Tensor, temperature: float, ignore_index: int,
+                      kept: Tensor, upstream: Tensor) -> Tensor:
+    return _ext.native().distill_grad(logits, _dense(teacher_ids), temperature, ignore_index,
+                                      _dense(kept), upstream)
+
+
+@distillation_grad.register_fake
+def _(logits, teacher_ids, temperature, ignore_index, kept, upstream):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _distillation_setup(ctx, inputs, output) -> None:
+    logits, ids, *_, ctx.temperature, ctx.ignore_index = inputs
+    ctx.save_for_backward(logits, ids, output[2])
+    ctx.mark_non_differentiable(output[1], output[2])
+
+
+def _distillation_backward(ctx, grad: Tensor, *_):
+    logits, ids, kept = ctx.saved_tensors
+    return (distillation_grad(logits, ids, ctx.temperature, ctx.ignore_index, kept, grad),
+            *(None,) * 8)
+
+
+torch.library.register_autograd(f"{_NS}::distillation", _distillation_backward,
+                                setup_context=_distillation_setup)
