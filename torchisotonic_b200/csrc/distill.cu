@@ -21,7 +21,8 @@ namespace tiso {
 namespace {
 
 constexpr int kMostListed = 128;
-constexpr size_t kSharedForBits = 160 * 1024;
+constexpr int kSmThreads = 1536;  // resident at 40 registers a thread
+constexpr int kSharedForBits = 160 * 1024;
 // the teacher's rest where it is divided by: a list's float log-probabilities say no less
 constexpr double kLeastRest = 1.0 / (1 << 24);
 
@@ -37,44 +38,66 @@ struct DistillArgs {
   double* coef;   // NULL, or per row the rest's factor for an upstream gradient of 1
   A* stats;       // per row the rest's base, and -1 where the row is left out
   A* listed;      // per row and entry the gradient for an upstream gradient of 1
-  A* terms;       // per row w D
+  A* terms;       // per unit (a row, or a CTA's rows) w D
   A* out;
   double* total;
   unsigned* done;
 };
 
+// Sums over the list's tokens: of q, q log q, q z, e = exp(z) and e (z - log q), z the logits from the
+// list's own maximum, over t; and how many tokens there are.
+struct ListSums {
+  double q, q_log_q, q_z, e, e_far;
+  int tokens;
+};
+
+// What the gradient of the list is made of, once the row's sum is known.
+struct Settled {
+  double c;      // the row's share of the loss, over t
+  double p;      // of an e: its probability
+  double log_p;  // of a z: its logarithm
+  double mean;   // sum P f
+  double list_q, whole;
+};
+
+constexpr int kListWarps = kMostListed / 32;
+
 // Shared memory of the threads that work on a row.
 template <typename A>
 struct ListSpace {
-  double *q, *log_q;     // the teacher's
+  double *q, *log_q, *e;  // the teacher's probabilities; exp(z)
+  ListSums* sums;         // of each warp that has entries
+  Settled* settled;
   A *logit, *gradient;
-  int *id, *lead;        // -1: no entry; the first entry of its id
-  unsigned* bits;        // of this CTA's share of the vectors: a bit an element
-  unsigned* edge_bits;   // of the single elements
-  int *bad, *twice;      // an id out of range; an id listed again
-  A *base, *scale;       // of the rest's gradient
+  A* most;                // of each of these warps, the largest logit
+  int *id, *lead;         // -1: no entry; the first entry of its id
+  int *bad, *twice;       // an id out of range; an id listed again
+  unsigned* edge_bits;    // of the single elements
+  unsigned* bits;         // of this CTA's share of the vectors: a bit an element
 
-  static size_t bytes(int top, size_t bits) {
-    const size_t n = (top + 3) / 4 * 4;
-    return n * (2 * sizeof(double) + 2 * sizeof(A) + 2 * sizeof(int)) + 4 * sizeof(double) +
-           (bits + 15) / 16 * 16;
+  static __host__ __device__ int entries(int top) { return (top + 3) / 4 * 4; }
+  static __host__ __device__ int bytes(int top, int bits) {
+    return entries(top) * static_cast<int>(3 * sizeof(double) + 2 * sizeof(A) + 2 * sizeof(int)) +
+           static_cast<int>(kListWarps * sizeof(ListSums) + sizeof(Settled) + kListWarps * sizeof(A)) +
+           16 + (bits + 15) / 16 * 16;
   }
 
   __device__ ListSpace(void* at, int top) {
-    const int n = (top + 3) / 4 * 4;
+    const int n = entries(top);
     q = static_cast<double*>(at);
     log_q = q + n;
-    A* numbers = reinterpret_cast<A*>(log_q + n);
-    base = numbers;
-    scale = numbers + 1;
-    logit = numbers + (sizeof(A) == 4 ? 4 : 2);  // 16 bytes on
+    e = log_q + n;
+    sums = reinterpret_cast<ListSums*>(e + n);
+    settled = reinterpret_cast<Settled*>(sums + kListWarps);
+    logit = reinterpret_cast<A*>(settled + 1);
     gradient = logit + n;
-    id = reinterpret_cast<int*>(gradient + n);
+    most = gradient + n;
+    id = reinterpret_cast<int*>(most + kListWarps);
     lead = id + n;
     bad = lead + n;
     twice = bad + 1;
     edge_bits = reinterpret_cast<unsigned*>(bad + 2);
-    bits = reinterpret_cast<unsigned*>(bad + 4);
+    bits = edge_bits + 2;
   }
 };
 
@@ -127,36 +150,29 @@ __device__ __forceinline__ void hide(uint4& q, unsigned bits) {
   }
 }
 
-// The part of the rest that a thread sees.
-template <int kThreads, typename T, typename A>
-__device__ __forceinline__ Part<A> rest_part(const RowView<T>& r, const Place<kThreads>& place,
-                                             const ListSpace<A>& space, A k) {
-  constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
-  const int e = place.edge();
-  const A edge = e < r.edges && !(*space.edge_bits >> e & 1) ? to_acc(r.x[r.edge(e)]) : lowest<A>();
-  Part<A> p{lowest<A>(), A(0)};
-  int local = 0;
-  for (int tile = place.cta * kTile; tile < r.vectors; tile += place.ctas * kTile, ++local) {
-    const int v = tile + place.tid;
-    uint4 q[kBatch];
-    if (tile + kTile <= r.vectors) {
-      load_vectors<kBatch, kThreads>(r, v, q);
-    } else {
+// Adds a tile's vectors but for the listed tokens.
+template <typename T, typename A>
+__device__ __forceinline__ void add_rest(Part<A>& p, uint4 (&q)[kBatch], unsigned bits, A k) {
+  constexpr int E = RowView<T>::E;
+  if (bits) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        q[i] = v + i * kThreads < r.vectors ? load_vector(r, v + i * kThreads) : no_vector<T>();
+    for (int i = 0; i < kBatch; ++i) {
+      const unsigned own = bits >> i * E & ((1u << E) - 1);
+      if (own) hide<T>(q[i], own);
     }
-    const unsigned bits = bits_of_tile<kThreads, T>(space.bits, local, place.tid);
-    if (bits) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) hide<T>(q[i], bits >> i * E & ((1u << E) - 1));
-    }
-    add_vectors<T>(p, q, k);
   }
+  add_vectors<T>(p, q, k);
+}
+
+// Adds one of the single elements, unless it is listed.
+template <typename T, int kThreads, typename A>
+__device__ __forceinline__ void add_edge(Part<A>& p, const RowView<T>& r, const Place<kThreads>& place,
+                                         unsigned edge_bits, A k) {
+  const int e = place.edge();
+  const A edge = e < r.edges && !(edge_bits >> e & 1) ? to_acc(r.x[r.edge(e)]) : lowest<A>();
   const A m = max_acc(p.m, edge), base = base_of(m);
   p.s = (p.m == m ? p.s : p.s * scaled_exp(p.m - base, k)) + scaled_exp(edge - base, k);
   p.m = m;
-  return p;
 }
 
 __device__ __forceinline__ double sum_of_warp(double v) {
@@ -167,111 +183,231 @@ __device__ __forceinline__ double sum_of_warp(double v) {
 
 __device__ __forceinline__ double product(double x, double y) { return x == 0 ? 0.0 : x * y; }
 
-// The steps over the list by a warp, in double: the divergence, and in `space` the gradient of the
-// listed tokens and the base and scale of the rest's, all times c.
-template <typename A>
-__device__ __forceinline__ double settle(const DistillArgs<A>& p, const ListSpace<A>& space,
-                                         const Part<A>& rest, int vocab, double inv_temp, double c,
-                                         double& scale) {
-  constexpr int kEach = kMostListed / 32;
-  const int lane = threadIdx.x & 31;
-  double q[kEach], log_q[kEach], z[kEach];
-  bool there[kEach];
-  A m = rest.m;
-  double listed_q = 0;
-  int tokens = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int k = lane + 32 * i;
-    there[i] = k < p.top && space.lead[k] == k;
-    q[i] = there[i] ? space.q[k] : 0.0;
-    log_q[i] = there[i] ? space.log_q[k] : 0.0;
-    z[i] = there[i] ? static_cast<double>(space.logit[k]) : static_cast<double>(lowest<A>());
-    m = max_acc(m, static_cast<A>(z[i]));
-    listed_q += q[i];
-    tokens += __popc(__ballot_sync(0xffffffffu, there[i]));
-  }
-  m = max_of_lanes<32>(m);
-  listed_q = sum_of_warp(listed_q);
-  // the student: z relative to the maximum, logarithms less log s
-  const double base = static_cast<double>(base_of(m));
-  double e[kEach], s = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    z[i] = (z[i] - base) * inv_temp;
-    e[i] = there[i] ? exp(z[i]) : 0.0;
-    s += e[i];
-  }
-  const double rest_z = (static_cast<double>(rest.m) - base) * inv_temp;
-  const double rest_e = rest.s == A(0) ? 0.0 : exp(rest_z) * static_cast<double>(rest.s);
-  s = sum_of_warp(s) + rest_e;
-  const double log_s = log(s), rest_p = rest_e / s;
-  const double rest_log_p = rest_z + log(static_cast<double>(rest.s)) - log_s;
-  // the teacher
-  double rest_q = tokens == vocab ? 0.0 : fmax(1.0 - listed_q, 0.0), whole = listed_q + rest_q;
-  if (p.drop) {
-    rest_q = 0.0;
-    whole = listed_q > 0 ? 1.0 : 0.0;
-    const double log_listed = log(listed_q);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      log_q[i] = q[i] > 0 ? log_q[i] - log_listed : log_q[i];
-      q[i] = q[i] > 0 ? q[i] / listed_q : q[i];
+// Warps with entries of a list, and the largest of its logits.
+template <int kThreads>
+__device__ __forceinline__ int warps_of(int top) {
+  return min((top + 31) / 32, kThreads / 32);
+}
+template <int kThreads, typename A>
+__device__ __forceinline__ A most_of(const ListSpace<A>& space, int top) {
+  A most = space.most[0];
+  for (int i = 1; i < warps_of<kThreads>(top); ++i) most = max_acc(most, space.most[i]);
+  return most;
+}
+
+// The list of row r into shared memory, its bits, and its sums (after the next meeting of the
+// threads).
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void read_list(const Rows& a, const DistillArgs<A>& p, int64_t r,
+                                          const RowView<T>& view, const Place<kThreads>& place,
+                                          int bit_words, double inv_temp, const ListSpace<A>& space) {
+  const Team<kThreads> team{place.tid};
+  for (int i = team.tid; i < bit_words; i += kThreads) space.bits[i] = 0;
+  if (team.tid == 0) *space.bad = *space.twice = static_cast<int>(*space.edge_bits = 0u);
+  team.sync();
+  const bool has_entries = team.tid / 32 * 32 < p.top;  // this warp
+  A most = lowest<A>();
+  for (int k = team.tid; k < p.top; k += kThreads) {
+    const int64_t id = p.ids[r * p.top + k];
+    const bool listed = id != a.ignore, in = id >= 0 && id < a.vocab;
+    if (listed && !in) *space.bad = 1;
+    space.id[k] = space.lead[k] = -1;
+    space.gradient[k] = A(0);
+    if (!listed || !in) continue;
+    const double log_q = static_cast<double>(p.logps[r * p.top + k]);
+    const A logit = to_acc(view.x[id]);
+    const Spot<kThreads, T> spot(view, place.ctas, static_cast<int>(id));
+    if (spot.cta == place.cta) {
+      unsigned* word = spot.edge ? space.edge_bits : space.bits + spot.bit / 32;
+      if (atomicOr(word, 1u << spot.bit % 32) >> spot.bit % 32 & 1) *space.twice = 1;
     }
-  } else if (p.kind == TISO_DISTILL_REVERSE && tokens < vocab) {
-    rest_q = fmax(rest_q, kLeastRest);
+    space.id[k] = static_cast<int>(id);
+    space.lead[k] = k;
+    space.logit[k] = logit;
+    space.log_q[k] = log_q;
+    space.q[k] = exp(log_q);
+    most = max_acc(most, logit);
   }
-  if (listed_q != listed_q) rest_q = listed_q;  // NaN
-  const double rest_log_q = log(rest_q);
-  double d = 0, factor;
-  if (p.kind == TISO_DISTILL_FORWARD) {
-    // p_v (f - sum P f) = p_v whole - q_v
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      d += product(q[i], log_q[i] - (z[i] - log_s));
-      if (there[i]) e[i] = e[i] / s * whole - q[i];
+  if (has_entries) {
+    most = max_of_lanes<32>(most);
+    if (team.tid % 32 == 0) space.most[team.tid / 32] = most;
+  }
+  team.sync();
+  if (place.ctas > 1 || *space.twice) {
+    // the same id again: its probabilities are added up in its first entry. (A CTA of a cluster sees
+    // only its own elements' bits, and looks through the list.)
+    for (int k = team.tid; k < p.top; k += kThreads) {
+      const int id = space.id[k];
+      if (id < 0) continue;
+      int first = k;
+      for (int j = k - 1; j >= 0; --j)
+        if (space.id[j] == id) first = j;
+      space.lead[k] = first;
     }
-    d = sum_of_warp(d) + product(rest_q, rest_log_q - rest_log_p);
-    factor = rest_p * whole - rest_q;
-  } else {
-    const double a = p.kind == TISO_DISTILL_REVERSE ? 0.0 : p.mix;
-    double f[kEach], mean = 0, cross = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const double prob = e[i] / s, log_p = z[i] - log_s;
-      const double log_m = a == 0 ? log_q[i] : log(a * q[i] + (1 - a) * prob);
-      e[i] = prob;
-      f[i] = (1 - a) * (log_p - log_m);
-      if (there[i]) {
-        mean += product(prob, f[i]);
-        cross += product(q[i], log_q[i] - log_m);
+    team.sync();
+    for (int k = team.tid; k < p.top; k += kThreads) {
+      if (space.lead[k] != k) continue;
+      double q = space.q[k];
+      bool more = false;
+      for (int j = k + 1; j < p.top; ++j)
+        if (space.lead[j] == k) {
+          q += space.q[j];
+          more = true;
+        }
+      if (more) {
+        space.q[k] = q;
+        space.log_q[k] = log(q);
       }
     }
-    const double log_m = a == 0 ? rest_log_q : log(a * rest_q + (1 - a) * rest_p);
-    const double rest_f = (1 - a) * (rest_log_p - log_m);
-    mean = sum_of_warp(mean) + product(rest_p, rest_f);
-    d = mean + a * (sum_of_warp(cross) + product(rest_q, rest_log_q - log_m));
-    if (a == 0) d = mean;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) e[i] = product(e[i], f[i] - mean);
-    factor = product(rest_p, rest_f - mean);
+    team.sync();
   }
-  const bool none = p.drop && listed_q == 0;  // nothing to compare with
-  const double unknown = *space.bad || s == 0 ? nan_of(0.0) : 0.0;
-  if (none) d = factor = 0;
-  d += unknown;
-  scale = rest.s == A(0) ? unknown : c * factor / static_cast<double>(rest.s) + unknown;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int k = lane + 32 * i;
-    if (there[i]) space.gradient[k] = static_cast<A>(none ? unknown : c * e[i] + unknown);
+  if (!has_entries) return;
+  const double base = base_of(most_of<kThreads>(space, p.top));
+  ListSums sums{};
+  for (int k = team.tid; k < p.top; k += kThreads) {
+    if (space.lead[k] != k) continue;
+    const double q = space.q[k], log_q = space.log_q[k];
+    const double z = (static_cast<double>(space.logit[k]) - base) * inv_temp, e = exp(z);
+    space.e[k] = e;
+    sums.q += q;
+    sums.q_log_q += product(q, log_q);
+    sums.q_z += product(q, z);
+    sums.e += e;
+    sums.e_far += product(e, z - log_q);
+    ++sums.tokens;
   }
-  if (lane == 0) {
-    *space.base = base_of(rest.m);
-    *space.scale = static_cast<A>(scale * p.upstream);
+  sums.q = sum_of_warp(sums.q);
+  sums.q_log_q = sum_of_warp(sums.q_log_q);
+  sums.q_z = sum_of_warp(sums.q_z);
+  sums.e = sum_of_warp(sums.e);
+  sums.e_far = sum_of_warp(sums.e_far);
+  sums.tokens = __reduce_add_sync(0xffffffffu, sums.tokens);
+  if (team.tid % 32 == 0) space.sums[team.tid / 32] = sums;
+}
+
+// The teacher's probabilities of the list and of the rest.
+struct Teacher {
+  double list_q, rest_q, whole;
+  __device__ __forceinline__ Teacher(double q, int tokens, int vocab, int kind, bool drop)
+      : list_q(q) {
+    rest_q = tokens == vocab ? 0.0 : fmax(1.0 - q, kind == TISO_DISTILL_REVERSE ? kLeastRest : 0.0);
+    if (drop) rest_q = 0.0;
+    if (q != q) rest_q = q;  // NaN
+    whole = drop ? (q > 0 ? 1.0 : 0.0) : q + rest_q;
   }
-  __syncwarp();
-  return d;
+};
+
+// The student's, from the parts' sums and maxima.
+template <typename A>
+struct Student {
+  double rest_z, list_z;  // the parts' maxima less the row's, over t
+  A s, rest_p, list_p;    // list_p: the probability of an e of 1
+
+  __device__ __forceinline__ Student(const Part<A>& rest, A most, double list_e, double inv_temp) {
+    const double base = base_of(max_acc(rest.m, most));
+    rest_z = (static_cast<double>(base_of(rest.m)) - base) * inv_temp;
+    list_z = (static_cast<double>(base_of(most)) - base) * inv_temp;
+    // a part that is empty, or hidden, has a sum of 0 and no maximum
+    const A of_rest = rest.s == A(0) ? A(0) : exp_as(A(0), rest_z) * rest.s;
+    const A of_list = list_e == 0 ? A(0) : exp_as(A(0), list_z);
+    s = of_rest + of_list * static_cast<A>(list_e);
+    rest_p = of_rest / s;
+    list_p = of_list / s;
+  }
+};
+
+// An entry's q, log q and log m (m the mixture of both), the q's renormalised where the rest is
+// dropped.
+template <typename A>
+__device__ __forceinline__ void entry_of(const DistillArgs<A>& p, const ListSpace<A>& space, int k,
+                                         const Settled& row, double prob, double& q, double& log_q,
+                                         double& log_m) {
+  q = space.q[k];
+  log_q = space.log_q[k];
+  if (p.drop && row.list_q > 0) {
+    q /= row.list_q;
+    log_q -= log(row.list_q);
+  }
+  log_m = p.kind == TISO_DISTILL_JENSEN ? log(p.mix * q + (1 - p.mix) * prob) : log_q;
+}
+
+// The steps after a row's sum, by a warp: the row's divergence, what the list's gradient is made of
+// into `settled`, and the rest's factor.
+template <int kThreads, typename A>
+__device__ __forceinline__ double settle(const DistillArgs<A>& p, const ListSpace<A>& space,
+                                         const Part<A>& rest, int vocab, double inv_temp,
+                                         double& factor) {
+  ListSums sums = space.sums[0];
+  for (int i = 1; i < warps_of<kThreads>(p.top); ++i) {
+    const ListSums& more = space.sums[i];
+    sums.q += more.q;
+    sums.q_log_q += more.q_log_q;
+    sums.q_z += more.q_z;
+    sums.e += more.e;
+    sums.e_far += more.e_far;
+    sums.tokens += more.tokens;
+  }
+  const Teacher teacher(sums.q, sums.tokens, vocab, p.kind, p.drop);
+  const A most = most_of<kThreads>(space, p.top);
+  const Student<A> student(rest, most, sums.e, inv_temp);
+  const double log_s = log(static_cast<double>(student.s));
+  const double rest_log_p = student.rest_z + log(static_cast<double>(rest.s)) - log_s;
+  const double rest_log_q = log(teacher.rest_q), rest_p = student.rest_p;
+  const double unknown = *space.bad || student.s == A(0) ? nan_of(0.0) : 0.0;
+  Settled row{space.settled->c + unknown, student.list_p, student.list_z - log_s, 0.0, sums.q,
+              teacher.whole};
+  double d;
+  if (p.drop && sums.q == 0) {  // nothing to compare with
+    d = factor = row.c = unknown;
+  } else if (p.kind == TISO_DISTILL_FORWARD) {
+    // p_v (f - sum P f) = p_v whole - q_v
+    const double each = p.drop ? 1 / sums.q : 1.0, shift = p.drop ? log(sums.q) : 0.0;
+    d = each * (sums.q_log_q - sums.q_z) - each * sums.q * (shift + row.log_p) +
+        product(teacher.rest_q, rest_log_q - rest_log_p);
+    factor = teacher.whole * rest_p - teacher.rest_q;
+  } else if (p.kind == TISO_DISTILL_REVERSE) {
+    const double rest_f = rest_log_p - rest_log_q;
+    d = row.mean = row.p * (sums.e_far + sums.e * row.log_p) + product(rest_p, rest_f);
+    factor = product(rest_p, rest_f - row.mean);
+  } else {
+    const double base = base_of(most);
+    double mean = 0, cross = 0;
+    for (int k = threadIdx.x & 31; k < p.top; k += 32) {
+      if (space.lead[k] != k) continue;
+      const double prob = space.e[k] * row.p;
+      const double log_p = (static_cast<double>(space.logit[k]) - base) * inv_temp + row.log_p;
+      double q, log_q, log_m;
+      entry_of(p, space, k, row, prob, q, log_q, log_m);
+      mean += product(prob, (1 - p.mix) * (log_p - log_m));
+      cross += product(q, log_q - log_m);
+    }
+    const double log_m = log(p.mix * teacher.rest_q + (1 - p.mix) * rest_p);
+    const double rest_f = (1 - p.mix) * (rest_log_p - log_m);
+    row.mean = sum_of_warp(mean) + product(rest_p, rest_f);
+    d = row.mean + p.mix * (sum_of_warp(cross) + product(teacher.rest_q, rest_log_q - log_m));
+    factor = product(rest_p, rest_f - row.mean);
+  }
+  factor = rest.s == A(0) ? unknown : row.c * factor / static_cast<double>(rest.s);
+  __syncwarp();  // every lane has read the share
+  if ((threadIdx.x & 31) == 0) *space.settled = row;
+  return d + unknown;
+}
+
+// The gradient of an entry's token.
+template <typename A>
+__device__ __forceinline__ A gradient_of(const DistillArgs<A>& p, const ListSpace<A>& space, int k,
+                                         const Settled& row, A most, double inv_temp) {
+  const double prob = space.e[k] * row.p;
+  double q, log_q, log_m;
+  if (p.kind == TISO_DISTILL_FORWARD) {
+    q = space.q[k];
+    if (p.drop && row.list_q > 0) q /= row.list_q;
+    return static_cast<A>(row.c * (prob * row.whole - q));
+  }
+  entry_of(p, space, k, row, prob, q, log_q, log_m);
+  const double z = (static_cast<double>(space.logit[k]) - static_cast<double>(base_of(most))) * inv_temp;
+  const double f = (p.kind == TISO_DISTILL_JENSEN ? 1 - p.mix : 1.0) * (z + row.log_p - log_m);
+  return static_cast<A>(row.c * product(prob, f - row.mean));
 }
 
 // The gradient of the rest: exp((x - base) / t) scale.
@@ -301,80 +437,77 @@ __device__ __forceinline__ void write_rest_of_tile(const RowView<T>& r, int tile
       store_once(to + i * kThreads, slope_vector<T>(load_vector(r, v + i * kThreads), slope));
 }
 
-// The list of row r into shared memory, and its bits. The threads have met when it returns.
+// The list's gradients, over what the pass wrote in their places. The threads have met since.
 template <int kThreads, typename T, typename A>
-__device__ __forceinline__ void read_list(const Rows& a, const DistillArgs<A>& p, int64_t r,
-                                          const RowView<T>& view, const Place<kThreads>& place,
-                                          int bit_words, const ListSpace<A>& space) {
+__device__ __forceinline__ void write_list(const Rows& a, const DistillArgs<A>& p, int64_t r,
+                                           const RowView<T>& view, const Place<kThreads>& place,
+                                           double inv_temp, bool with_grad,
+                                           const ListSpace<A>& space) {
   const Team<kThreads> team{place.tid};
-  for (int i = team.tid; i < bit_words; i += kThreads) space.bits[i] = 0;
-  if (team.tid == 0) *space.bad = *space.twice = static_cast<int>(*space.edge_bits = 0u);
-  team.sync();
-  for (int k = team.tid; k < p.top; k += kThreads) {
-    const int64_t id = p.ids[r * p.top + k];
-    const bool listed = id != a.ignore, in = id >= 0 && id < a.vocab;
-    if (listed && !in) *space.bad = 1;
-    const double log_q = listed && in ? static_cast<double>(p.logps[r * p.top + k])
-                                      : static_cast<double>(lowest<A>());
-    space.id[k] = space.lead[k] = -1;
-    space.log_q[k] = log_q;
-    space.q[k] = exp(log_q);
-    space.gradient[k] = A(0);
-    if (!listed || !in) continue;
-    space.id[k] = static_cast<int>(id);
-    space.lead[k] = k;
-    space.logit[k] = to_acc(view.x[id]);
-    const Spot<kThreads, T> spot(view, place.ctas, static_cast<int>(id));
-    if (spot.cta != place.cta) continue;
-    unsigned* word = spot.edge ? space.edge_bits : space.bits + spot.bit / 32;
-    if (atomicOr(word, 1u << spot.bit % 32) >> spot.bit % 32 & 1) *space.twice = 1;
-  }
-  team.sync();
-  // the same id again: its probabilities are added up in its first entry. (A CTA of a cluster sees
-  // only its own elements' bits, and looks through the list.)
-  if (place.ctas == 1 && !*space.twice) return;
-  for (int k = team.tid; k < p.top; k += kThreads) {
-    const int id = space.id[k];
-    if (id < 0) continue;
-    int first = k;
-    for (int j = k - 1; j >= 0; --j)
-      if (space.id[j] == id) first = j;
-    space.lead[k] = first;
-  }
-  team.sync();
+  const Settled row = *space.settled;
+  const A most = most_of<kThreads>(space, p.top);
   for (int k = team.tid; k < p.top; k += kThreads) {
     if (space.lead[k] != k) continue;
-    double q = space.q[k];
-    bool more = false;
-    for (int j = k + 1; j < p.top; ++j)
-      if (space.lead[j] == k) {
-        q += space.q[j];
-        more = true;
-      }
-    if (more) {
-      space.q[k] = q;
-      space.log_q[k] = log(q);
-    }
+    const A value = gradient_of(p, space, k, row, most, inv_temp);
+    space.gradient[k] = value;
+    const Spot<kThreads, T> spot(view, place.ctas, space.id[k]);
+    if (with_grad && spot.cta == place.cta)
+      view.g[space.id[k]] = from_acc<T>(static_cast<A>(value * p.upstream));
   }
+  if (!p.listed || place.cta != 0) return;
   team.sync();
+  for (int k = team.tid; k < p.top; k += kThreads)
+    p.listed[r * p.top + k] = space.lead[k] < 0 ? A(0) : space.gradient[space.lead[k]];
+}
+
+// A row's results but for the means' terms.
+template <typename A>
+__device__ __forceinline__ void write_row(const DistillArgs<A>& p, int64_t r, const Part<A>& rest,
+                                          double d, double factor) {
+  p.divergence[r] = static_cast<A>(d);
+  if (p.coef) {
+    p.coef[r] = factor;
+    p.stats[2 * r] = base_of(rest.m);
+    p.stats[2 * r + 1] = A(0);
+  }
+}
+
+template <typename A>
+__device__ __forceinline__ void write_left_out(const DistillArgs<A>& p, int64_t r) {
+  p.divergence[r] = A(0);
+  if (p.coef) p.stats[2 * r + 1] = A(kLeftOut);
+}
+
+// The row's share of the loss, into `settled`, by one thread while the row is read.
+template <typename A>
+__device__ __forceinline__ void read_share(const DistillArgs<A>& p, A w, double inv_temp,
+                                           const ListSpace<A>& space) {
+  cudaGridDependencySynchronize();  // the total's kernel is done
+  const double total = *p.total;
+  space.settled->c = total != 0 ? static_cast<double>(w) / total * inv_temp : 0.0;
+}
+
+template <typename T, typename A>
+__device__ __forceinline__ RowView<T> distill_view(const Rows& a, int64_t r, T* grad) {
+  T* g = grad + r * a.vocab;
+  return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
 }
 
 // Loss and gradient of a row by a CTA, or a cluster of them.
-template <typename T, typename A, int kThreads>
+template <int kThreads, typename T, typename A>
 __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>& p, double inv_temp,
                                             A k, T* grad, int bit_words, bool& last) {
   constexpr int kTile = kBatch * kThreads;
   extern __shared__ uint4 shared[];
+  __shared__ A slope_of[2];
   const Place<kThreads> place;
-  const Team<kThreads> team{place.tid};
   const int64_t r = place.row;
-  T* g = grad + r * a.vocab;
-  const RowView<T> view(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
+  const RowView<T> view = distill_view<T, A>(a, r, grad);
   const A w = p.weights.at(r);
   if (w == A(0)) {
     if (place.first()) {
-      p.divergence[r] = p.terms[r] = A(0);
-      if (p.coef) p.stats[2 * r + 1] = A(kLeftOut);
+      write_left_out(p, r);
+      p.terms[r] = A(0);
       cudaGridDependencySynchronize();
       last = last_unit(p.done, a.rows);
     }
@@ -385,53 +518,156 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
     return;
   }
   cluster_started(place.ctas);
-  const ListSpace<A> space(shared, p.top);
-  read_list(a, p, r, view, place, bit_words, space);
-  const Part<A> rest =
-      join_warps<kThreads>(join_lanes<32>(rest_part<kThreads>(view, place, space, k), k), k);
-  if (threadIdx.x < 32) {
-    cudaGridDependencySynchronize();
-    const double total = *p.total, c = total != 0 ? static_cast<double>(w) / total * inv_temp : 0.0;
-    double scale;
-    const double d = settle(p, space, rest, a.vocab, inv_temp, c, scale);
-    if (place.first()) {
-      p.divergence[r] = static_cast<A>(d);
-      p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
-      if (p.coef) {
-        p.coef[r] = scale;
-        p.stats[2 * r] = base_of(rest.m);
-        p.stats[2 * r + 1] = A(0);
+  const StagedTiles<kThreads, T> tiles(view, place, shared);
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) tiles.copy(j);
+  const ListSpace<A> space(shared + kStages * kTile, p.top);
+  read_list(a, p, r, view, place, bit_words, inv_temp, space);
+  if (place.tid == 0) read_share(p, w, inv_temp, space);
+
+  Part<A> rest{lowest<A>(), A(0)};
+  add_edge(rest, view, place, *space.edge_bits, k);
+  if (tiles.staged == 0)
+    for (int tile = place.cta * kTile, j = 0; tile < view.vectors; tile += place.ctas * kTile, ++j) {
+      uint4 q[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int v = tile + i * kThreads + place.tid;
+        q[i] = v < view.vectors ? load_vector(view, v) : no_vector<T>();
       }
+      add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, j, place.tid), k);
+    }
+  for (int j = 0; j < tiles.whole; ++j) {
+    uint4 q[kBatch];
+    tiles.fetch(j, q);
+    tiles.copy(j + kStages);
+    add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, j, place.tid), k);
+  }
+  if (tiles.cut) {
+    uint4 q[kBatch];
+    tiles.fetch_cut(q);
+    add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, tiles.whole, place.tid), k);
+    close_group();
+  }
+  rest = join_warps<kThreads>(join_lanes<32>(rest, k), k);
+  if (threadIdx.x < 32) {
+    double factor;
+    const double d = settle<kThreads>(p, space, rest, a.vocab, inv_temp, factor);
+    if (place.tid == 0) {
+      slope_of[0] = base_of(rest.m);
+      slope_of[1] = static_cast<A>(factor * p.upstream);
+    }
+    if (place.first()) {
+      write_row(p, r, rest, d, factor);
+      p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
       last = last_unit(p.done, a.rows);
     }
   }
   if (!grad && !p.listed) return;
-  team.sync();
-  if (p.listed && place.cta == 0)
-    for (int i = team.tid; i < p.top; i += kThreads)
-      p.listed[r * p.top + i] = space.lead[i] < 0 ? A(0) : space.gradient[space.lead[i]];
-  if (!grad) return;
-  const RestSlope<A> slope{*space.base, *space.scale, k};
-  if (place.edge() < view.edges) write_edge(view, place.edge(), slope);
-  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-    write_rest_of_tile<kThreads>(view, tile, place.tid, slope);
-  team.sync();  // the listed tokens' gradients over what the pass wrote there
-  for (int i = team.tid; i < p.top; i += kThreads) {
-    if (space.lead[i] < 0) continue;
-    const Spot<kThreads, T> spot(view, place.ctas, space.id[i]);
-    if (spot.cta == place.cta && space.lead[i] == i)
-      view.g[space.id[i]] = from_acc<T>(static_cast<A>(space.gradient[i] * p.upstream));
+  __syncthreads();
+  if (grad) {
+    const RestSlope<A> slope{slope_of[0], slope_of[1], k};
+    if (tiles.cut) {
+      uint4 q[kBatch];
+      tiles.fetch(tiles.whole, q);
+      tiles.copy(tiles.whole - kStages);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (tiles.has(i))
+          store_once(tiles.to(tiles.whole) + i * kThreads, slope_vector<T>(q[i], slope));
+    }
+    for (int j = tiles.whole - 1; j >= 0; --j) {
+      uint4 q[kBatch];
+      tiles.fetch(j, q);
+      tiles.copy(j - kStages);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        store_once(tiles.to(j) + i * kThreads, slope_vector<T>(q[i], slope));
+    }
+    write_edge(view, place.edge(), slope);
+    if (tiles.staged == 0)
+      for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+        write_rest_of_tile<kThreads>(view, tile, place.tid, slope);
+    __syncthreads();
   }
+  write_list(a, p, r, view, place, inv_temp, grad != nullptr, space);
 }
 
 template <typename T, typename A, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
     distill_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad, int bit_words) {
   __shared__ bool last;  // written by thread 0 alone
   if (threadIdx.x == 0) last = false;
-  distill_row<T, A, kThreads>(a, p, inv_temp, k, grad, bit_words, last);
+  distill_row<kThreads>(a, p, inv_temp, k, grad, bit_words, last);
   __syncthreads();
   if (last) write_means<1>(p.terms, *p.total, p.out, a.rows);
+}
+
+// Short rows: a warp to a row.
+template <typename T, typename A>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    distill_warp_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad, int bit_words) {
+  constexpr int kTile = kBatch * 32;
+  extern __shared__ uint4 shared[];
+  __shared__ A terms[kRowWarps];
+  __shared__ bool last;
+  const Place<32> place;
+  const int64_t r = place.row;
+  const int warp = threadIdx.x / 32;
+  const A w = r < a.rows ? p.weights.at(r) : A(0);
+  if (place.tid == 0) terms[warp] = A(0);
+  if (w != A(0)) {
+    const RowView<T> view = distill_view<T, A>(a, r, grad);
+    const ListSpace<A> space(
+        reinterpret_cast<char*>(shared) + warp * ListSpace<A>::bytes(p.top, 4 * bit_words), p.top);
+    read_list(a, p, r, view, place, bit_words, inv_temp, space);
+    if (place.tid == 0) read_share(p, w, inv_temp, space);
+    Part<A> rest{lowest<A>(), A(0)};
+    add_edge(rest, view, place, *space.edge_bits, k);
+    for (int tile = 0, j = 0; tile < view.vectors; tile += kTile, ++j) {
+      uint4 q[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int v = tile + i * 32 + place.tid;
+        q[i] = v < view.vectors ? load_vector(view, v) : no_vector<T>();
+      }
+      add_rest<T>(rest, q, bits_of_tile<32, T>(space.bits, j, place.tid), k);
+    }
+    rest = join_lanes<32>(rest, k);
+    __syncwarp();
+    double factor;
+    const double d = settle<32>(p, space, rest, a.vocab, inv_temp, factor);
+    if (place.tid == 0) {
+      write_row(p, r, rest, d, factor);
+      terms[warp] = static_cast<A>(static_cast<double>(w) * d);
+    }
+    if (grad) {
+      const RestSlope<A> slope{base_of(rest.m), static_cast<A>(factor * p.upstream), k};
+      write_edge(view, place.edge(), slope);
+      for (int tile = 0; tile < view.vectors; tile += kTile)
+        write_rest_of_tile<32>(view, tile, place.tid, slope);
+    }
+    __syncwarp();
+    if (grad || p.listed) write_list(a, p, r, view, place, inv_temp, grad != nullptr, space);
+  } else if (r < a.rows) {
+    if (place.tid == 0) write_left_out(p, r);
+    if (grad) {
+      const RowView<T> view = distill_view<T, A>(a, r, grad);
+      zero_edge(view, place.edge());
+      for (int tile = 0; tile < view.vectors; tile += kTile) zero_tile<32>(view, tile, place.tid);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    A sum = A(0);
+#pragma unroll
+    for (int i = 0; i < kRowWarps; ++i) sum += terms[i];
+    p.terms[blockIdx.x] = sum;
+    cudaGridDependencySynchronize();
+    last = last_unit(p.done, gridDim.x);
+  }
+  __syncthreads();
+  if (last) write_means<1>(p.terms, *p.total, p.out, gridDim.x);
 }
 
 // The gradient for another upstream gradient than the expected one, from what the loss left; nothing
@@ -474,12 +710,60 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------------------------
 // Host side
 
+// Bits of the vectors of a CTA's share of `vectors`, in bytes.
+template <typename T>
+int64_t bit_bytes(int64_t vectors, int threads, int ctas) {
+  const int64_t tile = int64_t{kBatch} * threads, tiles = (vectors + tile - 1) / tile;
+  return (tiles + ctas - 1) / ctas * tile * RowView<T>::E / 8;
+}
+
+template <typename T, int kThreads>
+int launch_distill_rows(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p,
+                        double inv_temp, T* grad, int sms, cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  constexpr int64_t kStaged = int64_t{kStages} * kBatch * kThreads * 16;
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  int ctas = ctas_for(a.rows, vectors, kThreads, sms);
+  while (ctas < 8 && int64_t{sms} * (kSmThreads / kThreads) * vectors * 16 / ctas > kRowsInL2)
+    ctas *= 2;
+  while (ctas < 8 && bit_bytes<T>(vectors, kThreads, ctas) > kSharedForBits) ctas *= 2;
+  const int64_t bits = bit_bytes<T>(vectors, kThreads, ctas);
+  if (bits > kSharedForBits)
+    return report_error(TISO_ERR_ARGUMENT, "a vocabulary too large for the distillation loss");
+  const size_t shared = kStaged + ListSpace<A>::bytes(p.top, static_cast<int>(bits));
+  const auto kernel = distill_kernel<T, A, kThreads>;
+  const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
+                              kStaged + ListSpace<A>::bytes(kMostListed, kSharedForBits));
+  if (rc) return rc;
+  return launch_clusters(kernel, a.rows, ctas, kThreads, shared, true, st, "distill_kernel launch", a,
+                         p, inv_temp, exp_factor(A(0), inv_temp), grad, static_cast<int>(bits / 4));
+}
+
+template <typename T>
+int launch_distill(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p, double inv_temp,
+                   T* grad, cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  const int sms = sm_count();
+  if (by_warps(a.rows, vectors, 1536, sms)) {
+    const int bits = static_cast<int>(bit_bytes<T>(vectors, 32, 1));
+    const size_t shared = size_t{kRowWarps} * ListSpace<A>::bytes(p.top, bits);
+    const auto kernel = distill_warp_kernel<T, A>;
+    const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
+                                size_t{kRowWarps} * ListSpace<A>::bytes(kMostListed, 1536 * 16 / 8));
+    if (rc) return rc;
+    return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps, shared,
+                           true, st, "distill_warp_kernel launch", a, p, inv_temp,
+                           exp_factor(A(0), inv_temp), grad, bits / 4);
+  }
+  return launch_distill_rows<T, 256>(a, p, inv_temp, grad, sms, st);
+}
+
 template <typename T>
 int run_distill(const Rows& a, const tiso_distill_args* q, double inv_temp, void* divergence,
                 double* coef, void* stats, void* listed, void* out, void* grad, void* workspace,
                 cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  constexpr int kThreads = 256, kTile = kBatch * kThreads, E = RowView<T>::E;
   DistillArgs<A> p{};
   p.weights = weights_of<A>(q->ids, q->top, a.ignore, q->weight, q->weight_is_byte);
   p.ids = q->ids;
@@ -499,19 +783,7 @@ int run_distill(const Rows& a, const tiso_distill_args* q, double inv_temp, void
   p.terms = reinterpret_cast<A*>(p.total + 2);
   int rc = launch_total(p.weights, a.rows, p.total, p.done, p.out, 1, st);
   if (rc || a.rows == 0) return rc;
-  const int64_t vectors = a.vocab / E, tiles = (vectors + kTile - 1) / kTile;
-  int ctas = ctas_for(a.rows, vectors, kThreads, sm_count());
-  const auto bits = [&] { return static_cast<size_t>((tiles + ctas - 1) / ctas) * kTile * E / 8; };
-  while (ctas < 8 && ListSpace<A>::bytes(p.top, bits()) > kSharedForBits) ctas *= 2;
-  const size_t shared = ListSpace<A>::bytes(p.top, bits());
-  if (shared > kSharedForBits)
-    return report_error(TISO_ERR_ARGUMENT, "a vocabulary too large for the distillation loss");
-  const auto kernel = distill_kernel<T, A, kThreads>;
-  rc = allow_shared(reinterpret_cast<const void*>(kernel), kSharedForBits);
-  if (rc) return rc;
-  return launch_clusters(kernel, a.rows, ctas, kThreads, shared, true, st, "distill_kernel launch", a,
-                         p, inv_temp, exp_factor(A(0), inv_temp), static_cast<T*>(grad),
-                         static_cast<int>(bits() / 4));
+  return launch_distill<T>(a, p, inv_temp, static_cast<T*>(grad), st);
 }
 
 template <typename T>

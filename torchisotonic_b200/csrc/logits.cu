@@ -146,16 +146,6 @@ struct TokenInput {
   }
 };
 
-// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest;
-// for |d| < kFar).
-__device__ __forceinline__ float exp_as(float, double d) {
-  const float hi = static_cast<float>(d);
-  const float lo = static_cast<double>(hi) == d ? 0.0f : static_cast<float>(d - hi);
-  const float e = expf(hi);
-  return __fmaf_rn(e, lo, e);
-}
-__device__ __forceinline__ double exp_as(double, double d) { return exp(d); }
-
 // exp(d) / s and exp(d) s, s a row's sum (up to 2^30). Beyond e^+-60 float has no room for them, nor
 // for exp(d) on the way: a token that the old policy all but excluded has a ratio of any size, which
 // the clip then cuts.
@@ -321,7 +311,6 @@ __global__ void __launch_bounds__(32 * kRowWarps)
 // A last tile that is cut goes this way too: loaded directly it is waited for twice (32000 to the
 // row: 306 us for 800 MB of bf16 logits, 320 with it loaded). The tiles of a row that is read and
 // written at different alignments are loaded directly, from two vectors each.
-constexpr int kStages = 2;
 constexpr int kSmThreads = 1536;  // resident at 40 registers a thread (spills: double 96 bytes, 16-bit types 8)
 
 template <int kThreads, typename T, typename A>
@@ -348,59 +337,25 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
     return;
   }
   cluster_started(place.ctas);
-  // this CTA's tiles that go through shared memory: its j-th is tile cta + j ctas; the row's last
-  // tile may be cut
-  const int staged = view.shift == 0 ? view.vectors : 0;
-  const int tiles = (staged + kTile - 1) / kTile;
-  const int mine = tiles > place.cta ? (tiles - place.cta + place.ctas - 1) / place.ctas : 0;
-  const bool cut = staged % kTile != 0 && (tiles - 1) % place.ctas == place.cta;
-  const int whole = mine - cut;
-  const int stride = place.ctas * kTile;
-  const int own = place.cta * kTile + place.tid;
-  const uint4* from = reinterpret_cast<const uint4*>(view.x + view.head) + own;
-  uint4* to = reinterpret_cast<uint4*>(view.g + view.head) + own;
-  const auto has = [&](int i) { return own + whole * stride + i * kThreads < staged; };  // if cut
-  const auto copy = [&](int j) {
-    uint4* at = stages + static_cast<unsigned>(j) % kStages * kTile + place.tid;
-    if (j >= 0 && j < whole) {
+  const StagedTiles<kThreads, T> tiles(view, place, stages);
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
-    } else if (cut && j == whole) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (has(i))
-          copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
-    }
-    close_group();
-  };
-  const auto fetch = [&](int j, uint4 (&q)[kBatch]) {
-    wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      q[i] = stages[static_cast<unsigned>(j) % kStages * kTile + i * kThreads + place.tid];
-  };
-#pragma unroll
-  for (int j = 0; j < kStages; ++j) copy(j);
+  for (int j = 0; j < kStages; ++j) tiles.copy(j);
   if (place.tid == 0) {
     token.w = w;
     token.read(a, p, r, target_logit<T, A>(view.x, a.vocab, a.targets[r]));
   }
 
   // the tiles that are loaded directly, and the single elements
-  Part<A> part = thread_part(view, place, staged ? staged : place.cta * kTile, k);
-  for (int j = 0; j < whole; ++j) {
+  Part<A> part = thread_part(view, place, tiles.staged ? tiles.staged : place.cta * kTile, k);
+  for (int j = 0; j < tiles.whole; ++j) {
     uint4 q[kBatch];
-    fetch(j, q);
-    copy(j + kStages);
+    tiles.fetch(j, q);
+    tiles.copy(j + kStages);
     add_vectors<T>(part, q, k);
   }
-  if (cut) {
+  if (tiles.cut) {
     uint4 q[kBatch];
-    fetch(whole, q);
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      if (!has(i)) q[i] = no_vector<T>();
+    tiles.fetch_cut(q);
     add_vectors<T>(part, q, k);
     close_group();
   }
@@ -416,32 +371,29 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   if (!grad) return;
   const Slope<A> slope(base_of(part.m), part.s, result.coef * inv_temp, k, token.target, a.vocab);
   const auto write_target = [&](int j) {
-    write_target_of_tile<kThreads, kTile>(view, own - place.tid + j * stride, place.tid, slope);
+    write_target_of_tile<kThreads, kTile>(view, tiles.tile(j), place.tid, slope);
   };
-  if (cut) {
+  if (tiles.cut) {
     uint4 q[kBatch];
-    fetch(whole, q);
-    copy(whole - kStages);
+    tiles.fetch(tiles.whole, q);
+    tiles.copy(tiles.whole - kStages);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      if (has(i))
-        store_once(to + static_cast<int64_t>(whole) * stride + i * kThreads,
-                   slope_vector<T>(q[i], slope));
-    write_target(whole);
+      if (tiles.has(i)) store_once(tiles.to(tiles.whole) + i * kThreads, slope_vector<T>(q[i], slope));
+    write_target(tiles.whole);
   }
-  for (int j = whole - 1; j >= 0; --j) {
+  for (int j = tiles.whole - 1; j >= 0; --j) {
     uint4 q[kBatch];
-    fetch(j, q);
-    copy(j - kStages);
+    tiles.fetch(j, q);
+    tiles.copy(j - kStages);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
-      store_once(to + static_cast<int64_t>(j) * stride + i * kThreads,
-                 slope_vector<T>(q[i], slope));
+      store_once(tiles.to(j) + i * kThreads, slope_vector<T>(q[i], slope));
     write_target(j);
   }
   write_edge(view, place.edge(), slope);
-  if (staged == 0)
-    for (int tile = place.cta * kTile; tile < view.vectors; tile += stride)
+  if (tiles.staged == 0)
+    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
       write_tile<kThreads>(view, tile, place.tid, slope);
 }
 
@@ -457,11 +409,6 @@ __global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
 
 // ---------------------------------------------------------------------------------------------
 // Host side
-
-// Bytes of rows in work at once that L2 is to hold from a row's first read to its
-// second. Rows of 256 KB: one CTA to a row (116 MB) reads 1.8 GB where two (58 MB) read 1.06 and
-// four 0.95 (0.94 is each byte once); two are fastest (828, 874 and 931 us with 2, 1 and 4).
-constexpr int64_t kRowsInL2 = 80 << 20;
 
 template <typename T>
 int run_logprobs(const Rows& a, double inv_temp, void* logps, void* stats, cudaStream_t st) {

@@ -258,6 +258,70 @@ __device__ __forceinline__ void zero_edge(const RowView<T>& r, int edge) {
   if (edge < r.edges) r.g[r.edge(edge)] = from_acc<T>(typename AccOf<T>::type(0));
 }
 
+// A CTA's tiles of a row that is read twice, for its sum and then in the reverse order: through kStages
+// places of shared memory, each thread copying and reading its own vectors there (no barrier). The
+// row's last tile may be cut. A row that is read and written at different alignments has none.
+constexpr int kStages = 2;
+
+template <int kThreads, typename T>
+struct StagedTiles {
+  static constexpr int kTile = kBatch * kThreads;
+  uint4* stages;  // [kStages][kTile]
+  const uint4* from;
+  uint4* first;
+  int staged, whole, stride, own, tid;
+  bool cut;
+
+  // this CTA's j-th tile is tile cta + j ctas
+  __device__ __forceinline__ StagedTiles(const RowView<T>& view, const Place<kThreads>& place,
+                                         uint4* stages_)
+      : stages(stages_), tid(place.tid) {
+    staged = view.shift == 0 ? view.vectors : 0;
+    const int tiles = (staged + kTile - 1) / kTile;
+    const int mine = tiles > place.cta ? (tiles - place.cta + place.ctas - 1) / place.ctas : 0;
+    cut = staged % kTile != 0 && (tiles - 1) % place.ctas == place.cta;
+    whole = mine - cut;
+    stride = place.ctas * kTile;
+    own = place.cta * kTile + place.tid;
+    from = reinterpret_cast<const uint4*>(view.x + view.head) + own;
+    first = reinterpret_cast<uint4*>(view.g + view.head) + own;
+  }
+  __device__ __forceinline__ int tile(int j) const { return own - tid + j * stride; }
+  __device__ __forceinline__ uint4* to(int j) const {
+    return first + static_cast<int64_t>(j) * stride;
+  }
+  // whether this thread has an i-th vector in the cut tile
+  __device__ __forceinline__ bool has(int i) const {
+    return own + whole * stride + i * kThreads < staged;
+  }
+  __device__ __forceinline__ void copy(int j) const {
+    uint4* at = stages + static_cast<unsigned>(j) % kStages * kTile + tid;
+    if (j >= 0 && j < whole) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
+    } else if (cut && j == whole) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (has(i))
+          copy_async(at + i * kThreads, from + static_cast<int64_t>(j) * stride + i * kThreads);
+    }
+    close_group();
+  }
+  __device__ __forceinline__ void fetch(int j, uint4 (&q)[kBatch]) const {
+    wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      q[i] = stages[static_cast<unsigned>(j) % kStages * kTile + i * kThreads + tid];
+  }
+  __device__ __forceinline__ void fetch_cut(uint4 (&q)[kBatch]) const {
+    fetch(whole, q);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (!has(i)) q[i] = no_vector<T>();
+  }
+};
+
 // A row that is left out (its target is the ignored index, or its weight is 0) is marked by a
 // negative sum in stats: its gradient is zeros and its logits are not read.
 constexpr int kLeftOut = -1;
@@ -481,6 +545,11 @@ constexpr int kWarpVectors = 256;
 inline bool by_warps(int64_t rows, int64_t vectors, int64_t most, int sms) {
   return vectors <= kWarpVectors || (vectors <= most && rows >= int64_t{16} * sms);
 }
+
+// Bytes of rows in work at once that L2 is to hold from a row's first read to its
+// second. Rows of 256 KB: one CTA to a row (116 MB) reads 1.8 GB where two (58 MB) read 1.06 and
+// four 0.95 (0.94 is each byte once); two are fastest (828, 874 and 931 us with 2, 1 and 4).
+constexpr int64_t kRowsInL2 = 80 << 20;
 
 // CTAs of `threads` to a row: doubled while rows are too few to fill the GPU and a CTA would have
 // more than a batch for each thread.
