@@ -21,8 +21,7 @@ namespace tiso {
 namespace {
 
 constexpr int kMostListed = 128;
-constexpr int kSmThreads = 1536;  // resident at 40 registers a thread
-constexpr int kSharedForBits = 160 * 1024;
+constexpr int kSmThreads = 1280;  // resident at 48 registers a thread
 // the teacher's rest where it is divided by: a list's float log-probabilities say no less
 constexpr double kLeastRest = 1.0 / (1 << 24);
 
@@ -44,137 +43,6 @@ struct DistillArgs {
   unsigned* done;
 };
 
-// Sums over the list's tokens: of q, q log q, q z, e = exp(z) and e (z - log q), z the logits from the
-// list's own maximum, over t; and how many tokens there are.
-struct ListSums {
-  double q, q_log_q, q_z, e, e_far;
-  int tokens;
-};
-
-// What the gradient of the list is made of, once the row's sum is known.
-struct Settled {
-  double c;      // the row's share of the loss, over t
-  double p;      // of an e: its probability
-  double log_p;  // of a z: its logarithm
-  double mean;   // sum P f
-  double list_q, whole;
-};
-
-constexpr int kListWarps = kMostListed / 32;
-
-// Shared memory of the threads that work on a row.
-template <typename A>
-struct ListSpace {
-  double *q, *log_q, *e;  // the teacher's probabilities; exp(z)
-  ListSums* sums;         // of each warp that has entries
-  Settled* settled;
-  A *logit, *gradient;
-  A* most;                // of each of these warps, the largest logit
-  int *id, *lead;         // -1: no entry; the first entry of its id
-  int *bad, *twice;       // an id out of range; an id listed again
-  unsigned* edge_bits;    // of the single elements
-  unsigned* bits;         // of this CTA's share of the vectors: a bit an element
-
-  static __host__ __device__ int entries(int top) { return (top + 3) / 4 * 4; }
-  static __host__ __device__ int bytes(int top, int bits) {
-    return entries(top) * static_cast<int>(3 * sizeof(double) + 2 * sizeof(A) + 2 * sizeof(int)) +
-           static_cast<int>(kListWarps * sizeof(ListSums) + sizeof(Settled) + kListWarps * sizeof(A)) +
-           16 + (bits + 15) / 16 * 16;
-  }
-
-  __device__ ListSpace(void* at, int top) {
-    const int n = entries(top);
-    q = static_cast<double*>(at);
-    log_q = q + n;
-    e = log_q + n;
-    sums = reinterpret_cast<ListSums*>(e + n);
-    settled = reinterpret_cast<Settled*>(sums + kListWarps);
-    logit = reinterpret_cast<A*>(settled + 1);
-    gradient = logit + n;
-    most = gradient + n;
-    id = reinterpret_cast<int*>(most + kListWarps);
-    lead = id + n;
-    bad = lead + n;
-    twice = bad + 1;
-    edge_bits = reinterpret_cast<unsigned*>(bad + 2);
-    bits = edge_bits + 2;
-  }
-};
-
-// Where an element lies among those of the threads that work on a row.
-template <int kThreads, typename T>
-struct Spot {
-  int cta, bit;  // of the bits of that CTA, or with `edge` of the edges'
-  bool edge;
-
-  __device__ __forceinline__ Spot(const RowView<T>& r, int ctas, int element) {
-    constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
-    edge = element < r.head || element >= r.head + r.vectors * E;
-    if (edge) {
-      cta = 0;
-      bit = element < r.head ? element : element - r.vectors * E;
-    } else {
-      const int v = (element - r.head) / E, tile = v / kTile, in = v % kTile;
-      cta = tile % ctas;
-      bit = ((tile / ctas * kThreads + in % kThreads) * kBatch + in / kThreads) * E +
-            (element - r.head) % E;
-    }
-  }
-};
-
-// The bits of the vectors that a thread takes of its CTA's tile `local`.
-template <int kThreads, typename T>
-__device__ __forceinline__ unsigned bits_of_tile(const unsigned* bits, int local, int tid) {
-  const int at = local * kThreads + tid;
-  if constexpr (RowView<T>::E == 8) return bits[at];
-  if constexpr (RowView<T>::E == 4) return reinterpret_cast<const uint16_t*>(bits)[at];
-  return reinterpret_cast<const uint8_t*>(bits)[at];
-}
-
-// -infinity for the elements whose bits are set.
-template <typename T>
-__device__ __forceinline__ void hide(uint4& q, unsigned bits) {
-  const uint4 none = no_vector<T>();
-  uint32_t* w = reinterpret_cast<uint32_t*>(&q);
-  const uint32_t* n = reinterpret_cast<const uint32_t*>(&none);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t gone = (bits >> 2 * i & 1 ? 0xffffu : 0u) | (bits >> 2 * i & 2 ? 0xffff0000u : 0u);
-      w[i] = (w[i] & ~gone) | (n[i] & gone);
-    } else if constexpr (sizeof(T) == 4) {
-      if (bits >> i & 1) w[i] = n[i];
-    } else {
-      if (bits >> (i / 2) & 1) w[i] = n[i];
-    }
-  }
-}
-
-// Adds a tile's vectors but for the listed tokens.
-template <typename T, typename A>
-__device__ __forceinline__ void add_rest(Part<A>& p, uint4 (&q)[kBatch], unsigned bits, A k) {
-  constexpr int E = RowView<T>::E;
-  if (bits) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const unsigned own = bits >> i * E & ((1u << E) - 1);
-      if (own) hide<T>(q[i], own);
-    }
-  }
-  add_vectors<T>(p, q, k);
-}
-
-// Adds one of the single elements, unless it is listed.
-template <typename T, int kThreads, typename A>
-__device__ __forceinline__ void add_edge(Part<A>& p, const RowView<T>& r, const Place<kThreads>& place,
-                                         unsigned edge_bits, A k) {
-  const int e = place.edge();
-  const A edge = e < r.edges && !(edge_bits >> e & 1) ? to_acc(r.x[r.edge(e)]) : lowest<A>();
-  const A m = max_acc(p.m, edge), base = base_of(m);
-  p.s = (p.m == m ? p.s : p.s * scaled_exp(p.m - base, k)) + scaled_exp(edge - base, k);
-  p.m = m;
-}
-
 __device__ __forceinline__ double sum_of_warp(double v) {
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -183,113 +51,238 @@ __device__ __forceinline__ double sum_of_warp(double v) {
 
 __device__ __forceinline__ double product(double x, double y) { return x == 0 ? 0.0 : x * y; }
 
-// Warps with entries of a list, and the largest of its logits.
+// Sums over the list's tokens (of a warp's entries, then of all): of q and of e = exp(z), z the logits
+// from the largest of them, over t; `far` of q (log q - z), in the reverse divergence of e (z - log q).
+template <typename A>
+struct ListSums {
+  double q, far;
+  A e, most;
+  int tokens;
+
+  // the same with z from another logit than the largest
+  __device__ __forceinline__ void move(A to, double inv_temp, A k, int kind) {
+    if (tokens == 0 || most == to) return;
+    const A d = base_of(most) - base_of(to), f = e == A(0) ? A(0) : scaled_exp(d, k);
+    const double z = static_cast<double>(d) * inv_temp;
+    if (kind == TISO_DISTILL_REVERSE) {
+      far = f == A(0) ? 0.0 : static_cast<double>(f) * (far + z * static_cast<double>(e));
+    } else if (q != 0) {
+      far -= q * z;
+    }
+    e *= f;
+  }
+};
+
+// What the gradients are made of, once the row's sum is known.
+struct Settled {
+  double c;         // the row's share of the loss, over t
+  double each;      // what the teacher's probabilities are multiplied with
+  double log_each;  // its logarithm
+  double whole;     // their sum with the rest's
+  double p;         // of an exp(z), z from the largest logit of the list: its probability
+  double log_p;     // of a z: its logarithm
+  double mean;      // sum P f
+  double factor;    // of the rest's gradient
+};
+
+constexpr int kListWarps = kMostListed / 32;
+
+// Shared memory of the kThreads threads that work on a row. An entry is handed to the thread that
+// reads and writes its token's element (its owner): each thread has a chain of its entries.
+template <typename A, int kThreads>
+struct ListSpace {
+  double *q, *log_q;     // the teacher's probabilities
+  double* share;         // the row's share of the loss, over t
+  ListSums<A>* sums;     // of each warp that has entries
+  Settled* settled;
+  A *logit, *gradient;
+  int *id, *lead;        // -1: no entry; the first entry of its id
+  int *next, *place;     // in its owner's chain; where among the owner's elements
+  int* head;             // of each thread's chain
+  int* bad;              // an id out of range
+
+  static __host__ __device__ constexpr int entries(int top) { return (top + 3) / 4 * 4; }
+  static __host__ __device__ constexpr int bytes(int top) {
+    return entries(top) * static_cast<int>(2 * sizeof(double) + 2 * sizeof(A) + 4 * sizeof(int)) +
+           static_cast<int>(kListWarps * sizeof(ListSums<A>) + sizeof(Settled)) + 16 +
+           kThreads * 4 + 16;
+  }
+
+  __device__ ListSpace(void* at, int top) {
+    const int n = entries(top);
+    q = static_cast<double*>(at);
+    log_q = q + n;
+    share = log_q + n;
+    sums = reinterpret_cast<ListSums<A>*>(share + 2);
+    settled = reinterpret_cast<Settled*>(sums + kListWarps);
+    logit = reinterpret_cast<A*>(settled + 1);
+    gradient = logit + n;
+    id = reinterpret_cast<int*>(gradient + n);
+    lead = id + n;
+    next = lead + n;
+    place = next + n;
+    head = place + n;
+    bad = head + kThreads;
+  }
+};
+
+// An element's owner: of a CTA's tiles (every ctas-th) the thread that has its vector, of the single
+// elements the thread of their number in the first CTA. place: its number among the owner's elements.
+constexpr int kNoPlace = -1, kEdgePlace = -2;
+
+template <int kThreads, typename T>
+__device__ __forceinline__ int owner_of(const RowView<T>& r, const Place<kThreads>& place, int element,
+                                        int& number) {
+  constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
+  if (element < r.head || element >= r.head + r.vectors * E) {
+    number = place.cta == 0 ? kEdgePlace : kNoPlace;
+    return element < r.head ? element : element - r.vectors * E;
+  }
+  const int v = (element - r.head) / E, tile = v / kTile, in = v % kTile;
+  const int local = tile / place.ctas;
+  number = tile - local * place.ctas == place.cta
+               ? (local * kBatch + in / kThreads) * E + (element - r.head) % E
+               : kNoPlace;
+  return in % kThreads;
+}
+
+// A thread's listed elements: in which tiles (bit j mod 32), and whether its single element is one.
+struct Own {
+  unsigned tiles;
+  bool edge;
+};
+
+// Calls fn(k, place) for the entries of a thread that this CTA has.
+template <int kThreads, typename A, typename F>
+__device__ __forceinline__ void for_own(const ListSpace<A, kThreads>& space, int tid, const F& fn) {
+  for (int k = space.head[tid]; k >= 0; k = space.next[k])
+    if (space.place[k] != kNoPlace) fn(k, space.place[k]);
+}
+
+// Row r's list is handed out. The threads have met when it returns.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ Own hand_out(const Rows& a, const DistillArgs<A>& p, int64_t r,
+                                        const RowView<T>& view, const Place<kThreads>& place,
+                                        const ListSpace<A, kThreads>& space) {
+  constexpr int kOfTile = kBatch * RowView<T>::E;
+  const Team<kThreads> team{place.tid};
+  space.head[team.tid] = -1;
+  if (team.tid == 0) *space.bad = 0;
+  for (int k = team.tid; k < p.top; k += kThreads) {
+    const int64_t id = p.ids[r * p.top + k];
+    space.id[k] = id == a.ignore ? -1 : id >= 0 && id < a.vocab ? static_cast<int>(id) : -2;
+  }
+  team.sync();
+  for (int k = team.tid; k < p.top; k += kThreads) {
+    const int id = space.id[k];
+    if (id == -2) *space.bad = 1;
+    if (id < 0) continue;
+    int number;
+    const int owner = owner_of<kThreads>(view, place, id, number);
+    space.place[k] = number;
+    space.next[k] = atomicExch(space.head + owner, k);
+  }
+  team.sync();
+  Own own{0, false};
+  for_own(space, team.tid, [&](int, int number) {
+    if (number == kEdgePlace) {
+      own.edge = true;
+    } else {
+      own.tiles |= 1u << number / kOfTile % 32;
+    }
+  });
+  return own;
+}
+
+// Warps with entries of a list.
 template <int kThreads>
 __device__ __forceinline__ int warps_of(int top) {
   return min((top + 31) / 32, kThreads / 32);
 }
-template <int kThreads, typename A>
-__device__ __forceinline__ A most_of(const ListSpace<A>& space, int top) {
-  A most = space.most[0];
-  for (int i = 1; i < warps_of<kThreads>(top); ++i) most = max_acc(most, space.most[i]);
-  return most;
-}
 
-// The list of row r into shared memory, its bits, and its sums (after the next meeting of the
-// threads).
+// The list's numbers and their sums, by each warp for its own entries (the others' are known after
+// the threads' next meeting). A token that is listed again counts in its first entry.
 template <int kThreads, typename T, typename A>
-__device__ __forceinline__ void read_list(const Rows& a, const DistillArgs<A>& p, int64_t r,
-                                          const RowView<T>& view, const Place<kThreads>& place,
-                                          int bit_words, double inv_temp, const ListSpace<A>& space) {
-  const Team<kThreads> team{place.tid};
-  for (int i = team.tid; i < bit_words; i += kThreads) space.bits[i] = 0;
-  if (team.tid == 0) *space.bad = *space.twice = static_cast<int>(*space.edge_bits = 0u);
-  team.sync();
-  const bool has_entries = team.tid / 32 * 32 < p.top;  // this warp
+__device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, const RowView<T>& view,
+                                          const Place<kThreads>& place, double inv_temp, A k,
+                                          const ListSpace<A, kThreads>& space) {
+  if (place.tid / 32 * 32 >= p.top) return;
   A most = lowest<A>();
-  for (int k = team.tid; k < p.top; k += kThreads) {
-    const int64_t id = p.ids[r * p.top + k];
-    const bool listed = id != a.ignore, in = id >= 0 && id < a.vocab;
-    if (listed && !in) *space.bad = 1;
-    space.id[k] = space.lead[k] = -1;
-    space.gradient[k] = A(0);
-    if (!listed || !in) continue;
-    const double log_q = static_cast<double>(p.logps[r * p.top + k]);
-    const A logit = to_acc(view.x[id]);
-    const Spot<kThreads, T> spot(view, place.ctas, static_cast<int>(id));
-    if (spot.cta == place.cta) {
-      unsigned* word = spot.edge ? space.edge_bits : space.bits + spot.bit / 32;
-      if (atomicOr(word, 1u << spot.bit % 32) >> spot.bit % 32 & 1) *space.twice = 1;
-    }
-    space.id[k] = static_cast<int>(id);
-    space.lead[k] = k;
-    space.logit[k] = logit;
-    space.log_q[k] = log_q;
-    space.q[k] = exp(log_q);
-    most = max_acc(most, logit);
-  }
-  if (has_entries) {
-    most = max_of_lanes<32>(most);
-    if (team.tid % 32 == 0) space.most[team.tid / 32] = most;
-  }
-  team.sync();
-  if (place.ctas > 1 || *space.twice) {
-    // the same id again: its probabilities are added up in its first entry. (A CTA of a cluster sees
-    // only its own elements' bits, and looks through the list.)
-    for (int k = team.tid; k < p.top; k += kThreads) {
-      const int id = space.id[k];
-      if (id < 0) continue;
-      int first = k;
-      for (int j = k - 1; j >= 0; --j)
-        if (space.id[j] == id) first = j;
-      space.lead[k] = first;
-    }
-    team.sync();
-    for (int k = team.tid; k < p.top; k += kThreads) {
-      if (space.lead[k] != k) continue;
-      double q = space.q[k];
+  for (int i = place.tid; i < p.top; i += kThreads) {
+    const int id = space.id[i];
+    int lead = -1;
+    if (id >= 0) {
+      const A logit = to_acc(view.x[id]);
+      double log_q = static_cast<double>(p.logps[r * p.top + i]), q = exp(log_q);
+      lead = i;
       bool more = false;
-      for (int j = k + 1; j < p.top; ++j)
-        if (space.lead[j] == k) {
-          q += space.q[j];
+      for (int j = 0; j < p.top; ++j) {
+        if (space.id[j] != id || j == i) continue;
+        if (j < i) {
+          lead = min(lead, j);
+        } else {
+          q += exp(static_cast<double>(p.logps[r * p.top + j]));
           more = true;
         }
-      if (more) {
-        space.q[k] = q;
-        space.log_q[k] = log(q);
       }
+      if (more) log_q = log(q);
+      space.logit[i] = logit;
+      space.log_q[i] = log_q;
+      space.q[i] = q;
+      most = max_acc(most, logit);
     }
-    team.sync();
+    space.lead[i] = lead;
   }
-  if (!has_entries) return;
-  const double base = base_of(most_of<kThreads>(space, p.top));
-  ListSums sums{};
-  for (int k = team.tid; k < p.top; k += kThreads) {
-    if (space.lead[k] != k) continue;
-    const double q = space.q[k], log_q = space.log_q[k];
-    const double z = (static_cast<double>(space.logit[k]) - base) * inv_temp, e = exp(z);
-    space.e[k] = e;
+  most = max_of_lanes<32>(most);
+  ListSums<A> sums{};
+  for (int i = place.tid; i < p.top; i += kThreads) {
+    if (space.lead[i] != i) continue;
+    const double q = space.q[i], log_q = space.log_q[i];
+    const A d = space.logit[i] - base_of(most), e = scaled_exp(d, k);
+    const double z = static_cast<double>(d) * inv_temp;
     sums.q += q;
-    sums.q_log_q += product(q, log_q);
-    sums.q_z += product(q, z);
+    sums.far += p.kind == TISO_DISTILL_REVERSE ? product(e, z - log_q) : product(q, log_q - z);
     sums.e += e;
-    sums.e_far += product(e, z - log_q);
     ++sums.tokens;
   }
-  sums.q = sum_of_warp(sums.q);
-  sums.q_log_q = sum_of_warp(sums.q_log_q);
-  sums.q_z = sum_of_warp(sums.q_z);
-  sums.e = sum_of_warp(sums.e);
-  sums.e_far = sum_of_warp(sums.e_far);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    sums.q += __shfl_xor_sync(0xffffffffu, sums.q, d);
+    sums.far += __shfl_xor_sync(0xffffffffu, sums.far, d);
+    sums.e += __shfl_xor_sync(0xffffffffu, sums.e, d);
+  }
   sums.tokens = __reduce_add_sync(0xffffffffu, sums.tokens);
-  if (team.tid % 32 == 0) space.sums[team.tid / 32] = sums;
+  sums.most = most;
+  if (place.tid % 32 == 0) space.sums[place.tid / 32] = sums;
+}
+
+// The sums over the whole list.
+template <int kThreads, typename A>
+__device__ __forceinline__ ListSums<A> list_sums(const ListSpace<A, kThreads>& space, int top, int kind,
+                                                 double inv_temp, A k) {
+  ListSums<A> sums = space.sums[0];
+  const int warps = warps_of<kThreads>(top);
+  if (warps > 1) {
+    A most = sums.most;
+    for (int i = 1; i < warps; ++i) most = max_acc(most, space.sums[i].most);
+    sums.move(most, inv_temp, k, kind);
+    for (int i = 1; i < warps; ++i) {
+      ListSums<A> more = space.sums[i];
+      more.move(most, inv_temp, k, kind);
+      sums.q += more.q;
+      sums.far += more.far;
+      sums.e += more.e;
+      sums.tokens += more.tokens;
+    }
+    sums.most = most;
+  }
+  return sums;
 }
 
 // The teacher's probabilities of the list and of the rest.
 struct Teacher {
-  double list_q, rest_q, whole;
-  __device__ __forceinline__ Teacher(double q, int tokens, int vocab, int kind, bool drop)
-      : list_q(q) {
+  double rest_q, whole;
+  __device__ __forceinline__ Teacher(double q, int tokens, int vocab, int kind, bool drop) {
     rest_q = tokens == vocab ? 0.0 : fmax(1.0 - q, kind == TISO_DISTILL_REVERSE ? kLeastRest : 0.0);
     if (drop) rest_q = 0.0;
     if (q != q) rest_q = q;  // NaN
@@ -297,89 +290,89 @@ struct Teacher {
   }
 };
 
-// The student's, from the parts' sums and maxima.
+// The student's, from the parts' sums and maxima; a part that is empty, or hidden, has a sum of 0 and no
+// maximum. list_p: the probability of an e of 1.
 template <typename A>
 struct Student {
-  double rest_z, list_z;  // the parts' maxima less the row's, over t
-  A s, rest_p, list_p;    // list_p: the probability of an e of 1
+  A base, s, rest_p, list_p;
 
-  __device__ __forceinline__ Student(const Part<A>& rest, A most, double list_e, double inv_temp) {
-    const double base = base_of(max_acc(rest.m, most));
-    rest_z = (static_cast<double>(base_of(rest.m)) - base) * inv_temp;
-    list_z = (static_cast<double>(base_of(most)) - base) * inv_temp;
-    // a part that is empty, or hidden, has a sum of 0 and no maximum
-    const A of_rest = rest.s == A(0) ? A(0) : exp_as(A(0), rest_z) * rest.s;
-    const A of_list = list_e == 0 ? A(0) : exp_as(A(0), list_z);
-    s = of_rest + of_list * static_cast<A>(list_e);
+  __device__ __forceinline__ Student(const Part<A>& rest, A most, A list_e, A k)
+      : base(base_of(max_acc(rest.m, most))) {
+    const A of_rest = rest.s == A(0) ? A(0) : scaled_exp(base_of(rest.m) - base, k) * rest.s;
+    const A of_list = list_e == A(0) ? A(0) : scaled_exp(base_of(most) - base, k);
+    s = of_rest + of_list * list_e;
     rest_p = of_rest / s;
     list_p = of_list / s;
   }
 };
 
-// An entry's q, log q and log m (m the mixture of both), the q's renormalised where the rest is
-// dropped.
-template <typename A>
-__device__ __forceinline__ void entry_of(const DistillArgs<A>& p, const ListSpace<A>& space, int k,
-                                         const Settled& row, double prob, double& q, double& log_q,
-                                         double& log_m) {
-  q = space.q[k];
-  log_q = space.log_q[k];
-  if (p.drop && row.list_q > 0) {
-    q /= row.list_q;
-    log_q -= log(row.list_q);
-  }
-  log_m = p.kind == TISO_DISTILL_JENSEN ? log(p.mix * q + (1 - p.mix) * prob) : log_q;
+// The first steps after a row's sum, by every warp: what a gradient of the forward divergence is made
+// of; without a logarithm, and in double only what cancels.
+template <typename A, int kThreads>
+__device__ __forceinline__ Settled settle(const DistillArgs<A>& p, const ListSpace<A, kThreads>& space,
+                                          const ListSums<A>& sums, const Part<A>& rest,
+                                          const Student<A>& student, int vocab) {
+  const Teacher teacher(sums.q, sums.tokens, vocab, p.kind, p.drop);
+  Settled row{};
+  row.c = *space.share;
+  if (*space.bad || student.s == A(0)) row.c = nan_of(0.0);
+  row.each = p.drop ? (sums.q > 0 ? 1 / sums.q : sums.q) : 1.0;  // nothing to compare with: 0
+  row.whole = teacher.whole;
+  row.p = student.list_p;
+  // p_v (f - sum P f) = p_v whole - q_v
+  const A factor = static_cast<A>(teacher.whole) * student.rest_p - static_cast<A>(teacher.rest_q);
+  row.factor = static_cast<A>(row.c) * (rest.s == A(0) ? A(0) : factor / rest.s);
+  return row;
 }
 
-// The steps after a row's sum, by a warp: the row's divergence, what the list's gradient is made of
-// into `settled`, and the rest's factor.
-template <int kThreads, typename A>
-__device__ __forceinline__ double settle(const DistillArgs<A>& p, const ListSpace<A>& space,
-                                         const Part<A>& rest, int vocab, double inv_temp,
-                                         double& factor) {
-  ListSums sums = space.sums[0];
-  for (int i = 1; i < warps_of<kThreads>(p.top); ++i) {
-    const ListSums& more = space.sums[i];
-    sums.q += more.q;
-    sums.q_log_q += more.q_log_q;
-    sums.q_z += more.q_z;
-    sums.e += more.e;
-    sums.e_far += more.e_far;
-    sums.tokens += more.tokens;
-  }
+// The steps that take logarithms, by a warp: the divergence, and what the gradients of the others than
+// the forward one are made of.
+template <typename A, int kThreads>
+__device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
+                                              const ListSpace<A, kThreads>& space,
+                                              const ListSums<A>& sums, const Part<A>& rest,
+                                              const Student<A>& student, int vocab, double inv_temp,
+                                              A k, Settled& row) {
   const Teacher teacher(sums.q, sums.tokens, vocab, p.kind, p.drop);
-  const A most = most_of<kThreads>(space, p.top);
-  const Student<A> student(rest, most, sums.e, inv_temp);
-  const double log_s = log(static_cast<double>(student.s));
-  const double rest_log_p = student.rest_z + log(static_cast<double>(rest.s)) - log_s;
-  const double rest_log_q = log(teacher.rest_q), rest_p = student.rest_p;
-  const double unknown = *space.bad || student.s == A(0) ? nan_of(0.0) : 0.0;
-  Settled row{space.settled->c + unknown, student.list_p, student.list_z - log_s, 0.0, sums.q,
-              teacher.whole};
-  double d;
+  const int lane = threadIdx.x & 31;
+  // a lane for each logarithm
+  const double of = lane == 0   ? static_cast<double>(student.s)
+                    : lane == 1 ? static_cast<double>(rest.s)
+                    : lane == 2 ? teacher.rest_q
+                                : sums.q;
+  const double logarithm = log(of), base = student.base;
+  const double log_s = __shfl_sync(0xffffffffu, logarithm, 0);
+  const double rest_log_p = (static_cast<double>(base_of(rest.m)) - base) * inv_temp - log_s +
+                            __shfl_sync(0xffffffffu, logarithm, 1);
+  const double rest_log_q = __shfl_sync(0xffffffffu, logarithm, 2), rest_p = student.rest_p;
+  row.log_each = p.drop ? -__shfl_sync(0xffffffffu, logarithm, 3) : 0.0;
+  row.log_p = (static_cast<double>(base_of(sums.most)) - base) * inv_temp - log_s;
+  double d, factor = 0;
   if (p.drop && sums.q == 0) {  // nothing to compare with
-    d = factor = row.c = unknown;
-  } else if (p.kind == TISO_DISTILL_FORWARD) {
-    // p_v (f - sum P f) = p_v whole - q_v
-    const double each = p.drop ? 1 / sums.q : 1.0, shift = p.drop ? log(sums.q) : 0.0;
-    d = each * (sums.q_log_q - sums.q_z) - each * sums.q * (shift + row.log_p) +
+    d = 0;
+    row.c *= 0;
+    row.factor *= 0;
+    return d + row.c;
+  }
+  if (p.kind == TISO_DISTILL_FORWARD) {
+    d = row.each * sums.far + row.each * sums.q * (row.log_each - row.log_p) +
         product(teacher.rest_q, rest_log_q - rest_log_p);
-    factor = teacher.whole * rest_p - teacher.rest_q;
-  } else if (p.kind == TISO_DISTILL_REVERSE) {
+    return row.c == row.c ? d : row.c;
+  }
+  if (p.kind == TISO_DISTILL_REVERSE) {
     const double rest_f = rest_log_p - rest_log_q;
-    d = row.mean = row.p * (sums.e_far + sums.e * row.log_p) + product(rest_p, rest_f);
+    d = row.mean = row.p * (sums.far + static_cast<double>(sums.e) * row.log_p) +
+                   product(rest_p, rest_f);
     factor = product(rest_p, rest_f - row.mean);
   } else {
-    const double base = base_of(most);
     double mean = 0, cross = 0;
-    for (int k = threadIdx.x & 31; k < p.top; k += 32) {
-      if (space.lead[k] != k) continue;
-      const double prob = space.e[k] * row.p;
-      const double log_p = (static_cast<double>(space.logit[k]) - base) * inv_temp + row.log_p;
-      double q, log_q, log_m;
-      entry_of(p, space, k, row, prob, q, log_q, log_m);
+    for (int i = lane; i < p.top; i += 32) {
+      if (space.lead[i] != i) continue;
+      const A z = space.logit[i] - base_of(sums.most);
+      const double prob = scaled_exp(z, k) * row.p, log_p = static_cast<double>(z) * inv_temp + row.log_p;
+      const double q = space.q[i] * row.each, log_m = log(p.mix * q + (1 - p.mix) * prob);
       mean += product(prob, (1 - p.mix) * (log_p - log_m));
-      cross += product(q, log_q - log_m);
+      cross += product(q, space.log_q[i] + row.log_each - log_m);
     }
     const double log_m = log(p.mix * teacher.rest_q + (1 - p.mix) * rest_p);
     const double rest_f = (1 - p.mix) * (rest_log_p - log_m);
@@ -387,27 +380,119 @@ __device__ __forceinline__ double settle(const DistillArgs<A>& p, const ListSpac
     d = row.mean + p.mix * (sum_of_warp(cross) + product(teacher.rest_q, rest_log_q - log_m));
     factor = product(rest_p, rest_f - row.mean);
   }
-  factor = rest.s == A(0) ? unknown : row.c * factor / static_cast<double>(rest.s);
-  __syncwarp();  // every lane has read the share
-  if ((threadIdx.x & 31) == 0) *space.settled = row;
-  return d + unknown;
+  row.factor = rest.s == A(0) ? 0 * row.c : row.c * factor / static_cast<double>(rest.s);
+  return row.c == row.c ? d : row.c;
 }
 
-// The gradient of an entry's token.
-template <typename A>
-__device__ __forceinline__ A gradient_of(const DistillArgs<A>& p, const ListSpace<A>& space, int k,
-                                         const Settled& row, A most, double inv_temp) {
-  const double prob = space.e[k] * row.p;
-  double q, log_q, log_m;
-  if (p.kind == TISO_DISTILL_FORWARD) {
-    q = space.q[k];
-    if (p.drop && row.list_q > 0) q /= row.list_q;
-    return static_cast<A>(row.c * (prob * row.whole - q));
+// The gradients of the list's tokens, by the threads of their entries.
+template <int kThreads, typename A>
+__device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t r,
+                                               const Place<kThreads>& place, double inv_temp, A k,
+                                               const Settled& row, A most,
+                                               const ListSpace<A, kThreads>& space) {
+  for (int i = place.tid; i < p.top; i += kThreads) {
+    const int lead = space.lead[i];
+    A value = A(0);
+    if (lead >= 0) {
+      const A z = space.logit[lead] - base_of(most);
+      const double prob = scaled_exp(z, k) * row.p, q = space.q[lead] * row.each;
+      if (p.kind == TISO_DISTILL_FORWARD) {
+        value = static_cast<A>(row.c * (prob * row.whole - q));
+      } else {
+        const double log_p = static_cast<double>(z) * inv_temp + row.log_p;
+        const double f = p.kind == TISO_DISTILL_REVERSE
+                             ? log_p - space.log_q[lead]
+                             : (1 - p.mix) * (log_p - log(p.mix * q + (1 - p.mix) * prob));
+        value = static_cast<A>(row.c * product(prob, f - row.mean));
+      }
+    }
+    space.gradient[i] = value;
+    if (p.listed && place.cta == 0) p.listed[r * p.top + i] = value;
   }
-  entry_of(p, space, k, row, prob, q, log_q, log_m);
-  const double z = (static_cast<double>(space.logit[k]) - static_cast<double>(base_of(most))) * inv_temp;
-  const double f = (p.kind == TISO_DISTILL_JENSEN ? 1 - p.mix : 1.0) * (z + row.log_p - log_m);
-  return static_cast<A>(row.c * product(prob, f - row.mean));
+}
+
+// Over what the pass wrote in their places. The threads have met since.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void write_list(const DistillArgs<A>& p, const RowView<T>& view,
+                                           const Place<kThreads>& place,
+                                           const ListSpace<A, kThreads>& space) {
+  for (int i = place.tid; i < p.top; i += kThreads)
+    if (space.lead[i] == i && space.place[i] != kNoPlace)
+      view.g[space.id[i]] = from_acc<T>(static_cast<A>(space.gradient[i] * p.upstream));
+}
+
+// ---------------------------------------------------------------------------------------------
+// The row's passes
+
+// -infinity for the listed elements of a tile that came through shared memory.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void hide_staged(const StagedTiles<kThreads, T>& tiles, int j, const Own& own,
+                                            const ListSpace<A, kThreads>& space) {
+  constexpr int E = RowView<T>::E, kOfTile = kBatch * E;
+  if (!(own.tiles >> j % 32 & 1)) return;
+  for_own(space, tiles.tid, [&](int, int number) {
+    if (number < 0 || number / kOfTile != j) return;
+    const T none = from_acc<T>(lowest<A>());
+    char* vector = reinterpret_cast<char*>(tiles.at(j) + number % kOfTile / E * kThreads);
+    memcpy(vector + number % E * sizeof(T), &none, sizeof(T));
+  });
+}
+
+// The same for a tile's vectors in registers.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void hide_loaded(uint4 (&q)[kBatch], int tid, int j, const Own& own,
+                                            const ListSpace<A, kThreads>& space) {
+  constexpr int E = RowView<T>::E, kOfTile = kBatch * E;
+  if (!(own.tiles >> j % 32 & 1)) return;
+  const uint4 none = no_vector<T>();
+  const uint32_t* n = reinterpret_cast<const uint32_t*>(&none);
+  for_own(space, tid, [&](int, int number) {
+    if (number < 0 || number / kOfTile != j) return;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&q[i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t gone = number % 2 ? 0xffff0000u : 0xffffu;
+          if (number % kOfTile / 2 == 4 * i + c) w[c] = (w[c] & ~gone) | (n[c] & gone);
+        } else if constexpr (sizeof(T) == 4) {
+          if (number % kOfTile == 4 * i + c) w[c] = n[c];
+        } else {
+          if (number % kOfTile == 2 * i + c / 2) w[c] = n[c];
+        }
+      }
+    }
+  });
+}
+
+// The rest's sum over tiles that are loaded directly.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ void add_loaded(Part<A>& rest, const RowView<T>& view,
+                                           const Place<kThreads>& place, const Own& own,
+                                           const ListSpace<A, kThreads>& space, A k) {
+  constexpr int kTile = kBatch * kThreads;
+  for (int tile = place.cta * kTile, j = 0; tile < view.vectors; tile += place.ctas * kTile, ++j) {
+    uint4 q[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int v = tile + i * kThreads + place.tid;
+      q[i] = v < view.vectors ? load_vector(view, v) : no_vector<T>();
+    }
+    hide_loaded<kThreads, T>(q, place.tid, j, own, space);
+    add_vectors<T>(rest, q, k);
+  }
+}
+
+// Adds one of the single elements, unless it is listed.
+template <typename T, int kThreads, typename A>
+__device__ __forceinline__ void add_edge(Part<A>& p, const RowView<T>& r, const Place<kThreads>& place,
+                                         const Own& own, A k) {
+  const int e = place.edge();
+  const A edge = e < r.edges && !own.edge ? to_acc(r.x[r.edge(e)]) : lowest<A>();
+  const A m = max_acc(p.m, edge), base = base_of(m);
+  p.s = (p.m == m ? p.s : p.s * scaled_exp(p.m - base, k)) + scaled_exp(edge - base, k);
+  p.m = m;
 }
 
 // The gradient of the rest: exp((x - base) / t) scale.
@@ -437,30 +522,7 @@ __device__ __forceinline__ void write_rest_of_tile(const RowView<T>& r, int tile
       store_once(to + i * kThreads, slope_vector<T>(load_vector(r, v + i * kThreads), slope));
 }
 
-// The list's gradients, over what the pass wrote in their places. The threads have met since.
-template <int kThreads, typename T, typename A>
-__device__ __forceinline__ void write_list(const Rows& a, const DistillArgs<A>& p, int64_t r,
-                                           const RowView<T>& view, const Place<kThreads>& place,
-                                           double inv_temp, bool with_grad,
-                                           const ListSpace<A>& space) {
-  const Team<kThreads> team{place.tid};
-  const Settled row = *space.settled;
-  const A most = most_of<kThreads>(space, p.top);
-  for (int k = team.tid; k < p.top; k += kThreads) {
-    if (space.lead[k] != k) continue;
-    const A value = gradient_of(p, space, k, row, most, inv_temp);
-    space.gradient[k] = value;
-    const Spot<kThreads, T> spot(view, place.ctas, space.id[k]);
-    if (with_grad && spot.cta == place.cta)
-      view.g[space.id[k]] = from_acc<T>(static_cast<A>(value * p.upstream));
-  }
-  if (!p.listed || place.cta != 0) return;
-  team.sync();
-  for (int k = team.tid; k < p.top; k += kThreads)
-    p.listed[r * p.top + k] = space.lead[k] < 0 ? A(0) : space.gradient[space.lead[k]];
-}
-
-// A row's results but for the means' terms.
+// A row's results but for the means' terms. factor: of the rest's gradient for an upstream one of 1.
 template <typename A>
 __device__ __forceinline__ void write_row(const DistillArgs<A>& p, int64_t r, const Part<A>& rest,
                                           double d, double factor) {
@@ -478,16 +540,16 @@ __device__ __forceinline__ void write_left_out(const DistillArgs<A>& p, int64_t 
   if (p.coef) p.stats[2 * r + 1] = A(kLeftOut);
 }
 
-// The row's share of the loss, into `settled`, by one thread while the row is read.
-template <typename A>
+// The row's share of the loss, by one thread while the row is read.
+template <typename A, int kThreads>
 __device__ __forceinline__ void read_share(const DistillArgs<A>& p, A w, double inv_temp,
-                                           const ListSpace<A>& space) {
+                                           const ListSpace<A, kThreads>& space) {
   cudaGridDependencySynchronize();  // the total's kernel is done
   const double total = *p.total;
-  space.settled->c = total != 0 ? static_cast<double>(w) / total * inv_temp : 0.0;
+  *space.share = total != 0 ? static_cast<double>(w) / total * inv_temp : 0.0;
 }
 
-template <typename T, typename A>
+template <typename T>
 __device__ __forceinline__ RowView<T> distill_view(const Rows& a, int64_t r, T* grad) {
   T* g = grad + r * a.vocab;
   return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
@@ -496,13 +558,12 @@ __device__ __forceinline__ RowView<T> distill_view(const Rows& a, int64_t r, T* 
 // Loss and gradient of a row by a CTA, or a cluster of them.
 template <int kThreads, typename T, typename A>
 __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>& p, double inv_temp,
-                                            A k, T* grad, int bit_words, bool& last) {
+                                            A k, T* grad, bool& last) {
   constexpr int kTile = kBatch * kThreads;
   extern __shared__ uint4 shared[];
-  __shared__ A slope_of[2];
   const Place<kThreads> place;
   const int64_t r = place.row;
-  const RowView<T> view = distill_view<T, A>(a, r, grad);
+  const RowView<T> view = distill_view<T>(a, r, grad);
   const A w = p.weights.at(r);
   if (w == A(0)) {
     if (place.first()) {
@@ -521,84 +582,90 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   const StagedTiles<kThreads, T> tiles(view, place, shared);
 #pragma unroll
   for (int j = 0; j < kStages; ++j) tiles.copy(j);
-  const ListSpace<A> space(shared + kStages * kTile, p.top);
-  read_list(a, p, r, view, place, bit_words, inv_temp, space);
+  const ListSpace<A, kThreads> space(shared + kStages * kTile, p.top);
+  const Own own = hand_out(a, p, r, view, place, space);
+  read_list(p, r, view, place, inv_temp, k, space);
   if (place.tid == 0) read_share(p, w, inv_temp, space);
 
   Part<A> rest{lowest<A>(), A(0)};
-  add_edge(rest, view, place, *space.edge_bits, k);
-  if (tiles.staged == 0)
-    for (int tile = place.cta * kTile, j = 0; tile < view.vectors; tile += place.ctas * kTile, ++j) {
-      uint4 q[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int v = tile + i * kThreads + place.tid;
-        q[i] = v < view.vectors ? load_vector(view, v) : no_vector<T>();
-      }
-      add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, j, place.tid), k);
-    }
+  add_edge(rest, view, place, own, k);
+  if (tiles.staged == 0) add_loaded(rest, view, place, own, space, k);
   for (int j = 0; j < tiles.whole; ++j) {
     uint4 q[kBatch];
-    tiles.fetch(j, q);
+    tiles.arrived();
+    hide_staged(tiles, j, own, space);
+    tiles.read(j, q);
     tiles.copy(j + kStages);
-    add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, j, place.tid), k);
+    add_vectors<T>(rest, q, k);
   }
   if (tiles.cut) {
     uint4 q[kBatch];
-    tiles.fetch_cut(q);
-    add_rest<T>(rest, q, bits_of_tile<kThreads, T>(space.bits, tiles.whole, place.tid), k);
+    tiles.arrived();
+    hide_staged(tiles, tiles.whole, own, space);
+    tiles.read_cut(q);
+    add_vectors<T>(rest, q, k);
     close_group();
   }
   rest = join_warps<kThreads>(join_lanes<32>(rest, k), k);
-  if (threadIdx.x < 32) {
-    double factor;
-    const double d = settle<kThreads>(p, space, rest, a.vocab, inv_temp, factor);
-    if (place.tid == 0) {
-      slope_of[0] = base_of(rest.m);
-      slope_of[1] = static_cast<A>(factor * p.upstream);
+  const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
+  const Student<A> student(rest, sums.most, sums.e, k);
+  // every warp takes the few steps to the rest's factor by itself, where they need no logarithm
+  Settled row = settle(p, space, sums, rest, student, a.vocab);
+  const auto write_results = [&](double d) {
+    write_row(p, r, rest, d, row.factor);
+    p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
+    last = last_unit(p.done, a.rows);
+  };
+  if (p.kind != TISO_DISTILL_FORWARD) {
+    double d = 0;
+    if (threadIdx.x < 32) {
+      d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, row);
+      if (place.tid == 0) *space.settled = row;
     }
-    if (place.first()) {
-      write_row(p, r, rest, d, factor);
-      p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
-      last = last_unit(p.done, a.rows);
-    }
-  }
-  if (!grad && !p.listed) return;
-  __syncthreads();
-  if (grad) {
-    const RestSlope<A> slope{slope_of[0], slope_of[1], k};
-    if (tiles.cut) {
-      uint4 q[kBatch];
-      tiles.fetch(tiles.whole, q);
-      tiles.copy(tiles.whole - kStages);
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (tiles.has(i))
-          store_once(tiles.to(tiles.whole) + i * kThreads, slope_vector<T>(q[i], slope));
-    }
-    for (int j = tiles.whole - 1; j >= 0; --j) {
-      uint4 q[kBatch];
-      tiles.fetch(j, q);
-      tiles.copy(j - kStages);
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        store_once(tiles.to(j) + i * kThreads, slope_vector<T>(q[i], slope));
-    }
-    write_edge(view, place.edge(), slope);
-    if (tiles.staged == 0)
-      for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-        write_rest_of_tile<kThreads>(view, tile, place.tid, slope);
     __syncthreads();
+    row = *space.settled;
+    if (place.first()) write_results(d);
   }
-  write_list(a, p, r, view, place, inv_temp, grad != nullptr, space);
+  if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, sums.most, space);
+  if (p.kind == TISO_DISTILL_FORWARD && place.tid >= kThreads - 32 && place.cta == 0) {
+    // by the last warp: the first ones have the list
+    Settled all = row;
+    const double d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, all);
+    if (place.tid == kThreads - 32) write_results(d);
+  }
+  if (!grad) return;
+  const RestSlope<A> slope{base_of(rest.m), static_cast<A>(row.factor * p.upstream), k};
+  if (tiles.cut) {
+    uint4 q[kBatch];
+    tiles.fetch(tiles.whole, q);
+    tiles.copy(tiles.whole - kStages);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (tiles.has(i))
+        store_once(tiles.to(tiles.whole) + i * kThreads, slope_vector<T>(q[i], slope));
+  }
+  for (int j = tiles.whole - 1; j >= 0; --j) {
+    uint4 q[kBatch];
+    tiles.fetch(j, q);
+    tiles.copy(j - kStages);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      store_once(tiles.to(j) + i * kThreads, slope_vector<T>(q[i], slope));
+  }
+  write_edge(view, place.edge(), slope);
+  if (tiles.staged == 0)
+    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+      write_rest_of_tile<kThreads>(view, tile, place.tid, slope);
+  __syncthreads();
+  write_list(p, view, place, space);
 }
 
 template <typename T, typename A, int kThreads>
-__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
-    distill_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad, int bit_words) {
-  __shared__ bool last;  // written by thread 0 alone
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads / (sizeof(T) == 8 ? 2 : 1))
+    distill_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad) {
+  __shared__ bool last;  // written by one thread of a CTA, after its start
   if (threadIdx.x == 0) last = false;
-  distill_row<kThreads>(a, p, inv_temp, k, grad, bit_words, last);
+  distill_row<kThreads>(a, p, inv_temp, k, grad, last);
   __syncthreads();
   if (last) write_means<1>(p.terms, *p.total, p.out, a.rows);
 }
@@ -606,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
 // Short rows: a warp to a row.
 template <typename T, typename A>
 __global__ void __launch_bounds__(32 * kRowWarps)
-    distill_warp_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad, int bit_words) {
+    distill_warp_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad) {
   constexpr int kTile = kBatch * 32;
   extern __shared__ uint4 shared[];
   __shared__ A terms[kRowWarps];
@@ -617,42 +684,38 @@ __global__ void __launch_bounds__(32 * kRowWarps)
   const A w = r < a.rows ? p.weights.at(r) : A(0);
   if (place.tid == 0) terms[warp] = A(0);
   if (w != A(0)) {
-    const RowView<T> view = distill_view<T, A>(a, r, grad);
-    const ListSpace<A> space(
-        reinterpret_cast<char*>(shared) + warp * ListSpace<A>::bytes(p.top, 4 * bit_words), p.top);
-    read_list(a, p, r, view, place, bit_words, inv_temp, space);
+    const RowView<T> view = distill_view<T>(a, r, grad);
+    const ListSpace<A, 32> space(
+        reinterpret_cast<char*>(shared) + warp * ListSpace<A, 32>::bytes(p.top), p.top);
+    const Own own = hand_out(a, p, r, view, place, space);
+    read_list(p, r, view, place, inv_temp, k, space);
     if (place.tid == 0) read_share(p, w, inv_temp, space);
     Part<A> rest{lowest<A>(), A(0)};
-    add_edge(rest, view, place, *space.edge_bits, k);
-    for (int tile = 0, j = 0; tile < view.vectors; tile += kTile, ++j) {
-      uint4 q[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int v = tile + i * 32 + place.tid;
-        q[i] = v < view.vectors ? load_vector(view, v) : no_vector<T>();
-      }
-      add_rest<T>(rest, q, bits_of_tile<32, T>(space.bits, j, place.tid), k);
-    }
+    add_edge(rest, view, place, own, k);
+    add_loaded(rest, view, place, own, space, k);
     rest = join_lanes<32>(rest, k);
     __syncwarp();
-    double factor;
-    const double d = settle<32>(p, space, rest, a.vocab, inv_temp, factor);
+    const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
+    const Student<A> student(rest, sums.most, sums.e, k);
+    Settled row = settle(p, space, sums, rest, student, a.vocab);
+    const double d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, row);
     if (place.tid == 0) {
-      write_row(p, r, rest, d, factor);
+      write_row(p, r, rest, d, row.factor);
       terms[warp] = static_cast<A>(static_cast<double>(w) * d);
     }
+    if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, sums.most, space);
     if (grad) {
-      const RestSlope<A> slope{base_of(rest.m), static_cast<A>(factor * p.upstream), k};
+      const RestSlope<A> slope{base_of(rest.m), static_cast<A>(row.factor * p.upstream), k};
       write_edge(view, place.edge(), slope);
       for (int tile = 0; tile < view.vectors; tile += kTile)
         write_rest_of_tile<32>(view, tile, place.tid, slope);
+      __syncwarp();
+      write_list(p, view, place, space);
     }
-    __syncwarp();
-    if (grad || p.listed) write_list(a, p, r, view, place, inv_temp, grad != nullptr, space);
   } else if (r < a.rows) {
     if (place.tid == 0) write_left_out(p, r);
     if (grad) {
-      const RowView<T> view = distill_view<T, A>(a, r, grad);
+      const RowView<T> view = distill_view<T>(a, r, grad);
       zero_edge(view, place.edge());
       for (int tile = 0; tile < view.vectors; tile += kTile) zero_tile<32>(view, tile, place.tid);
     }
@@ -710,33 +773,22 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------------------------
 // Host side
 
-// Bits of the vectors of a CTA's share of `vectors`, in bytes.
-template <typename T>
-int64_t bit_bytes(int64_t vectors, int threads, int ctas) {
-  const int64_t tile = int64_t{kBatch} * threads, tiles = (vectors + tile - 1) / tile;
-  return (tiles + ctas - 1) / ctas * tile * RowView<T>::E / 8;
-}
-
 template <typename T, int kThreads>
 int launch_distill_rows(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p,
                         double inv_temp, T* grad, int sms, cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  constexpr int64_t kStaged = int64_t{kStages} * kBatch * kThreads * 16;
+  constexpr size_t kStaged = size_t{kStages} * kBatch * kThreads * 16;
   const int64_t vectors = a.vocab / RowView<T>::E;
   int ctas = ctas_for(a.rows, vectors, kThreads, sms);
   while (ctas < 8 && int64_t{sms} * (kSmThreads / kThreads) * vectors * 16 / ctas > kRowsInL2)
     ctas *= 2;
-  while (ctas < 8 && bit_bytes<T>(vectors, kThreads, ctas) > kSharedForBits) ctas *= 2;
-  const int64_t bits = bit_bytes<T>(vectors, kThreads, ctas);
-  if (bits > kSharedForBits)
-    return report_error(TISO_ERR_ARGUMENT, "a vocabulary too large for the distillation loss");
-  const size_t shared = kStaged + ListSpace<A>::bytes(p.top, static_cast<int>(bits));
   const auto kernel = distill_kernel<T, A, kThreads>;
   const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
-                              kStaged + ListSpace<A>::bytes(kMostListed, kSharedForBits));
+                              kStaged + ListSpace<A, kThreads>::bytes(kMostListed));
   if (rc) return rc;
-  return launch_clusters(kernel, a.rows, ctas, kThreads, shared, true, st, "distill_kernel launch", a,
-                         p, inv_temp, exp_factor(A(0), inv_temp), grad, static_cast<int>(bits / 4));
+  return launch_clusters(kernel, a.rows, ctas, kThreads,
+                         kStaged + ListSpace<A, kThreads>::bytes(p.top), true, st,
+                         "distill_kernel launch", a, p, inv_temp, exp_factor(A(0), inv_temp), grad);
 }
 
 template <typename T>
@@ -746,15 +798,14 @@ int launch_distill(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p,
   const int64_t vectors = a.vocab / RowView<T>::E;
   const int sms = sm_count();
   if (by_warps(a.rows, vectors, 1536, sms)) {
-    const int bits = static_cast<int>(bit_bytes<T>(vectors, 32, 1));
-    const size_t shared = size_t{kRowWarps} * ListSpace<A>::bytes(p.top, bits);
     const auto kernel = distill_warp_kernel<T, A>;
     const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
-                                size_t{kRowWarps} * ListSpace<A>::bytes(kMostListed, 1536 * 16 / 8));
+                                size_t{kRowWarps} * ListSpace<A, 32>::bytes(kMostListed));
     if (rc) return rc;
-    return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps, shared,
-                           true, st, "distill_warp_kernel launch", a, p, inv_temp,
-                           exp_factor(A(0), inv_temp), grad, bits / 4);
+    return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps,
+                           size_t{kRowWarps} * ListSpace<A, 32>::bytes(p.top), true, st,
+                           "distill_warp_kernel launch", a, p, inv_temp, exp_factor(A(0), inv_temp),
+                           grad);
   }
   return launch_distill_rows<T, 256>(a, p, inv_temp, grad, sms, st);
 }

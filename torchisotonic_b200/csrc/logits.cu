@@ -355,7 +355,8 @@ __device__ __forceinline__ void policy_row(const Rows& a, const PolicyArgs<A>& p
   }
   if (tiles.cut) {
     uint4 q[kBatch];
-    tiles.fetch_cut(q);
+    tiles.arrived();
+    tiles.read_cut(q);
     add_vectors<T>(part, q, k);
     close_group();
   }

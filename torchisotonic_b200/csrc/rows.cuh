@@ -295,7 +295,7 @@ struct StagedTiles {
     return own + whole * stride + i * kThreads < staged;
   }
   __device__ __forceinline__ void copy(int j) const {
-    uint4* at = stages + static_cast<unsigned>(j) % kStages * kTile + tid;
+    uint4* at = this->at(j);
     if (j >= 0 && j < whole) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
@@ -308,17 +308,25 @@ struct StagedTiles {
     }
     close_group();
   }
-  __device__ __forceinline__ void fetch(int j, uint4 (&q)[kBatch]) const {
-    wait_groups<kStages - 1>();  // tile j's, closed kStages - 1 groups before the last
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      q[i] = stages[static_cast<unsigned>(j) % kStages * kTile + i * kThreads + tid];
+  // waits for the tile that is read next: kStages - 1 groups were closed after its own
+  __device__ __forceinline__ void arrived() const { wait_groups<kStages - 1>(); }
+  // this thread's vectors of tile j in shared memory, kThreads apart
+  __device__ __forceinline__ uint4* at(int j) const {
+    return stages + static_cast<unsigned>(j) % kStages * kTile + tid;
   }
-  __device__ __forceinline__ void fetch_cut(uint4 (&q)[kBatch]) const {
-    fetch(whole, q);
+  __device__ __forceinline__ void read(int j, uint4 (&q)[kBatch]) const {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) q[i] = at(j)[i * kThreads];
+  }
+  __device__ __forceinline__ void read_cut(uint4 (&q)[kBatch]) const {
+    read(whole, q);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i)
       if (!has(i)) q[i] = no_vector<T>();
+  }
+  __device__ __forceinline__ void fetch(int j, uint4 (&q)[kBatch]) const {
+    arrived();
+    read(j, q);
   }
 };
 
