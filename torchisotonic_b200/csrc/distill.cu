@@ -99,7 +99,7 @@ struct ListSpace {
   int *id, *lead;        // -1: no entry; the first entry of its id
   int *next, *place;     // in its owner's chain; where among the owner's elements
   int* head;             // of each thread's chain
-  int* bad;              // an id out of range
+  int *bad, *twice;      // an id out of range; a token that is listed again
 
   static __host__ __device__ constexpr int entries(int top) { return (top + 3) / 4 * 4; }
   static __host__ __device__ constexpr int bytes(int top) {
@@ -123,6 +123,7 @@ struct ListSpace {
     place = next + n;
     head = place + n;
     bad = head + kThreads;
+    twice = bad + 1;
   }
 };
 
@@ -167,7 +168,7 @@ __device__ __forceinline__ Own hand_out(const Rows& a, const DistillArgs<A>& p, 
   constexpr int kOfTile = kBatch * RowView<T>::E;
   const Team<kThreads> team{place.tid};
   space.head[team.tid] = -1;
-  if (team.tid == 0) *space.bad = 0;
+  if (team.tid == 0) *space.bad = *space.twice = 0;
   for (int k = team.tid; k < p.top; k += kThreads) {
     const int64_t id = p.ids[r * p.top + k];
     space.id[k] = id == a.ignore ? -1 : id >= 0 && id < a.vocab ? static_cast<int>(id) : -2;
@@ -184,6 +185,9 @@ __device__ __forceinline__ Own hand_out(const Rows& a, const DistillArgs<A>& p, 
   }
   team.sync();
   Own own{0, false};
+  for (int k = space.head[team.tid]; k >= 0; k = space.next[k])
+    for (int j = space.next[k]; j >= 0; j = space.next[j])
+      if (space.id[j] == space.id[k]) *space.twice = 1;
   for_own(space, team.tid, [&](int, int number) {
     if (number == kEdgePlace) {
       own.edge = true;
@@ -201,8 +205,9 @@ __device__ __forceinline__ int warps_of(int top) {
 }
 
 // The list's numbers and their sums, by each warp for its own entries (the others' are known after
-// the threads' next meeting). A token that is listed again counts in its first entry.
-template <int kThreads, typename T, typename A>
+// the threads' next meeting). kAgain: tokens are listed more than once, each counts in its first entry
+// with the sum of its probabilities.
+template <bool kAgain, int kThreads, typename T, typename A>
 __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, const RowView<T>& view,
                                           const Place<kThreads>& place, double inv_temp, A k,
                                           const ListSpace<A, kThreads>& space) {
@@ -215,17 +220,19 @@ __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, co
       const A logit = to_acc(view.x[id]);
       double log_q = static_cast<double>(p.logps[r * p.top + i]), q = exp(log_q);
       lead = i;
-      bool more = false;
-      for (int j = 0; j < p.top; ++j) {
-        if (space.id[j] != id || j == i) continue;
-        if (j < i) {
-          lead = min(lead, j);
-        } else {
-          q += exp(static_cast<double>(p.logps[r * p.top + j]));
-          more = true;
+      if constexpr (kAgain) {
+        bool more = false;
+        for (int j = 0; j < p.top; ++j) {
+          if (space.id[j] != id || j == i) continue;
+          if (j < i) {
+            lead = min(lead, j);
+          } else {
+            q += exp(static_cast<double>(p.logps[r * p.top + j]));
+            more = true;
+          }
         }
+        if (more) log_q = log(q);
       }
-      if (more) log_q = log(q);
       space.logit[i] = logit;
       space.log_q[i] = log_q;
       space.q[i] = q;
@@ -584,7 +591,7 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   for (int j = 0; j < kStages; ++j) tiles.copy(j);
   const ListSpace<A, kThreads> space(shared + kStages * kTile, p.top);
   const Own own = hand_out(a, p, r, view, place, space);
-  read_list(p, r, view, place, inv_temp, k, space);
+  read_list<false>(p, r, view, place, inv_temp, k, space);
   if (place.tid == 0) read_share(p, w, inv_temp, space);
 
   Part<A> rest{lowest<A>(), A(0)};
@@ -607,6 +614,10 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
     close_group();
   }
   rest = join_warps<kThreads>(join_lanes<32>(rest, k), k);
+  if (*space.twice) {
+    read_list<true>(p, r, view, place, inv_temp, k, space);
+    __syncthreads();
+  }
   const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
   const Student<A> student(rest, sums.most, sums.e, k);
   // every warp takes the few steps to the rest's factor by itself, where they need no logarithm
@@ -688,13 +699,17 @@ __global__ void __launch_bounds__(32 * kRowWarps)
     const ListSpace<A, 32> space(
         reinterpret_cast<char*>(shared) + warp * ListSpace<A, 32>::bytes(p.top), p.top);
     const Own own = hand_out(a, p, r, view, place, space);
-    read_list(p, r, view, place, inv_temp, k, space);
+    read_list<false>(p, r, view, place, inv_temp, k, space);
     if (place.tid == 0) read_share(p, w, inv_temp, space);
     Part<A> rest{lowest<A>(), A(0)};
     add_edge(rest, view, place, own, k);
     add_loaded(rest, view, place, own, space, k);
     rest = join_lanes<32>(rest, k);
     __syncwarp();
+    if (*space.twice) {
+      read_list<true>(p, r, view, place, inv_temp, k, space);
+      __syncwarp();
+    }
     const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
     const Student<A> student(rest, sums.most, sums.e, k);
     Settled row = settle(p, space, sums, rest, student, a.vocab);
