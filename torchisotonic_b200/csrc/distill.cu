@@ -127,6 +127,12 @@ struct ListSpace {
   }
 };
 
+// The same with the staged tiles, in bytes (whole vectors).
+template <typename A, int kThreads>
+__host__ __device__ constexpr int row_bytes(int top) {
+  return (kStages * kBatch * kThreads * 16 + ListSpace<A, kThreads>::bytes(top) + 15) / 16 * 16;
+}
+
 // An element's owner: of a CTA's tiles (every ctas-th) the thread that has its vector, of the single
 // elements the thread of their number in the first CTA. place: its number among the owner's elements.
 constexpr int kNoPlace = -1, kEdgePlace = -2;
@@ -562,37 +568,32 @@ __device__ __forceinline__ RowView<T> distill_view(const Rows& a, int64_t r, T* 
   return RowView<T>(row_at<T>(a, r), g, reinterpret_cast<uintptr_t>(g), a.vocab);
 }
 
-// Loss and gradient of a row by a CTA, or a cluster of them.
-template <int kThreads, typename T, typename A>
-__device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>& p, double inv_temp,
-                                            A k, T* grad, bool& last) {
+// A row that is left out: its gradient is zeros.
+template <int kThreads, typename T>
+__device__ __forceinline__ void zero_row(const RowView<T>& view, const Place<kThreads>& place) {
   constexpr int kTile = kBatch * kThreads;
-  extern __shared__ uint4 shared[];
-  const Place<kThreads> place;
+  zero_edge(view, place.edge());
+  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
+    zero_tile<kThreads>(view, tile, place.tid);
+}
+
+// Loss and gradient of a row by a warp, a CTA, or a cluster of them. finish(d) is called by one thread
+// with the row's divergence, after the row's other results are written.
+template <int kThreads, typename T, typename A, typename F>
+__device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>& p, double inv_temp,
+                                            A k, T* grad, const Place<kThreads>& place, A w,
+                                            uint4* shared, const F& finish) {
+  constexpr int kTile = kBatch * kThreads;
+  const Team<kThreads> team{place.tid};
   const int64_t r = place.row;
   const RowView<T> view = distill_view<T>(a, r, grad);
-  const A w = p.weights.at(r);
-  if (w == A(0)) {
-    if (place.first()) {
-      write_left_out(p, r);
-      p.terms[r] = A(0);
-      cudaGridDependencySynchronize();
-      last = last_unit(p.done, a.rows);
-    }
-    if (!grad) return;
-    zero_edge(view, place.edge());
-    for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
-      zero_tile<kThreads>(view, tile, place.tid);
-    return;
-  }
-  cluster_started(place.ctas);
   const StagedTiles<kThreads, T> tiles(view, place, shared);
 #pragma unroll
   for (int j = 0; j < kStages; ++j) tiles.copy(j);
   const ListSpace<A, kThreads> space(shared + kStages * kTile, p.top);
   const Own own = hand_out(a, p, r, view, place, space);
   read_list<false>(p, r, view, place, inv_temp, k, space);
-  if (place.tid == 0) read_share(p, w, inv_temp, space);
+  if (place.tid == kThreads - 1) read_share(p, w, inv_temp, space);
 
   Part<A> rest{lowest<A>(), A(0)};
   add_edge(rest, view, place, own, k);
@@ -614,9 +615,10 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
     close_group();
   }
   rest = join_warps<kThreads>(join_lanes<32>(rest, k), k);
+  if constexpr (kThreads == 32) team.sync();
   if (*space.twice) {
     read_list<true>(p, r, view, place, inv_temp, k, space);
-    __syncthreads();
+    team.sync();
   }
   const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
   const Student<A> student(rest, sums.most, sums.e, k);
@@ -624,16 +626,15 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   Settled row = settle(p, space, sums, rest, student, a.vocab);
   const auto write_results = [&](double d) {
     write_row(p, r, rest, d, row.factor);
-    p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
-    last = last_unit(p.done, a.rows);
+    finish(d);
   };
   if (p.kind != TISO_DISTILL_FORWARD) {
     double d = 0;
-    if (threadIdx.x < 32) {
+    if (place.tid < 32) {
       d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, row);
       if (place.tid == 0) *space.settled = row;
     }
-    __syncthreads();
+    team.sync();
     row = *space.settled;
     if (place.first()) write_results(d);
   }
@@ -667,25 +668,42 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   if (tiles.staged == 0)
     for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile)
       write_rest_of_tile<kThreads>(view, tile, place.tid, slope);
-  __syncthreads();
+  team.sync();
   write_list(p, view, place, space);
 }
 
 template <typename T, typename A, int kThreads>
 __global__ void __launch_bounds__(kThreads, kSmThreads / kThreads / (sizeof(T) == 8 ? 2 : 1))
     distill_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad) {
+  extern __shared__ uint4 shared[];
   __shared__ bool last;  // written by one thread of a CTA, after its start
   if (threadIdx.x == 0) last = false;
-  distill_row<kThreads>(a, p, inv_temp, k, grad, last);
+  const Place<kThreads> place;
+  const int64_t r = place.row;
+  const A w = p.weights.at(r);
+  if (w != A(0)) {
+    cluster_started(place.ctas);
+    distill_row(a, p, inv_temp, k, grad, place, w, shared, [&](double d) {
+      p.terms[r] = static_cast<A>(static_cast<double>(w) * d);
+      last = last_unit(p.done, a.rows);
+    });
+  } else {
+    if (place.first()) {
+      write_left_out(p, r);
+      p.terms[r] = A(0);
+      cudaGridDependencySynchronize();
+      last = last_unit(p.done, a.rows);
+    }
+    if (grad) zero_row(distill_view<T>(a, r, grad), place);
+  }
   __syncthreads();
   if (last) write_means<1>(p.terms, *p.total, p.out, a.rows);
 }
 
 // Short rows: a warp to a row.
 template <typename T, typename A>
-__global__ void __launch_bounds__(32 * kRowWarps)
+__global__ void __launch_bounds__(32 * kRowWarps, sizeof(T) == 8 ? 2 : 4)
     distill_warp_kernel(Rows a, DistillArgs<A> p, double inv_temp, A k, T* grad) {
-  constexpr int kTile = kBatch * 32;
   extern __shared__ uint4 shared[];
   __shared__ A terms[kRowWarps];
   __shared__ bool last;
@@ -695,45 +713,12 @@ __global__ void __launch_bounds__(32 * kRowWarps)
   const A w = r < a.rows ? p.weights.at(r) : A(0);
   if (place.tid == 0) terms[warp] = A(0);
   if (w != A(0)) {
-    const RowView<T> view = distill_view<T>(a, r, grad);
-    const ListSpace<A, 32> space(
-        reinterpret_cast<char*>(shared) + warp * ListSpace<A, 32>::bytes(p.top), p.top);
-    const Own own = hand_out(a, p, r, view, place, space);
-    read_list<false>(p, r, view, place, inv_temp, k, space);
-    if (place.tid == 0) read_share(p, w, inv_temp, space);
-    Part<A> rest{lowest<A>(), A(0)};
-    add_edge(rest, view, place, own, k);
-    add_loaded(rest, view, place, own, space, k);
-    rest = join_lanes<32>(rest, k);
-    __syncwarp();
-    if (*space.twice) {
-      read_list<true>(p, r, view, place, inv_temp, k, space);
-      __syncwarp();
-    }
-    const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
-    const Student<A> student(rest, sums.most, sums.e, k);
-    Settled row = settle(p, space, sums, rest, student, a.vocab);
-    const double d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, row);
-    if (place.tid == 0) {
-      write_row(p, r, rest, d, row.factor);
-      terms[warp] = static_cast<A>(static_cast<double>(w) * d);
-    }
-    if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, sums.most, space);
-    if (grad) {
-      const RestSlope<A> slope{base_of(rest.m), static_cast<A>(row.factor * p.upstream), k};
-      write_edge(view, place.edge(), slope);
-      for (int tile = 0; tile < view.vectors; tile += kTile)
-        write_rest_of_tile<32>(view, tile, place.tid, slope);
-      __syncwarp();
-      write_list(p, view, place, space);
-    }
+    uint4* own = shared + warp * (row_bytes<A, 32>(p.top) / 16);
+    distill_row(a, p, inv_temp, k, grad, place, w, own,
+                [&](double d) { terms[warp] = static_cast<A>(static_cast<double>(w) * d); });
   } else if (r < a.rows) {
     if (place.tid == 0) write_left_out(p, r);
-    if (grad) {
-      const RowView<T> view = distill_view<T>(a, r, grad);
-      zero_edge(view, place.edge());
-      for (int tile = 0; tile < view.vectors; tile += kTile) zero_tile<32>(view, tile, place.tid);
-    }
+    if (grad) zero_row(distill_view<T>(a, r, grad), place);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -792,17 +777,15 @@ template <typename T, int kThreads>
 int launch_distill_rows(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p,
                         double inv_temp, T* grad, int sms, cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  constexpr size_t kStaged = size_t{kStages} * kBatch * kThreads * 16;
   const int64_t vectors = a.vocab / RowView<T>::E;
   int ctas = ctas_for(a.rows, vectors, kThreads, sms);
   while (ctas < 8 && int64_t{sms} * (kSmThreads / kThreads) * vectors * 16 / ctas > kRowsInL2)
     ctas *= 2;
   const auto kernel = distill_kernel<T, A, kThreads>;
-  const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
-                              kStaged + ListSpace<A, kThreads>::bytes(kMostListed));
+  const int rc =
+      allow_shared(reinterpret_cast<const void*>(kernel), row_bytes<A, kThreads>(kMostListed));
   if (rc) return rc;
-  return launch_clusters(kernel, a.rows, ctas, kThreads,
-                         kStaged + ListSpace<A, kThreads>::bytes(p.top), true, st,
+  return launch_clusters(kernel, a.rows, ctas, kThreads, row_bytes<A, kThreads>(p.top), true, st,
                          "distill_kernel launch", a, p, inv_temp, exp_factor(A(0), inv_temp), grad);
 }
 
@@ -815,10 +798,10 @@ int launch_distill(const Rows& a, const DistillArgs<typename AccOf<T>::type>& p,
   if (by_warps(a.rows, vectors, 1536, sms)) {
     const auto kernel = distill_warp_kernel<T, A>;
     const int rc = allow_shared(reinterpret_cast<const void*>(kernel),
-                                size_t{kRowWarps} * ListSpace<A, 32>::bytes(kMostListed));
+                                kRowWarps * row_bytes<A, 32>(kMostListed));
     if (rc) return rc;
     return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps,
-                           size_t{kRowWarps} * ListSpace<A, 32>::bytes(p.top), true, st,
+                           kRowWarps * row_bytes<A, 32>(p.top), true, st,
                            "distill_warp_kernel launch", a, p, inv_temp, exp_factor(A(0), inv_temp),
                            grad);
   }
@@ -847,7 +830,7 @@ int run_distill(const Rows& a, const tiso_distill_args* q, double inv_temp, void
   p.total = static_cast<double*>(workspace);
   p.done = reinterpret_cast<unsigned*>(p.total + 1);
   p.terms = reinterpret_cast<A*>(p.total + 2);
-  int rc = launch_total(p.weights, a.rows, p.total, p.done, p.out, 1, st);
+  int rc = launch_total(p.weights, a.rows, kTotalThreads, p.total, p.done, p.out, 1, st);
   if (rc || a.rows == 0) return rc;
   return launch_distill<T>(a, p, inv_temp, static_cast<T*>(grad), st);
 }

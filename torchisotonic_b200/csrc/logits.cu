@@ -504,7 +504,7 @@ int run_policy(const Rows& a, const tiso_policy_args* q, double inv_temp, void* 
   p.total = static_cast<double*>(workspace);
   p.done = reinterpret_cast<unsigned*>(p.total + 1);
   p.terms = reinterpret_cast<A*>(p.total + 2);
-  const int rc = launch_total(p.weights, a.rows, p.total, p.done, p.out, 3, st);
+  const int rc = launch_total(p.weights, a.rows, 8 * kTotalThreads, p.total, p.done, p.out, 3, st);
   if (rc || a.rows == 0) return rc;
   return launch_policy<T>(a, p, inv_temp, static_cast<T*>(grad), st);
 }

@@ -535,13 +535,13 @@ TokenWeights<A> weights_of(const int64_t* marks, int64_t stride, int64_t ignore,
           !weight ? kNoWeight : weight_is_byte ? kByteWeight : kAccWeight};
 }
 
-// 8192 rows: 7 us by one CTA
+// `alone`: up to so many rows by one CTA (8192 rows: 7 us)
 template <typename A>
-int launch_total(const TokenWeights<A>& weights, int64_t rows, double* total, unsigned* done, A* out,
-                 int means, cudaStream_t st) {
-  return launch_clusters(weights_total_kernel<A>, 1, rows > 8 * kTotalThreads ? kTotalCtas : 1,
-                         kTotalThreads, 0, false, st, "weights_total_kernel launch", weights, rows,
-                         total, done, out, means);
+int launch_total(const TokenWeights<A>& weights, int64_t rows, int64_t alone, double* total,
+                 unsigned* done, A* out, int means, cudaStream_t st) {
+  return launch_clusters(weights_total_kernel<A>, 1, rows > alone ? kTotalCtas : 1, kTotalThreads, 0,
+                         false, st, "weights_total_kernel launch", weights, rows, total, done, out,
+                         means);
 }
 
 // Rows of at most kWarpVectors vectors go to a warp each; of up to `most` of them where there are
