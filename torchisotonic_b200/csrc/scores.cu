@@ -7,10 +7,15 @@
 // neither a difference of large numbers (s >= 1, u <= 0). Parts of a row join as for s alone: with
 // d = (m1 - M) / t, s1 and u1 become s1 exp(d) and exp(d) (u1 + d s1).
 //
-// Top alternatives: the row's body is cut into groups of neighbouring vectors, whose maxima the pass
-// leaves in shared memory. The k best groups (equal maxima: the first) hold the k largest elements,
-// for each of the others has an element in each of these before it. Those groups are read again and
-// their elements, all at least the k-th maximum, are ranked.
+// Top alternatives: each thread keeps the maximum of every batch of vectors it reads. Of the maxima that
+// the lanes of a warp have seen, the q-th largest is taken, q = top / warps rounded up: the least of
+// these over the warps is reached by `top` elements at least, so that the alternatives are among the
+// elements that reach it. The batches whose maximum does are read again, and what is found there, a
+// few times `top` elements as a rule, is ranked. Where it is more than there is room for (equal
+// logits, rows in order) the selection is by groups instead: the row is read again for the maxima of
+// groups of neighbouring vectors; the `top` best groups (equal maxima: the first) hold the top
+// elements, for each of the others has an element in each of these before it; and so on with their
+// vectors and elements, each step an exact selection that no data makes longer.
 #include "rows.cuh"
 #include "select.cuh"
 
@@ -18,7 +23,7 @@ namespace tiso {
 namespace {
 
 constexpr int kMostTop = 128;
-constexpr size_t kSharedForTop = 160 * 1024;
+constexpr int kSharedForTop = 160 * 1024;
 
 // What a thread has seen of a row; u in the exponent's unit (log 2 in float, 1 in double).
 template <typename A>
@@ -39,6 +44,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where eithe
   return r;
 }
 __device__ __forceinline__ double max_nan(double a, double b) { return a != a || a > b ? a : b; }
+__device__ __forceinline__ float min_acc(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double min_acc(double a, double b) { return fmin(a, b); }
 __device__ __forceinline__ float exp_of(float a) { return exp2_of(a); }
 __device__ __forceinline__ double exp_of(double a) { return exp(a); }
 
@@ -134,40 +141,102 @@ __device__ __forceinline__ Scored<A> join_scores_of_warps(Scored<A> p, A k) {
 // ---------------------------------------------------------------------------------------------
 // Top alternatives
 
-// A row's element; the larger one, of equal ones the first, is before the other.
+// A row's element: the larger one, of equal ones the first, is before the other. In float as one
+// integer, the number's key over the complement of its place.
 template <typename A>
-struct Element {
-  A value;
-  int at;
-  __device__ __forceinline__ bool before(const Element& o) const {
-    return value > o.value || (value == o.value && at < o.at);
+struct Ranked;
+template <>
+struct Ranked<float> {
+  uint64_t key;
+  Ranked() = default;
+  __device__ __forceinline__ Ranked(float value, int at)
+      : key(static_cast<uint64_t>(ordered(value)) << 32 | (0xffffffffu - static_cast<unsigned>(at))) {}
+  __device__ __forceinline__ bool before(const Ranked& o) const { return key > o.key; }
+  __device__ __forceinline__ uint32_t number() const { return static_cast<uint32_t>(key >> 32); }
+  __device__ __forceinline__ float value() const {
+    const uint32_t b = number();
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+  }
+  __device__ __forceinline__ int at() const {
+    return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
   }
 };
+template <>
+struct Ranked<double> {
+  uint64_t key;
+  int place;
+  Ranked() = default;
+  __device__ __forceinline__ Ranked(double value, int at) : key(ordered(value)), place(at) {}
+  __device__ __forceinline__ bool before(const Ranked& o) const {
+    return key > o.key || (key == o.key && place < o.place);
+  }
+  __device__ __forceinline__ uint64_t number() const { return key; }
+  __device__ __forceinline__ double value() const {
+    return __longlong_as_double(
+        static_cast<long long>(key >> 63 ? key & 0x7fffffffffffffffULL : ~key));
+  }
+  __device__ __forceinline__ int at() const { return place; }
+};
 
-// Shared memory of the threads that work on a row (a cluster's CTAs have one each).
+constexpr int kNowhere = 0x7fffffff;  // the place of an element that is not there
+
 template <typename A>
-struct TopSpace {
-  Element<A>* candidates;  // 8 top + 32
-  Element<A>* best;        // top; of the first CTA of a cluster top for each CTA
-  A* maxima;               // of the groups; 32 top at least
-  int* picked;             // top
-  unsigned* histogram;
-  int* count;              // 2
+__device__ __forceinline__ A number_of(A x) {  // NaN in the order of -infinity
+  return x == x ? x : lowest<A>();
+}
 
-  static size_t bytes(int top, int groups, int ctas) {
-    const size_t numbers = groups > 32 * top ? groups : 32 * top;
-    return sizeof(Element<A>) * (8 * top + 32 + static_cast<size_t>(top) * ctas) +
-           sizeof(A) * ((numbers + 3) / 4 * 4) + sizeof(int) * ((top + 3) / 4 * 4 + kHistogram + 4);
+// At least x, in the upper half of a float.
+__device__ __forceinline__ uint16_t upper_half(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return static_cast<uint16_t>((b >> 31 ? b : b + 0xffffu) >> 16);
+}
+__device__ __forceinline__ uint16_t upper_half(double x) { return upper_half(__double2float_ru(x)); }
+__device__ __forceinline__ float from_upper_half(uint16_t h) {
+  return __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
+
+// What the threads that work on a row have to choose from (a cluster's CTAs each for their share).
+struct TopSizes {
+  int top, tiles;  // of this CTA's share, at most
+  int groups;      // and groups of vectors
+  bool whole;      // 32 vectors to a group, else one
+
+  __host__ __device__ int room() const { return 8 * (top + 32) + 32; }
+  __host__ __device__ int batches() const { return 4 * top + 64; }
+};
+
+// Their shared memory.
+template <typename A, int kThreads>
+struct TopSpace {
+  static constexpr int kWarps = kThreads / 32;
+  Ranked<A>* candidates;  // room
+  Ranked<A>* best;        // top; in the first CTA of a cluster top for each CTA
+  double* log_s;
+  A* kth;                 // of each warp
+  int* picked;            // batches, or top groups
+  int* count;             // 2: candidates, picked
+  unsigned* histogram;
+  uint16_t* batch_max;    // tiles x threads
+  A* maxima;              // of the groups, 32 top at least: in the same place
+
+  static __host__ __device__ int bytes(const TopSizes& z, int ctas) {
+    const int numbers = z.groups > 32 * z.top ? z.groups : 32 * z.top;
+    const int maxima = numbers * static_cast<int>(sizeof(A)), batches = z.tiles * kThreads * 2;
+    return static_cast<int>(sizeof(Ranked<A>)) * (z.room() + (z.top + 1) / 2 * 2 * ctas) + 16 +
+           static_cast<int>(sizeof(A)) * ((kWarps + 3) / 4 * 4) + 4 * (z.batches() + 4 + kHistogram) +
+           ((maxima > batches ? maxima : batches) + 15) / 16 * 16;
   }
 
-  __device__ TopSpace(void* at, int top, int groups, int ctas) {
-    const int numbers = max(groups, 32 * top);
-    candidates = static_cast<Element<A>*>(at);
-    best = candidates + 8 * top + 32;
-    maxima = reinterpret_cast<A*>(best + top * ctas);
-    histogram = reinterpret_cast<unsigned*>(maxima + (numbers + 3) / 4 * 4);
-    picked = reinterpret_cast<int*>(histogram + kHistogram);
-    count = picked + (top + 3) / 4 * 4;
+  __device__ TopSpace(void* at, const TopSizes& z, int ctas) {
+    candidates = static_cast<Ranked<A>*>(at);
+    best = candidates + z.room();
+    log_s = reinterpret_cast<double*>(best + (z.top + 1) / 2 * 2 * ctas);
+    kth = reinterpret_cast<A*>(log_s + 2);
+    picked = reinterpret_cast<int*>(kth + (kWarps + 3) / 4 * 4);
+    count = picked + z.batches();
+    histogram = reinterpret_cast<unsigned*>(count + 4);
+    maxima = reinterpret_cast<A*>(histogram + kHistogram);
+    batch_max = reinterpret_cast<uint16_t*>(maxima);
   }
 };
 
@@ -181,28 +250,62 @@ struct Share {
   }
 };
 
+// The q-th largest of a warp's numbers (1 <= q <= 32): they are sorted, in every lane its own.
 template <typename A>
-__device__ __forceinline__ A number_of(A x) {  // NaN in the order of -infinity
-  return x == x ? x : lowest<A>();
+__device__ __forceinline__ A largest_of_warp(A v, int q) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int d = size / 2; d; d /= 2) {
+      const A other = __shfl_xor_sync(0xffffffffu, v, d);
+      const bool first = (lane & d) == 0, down = (lane & size) == 0;
+      v = first == down ? max_acc(v, other) : min_acc(v, other);
+    }
+  return __shfl_sync(0xffffffffu, v, q - 1);
 }
 
-// The row's `top` best elements of this CTA's share to space.best, in order; elements that are not
-// there (a share of fewer) stand at the end, at an impossible place. kGroup: vectors to a maximum (32
-// or 1), `groups` of them. The maxima are written and the threads have met.
+// How many of each warp's lanes are to reach the bound: over the warps whose lanes all have a vector;
+// 0 where they are too few to give one.
+template <int kThreads, typename T>
+__device__ __forceinline__ int quota_of(const RowView<T>& r, const Place<kThreads>& place, int top,
+                                        int& warps) {
+  const int own = min(max(r.vectors - place.cta * kBatch * kThreads, 0), kThreads);
+  warps = own / 32;
+  const int q = warps > 0 ? (top + warps - 1) / warps : 33;
+  return q <= 32 ? q : 0;
+}
+
+// The largest elements of this CTA's share by groups, for any data: to space.candidates, not in order;
+// returns how many.
 template <int kGroup, int kThreads, typename T, typename A>
-__device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThreads>& place, int top,
-                                           int groups, const TopSpace<A>& space) {
-  constexpr int E = RowView<T>::E;
+__device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kThreads> place, int top,
+                                             int room, const TopSpace<A, kThreads> space) {
+  constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
   const Team<kThreads> team{place.tid};
   const Share<kThreads> share{place.cta, place.ctas};
-  const int room = 8 * top;
-  Cut<A> cut{0, 0xffffffffu};
+  int groups = 0;
+  for (int tile = place.cta * kTile, l = 0; tile < r.vectors; tile += place.ctas * kTile, l += kTile) {
+    for (int i = 0; i < kBatch; ++i) {
+      const int v = tile + i * kThreads + place.tid;
+      const uint4 q[1] = {v < r.vectors ? load_vector(r, v) : no_vector<T>()};
+      A most = vector_max<T>(q);
+      if (kGroup == 1) {
+        space.maxima[l + i * kThreads + place.tid] = most;
+      } else {
+        most = max_of_lanes<32>(most);
+        if (place.tid % 32 == 0) space.maxima[(l + i * kThreads + place.tid) / 32] = most;
+      }
+    }
+    groups += kTile / kGroup;
+  }
   if (team.tid < 2) space.count[team.tid] = 0;
+  team.sync();
+  Cut<A> cut{0, 0xffffffffu};
   if (groups > top)
     cut = find_cut<2, kThreads, A>(
         team, groups, top, [&](int i) { return ordered(space.maxima[i]); },
         [](int i) { return static_cast<uint32_t>(i); }, space.histogram);
-  team.sync();
   for (int i = team.tid; i < groups; i += kThreads)
     if (cut.takes(ordered(space.maxima[i]), static_cast<uint32_t>(i)))
       space.picked[atomicAdd(space.count + 1, 1)] = i;
@@ -211,12 +314,11 @@ __device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThr
   const auto add = [&](int v, KeyOf<A> least) {  // a vector's elements from `least` on
     A x[E];
     unpack<T>(load_vector(r, v), x);
-#pragma unroll
     for (int j = 0; j < E; ++j) {
       x[j] = number_of(x[j]);
       if (ordered(x[j]) >= least) {
         const int slot = atomicAdd(space.count, 1);
-        if (slot < room) space.candidates[slot] = {x[j], r.element(v) + j};
+        if (slot < room) space.candidates[slot] = Ranked<A>(x[j], r.element(v) + j);
       }
     }
   };
@@ -225,13 +327,14 @@ __device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThr
     if (v < r.vectors) add(v, cut.key);
   }
   team.sync();
-  if (kGroup > 1 && space.count[0] > room) {
-    // more than 8 elements each: the best vectors of these groups first
+  const int found = space.count[0];
+  team.sync();  // every thread has read it
+  if (kGroup > 1 && found > room) {  // the best vectors of these groups first
     for (int i = team.tid; i < picked * kGroup; i += kThreads) {
       const int v = share.vector(space.picked[i / kGroup] * kGroup + i % kGroup);
       A most = lowest<A>();
       if (v < r.vectors) {
-        uint4 q[1] = {load_vector(r, v)};
+        const uint4 q[1] = {load_vector(r, v)};
         most = vector_max<T>(q);
       }
       space.maxima[i] = most;
@@ -242,7 +345,9 @@ __device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThr
     };
     if (team.tid == 0) space.count[0] = 0;
     team.sync();
-    const Cut<A> best = find_cut<4, kThreads, A>(team, picked * kGroup, top, key, at, space.histogram);
+    Cut<A> best{0, 0xffffffffu};
+    if (picked * kGroup > top)
+      best = find_cut<4, kThreads, A>(team, picked * kGroup, top, key, at, space.histogram);
     for (int i = team.tid; i < picked * kGroup; i += kThreads) {
       const int v = share.vector(static_cast<int>(at(i)));
       if (v < r.vectors && best.takes(key(i), at(i))) add(v, 0);
@@ -252,23 +357,86 @@ __device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThr
   const int body = space.count[0];
   if (place.cta == 0) {
     for (int e = team.tid; e < r.edges; e += kThreads)
-      space.candidates[body + e] = {number_of(to_acc(r.x[r.edge(e)])), r.edge(e)};
+      space.candidates[body + e] = Ranked<A>(number_of(to_acc(r.x[r.edge(e)])), r.edge(e));
     team.sync();
   }
   const int n = body + (place.cta == 0 ? r.edges : 0);
-  Cut<A> last{0, 0xffffffffu};
-  const auto key = [&](int i) { return ordered(space.candidates[i].value); };
-  const auto at = [&](int i) { return static_cast<uint32_t>(space.candidates[i].at); };
-  if (n > top) last = find_cut<4, kThreads, A>(team, n, top, key, at, space.histogram);
-  for (int i = team.tid; i < n; i += kThreads) {
-    if (!last.takes(key(i), at(i))) continue;
-    const Element<A> own = space.candidates[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += space.candidates[j].before(own);
-    space.best[rank] = own;
-  }
-  for (int i = n + team.tid; i < top; i += kThreads) space.best[i] = {lowest<A>(), 0x7fffffff};
+  if (n <= 256) return n;
+  // the best of them to the front
+  const auto key = [&](int i) { return space.candidates[i].number(); };
+  const auto at = [&](int i) { return static_cast<uint32_t>(space.candidates[i].at()); };
+  const Cut<A> last = find_cut<4, kThreads, A>(team, n, top, key, at, space.histogram);
+  if (team.tid == 0) space.count[1] = 0;
   team.sync();
+  for (int i = team.tid; i < n; i += kThreads)
+    if (last.takes(key(i), at(i))) space.best[atomicAdd(space.count + 1, 1)] = space.candidates[i];
+  team.sync();
+  for (int i = team.tid; i < top; i += kThreads) space.candidates[i] = space.best[i];
+  team.sync();
+  return top;
+}
+
+// The elements of this CTA's share among which its `top` best are, to space.candidates; returns how
+// many. own: the thread's largest; edge: its single element. The maxima, the warps' bounds and counts
+// of 0 are written and the threads have met.
+template <int kThreads, typename T, typename A>
+__device__ __forceinline__ int choose_top(const RowView<T>& r, const Place<kThreads>& place,
+                                          const TopSizes& z, A own, A edge,
+                                          const TopSpace<A, kThreads>& space) {
+  constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
+  const Team<kThreads> team{place.tid};
+  const Share<kThreads> share{place.cta, place.ctas};
+  int warps;
+  A bound = lowest<A>();
+  if (quota_of(r, place, z.top, warps) > 0) {
+    bound = space.kth[0];
+    for (int i = 1; i < warps; ++i) bound = min_acc(bound, space.kth[i]);
+  }
+  const auto add = [&](A x, int at) {
+    const int slot = atomicAdd(space.count, 1);
+    if (slot < z.room()) space.candidates[slot] = Ranked<A>(x, at);
+  };
+  if (own >= bound) {
+    for (int tile = place.cta * kTile, j = 0; tile < r.vectors; tile += place.ctas * kTile, ++j) {
+      const A most = static_cast<A>(from_upper_half(space.batch_max[j * kThreads + team.tid]));
+      if (tile + team.tid >= r.vectors || !(most >= bound)) continue;
+      const int slot = atomicAdd(space.count + 1, 1);
+      if (slot < z.batches()) space.picked[slot] = j * kThreads + team.tid;
+    }
+  }
+  if (place.edge() < r.edges && number_of(edge) >= bound) add(number_of(edge), r.edge(place.edge()));
+  team.sync();
+  const int picked = space.count[1];
+  if (picked <= z.batches()) {
+    for (int i = team.tid; i < picked * kBatch; i += kThreads) {
+      const int batch = space.picked[i / kBatch];
+      const int v = share.vector(batch / kThreads * kTile + i % kBatch * kThreads + batch % kThreads);
+      if (v >= r.vectors) continue;
+      A x[E];
+      unpack<T>(load_vector(r, v), x);
+#pragma unroll
+      for (int c = 0; c < E; ++c)
+        if (number_of(x[c]) >= bound) add(number_of(x[c]), r.element(v) + c);
+    }
+    team.sync();
+    if (space.count[0] <= z.room()) return space.count[0];
+  }
+  team.sync();  // the counts have been read
+  return z.whole ? choose_by_groups<32>(r, place, z.top, z.room(), space)
+                 : choose_by_groups<1>(r, place, z.top, z.room(), space);
+}
+
+// Calls fn(rank, element) for the `top` best of the candidates, each by one thread.
+template <int kThreads, typename A, typename F>
+__device__ __forceinline__ void rank_candidates(int tid, int n, int top,
+                                                const TopSpace<A, kThreads>& space, const F& fn) {
+  for (int i = tid; i < n; i += kThreads) {
+    const Ranked<A> own = space.candidates[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += space.candidates[j].before(own);
+    if (rank < top) fn(rank, own);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -276,60 +444,65 @@ __device__ __forceinline__ void choose_top(const RowView<T>& r, const Place<kThr
 
 template <typename A>
 struct ScoresArgs {
-  int top, groups;     // of a CTA
+  TopSizes sizes;
   A *logps, *entropy;  // logps may be NULL (no targets)
   A* top_logps;
   int64_t* top_ids;
   A* stats;  // NULL, or per row the base, the sum and the mean of z
 };
 
+// By one thread; returns log s.
 template <typename A>
-__device__ __forceinline__ void write_scores(const ScoresArgs<A>& p, int64_t r, A logit,
-                                             const Scored<A>& part, double inv_temp) {
-  const double s = part.s, mean = part.u * unit_of(part.u) / s;
-  if (p.logps) p.logps[r] = static_cast<A>(logp_of(logit, Part<A>{part.m, part.s}, inv_temp));
-  p.entropy[r] = static_cast<A>(log(s) - mean);
+__device__ __forceinline__ double write_scores(const ScoresArgs<A>& p, int64_t r, A logit,
+                                               const Scored<A>& part, double inv_temp) {
+  const double s = part.s, mean = part.u * unit_of(part.u) / s, log_s = log(s);
+  if (p.logps)
+    p.logps[r] = static_cast<A>(
+        (static_cast<double>(logit) - static_cast<double>(base_of(part.m))) * inv_temp - log_s);
+  p.entropy[r] = static_cast<A>(log_s - mean);
   if (p.stats) {
     p.stats[3 * r] = base_of(part.m);
     p.stats[3 * r + 1] = part.s;
     p.stats[3 * r + 2] = static_cast<A>(mean);
   }
+  return log_s;
 }
 
-// One pass over a row by a CTA, or where rows are few by a cluster. kGroup: 0 where no alternatives
-// are asked for, else the vectors to a maximum.
-template <typename T, typename A, int kThreads, int kGroup>
-__global__ void __launch_bounds__(kThreads)
-    scores_kernel(Rows a, ScoresArgs<A> p, double inv_temp, A k) {
-  constexpr int kTile = kBatch * kThreads, kWarps = kThreads / 32;
-  extern __shared__ uint4 shared[];
-  const Place<kThreads> place;
+// A row that is left out.
+template <int kThreads, typename A>
+__device__ __forceinline__ void write_no_scores(const Rows& a, const ScoresArgs<A>& p,
+                                                const Place<kThreads>& place) {
   const int64_t r = place.row;
-  const int64_t target = a.targets ? a.targets[r] : 0;
-  if (a.targets && target == a.ignore) {
-    if (place.first()) {
-      p.logps[r] = A(0);
-      p.entropy[r] = A(0);
-      if (p.stats) p.stats[3 * r + 1] = A(kLeftOut);
-    }
-    if (place.cta == 0)
-      for (int i = place.tid; i < p.top; i += kThreads) {
-        p.top_logps[r * p.top + i] = A(0);
-        p.top_ids[r * p.top + i] = a.ignore;
-      }
-    return;
+  const int top = p.sizes.top;
+  if (place.first()) {
+    p.logps[r] = A(0);
+    p.entropy[r] = A(0);
+    if (p.stats) p.stats[3 * r + 1] = A(kLeftOut);
   }
-  cluster_started(place.ctas);
+  if (place.cta == 0)
+    for (int i = place.tid; i < top; i += kThreads) {
+      p.top_logps[r * top + i] = A(0);
+      p.top_ids[r * top + i] = a.ignore;
+    }
+}
+
+// One pass over a row by a warp, a CTA or a cluster; its alternatives if kTop.
+template <bool kTop, int kThreads, typename T, typename A>
+__device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p, double inv_temp, A k,
+                                           const Place<kThreads>& place, int64_t target, void* shared) {
+  constexpr int kTile = kBatch * kThreads;
+  const Team<kThreads> team{place.tid};
+  const int64_t r = place.row;
   const T* x = row_at<T>(a, r);
   const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
   A logit = A(0);
   if (place.first() && a.targets) logit = target_logit<T, A>(x, a.vocab, target);
-  const TopSpace<A> space(shared, p.top, p.groups, place.ctas);
+  const TopSpace<A, kThreads> space(shared, p.sizes, place.ctas);
+  if (kTop && team.tid < 2) space.count[team.tid] = 0;
 
   const A edge = place.edge() < view.edges ? to_acc(x[view.edge(place.edge())]) : lowest<A>();
   Scored<A> part{lowest<A>(), A(0), A(0)};
-  int local = 0, groups = 0;
-  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile) {
+  for (int tile = place.cta * kTile, j = 0; tile < view.vectors; tile += place.ctas * kTile, ++j) {
     const int v = tile + place.tid;
     uint4 q[kBatch];
     if (tile + kTile <= view.vectors) {
@@ -339,21 +512,8 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < kBatch; ++i)
         q[i] = v + i * kThreads < view.vectors ? load_vector(view, v + i * kThreads) : no_vector<T>();
     }
-    A m = part.m;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const uint4 one[1] = {q[i]};
-      A most = vector_max<T>(one);
-      m = max_acc(m, most);
-      if constexpr (kGroup == 1) space.maxima[local + i * kThreads + place.tid] = most;
-      if constexpr (kGroup == 32) {
-        most = max_of_lanes<32>(most);
-        if ((place.tid & 31) == 0)
-          space.maxima[(local + i * kThreads) / 32 + place.tid / 32] = most;
-      }
-    }
-    local += kTile;
-    groups += kBatch * (kGroup == 32 ? kWarps : kThreads);
+    const A most = vector_max<T>(q), m = max_acc(part.m, most);
+    if constexpr (kTop) space.batch_max[j * kThreads + place.tid] = upper_half(most);
     move_base(part, m, k);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -363,6 +523,15 @@ __global__ void __launch_bounds__(kThreads)
       add_scores(z, part.s, part.u);
     }
   }
+  const A own = part.m;
+  if constexpr (kTop) {
+    int warps;
+    const int quota = quota_of(view, place, p.sizes.top, warps);
+    if (quota > 0) {
+      const A kth = largest_of_warp(own, quota);
+      if (team.tid % 32 == 0) space.kth[team.tid / 32] = kth;
+    }
+  }
   move_base(part, max_acc(part.m, edge), k);
   if (place.edge() < view.edges) {
     const A z = max_nan(mul_rn(edge - base_of(part.m), k), least_argument(k)), e = exp_of(z);
@@ -370,36 +539,43 @@ __global__ void __launch_bounds__(kThreads)
     part.u += e * z;
   }
   part = join_scores_of_warps<kThreads>(join_scores<32>(part, k), k);
-  if (place.first()) write_scores(p, r, logit, part, inv_temp);
-  if constexpr (kGroup > 0) {
-    choose_top<kGroup>(view, place, p.top, groups, space);
-    const auto write = [&](int rank, const Element<A>& e) {
-      p.top_logps[r * p.top + rank] =
-          static_cast<A>(logp_of(e.value, Part<A>{part.m, part.s}, inv_temp));
-      p.top_ids[r * p.top + rank] = e.at;
+  if constexpr (kThreads == 32) team.sync();
+  if (place.first()) {
+    const double log_s = write_scores(p, r, logit, part, inv_temp);
+    if (kTop) *space.log_s = log_s;
+  }
+  if constexpr (kTop) {
+    const int top = p.sizes.top;
+    const int n = choose_top(view, place, p.sizes, own, edge, space);
+    const double base = base_of(part.m);
+    const auto write = [&](int rank, const Ranked<A>& e) {
+      p.top_logps[r * top + rank] =
+          static_cast<A>((static_cast<double>(e.value()) - base) * inv_temp - *space.log_s);
+      p.top_ids[r * top + rank] = e.at();
     };
     if (place.ctas == 1) {
-      for (int i = place.tid; i < p.top; i += kThreads) write(i, space.best[i]);
-    } else {
+      rank_candidates<kThreads>(place.tid, n, top, space, write);
+    } else if constexpr (kThreads > 32) {
       // the CTAs' lists to the first CTA, where an element's rank is its place in its own list and
       // what of the others is before it
       auto cluster = cg::this_cluster();
-      Element<A>* to = of_peer(space.best, 0, false) + place.cta * p.top;
-      if (place.cta != 0)
-        for (int i = place.tid; i < p.top; i += kThreads) to[i] = space.best[i];
+      Ranked<A>* to = of_peer(space.best, 0, false) + place.cta * top;
+      rank_candidates<kThreads>(place.tid, n, top, space,
+                                [&](int rank, const Ranked<A>& e) { to[rank] = e; });
+      for (int i = n + place.tid; i < top; i += kThreads) to[i] = Ranked<A>(lowest<A>(), kNowhere);
       cluster.sync();
       if (place.cta == 0)
-        for (int i = place.tid; i < p.top * place.ctas; i += kThreads) {
-          const Element<A> own = space.best[i];
-          const int list = i / p.top;
-          int rank = i % p.top;
+        for (int i = place.tid; i < top * place.ctas; i += kThreads) {
+          const Ranked<A> own_element = space.best[i];
+          const int list = i / top;
+          int rank = i % top;
           for (int other = 0; other < place.ctas; ++other) {
             if (other == list) continue;
-            const Element<A>* of = space.best + other * p.top;
-            int low = 0, high = p.top;  // the first that is not before it
+            const Ranked<A>* of = space.best + other * top;
+            int low = 0, high = top;  // the first that is not before it
             while (low < high) {
               const int mid = (low + high) / 2;
-              if (of[mid].before(own)) {
+              if (of[mid].before(own_element)) {
                 low = mid + 1;
               } else {
                 high = mid;
@@ -407,10 +583,41 @@ __global__ void __launch_bounds__(kThreads)
             }
             rank += low;
           }
-          if (rank < p.top && own.at != 0x7fffffff) write(rank, own);
+          if (rank < top && own_element.at() != kNowhere) write(rank, own_element);
         }
     }
   }
+}
+
+template <typename T, typename A, int kThreads, bool kTop>
+__global__ void __launch_bounds__(kThreads)
+    scores_kernel(Rows a, ScoresArgs<A> p, double inv_temp, A k) {
+  extern __shared__ uint4 shared[];
+  const Place<kThreads> place;
+  const int64_t target = a.targets ? a.targets[place.row] : 0;
+  if (a.targets && target == a.ignore) {
+    write_no_scores(a, p, place);
+    return;
+  }
+  cluster_started(place.ctas);
+  scores_row<kTop, kThreads, T>(a, p, inv_temp, k, place, target, shared);
+}
+
+// Short rows: a warp to a row.
+template <typename T, typename A, bool kTop>
+__global__ void __launch_bounds__(32 * kRowWarps)
+    scores_warp_kernel(Rows a, ScoresArgs<A> p, double inv_temp, A k) {
+  extern __shared__ uint4 shared[];
+  const Place<32> place;
+  if (place.row >= a.rows) return;
+  const int64_t target = a.targets ? a.targets[place.row] : 0;
+  if (a.targets && target == a.ignore) {
+    write_no_scores(a, p, place);
+    return;
+  }
+  char* own = reinterpret_cast<char*>(shared) +
+              static_cast<int>(threadIdx.x / 32) * TopSpace<A, 32>::bytes(p.sizes, 1);
+  scores_row<kTop, 32, T>(a, p, inv_temp, k, place, target, own);
 }
 
 // The gradient of c log p_y + h entropy, both divided by t: exp(z) (alpha + beta z), and c at the
@@ -479,48 +686,63 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------------------------
 // Host side
 
-template <typename T, int kGroup>
-int launch_scores(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double inv_temp, int ctas,
+// What there is to choose from where `threads` threads and `ctas` CTAs take a row.
+template <typename T>
+TopSizes top_sizes(int top, int64_t vectors, int threads, int ctas) {
+  const int64_t tile = int64_t{kBatch} * threads, tiles = (vectors + tile - 1) / tile;
+  const int64_t share = (tiles + ctas - 1) / ctas;
+  const bool whole = share * tile / 32 >= 2 * top;
+  const int64_t groups = whole ? share * tile / 32 : share * tile;
+  return {top, static_cast<int>(share), static_cast<int>(groups), whole};
+}
+
+template <typename T, bool kTop>
+int launch_scores(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double inv_temp,
                   cudaStream_t st) {
   using A = typename AccOf<T>::type;
   constexpr int kThreads = 256;
-  const auto kernel = scores_kernel<T, A, kThreads, kGroup>;
-  const size_t shared = kGroup ? TopSpace<A>::bytes(p.top, p.groups, ctas) : 0;
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  const int top = p.sizes.top, sms = sm_count();
+  const A k = exp_factor(A(0), inv_temp);
+  // a warp's lanes are enough to bound up to 32 alternatives
+  p.sizes = top_sizes<T>(top, vectors, 32, 1);
+  const int by_warp = kTop ? kRowWarps * TopSpace<A, 32>::bytes(p.sizes, 1) : 0;
+  if (top <= 32 && by_warps(a.rows, vectors, 2048, sms) && by_warp <= kSharedForTop) {
+    const auto kernel = scores_warp_kernel<T, A, kTop>;
+    const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSharedForTop);
+    if (rc) return rc;
+    return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps, by_warp,
+                           false, st, "scores_warp_kernel launch", a, p, inv_temp, k);
+  }
+  int ctas = ctas_for(a.rows, vectors, kThreads, sms);
+  const auto fits = [&] {
+    p.sizes = top_sizes<T>(top, vectors, kThreads, ctas);
+    return !kTop || (p.sizes.groups < 1 << 16 && p.sizes.tiles < 1 << 15 &&
+                     TopSpace<A, kThreads>::bytes(p.sizes, ctas) <= kSharedForTop);
+  };
+  while (!fits() && ctas < 8) ctas *= 2;
+  if (!fits())
+    return report_error(TISO_ERR_ARGUMENT, "a vocabulary too large for top alternatives");
+  const auto kernel = scores_kernel<T, A, kThreads, kTop>;
   const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSharedForTop);
   if (rc) return rc;
+  const size_t shared = kTop ? TopSpace<A, kThreads>::bytes(p.sizes, ctas) : 0;
   return launch_clusters(kernel, a.rows, ctas, kThreads, shared, false, st, "scores_kernel launch", a,
-                         p, inv_temp, exp_factor(A(0), inv_temp));
+                         p, inv_temp, k);
 }
 
 template <typename T>
 int run_scores(const Rows& a, int top, double inv_temp, void* logps, void* entropy, void* top_logps,
                int64_t* top_ids, void* stats, cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  constexpr int kTile = kBatch * 256;
-  const int64_t vectors = a.vocab / RowView<T>::E, tiles = (vectors + kTile - 1) / kTile;
-  int ctas = ctas_for(a.rows, vectors, 256, sm_count());
-  ScoresArgs<A> p{top,
-                  0,
-                  static_cast<A*>(logps),
-                  static_cast<A*>(entropy),
-                  static_cast<A*>(top_logps),
-                  top_ids,
-                  static_cast<A*>(stats)};
-  if (top == 0) return launch_scores<T, 0>(a, p, inv_temp, ctas, st);
-  const auto share = [&] { return (tiles + ctas - 1) / ctas * kTile; };  // vectors of a CTA
-  // maxima of whole groups of 32 vectors where there are enough of them to choose from
-  const auto whole = [&] { return share() / 32 >= 2 * top; };
-  const auto fits = [&] {
-    const int64_t groups = whole() ? share() / 32 : share();
-    return groups < 1 << 16 &&
-           TopSpace<A>::bytes(top, static_cast<int>(groups), ctas) <= kSharedForTop;
-  };
-  while (ctas < 8 && !fits()) ctas *= 2;
-  if (!fits())
-    return report_error(TISO_ERR_ARGUMENT, "a vocabulary too large for top alternatives");
-  p.groups = static_cast<int>(whole() ? share() / 32 : share());
-  return whole() ? launch_scores<T, 32>(a, p, inv_temp, ctas, st)
-                 : launch_scores<T, 1>(a, p, inv_temp, ctas, st);
+  ScoresArgs<A> p{};
+  p.sizes.top = top;
+  p.logps = static_cast<A*>(logps);
+  p.entropy = static_cast<A*>(entropy);
+  p.top_logps = static_cast<A*>(top_logps);
+  p.top_ids = top_ids;
+  p.stats = static_cast<A*>(stats);
+  return top ? launch_scores<T, true>(a, p, inv_temp, st) : launch_scores<T, false>(a, p, inv_temp, st);
 }
 
 template <typename T>
