@@ -7,15 +7,18 @@
 // neither a difference of large numbers (s >= 1, u <= 0). Parts of a row join as for s alone: with
 // d = (m1 - M) / t, s1 and u1 become s1 exp(d) and exp(d) (u1 + d s1).
 //
-// Top alternatives: each thread keeps the maximum of every batch of vectors it reads. Of the maxima that
-// the lanes of a warp have seen, the q-th largest is taken, q = top / warps rounded up: the least of
-// these over the warps is reached by `top` elements at least, so that the alternatives are among the
-// elements that reach it. The batches whose maximum does are read again, and what is found there, a
-// few times `top` elements as a rule, is ranked. Where it is more than there is room for (equal
-// logits, rows in order) the selection is by groups instead: the row is read again for the maxima of
-// groups of neighbouring vectors; the `top` best groups (equal maxima: the first) hold the top
-// elements, for each of the others has an element in each of these before it; and so on with their
-// vectors and elements, each step an exact selection that no data makes longer.
+// Top alternatives: the upper 16 bits of a number's key (its order as an integer) make it coarse. The
+// pass leaves the coarse maximum of each unit of vectors in shared memory and finds a bound that `top`
+// units reach at least: the alternatives are then among the elements that reach it. The units that do
+// are read again, and what is found there, once or twice `top` elements as a rule, is sorted. The bound
+// is the least of what the warps find for themselves, the q-th largest of their lanes' maxima, q = top
+// / warps rounded up; where a warp alone has a row and q is large the top-th largest of the units'
+// maxima, by bisection.
+// Where more elements reach the bound than there is room for (equal logits, rows in order) the
+// selection is by groups instead: the row is read again for the maxima of groups of neighbouring
+// vectors; the `top` best groups (equal maxima: the first) hold the top elements, for each of the
+// others has an element in each of these before it; and so on with their vectors and elements, each
+// step an exact selection that no data makes longer.
 #include "rows.cuh"
 #include "select.cuh"
 
@@ -44,8 +47,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN where eithe
   return r;
 }
 __device__ __forceinline__ double max_nan(double a, double b) { return a != a || a > b ? a : b; }
-__device__ __forceinline__ float min_acc(float a, float b) { return fminf(a, b); }
-__device__ __forceinline__ double min_acc(double a, double b) { return fmin(a, b); }
 __device__ __forceinline__ float exp_of(float a) { return exp2_of(a); }
 __device__ __forceinline__ double exp_of(double a) { return exp(a); }
 
@@ -185,58 +186,60 @@ __device__ __forceinline__ A number_of(A x) {  // NaN in the order of -infinity
   return x == x ? x : lowest<A>();
 }
 
-// At least x, in the upper half of a float.
-__device__ __forceinline__ uint16_t upper_half(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return static_cast<uint16_t>((b >> 31 ? b : b + 0xffffu) >> 16);
+// The upper 16 bits of a number's key.
+__device__ __forceinline__ uint32_t coarse(float x) { return ordered(x) >> 16; }
+__device__ __forceinline__ uint32_t coarse(double x) {
+  return static_cast<uint32_t>(ordered(x) >> 48);
 }
-__device__ __forceinline__ uint16_t upper_half(double x) { return upper_half(__double2float_ru(x)); }
-__device__ __forceinline__ float from_upper_half(uint16_t h) {
-  return __uint_as_float(static_cast<uint32_t>(h) << 16);
-}
+
+constexpr int kMostUnits = 16;  // of a warp's lane
 
 // What the threads that work on a row have to choose from (a cluster's CTAs each for their share).
 struct TopSizes {
   int top, tiles;  // of this CTA's share, at most
   int groups;      // and groups of vectors
   bool whole;      // 32 vectors to a group, else one
+  bool fine;       // a unit is one vector, else a batch of a thread's
 
-  __host__ __device__ int room() const { return 8 * (top + 32) + 32; }
-  __host__ __device__ int batches() const { return 4 * top + 64; }
+  __host__ __device__ int rows() const { return fine ? tiles * kBatch : tiles; }  // of units
+  __host__ __device__ int room() const { return 3 * top + 128; }
+  __host__ __device__ int units() const { return (3 * top + 99) / 4 * 4; }
+  // of a selection by groups
+  __host__ __device__ int numbers() const { return whole && groups < 32 * top ? 32 * top : groups; }
 };
 
 // Their shared memory.
 template <typename A, int kThreads>
 struct TopSpace {
   static constexpr int kWarps = kThreads / 32;
-  Ranked<A>* candidates;  // room
-  Ranked<A>* best;        // top; in the first CTA of a cluster top for each CTA
+  Ranked<A>* candidates;  // room, and up to a multiple of 32
+  Ranked<A>* best;        // in the first CTA of a cluster top for each CTA
   double* log_s;
-  A* kth;                 // of each warp
-  int* picked;            // batches, or top groups
+  unsigned* kth;          // of each warp
+  int* picked;            // units, or top groups
   int* count;             // 2: candidates, picked
   unsigned* histogram;
-  uint16_t* batch_max;    // tiles x threads
-  A* maxima;              // of the groups, 32 top at least: in the same place
+  uint16_t* unit_max;     // rows of units x threads
+  A* maxima;              // of the groups: in the same place
 
+  static __host__ __device__ int rounded(const TopSizes& z) { return (z.room() + 31) / 32 * 32; }
   static __host__ __device__ int bytes(const TopSizes& z, int ctas) {
-    const int numbers = z.groups > 32 * z.top ? z.groups : 32 * z.top;
-    const int maxima = numbers * static_cast<int>(sizeof(A)), batches = z.tiles * kThreads * 2;
-    return static_cast<int>(sizeof(Ranked<A>)) * (z.room() + (z.top + 1) / 2 * 2 * ctas) + 16 +
-           static_cast<int>(sizeof(A)) * ((kWarps + 3) / 4 * 4) + 4 * (z.batches() + 4 + kHistogram) +
-           ((maxima > batches ? maxima : batches) + 15) / 16 * 16;
+    const int maxima = z.numbers() * static_cast<int>(sizeof(A)), units = z.rows() * kThreads * 2;
+    return static_cast<int>(sizeof(Ranked<A>)) * (rounded(z) + (z.top + 1) / 2 * 2 * ctas) + 16 +
+           4 * ((kWarps + 3) / 4 * 4 + z.units() + 4 + kHistogram) +
+           ((maxima > units ? maxima : units) + 15) / 16 * 16;
   }
 
   __device__ TopSpace(void* at, const TopSizes& z, int ctas) {
     candidates = static_cast<Ranked<A>*>(at);
-    best = candidates + z.room();
+    best = candidates + rounded(z);
     log_s = reinterpret_cast<double*>(best + (z.top + 1) / 2 * 2 * ctas);
-    kth = reinterpret_cast<A*>(log_s + 2);
+    kth = reinterpret_cast<unsigned*>(log_s + 2);
     picked = reinterpret_cast<int*>(kth + (kWarps + 3) / 4 * 4);
-    count = picked + z.batches();
+    count = picked + z.units();
     histogram = reinterpret_cast<unsigned*>(count + 4);
     maxima = reinterpret_cast<A*>(histogram + kHistogram);
-    batch_max = reinterpret_cast<uint16_t*>(maxima);
+    unit_max = reinterpret_cast<uint16_t*>(maxima);
   }
 };
 
@@ -250,23 +253,55 @@ struct Share {
   }
 };
 
-// The q-th largest of a warp's numbers (1 <= q <= 32): they are sorted, in every lane its own.
-template <typename A>
-__device__ __forceinline__ A largest_of_warp(A v, int q) {
+// The q-th largest of a warp's numbers (1 <= q <= 32): by taking out the largest, or by sorting.
+__device__ __forceinline__ unsigned largest_of_warp(unsigned v, int q) {
   const int lane = threadIdx.x & 31;
+  if (q <= 6) {
+    unsigned most = 0;
+    for (int i = 0; i < q; ++i) {
+      most = __reduce_max_sync(0xffffffffu, v);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, v == most)) - 1) v = 0;
+    }
+    return most;
+  }
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int d = size / 2; d; d /= 2) {
-      const A other = __shfl_xor_sync(0xffffffffu, v, d);
+      const unsigned other = __shfl_xor_sync(0xffffffffu, v, d);
       const bool first = (lane & d) == 0, down = (lane & size) == 0;
-      v = first == down ? max_acc(v, other) : min_acc(v, other);
+      v = first == down ? max(v, other) : min(v, other);
     }
   return __shfl_sync(0xffffffffu, v, q - 1);
 }
 
-// How many of each warp's lanes are to reach the bound: over the warps whose lanes all have a vector;
-// 0 where they are too few to give one.
+// A number that `top` of a warp's units' maxima reach, 0 where they are fewer: the top-th largest, or
+// less where no more reach it.
+__device__ __forceinline__ unsigned bound_of_warp(const uint16_t* unit_max, int rows, int top) {
+  unsigned v[kMostUnits];
+#pragma unroll
+  for (int i = 0; i < kMostUnits; ++i)
+    v[i] = i < rows ? unit_max[32 * i + (threadIdx.x & 31)] : 0u;
+  unsigned bound = 0;
+#pragma unroll 1
+  for (int bit = 15; bit >= 0; --bit) {
+    const unsigned more = bound | 1u << bit;
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < kMostUnits; ++i) reach += v[i] >= more;
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (reach >= top) bound = more;
+    if (reach == top) break;
+  }
+  return bound;
+}
+
+// Up to so many alternatives a warp alone takes its bound from its lanes: 200000 x 2048 bf16, 1 and 20
+// of them, 256 and 518 us so, 472 and 552 us by bisection over the units; 32: 2211 and 826.
+constexpr int kMostByLanes = 16;
+
+// How many of each warp's lanes are to reach the bound, over the warps whose lanes all have a vector;
+// 0 where these are too few to give one.
 template <int kThreads, typename T>
 __device__ __forceinline__ int quota_of(const RowView<T>& r, const Place<kThreads>& place, int top,
                                         int& warps) {
@@ -276,11 +311,11 @@ __device__ __forceinline__ int quota_of(const RowView<T>& r, const Place<kThread
   return q <= 32 ? q : 0;
 }
 
-// The largest elements of this CTA's share by groups, for any data: to space.candidates, not in order;
-// returns how many.
+// The `top` best elements of this CTA's share (all, if fewer), for any data: to space.candidates, not in
+// order; returns how many.
 template <int kGroup, int kThreads, typename T, typename A>
 __device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kThreads> place, int top,
-                                             int room, const TopSpace<A, kThreads> space) {
+                                             const TopSpace<A, kThreads> space) {
   constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
   const Team<kThreads> team{place.tid};
   const Share<kThreads> share{place.cta, place.ctas};
@@ -301,35 +336,20 @@ __device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kTh
   }
   if (team.tid < 2) space.count[team.tid] = 0;
   team.sync();
-  Cut<A> cut{0, 0xffffffffu};
-  if (groups > top)
-    cut = find_cut<2, kThreads, A>(
-        team, groups, top, [&](int i) { return ordered(space.maxima[i]); },
-        [](int i) { return static_cast<uint32_t>(i); }, space.histogram);
-  for (int i = team.tid; i < groups; i += kThreads)
-    if (cut.takes(ordered(space.maxima[i]), static_cast<uint32_t>(i)))
-      space.picked[atomicAdd(space.count + 1, 1)] = i;
-  team.sync();
-  const int picked = space.count[1];
-  const auto add = [&](int v, KeyOf<A> least) {  // a vector's elements from `least` on
-    A x[E];
-    unpack<T>(load_vector(r, v), x);
-    for (int j = 0; j < E; ++j) {
-      x[j] = number_of(x[j]);
-      if (ordered(x[j]) >= least) {
-        const int slot = atomicAdd(space.count, 1);
-        if (slot < room) space.candidates[slot] = Ranked<A>(x[j], r.element(v) + j);
-      }
-    }
+  // puts down the places of the numbers that are among the `top` largest of n
+  const auto choose = [&](int n, const auto& key, const auto& at, int* places, int* count) {
+    Cut<A> cut{0, 0xffffffffu};
+    if (n > top) cut = find_cut<4, kThreads, A>(team, n, top, key, at, space.histogram);
+    for (int i = team.tid; i < n; i += kThreads)
+      if (cut.takes(key(i), at(i))) places[atomicAdd(count, 1)] = static_cast<int>(at(i));
+    team.sync();
+    return min(n, top);
   };
-  for (int i = team.tid; i < picked * kGroup; i += kThreads) {
-    const int v = share.vector(space.picked[i / kGroup] * kGroup + i % kGroup);
-    if (v < r.vectors) add(v, cut.key);
-  }
-  team.sync();
-  const int found = space.count[0];
-  team.sync();  // every thread has read it
-  if (kGroup > 1 && found > room) {  // the best vectors of these groups first
+  const auto maximum = [&](int i) { return ordered(space.maxima[i]); };
+  int picked = choose(groups, maximum, [](int i) { return static_cast<uint32_t>(i); }, space.picked,
+                      space.count);
+  const int* vectors = space.picked;  // local ones
+  if constexpr (kGroup > 1) {
     for (int i = team.tid; i < picked * kGroup; i += kThreads) {
       const int v = share.vector(space.picked[i / kGroup] * kGroup + i % kGroup);
       A most = lowest<A>();
@@ -339,103 +359,156 @@ __device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kTh
       }
       space.maxima[i] = most;
     }
-    const auto key = [&](int i) { return ordered(space.maxima[i]); };
-    const auto at = [&](int i) {
-      return static_cast<uint32_t>(space.picked[i / kGroup] * kGroup + i % kGroup);
-    };
-    if (team.tid == 0) space.count[0] = 0;
     team.sync();
-    Cut<A> best{0, 0xffffffffu};
-    if (picked * kGroup > top)
-      best = find_cut<4, kThreads, A>(team, picked * kGroup, top, key, at, space.histogram);
-    for (int i = team.tid; i < picked * kGroup; i += kThreads) {
-      const int v = share.vector(static_cast<int>(at(i)));
-      if (v < r.vectors && best.takes(key(i), at(i))) add(v, 0);
-    }
+    int* chosen = reinterpret_cast<int*>(space.candidates);
+    picked = choose(picked * kGroup, maximum,
+                    [&](int i) {
+                      return static_cast<uint32_t>(space.picked[i / kGroup] * kGroup + i % kGroup);
+                    },
+                    chosen, space.count + 1);
+    for (int i = team.tid; i < picked; i += kThreads) space.picked[i] = chosen[i];
     team.sync();
   }
-  const int body = space.count[0];
-  if (place.cta == 0) {
-    for (int e = team.tid; e < r.edges; e += kThreads)
-      space.candidates[body + e] = Ranked<A>(number_of(to_acc(r.x[r.edge(e)])), r.edge(e));
-    team.sync();
+  // their elements, and the single ones
+  if (team.tid == 0) *space.count = 0;
+  const int body = picked * E, edges = place.cta == 0 ? r.edges : 0, n = body + edges;
+  const auto element = [&](int i) {
+    if (i >= body) return r.edge(i - body);
+    const int v = share.vector(vectors[i / E]);
+    return v < r.vectors ? r.element(v) + i % E : kNowhere - i;  // distinct, behind all others
+  };
+  const auto number = [&](int i) {
+    const int at = element(i);
+    return at <= kNowhere - n ? number_of(to_acc(r.x[at])) : lowest<A>();
+  };
+  Cut<A> cut{0, 0xffffffffu};
+  if (n > top)
+    cut = find_cut<4, kThreads, A>(
+        team, n, top, [&](int i) { return ordered(number(i)); },
+        [&](int i) { return static_cast<uint32_t>(element(i)); }, space.histogram);
+  team.sync();
+  for (int i = team.tid; i < n; i += kThreads) {
+    const int at = element(i);
+    if (at > kNowhere - n || !cut.takes(ordered(number(i)), static_cast<uint32_t>(at))) continue;
+    space.candidates[atomicAdd(space.count, 1)] = Ranked<A>(number(i), at);
   }
-  const int n = body + (place.cta == 0 ? r.edges : 0);
-  if (n <= 256) return n;
-  // the best of them to the front
-  const auto key = [&](int i) { return space.candidates[i].number(); };
-  const auto at = [&](int i) { return static_cast<uint32_t>(space.candidates[i].at()); };
-  const Cut<A> last = find_cut<4, kThreads, A>(team, n, top, key, at, space.histogram);
-  if (team.tid == 0) space.count[1] = 0;
   team.sync();
-  for (int i = team.tid; i < n; i += kThreads)
-    if (last.takes(key(i), at(i))) space.best[atomicAdd(space.count + 1, 1)] = space.candidates[i];
-  team.sync();
-  for (int i = team.tid; i < top; i += kThreads) space.candidates[i] = space.best[i];
-  team.sync();
-  return top;
+  return *space.count;
 }
 
 // The elements of this CTA's share among which its `top` best are, to space.candidates; returns how
-// many. own: the thread's largest; edge: its single element. The maxima, the warps' bounds and counts
-// of 0 are written and the threads have met.
-template <int kThreads, typename T, typename A>
+// many. tiles: of the share; own: the thread's coarse maximum; edge: its single element. The maxima, the
+// warps' bounds and counts of 0 are written and the threads have met. meanwhile() is called between two more meetings.
+template <int kThreads, typename T, typename A, typename F>
 __device__ __forceinline__ int choose_top(const RowView<T>& r, const Place<kThreads>& place,
-                                          const TopSizes& z, A own, A edge,
-                                          const TopSpace<A, kThreads>& space) {
+                                          const TopSizes& z, int tiles, unsigned own, A edge,
+                                          const TopSpace<A, kThreads>& space, const F& meanwhile) {
   constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
   const Team<kThreads> team{place.tid};
   const Share<kThreads> share{place.cta, place.ctas};
-  int warps;
-  A bound = lowest<A>();
-  if (quota_of(r, place, z.top, warps) > 0) {
-    bound = space.kth[0];
-    for (int i = 1; i < warps; ++i) bound = min_acc(bound, space.kth[i]);
+  const int rows = z.fine ? tiles * kBatch : tiles;  // of units
+  unsigned bound = 0;
+  if (kThreads == 32 && z.top > kMostByLanes) {
+    bound = bound_of_warp(space.unit_max, rows, z.top);
+  } else {
+    int warps;
+    if (quota_of(r, place, z.top, warps) > 0) {
+      bound = space.kth[0];
+      for (int i = 1; i < warps; ++i) bound = min(bound, space.kth[i]);
+    }
   }
   const auto add = [&](A x, int at) {
     const int slot = atomicAdd(space.count, 1);
     if (slot < z.room()) space.candidates[slot] = Ranked<A>(x, at);
   };
+  // a unit's first vector; a batch's others are kThreads apart
+  const int each = z.fine ? 1 : kBatch;
+  const auto first = [&](int unit) {
+    return share.vector(z.fine ? unit : unit / kThreads * kTile + unit % kThreads);
+  };
   if (own >= bound) {
-    for (int tile = place.cta * kTile, j = 0; tile < r.vectors; tile += place.ctas * kTile, ++j) {
-      const A most = static_cast<A>(from_upper_half(space.batch_max[j * kThreads + team.tid]));
-      if (tile + team.tid >= r.vectors || !(most >= bound)) continue;
-      const int slot = atomicAdd(space.count + 1, 1);
-      if (slot < z.batches()) space.picked[slot] = j * kThreads + team.tid;
+    constexpr int kAhead = 4;
+    for (int row = 0; row < rows; row += kAhead) {
+      unsigned most[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        most[i] = row + i < rows ? space.unit_max[(row + i) * kThreads + team.tid] : 0u;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int unit = (row + i) * kThreads + team.tid;
+        if (most[i] == 0 || most[i] < bound || row + i >= rows) continue;  // 0: no vector
+        const int slot = atomicAdd(space.count + 1, 1);
+        if (slot < z.units()) space.picked[slot] = unit;
+      }
     }
   }
-  if (place.edge() < r.edges && number_of(edge) >= bound) add(number_of(edge), r.edge(place.edge()));
+  if (place.edge() < r.edges && coarse(edge) >= bound) add(number_of(edge), r.edge(place.edge()));
   team.sync();
   const int picked = space.count[1];
-  if (picked <= z.batches()) {
-    for (int i = team.tid; i < picked * kBatch; i += kThreads) {
-      const int batch = space.picked[i / kBatch];
-      const int v = share.vector(batch / kThreads * kTile + i % kBatch * kThreads + batch % kThreads);
+  if (picked <= z.units()) {
+    for (int i = team.tid; i < picked * each; i += kThreads) {
+      const int v = first(space.picked[i / each]) + i % each * kThreads;
       if (v >= r.vectors) continue;
       A x[E];
       unpack<T>(load_vector(r, v), x);
 #pragma unroll
       for (int c = 0; c < E; ++c)
-        if (number_of(x[c]) >= bound) add(number_of(x[c]), r.element(v) + c);
+        if (coarse(x[c]) >= bound) add(number_of(x[c]), r.element(v) + c);
     }
-    team.sync();
-    if (space.count[0] <= z.room()) return space.count[0];
   }
+  meanwhile();
+  team.sync();
+  const int n = space.count[0];
+  if (picked <= z.units() && n <= z.room()) return n;
   team.sync();  // the counts have been read
-  return z.whole ? choose_by_groups<32>(r, place, z.top, z.room(), space)
-                 : choose_by_groups<1>(r, place, z.top, z.room(), space);
+  return z.whole ? choose_by_groups<32>(r, place, z.top, space)
+                 : choose_by_groups<1>(r, place, z.top, space);
 }
 
-// Calls fn(rank, element) for the `top` best of the candidates, each by one thread.
+template <typename A>
+__device__ __forceinline__ Ranked<A> of_lane(const Ranked<A>& v, int d) {
+  Ranked<A> r = v;
+  r.key = __shfl_xor_sync(0xffffffffu, v.key, d);
+  if constexpr (sizeof(A) == 8) r.place = __shfl_xor_sync(0xffffffffu, v.place, d);
+  return r;
+}
+
+// Calls fn(rank, element) for the `top` best of the n candidates, each by one thread: 32 at a time are
+// sorted by a warp; a rank is the place among these and, by halving, what of the others is before it.
 template <int kThreads, typename A, typename F>
-__device__ __forceinline__ void rank_candidates(int tid, int n, int top,
+__device__ __forceinline__ void rank_candidates(const Team<kThreads>& team, int n, int top,
                                                 const TopSpace<A, kThreads>& space, const F& fn) {
-  for (int i = tid; i < n; i += kThreads) {
+  const int lane = team.tid & 31, runs = (n + 31) / 32;
+  for (int run = team.tid / 32; run < runs; run += kThreads / 32) {
+    const int i = 32 * run + lane;
+    Ranked<A> v = i < n ? space.candidates[i] : Ranked<A>(lowest<A>(), kNowhere);
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int d = size / 2; d; d /= 2) {
+        const Ranked<A> other = of_lane(v, d);
+        const bool first = (lane & d) == 0, down = (lane & size) == 0;
+        if (other.before(v) == (first == down)) v = other;
+      }
+    space.candidates[i] = v;
+  }
+  if (runs > 1) {
+    team.sync();
+  } else if (team.tid >= 32) {
+    return;
+  }
+  for (int i = team.tid; i < 32 * runs; i += kThreads) {
     const Ranked<A> own = space.candidates[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += space.candidates[j].before(own);
-    if (rank < top) fn(rank, own);
+    int rank = lane;
+    for (int run = 0; run < runs && rank < top; ++run) {
+      if (run == i / 32) continue;
+      const Ranked<A>* of = space.candidates + 32 * run;
+      int before = 0;
+#pragma unroll
+      for (int d = 16; d; d /= 2) before += of[before + d - 1].before(own) ? d : 0;
+      rank += before + of[before].before(own);
+    }
+    if (rank < top && own.at() != kNowhere) fn(rank, own);
   }
 }
 
@@ -496,13 +569,15 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
   const T* x = row_at<T>(a, r);
   const RowView<T> view(x, nullptr, reinterpret_cast<uintptr_t>(x), a.vocab);
   A logit = A(0);
-  if (place.first() && a.targets) logit = target_logit<T, A>(x, a.vocab, target);
+  if (place.cta == 0 && place.tid == kThreads - 1 && a.targets)
+    logit = target_logit<T, A>(x, a.vocab, target);
   const TopSpace<A, kThreads> space(shared, p.sizes, place.ctas);
   if (kTop && team.tid < 2) space.count[team.tid] = 0;
 
   const A edge = place.edge() < view.edges ? to_acc(x[view.edge(place.edge())]) : lowest<A>();
   Scored<A> part{lowest<A>(), A(0), A(0)};
-  for (int tile = place.cta * kTile, j = 0; tile < view.vectors; tile += place.ctas * kTile, ++j) {
+  int j = 0;
+  for (int tile = place.cta * kTile; tile < view.vectors; tile += place.ctas * kTile, ++j) {
     const int v = tile + place.tid;
     uint4 q[kBatch];
     if (tile + kTile <= view.vectors) {
@@ -512,8 +587,22 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
       for (int i = 0; i < kBatch; ++i)
         q[i] = v + i * kThreads < view.vectors ? load_vector(view, v + i * kThreads) : no_vector<T>();
     }
-    const A most = vector_max<T>(q), m = max_acc(part.m, most);
-    if constexpr (kTop) space.batch_max[j * kThreads + place.tid] = upper_half(most);
+    A m = part.m;
+    if (kTop && kThreads == 32 && p.sizes.fine) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint4 one[1] = {q[i]};
+        const A most = vector_max<T>(one);
+        space.unit_max[(j * kBatch + i) * kThreads + place.tid] =
+            v + i * kThreads < view.vectors ? coarse(most) : 0u;
+        m = max_acc(m, most);
+      }
+    } else {
+      const A most = vector_max<T>(q);
+      if constexpr (kTop)
+        space.unit_max[j * kThreads + place.tid] = v < view.vectors ? coarse(most) : 0u;
+      m = max_acc(m, most);
+    }
     move_base(part, m, k);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -523,12 +612,12 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
       add_scores(z, part.s, part.u);
     }
   }
-  const A own = part.m;
+  const unsigned own = coarse(part.m);
   if constexpr (kTop) {
     int warps;
     const int quota = quota_of(view, place, p.sizes.top, warps);
-    if (quota > 0) {
-      const A kth = largest_of_warp(own, quota);
+    if (quota > 0 && (kThreads > 32 || p.sizes.top <= kMostByLanes)) {
+      const unsigned kth = largest_of_warp(own, quota);
       if (team.tid % 32 == 0) space.kth[team.tid / 32] = kth;
     }
   }
@@ -540,13 +629,17 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
   }
   part = join_scores_of_warps<kThreads>(join_scores<32>(part, k), k);
   if constexpr (kThreads == 32) team.sync();
-  if (place.first()) {
-    const double log_s = write_scores(p, r, logit, part, inv_temp);
-    if (kTop) *space.log_s = log_s;
-  }
-  if constexpr (kTop) {
+  const auto write_first = [&] {
+    if (place.cta == 0 && place.tid == kThreads - 1) {
+      const double log_s = write_scores(p, r, logit, part, inv_temp);
+      if (kTop) *space.log_s = log_s;
+    }
+  };
+  if constexpr (!kTop) {
+    write_first();
+  } else {
     const int top = p.sizes.top;
-    const int n = choose_top(view, place, p.sizes, own, edge, space);
+    const int n = choose_top(view, place, p.sizes, j, own, edge, space, write_first);
     const double base = base_of(part.m);
     const auto write = [&](int rank, const Ranked<A>& e) {
       p.top_logps[r * top + rank] =
@@ -554,14 +647,13 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
       p.top_ids[r * top + rank] = e.at();
     };
     if (place.ctas == 1) {
-      rank_candidates<kThreads>(place.tid, n, top, space, write);
+      rank_candidates(team, n, top, space, write);
     } else if constexpr (kThreads > 32) {
       // the CTAs' lists to the first CTA, where an element's rank is its place in its own list and
       // what of the others is before it
       auto cluster = cg::this_cluster();
       Ranked<A>* to = of_peer(space.best, 0, false) + place.cta * top;
-      rank_candidates<kThreads>(place.tid, n, top, space,
-                                [&](int rank, const Ranked<A>& e) { to[rank] = e; });
+      rank_candidates(team, n, top, space, [&](int rank, const Ranked<A>& e) { to[rank] = e; });
       for (int i = n + place.tid; i < top; i += kThreads) to[i] = Ranked<A>(lowest<A>(), kNowhere);
       cluster.sync();
       if (place.cta == 0)
@@ -589,8 +681,10 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
   }
 }
 
+constexpr int kSmThreads = 1280;  // resident at 48 registers a thread
+
 template <typename T, typename A, int kThreads, bool kTop>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads / (sizeof(T) == 8 ? 2 : 1))
     scores_kernel(Rows a, ScoresArgs<A> p, double inv_temp, A k) {
   extern __shared__ uint4 shared[];
   const Place<kThreads> place;
@@ -691,32 +785,21 @@ template <typename T>
 TopSizes top_sizes(int top, int64_t vectors, int threads, int ctas) {
   const int64_t tile = int64_t{kBatch} * threads, tiles = (vectors + tile - 1) / tile;
   const int64_t share = (tiles + ctas - 1) / ctas;
-  const bool whole = share * tile / 32 >= 2 * top;
+  const bool whole = share * tile > 1024 && share * tile / 32 >= 2 * top;
   const int64_t groups = whole ? share * tile / 32 : share * tile;
-  return {top, static_cast<int>(share), static_cast<int>(groups), whole};
+  const bool fine = threads == 32 && share * kBatch <= kMostUnits;
+  return {top, static_cast<int>(share), static_cast<int>(groups), whole, fine};
 }
 
-template <typename T, bool kTop>
-int launch_scores(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double inv_temp,
-                  cudaStream_t st) {
+// By CTAs of kThreads, or clusters of them.
+template <typename T, bool kTop, int kThreads>
+int launch_score_rows(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double inv_temp, int sms,
+                      cudaStream_t st) {
   using A = typename AccOf<T>::type;
-  constexpr int kThreads = 256;
   const int64_t vectors = a.vocab / RowView<T>::E;
-  const int top = p.sizes.top, sms = sm_count();
-  const A k = exp_factor(A(0), inv_temp);
-  // a warp's lanes are enough to bound up to 32 alternatives
-  p.sizes = top_sizes<T>(top, vectors, 32, 1);
-  const int by_warp = kTop ? kRowWarps * TopSpace<A, 32>::bytes(p.sizes, 1) : 0;
-  if (top <= 32 && by_warps(a.rows, vectors, 2048, sms) && by_warp <= kSharedForTop) {
-    const auto kernel = scores_warp_kernel<T, A, kTop>;
-    const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSharedForTop);
-    if (rc) return rc;
-    return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps, by_warp,
-                           false, st, "scores_warp_kernel launch", a, p, inv_temp, k);
-  }
   int ctas = ctas_for(a.rows, vectors, kThreads, sms);
   const auto fits = [&] {
-    p.sizes = top_sizes<T>(top, vectors, kThreads, ctas);
+    p.sizes = top_sizes<T>(p.sizes.top, vectors, kThreads, ctas);
     return !kTop || (p.sizes.groups < 1 << 16 && p.sizes.tiles < 1 << 15 &&
                      TopSpace<A, kThreads>::bytes(p.sizes, ctas) <= kSharedForTop);
   };
@@ -728,7 +811,37 @@ int launch_scores(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double i
   if (rc) return rc;
   const size_t shared = kTop ? TopSpace<A, kThreads>::bytes(p.sizes, ctas) : 0;
   return launch_clusters(kernel, a.rows, ctas, kThreads, shared, false, st, "scores_kernel launch", a,
-                         p, inv_temp, k);
+                         p, inv_temp, exp_factor(A(0), inv_temp));
+}
+
+// Rows of up to kFewVectors vectors, where there are many, take CTAs of 128 threads for up to 64
+// alternatives: the few steps after a row's sum are short of work, and more rows hide them. 16384 x
+// 32000 bf16, 1, 20 and 64 alternatives: 232, 257 and 338 us by 128 threads, 279, 307 and 373 by 256;
+// 4096 x 131072, 64: 237 and 228. (More alternatives than half the threads, and the bound is loose.)
+constexpr int kFewVectors = 8192, kMostByHalf = 64;
+
+template <typename T, bool kTop>
+int launch_scores(const Rows& a, ScoresArgs<typename AccOf<T>::type> p, double inv_temp,
+                  cudaStream_t st) {
+  using A = typename AccOf<T>::type;
+  const int64_t vectors = a.vocab / RowView<T>::E;
+  const int top = p.sizes.top, sms = sm_count();
+  if (by_warps(a.rows, vectors, 2048, sms)) {
+    p.sizes = top_sizes<T>(top, vectors, 32, 1);
+    const int64_t shared = kTop ? int64_t{kRowWarps} * TopSpace<A, 32>::bytes(p.sizes, 1) : 0;
+    if (shared <= kSharedForTop) {
+      const auto kernel = scores_warp_kernel<T, A, kTop>;
+      const int rc = allow_shared(reinterpret_cast<const void*>(kernel), kSharedForTop);
+      if (rc) return rc;
+      return launch_clusters(kernel, (a.rows + kRowWarps - 1) / kRowWarps, 1, 32 * kRowWarps, shared,
+                             false, st, "scores_warp_kernel launch", a, p, inv_temp,
+                             exp_factor(A(0), inv_temp));
+    }
+  }
+  if constexpr (kTop)
+    if (vectors <= kFewVectors && top <= kMostByHalf && a.rows >= int64_t{16} * sms)
+      return launch_score_rows<T, kTop, 128>(a, p, inv_temp, sms, st);
+  return launch_score_rows<T, kTop, 256>(a, p, inv_temp, sms, st);
 }
 
 template <typename T>
