@@ -114,30 +114,47 @@ __device__ __forceinline__ Scored<A> join_scores(Scored<A> p, A k) {
   return p;
 }
 
-// As join_warps of rows.cuh.
+// The parts of a row's threads joined, first in each CTA (the threads have met then), and from there
+// across a cluster in two steps: the CTAs send their parts, and wait for one another's later. Called
+// by all threads, after cluster_started.
 template <int kThreads, typename A>
-__device__ __forceinline__ Scored<A> join_scores_of_warps(Scored<A> p, A k) {
-  if constexpr (kThreads > 32) {
-    constexpr int kWarps = kThreads / 32, kMostCtas = 8;
-    __shared__ Scored<A> of_warp[kWarps], of_cta[kMostCtas];
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) of_warp[threadIdx.x >> 5] = p;
-    __syncthreads();
-    p = join_scores<kWarps>(of_warp[lane % kWarps], k);
-    auto cluster = cg::this_cluster();
-    const int ctas = static_cast<int>(cluster.num_blocks());
-    if (ctas > 1) {
-      const int rank = min(static_cast<int>(threadIdx.x), ctas - 1);
-      Scored<A>* there = of_peer(&of_cta[cluster.block_rank()], rank, true);
-      if (threadIdx.x < ctas) *there = p;
-      cluster.sync();
+struct JoinScores {
+  static constexpr int kMostCtas = 8;
+  Scored<A>* of_cta;  // kMostCtas, shared
+  int ctas;
+
+  __device__ __forceinline__ Scored<A> send(Scored<A> p, A k) const {
+    p = join_scores<32>(p, k);
+    if constexpr (kThreads > 32) {
+      constexpr int kWarps = kThreads / 32;
+      __shared__ Scored<A> of_warp[kWarps];
+      const int lane = threadIdx.x & 31;
+      if (lane == 0) of_warp[threadIdx.x >> 5] = p;
+      __syncthreads();
+      p = join_scores<kWarps>(of_warp[lane % kWarps], k);
+      if (ctas > 1) {
+        auto cluster = cg::this_cluster();
+        const int rank = min(static_cast<int>(threadIdx.x), ctas - 1);
+        Scored<A>* there = of_peer(&of_cta[cluster.block_rank()], rank, true);
+        if (threadIdx.x < ctas) *there = p;
+        cluster.barrier_arrive();
+      }
+    } else {
+      __syncwarp();
+    }
+    return p;
+  }
+  __device__ __forceinline__ Scored<A> receive(Scored<A> p, A k) const {
+    if (kThreads > 32 && ctas > 1) {
+      cg::this_cluster().barrier_wait();
+      const int at = threadIdx.x % kMostCtas;
       p = {lowest<A>(), A(0), A(0)};
-      if (lane % kMostCtas < ctas) p = of_cta[lane % kMostCtas];
+      if (at < ctas) p = of_cta[at];
       p = join_scores<kMostCtas>(p, k);
     }
+    return p;
   }
-  return p;
-}
+};
 
 // ---------------------------------------------------------------------------------------------
 // Top alternatives
@@ -627,9 +644,11 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
     part.s += e;
     part.u += e * z;
   }
-  part = join_scores_of_warps<kThreads>(join_scores<32>(part, k), k);
-  if constexpr (kThreads == 32) team.sync();
+  __shared__ Scored<A> of_cta[JoinScores<kThreads, A>::kMostCtas];
+  const JoinScores<kThreads, A> join{of_cta, place.ctas};
+  part = join.send(part, k);
   const auto write_first = [&] {
+    part = join.receive(part, k);
     if (place.cta == 0 && place.tid == kThreads - 1) {
       const double log_s = write_scores(p, r, logit, part, inv_temp);
       if (kTop) *space.log_s = log_s;
