@@ -490,11 +490,24 @@ __device__ __forceinline__ Ranked<A> of_lane(const Ranked<A>& v, int d) {
   return r;
 }
 
-// Calls fn(rank, element) for the `top` best of the n candidates, each by one thread: 32 at a time are
-// sorted by a warp; a rank is the place among these and, by halving, what of the others is before it.
+// Calls fn(rank, element) for the `top` best of the n candidates, each by one thread. Few are counted
+// through; of more 32 at a time are sorted by a warp, and a rank is the place among these and, by
+// halving, what of the others is before it.
+constexpr int kFewCandidates = 48;
+
 template <int kThreads, typename A, typename F>
 __device__ __forceinline__ void rank_candidates(const Team<kThreads>& team, int n, int top,
                                                 const TopSpace<A, kThreads>& space, const F& fn) {
+  if (n <= kFewCandidates) {
+    for (int i = team.tid; i < n; i += kThreads) {
+      const Ranked<A> own = space.candidates[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += space.candidates[j].before(own);
+      if (rank < top) fn(rank, own);
+    }
+    return;
+  }
   const int lane = team.tid & 31, runs = (n + 31) / 32;
   for (int run = team.tid / 32; run < runs; run += kThreads / 32) {
     const int i = 32 * run + lane;
@@ -509,11 +522,7 @@ __device__ __forceinline__ void rank_candidates(const Team<kThreads>& team, int 
       }
     space.candidates[i] = v;
   }
-  if (runs > 1) {
-    team.sync();
-  } else if (team.tid >= 32) {
-    return;
-  }
+  team.sync();
   for (int i = team.tid; i < 32 * runs; i += kThreads) {
     const Ranked<A> own = space.candidates[i];
     int rank = lane;
