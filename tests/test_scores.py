@@ -215,6 +215,23 @@ def test_scores_ties_and_orders(vocab: int, dtype: torch.dtype) -> None:
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(2500, 300), (2500, 2000), (2500, 9000), (2500, 20000), (300, 70001)])
+def test_scores_alternatives_of_many_rows(rows: int, vocab: int, dtype: torch.dtype) -> None:
+    # as many as a warp, a small and a large CTA and a cluster choose from, also where many are equal
+    x, _ = logits_of((rows, vocab), dtype, seed=rows + vocab)
+    flat = (x * 0.5).round()
+    offset = x + 200  # what is left of the differences is below the upper 16 bits of a float
+    for z in (x, flat, offset):
+        want = ranked(z, 128)
+        lp = torch.log_softmax(z.double(), -1).gather(-1, want)
+        for top in (1, 16, 17, 33, 64, 65, 128):
+            got = ti.token_scores(z, None, top=top)
+            assert torch.equal(got.top_ids, want[:, :top])
+            close(got.top_logps, lp[:, :top], sum_error(dtype, vocab), 2 * unit(dtype))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("vocab", [40, 2500, 40007])
 def test_scores_masked_vocabulary(vocab: int, dtype: torch.dtype) -> None:
@@ -570,6 +587,30 @@ def test_distill_lists(vocab: int, kind: str, rest: str) -> None:
             if rest == "drop":
                 none[3] = -math.inf  # nothing to compare with
                 assert check_distill(x, ids, none, kind=kind, rest=rest).divergence[3] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(2, 131075), (400, 20011), (2500, 1003)])
+def test_distill_lists_in_one_place(rows: int, vocab: int) -> None:
+    # tokens 2048 apart (one thread has them all), side by side at either end of the row, and all of them
+    # listed twice
+    x, _ = logits_of((rows, vocab), torch.bfloat16, seed=vocab)
+    apart = torch.arange(5, vocab, 2048, device="cuda")[:64]
+    ends = torch.cat([torch.arange(20, device="cuda"), torch.arange(vocab - 20, vocab, device="cuda")])
+    few = slice(0, 3)
+    for ids in (apart, ends, torch.cat([apart, apart.flip(0)]), torch.cat([ends, ends])):
+        lists = ids.expand(rows, len(ids)).contiguous()
+        logps = torch.full(lists.shape, -math.log(len(ids) + 3.0), device="cuda")
+        leaf = x.detach().requires_grad_()
+        got = ti.distillation_loss(leaf, lists, logps, upstream=float(rows))
+        (gx,) = torch.autograd.grad(got.loss * rows, leaf)
+        part = check_distill(x[few], lists[few], logps[few])
+        close(got.divergence[few], part.divergence, 12 * sum_error(x.dtype, vocab), 2.0**-22)
+        leaf = x[few].detach().requires_grad_()
+        n = len(leaf)
+        (gp,) = torch.autograd.grad(ti.distillation_loss(leaf, lists[few], logps[few],
+                                                         upstream=float(n)).loss * n, leaf)
+        close(gx[few], gp.double(), 12 * sum_error(x.dtype, vocab), HALF_ULP[x.dtype] * 2.02)
 
 
 @pytest.mark.gpu
@@ -1054,6 +1095,8 @@ def test_abi_refusals() -> None:
                 dict(rows=_ext.Rows(16, 4, 4, 0, -8, 8)), dict(rows=_ext.Rows(17, 4, 4, 0, 8, 8))):
         assert scores(**bad) == 1, bad
     assert scores(rows=_ext.Rows(none, 0, 1, 0, 8, 8), logps=none, entropy=none, tops=none, ids=none) == 0
+    huge = _ext.Rows(16, 1, 1, 0, 1 << 28, 1 << 28)
+    assert scores(dtype=1, rows=huge, top=5) == 1 and b"vocabulary" in so.tiso_last_error()
     assert so.tiso_scores_grad(2, rows, p, 1.0, none, p, p, p, none) == 1
     assert so.tiso_scores_grad(2, rows, none, 1.0, p, p, p, p, none) == 1
     assert b"targets" in so.tiso_last_error()
