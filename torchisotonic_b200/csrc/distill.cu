@@ -51,26 +51,13 @@ __device__ __forceinline__ double sum_of_warp(double v) {
 
 __device__ __forceinline__ double product(double x, double y) { return x == 0 ? 0.0 : x * y; }
 
-// Sums over the list's tokens (of a warp's entries, then of all): of q and of e = exp(z), z the logits
-// from the largest of them, over t; `far` of q (log q - z), in the reverse divergence of e (z - log q).
+// Sums over the list's tokens, of a warp's entries: of q and of e = exp(z), z the logits from the
+// largest of them, over t; `far` of q (log q - z), in the reverse divergence of e (z - log q).
 template <typename A>
 struct ListSums {
-  double q, far;
-  A e, most;
+  double q, far, e;
+  A most;
   int tokens;
-
-  // the same with z from another logit than the largest
-  __device__ __forceinline__ void move(A to, double inv_temp, A k, int kind) {
-    if (tokens == 0 || most == to) return;
-    const A d = base_of(most) - base_of(to), f = e == A(0) ? A(0) : scaled_exp(d, k);
-    const double z = static_cast<double>(d) * inv_temp;
-    if (kind == TISO_DISTILL_REVERSE) {
-      far = f == A(0) ? 0.0 : static_cast<double>(f) * (far + z * static_cast<double>(e));
-    } else if (q != 0) {
-      far -= q * z;
-    }
-    e *= f;
-  }
 };
 
 // What the gradients are made of, once the row's sum is known.
@@ -215,7 +202,7 @@ __device__ __forceinline__ int warps_of(int top) {
 // with the sum of its probabilities.
 template <bool kAgain, int kThreads, typename T, typename A>
 __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, const RowView<T>& view,
-                                          const Place<kThreads>& place, double inv_temp, A k,
+                                          const Place<kThreads>& place, double inv_temp,
                                           const ListSpace<A, kThreads>& space) {
   if (place.tid / 32 * 32 >= p.top) return;
   A most = lowest<A>();
@@ -247,12 +234,12 @@ __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, co
     space.lead[i] = lead;
   }
   most = max_of_lanes<32>(most);
+  const double base = base_of(most);
   ListSums<A> sums{};
   for (int i = place.tid; i < p.top; i += kThreads) {
     if (space.lead[i] != i) continue;
     const double q = space.q[i], log_q = space.log_q[i];
-    const A d = space.logit[i] - base_of(most), e = scaled_exp(d, k);
-    const double z = static_cast<double>(d) * inv_temp;
+    const double z = (static_cast<double>(space.logit[i]) - base) * inv_temp, e = exp(z);
     sums.q += q;
     sums.far += p.kind == TISO_DISTILL_REVERSE ? product(e, z - log_q) : product(q, log_q - z);
     sums.e += e;
@@ -269,28 +256,35 @@ __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, co
   if (place.tid % 32 == 0) space.sums[place.tid / 32] = sums;
 }
 
-// The sums over the whole list.
-template <int kThreads, typename A>
-__device__ __forceinline__ ListSums<A> list_sums(const ListSpace<A, kThreads>& space, int top, int kind,
-                                                 double inv_temp, A k) {
-  ListSums<A> sums = space.sums[0];
-  const int warps = warps_of<kThreads>(top);
-  if (warps > 1) {
-    A most = sums.most;
-    for (int i = 1; i < warps; ++i) most = max_acc(most, space.sums[i].most);
-    sums.move(most, inv_temp, k, kind);
-    for (int i = 1; i < warps; ++i) {
-      ListSums<A> more = space.sums[i];
-      more.move(most, inv_temp, k, kind);
-      sums.q += more.q;
-      sums.far += more.far;
-      sums.e += more.e;
-      sums.tokens += more.tokens;
+// What the first steps need of the whole list: the sums of q and of exp(z), z from its largest logit,
+// this one in the accumulation type.
+template <typename A>
+struct WholeList {
+  double q;
+  A e, most;
+  int tokens;
+
+  template <int kThreads>
+  __device__ __forceinline__ WholeList(const ListSpace<A, kThreads>& space, int top, A k) {
+    const ListSums<A>* sums = space.sums;
+    const int warps = warps_of<kThreads>(top);
+    q = sums[0].q;
+    e = static_cast<A>(sums[0].e);
+    most = sums[0].most;
+    tokens = sums[0].tokens;
+    if (warps > 1) {
+      for (int i = 1; i < warps; ++i) {
+        most = max_acc(most, sums[i].most);
+        q += sums[i].q;
+        tokens += sums[i].tokens;
+      }
+      e = A(0);
+      for (int i = 0; i < warps; ++i)
+        if (sums[i].e != 0)  // (a part that is hidden has no maximum)
+          e += static_cast<A>(sums[i].e) * scaled_exp(base_of(sums[i].most) - base_of(most), k);
     }
-    sums.most = most;
   }
-  return sums;
-}
+};
 
 // The teacher's probabilities of the list and of the rest.
 struct Teacher {
@@ -323,13 +317,14 @@ struct Student {
 // of; without a logarithm, and in double only what cancels.
 template <typename A, int kThreads>
 __device__ __forceinline__ Settled settle(const DistillArgs<A>& p, const ListSpace<A, kThreads>& space,
-                                          const ListSums<A>& sums, const Part<A>& rest,
-                                          const Student<A>& student, int vocab) {
-  const Teacher teacher(sums.q, sums.tokens, vocab, p.kind, p.drop);
+                                          const WholeList<A>& list, const Part<A>& rest, int vocab,
+                                          A k) {
+  const Teacher teacher(list.q, list.tokens, vocab, p.kind, p.drop);
+  const Student<A> student(rest, list.most, list.e, k);
   Settled row{};
   row.c = *space.share;
   if (*space.bad || student.s == A(0)) row.c = nan_of(0.0);
-  row.each = p.drop ? (sums.q > 0 ? 1 / sums.q : sums.q) : 1.0;  // nothing to compare with: 0
+  row.each = p.drop ? (list.q > 0 ? 1 / list.q : list.q) : 1.0;  // nothing to compare with: 0
   row.whole = teacher.whole;
   row.p = student.list_p;
   // p_v (f - sum P f) = p_v whole - q_v
@@ -338,52 +333,77 @@ __device__ __forceinline__ Settled settle(const DistillArgs<A>& p, const ListSpa
   return row;
 }
 
-// The steps that take logarithms, by a warp: the divergence, and what the gradients of the others than
-// the forward one are made of.
+// The steps to the divergence, by a warp, in double (it is small beside its terms where the student is
+// near the teacher); and what the gradients of the others than the forward one are made of. A lane for
+// each exponential and logarithm that can be taken at once.
 template <typename A, int kThreads>
 __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
                                               const ListSpace<A, kThreads>& space,
-                                              const ListSums<A>& sums, const Part<A>& rest,
-                                              const Student<A>& student, int vocab, double inv_temp,
-                                              A k, Settled& row) {
-  const Teacher teacher(sums.q, sums.tokens, vocab, p.kind, p.drop);
+                                              const WholeList<A>& list, const Part<A>& rest, int vocab,
+                                              double inv_temp, Settled& row) {
+  const Teacher teacher(list.q, list.tokens, vocab, p.kind, p.drop);
   const int lane = threadIdx.x & 31;
-  // a lane for each logarithm
-  const double of = lane == 0   ? static_cast<double>(student.s)
-                    : lane == 1 ? static_cast<double>(rest.s)
-                    : lane == 2 ? teacher.rest_q
-                                : sums.q;
-  const double logarithm = log(of), base = student.base;
-  const double log_s = __shfl_sync(0xffffffffu, logarithm, 0);
-  const double rest_log_p = (static_cast<double>(base_of(rest.m)) - base) * inv_temp - log_s +
-                            __shfl_sync(0xffffffffu, logarithm, 1);
-  const double rest_log_q = __shfl_sync(0xffffffffu, logarithm, 2), rest_p = student.rest_p;
-  row.log_each = p.drop ? -__shfl_sync(0xffffffffu, logarithm, 3) : 0.0;
-  row.log_p = (static_cast<double>(base_of(sums.most)) - base) * inv_temp - log_s;
+  const auto of_lane = [](double v, int from) { return __shfl_sync(0xffffffffu, v, from); };
+  const double most = base_of(list.most);
+  // the list's sums with z from its largest logit
+  double far = 0, e = 0;
+  if (lane < warps_of<kThreads>(p.top)) {
+    const ListSums<A> part = space.sums[lane];
+    far = part.far;
+    e = part.e;
+    const double d = (static_cast<double>(base_of(part.most)) - most) * inv_temp;
+    if (part.tokens > 0 && part.most != list.most) {
+      const double f = e == 0 ? 0.0 : exp(d);
+      if (p.kind == TISO_DISTILL_REVERSE) {
+        far = f == 0 ? 0.0 : f * (far + d * e);
+      } else if (part.q != 0) {
+        far -= part.q * d;
+      }
+      e *= f;
+    }
+  }
+#pragma unroll
+  for (int d = kListWarps / 2; d; d /= 2) {
+    far += __shfl_xor_sync(0xffffffffu, far, d);
+    e += __shfl_xor_sync(0xffffffffu, e, d);
+  }
+  far = of_lane(far, 0);
+  e = of_lane(e, 0);
+  // both parts' sums from the row's maximum
+  const double base = base_of(max_acc(rest.m, list.most)), rest_s = rest.s;
+  const double rest_z = (static_cast<double>(base_of(rest.m)) - base) * inv_temp;
+  const double list_z = (most - base) * inv_temp;
+  const double z = lane == 0 ? rest_z : list_z, from_base = z == 0 ? 1.0 : exp(z);
+  const double of_rest = rest_s == 0 ? 0.0 : of_lane(from_base, 0) * rest_s;
+  const double of_list = e == 0 ? 0.0 : of_lane(from_base, 1), s = of_rest + of_list * e;
+  const double rest_p = of_rest / s;
+  const double logarithm = log(lane == 0 ? s : lane == 1 ? rest_s : lane == 2 ? teacher.rest_q : list.q);
+  const double log_s = of_lane(logarithm, 0), rest_log_p = rest_z + of_lane(logarithm, 1) - log_s;
+  const double rest_log_q = of_lane(logarithm, 2);
+  row.log_each = p.drop ? -of_lane(logarithm, 3) : 0.0;
+  row.log_p = list_z - log_s;
   double d, factor = 0;
-  if (p.drop && sums.q == 0) {  // nothing to compare with
-    d = 0;
+  if (p.drop && list.q == 0) {  // nothing to compare with
     row.c *= 0;
     row.factor *= 0;
-    return d + row.c;
+    return row.c;
   }
   if (p.kind == TISO_DISTILL_FORWARD) {
-    d = row.each * sums.far + row.each * sums.q * (row.log_each - row.log_p) +
+    d = row.each * far + row.each * list.q * (row.log_each - row.log_p) +
         product(teacher.rest_q, rest_log_q - rest_log_p);
     return row.c == row.c ? d : row.c;
   }
   if (p.kind == TISO_DISTILL_REVERSE) {
     const double rest_f = rest_log_p - rest_log_q;
-    d = row.mean = row.p * (sums.far + static_cast<double>(sums.e) * row.log_p) +
-                   product(rest_p, rest_f);
+    d = row.mean = of_list / s * (far + e * row.log_p) + product(rest_p, rest_f);
     factor = product(rest_p, rest_f - row.mean);
   } else {
     double mean = 0, cross = 0;
     for (int i = lane; i < p.top; i += 32) {
       if (space.lead[i] != i) continue;
-      const A z = space.logit[i] - base_of(sums.most);
-      const double prob = scaled_exp(z, k) * row.p, log_p = static_cast<double>(z) * inv_temp + row.log_p;
-      const double q = space.q[i] * row.each, log_m = log(p.mix * q + (1 - p.mix) * prob);
+      const double log_p = (static_cast<double>(space.logit[i]) - most) * inv_temp + row.log_p;
+      const double prob = exp(log_p), q = space.q[i] * row.each;
+      const double log_m = log(p.mix * q + (1 - p.mix) * prob);
       mean += product(prob, (1 - p.mix) * (log_p - log_m));
       cross += product(q, space.log_q[i] + row.log_each - log_m);
     }
@@ -393,7 +413,7 @@ __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
     d = row.mean + p.mix * (sum_of_warp(cross) + product(teacher.rest_q, rest_log_q - log_m));
     factor = product(rest_p, rest_f - row.mean);
   }
-  row.factor = rest.s == A(0) ? 0 * row.c : row.c * factor / static_cast<double>(rest.s);
+  row.factor = rest.s == A(0) ? 0 * row.c : row.c * factor / rest_s;
   return row.c == row.c ? d : row.c;
 }
 
@@ -408,11 +428,14 @@ __device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t 
     A value = A(0);
     if (lead >= 0) {
       const A z = space.logit[lead] - base_of(most);
-      const double prob = scaled_exp(z, k) * row.p, q = space.q[lead] * row.each;
+      const double q = space.q[lead] * row.each;
       if (p.kind == TISO_DISTILL_FORWARD) {
-        value = static_cast<A>(row.c * (prob * row.whole - q));
+        value = static_cast<A>(row.c * (scaled_exp(z, k) * row.p * row.whole - q));
       } else {
-        const double log_p = static_cast<double>(z) * inv_temp + row.log_p;
+        const double log_p =
+            (static_cast<double>(space.logit[lead]) - static_cast<double>(base_of(most))) * inv_temp +
+            row.log_p;
+        const double prob = exp(log_p);
         const double f = p.kind == TISO_DISTILL_REVERSE
                              ? log_p - space.log_q[lead]
                              : (1 - p.mix) * (log_p - log(p.mix * q + (1 - p.mix) * prob));
@@ -592,7 +615,7 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   for (int j = 0; j < kStages; ++j) tiles.copy(j);
   const ListSpace<A, kThreads> space(shared + kStages * kTile, p.top);
   const Own own = hand_out(a, p, r, view, place, space);
-  read_list<false>(p, r, view, place, inv_temp, k, space);
+  read_list<false>(p, r, view, place, inv_temp, space);
   if (place.tid == kThreads - 1) read_share(p, w, inv_temp, space);
 
   Part<A> rest{lowest<A>(), A(0)};
@@ -617,13 +640,12 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   rest = join_warps<kThreads>(join_lanes<32>(rest, k), k);
   if constexpr (kThreads == 32) team.sync();
   if (*space.twice) {
-    read_list<true>(p, r, view, place, inv_temp, k, space);
+    read_list<true>(p, r, view, place, inv_temp, space);
     team.sync();
   }
-  const ListSums<A> sums = list_sums(space, p.top, p.kind, inv_temp, k);
-  const Student<A> student(rest, sums.most, sums.e, k);
+  const WholeList<A> list(space, p.top, k);
   // every warp takes the few steps to the rest's factor by itself, where they need no logarithm
-  Settled row = settle(p, space, sums, rest, student, a.vocab);
+  Settled row = settle(p, space, list, rest, a.vocab, k);
   const auto write_results = [&](double d) {
     write_row(p, r, rest, d, row.factor);
     finish(d);
@@ -631,18 +653,18 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   if (p.kind != TISO_DISTILL_FORWARD) {
     double d = 0;
     if (place.tid < 32) {
-      d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, row);
+      d = settle_logs(p, space, list, rest, a.vocab, inv_temp, row);
       if (place.tid == 0) *space.settled = row;
     }
     team.sync();
     row = *space.settled;
     if (place.first()) write_results(d);
   }
-  if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, sums.most, space);
+  if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, list.most, space);
   if (p.kind == TISO_DISTILL_FORWARD && place.tid >= kThreads - 32 && place.cta == 0) {
     // by the last warp: the first ones have the list
     Settled all = row;
-    const double d = settle_logs(p, space, sums, rest, student, a.vocab, inv_temp, k, all);
+    const double d = settle_logs(p, space, list, rest, a.vocab, inv_temp, all);
     if (place.tid == kThreads - 32) write_results(d);
   }
   if (!grad) return;
