@@ -755,10 +755,11 @@ struct ScoresSlope {
                                          int64_t target_, int vocab)
       : base(stats[0]), k(k_), c(c_) {
     const bool in = target_ >= 0 && target_ < vocab;
-    const double s = stats[1], mean = stats[2];
+    const A s = stats[1], mean = stats[2], of_entropy = static_cast<A>(h);
     target = in && wanted ? static_cast<int>(target_) : -1;
-    alpha = in || !wanted ? static_cast<A>((h * mean - c) / s) : nan_of(A(0));
-    beta = static_cast<A>(-h * unit_of(k_) / s);
+    // (not in double: two divisions a thread would be a third of a tile's instructions)
+    alpha = in || !wanted ? (of_entropy * mean - static_cast<A>(c)) / s : nan_of(A(0));
+    beta = -of_entropy * static_cast<A>(unit_of(k_)) / s;
   }
   __device__ __forceinline__ A at(A x, int v) const {
     const A z = max_nan(mul_rn(x - base, k), least_argument(k));
