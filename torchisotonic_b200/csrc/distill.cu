@@ -12,8 +12,8 @@
 //
 // The rest's probability is summed from the rest's own exponentials, taken from the rest's own
 // maximum: as the row's sum less the listed ones it would cancel where the list holds nearly all, and
-// taken from the row's maximum it would underflow where the student is sure of a listed token. The
-// row's pass leaves the listed tokens out by a bit for each of its elements in shared memory.
+// taken from the row's maximum it would underflow where the student is sure of a listed token. Each
+// listed token is handed to the thread that reads its element, which puts -infinity in its place.
 #include "rows.cuh"
 #include "select.cuh"
 

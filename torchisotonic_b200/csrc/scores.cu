@@ -209,6 +209,18 @@ __device__ __forceinline__ uint32_t coarse(double x) {
   return static_cast<uint32_t>(ordered(x) >> 48);
 }
 
+// The least number of a coarse key, or of all.
+__device__ __forceinline__ float least_of(uint32_t key, float) {
+  const uint32_t b = key << 16;
+  return key <= 0x7fu ? lowest<float>() : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ double least_of(uint32_t key, double) {
+  const uint64_t b = static_cast<uint64_t>(key) << 48;
+  return key <= 0xfu ? lowest<double>()
+                     : __longlong_as_double(static_cast<long long>(
+                           b >> 63 ? b & 0x7fffffffffffffffULL : ~b));
+}
+
 constexpr int kMostUnits = 16;  // of a warp's lane
 
 // What the threads that work on a row have to choose from (a cluster's CTAs each for their share).
@@ -322,8 +334,10 @@ constexpr int kMostByLanes = 16;
 template <int kThreads, typename T>
 __device__ __forceinline__ int quota_of(const RowView<T>& r, const Place<kThreads>& place, int top,
                                         int& warps) {
-  const int own = min(max(r.vectors - place.cta * kBatch * kThreads, 0), kThreads);
-  warps = own / 32;
+  const int own = r.vectors - place.cta * kBatch * kThreads;
+  warps = kThreads / 32;
+  if (own >= kThreads) return (top + warps - 1) / warps;
+  warps = max(own, 0) / 32;
   const int q = warps > 0 ? (top + warps - 1) / warps : 33;
   return q <= 32 ? q : 0;
 }
@@ -423,7 +437,7 @@ __device__ __forceinline__ int choose_top(const RowView<T>& r, const Place<kThre
   constexpr int E = RowView<T>::E, kTile = kBatch * kThreads;
   const Team<kThreads> team{place.tid};
   const Share<kThreads> share{place.cta, place.ctas};
-  const int rows = z.fine ? tiles * kBatch : tiles;  // of units
+  const int rows = kThreads == 32 && z.fine ? tiles * kBatch : tiles;  // of units
   unsigned bound = 0;
   if (kThreads == 32 && z.top > kMostByLanes) {
     bound = bound_of_warp(space.unit_max, rows, z.top);
@@ -439,10 +453,13 @@ __device__ __forceinline__ int choose_top(const RowView<T>& r, const Place<kThre
     if (slot < z.room()) space.candidates[slot] = Ranked<A>(x, at);
   };
   // a unit's first vector; a batch's others are kThreads apart
-  const int each = z.fine ? 1 : kBatch;
+  const bool fine = kThreads == 32 && z.fine;
+  const int each = fine ? 1 : kBatch, log_each = fine ? 0 : 2;
+  static_assert(kBatch == 4, "log_each");
   const auto first = [&](int unit) {
-    return share.vector(z.fine ? unit : unit / kThreads * kTile + unit % kThreads);
+    return share.vector(fine ? unit : unit / kThreads * kTile + unit % kThreads);
   };
+  const A least = least_of(bound, A(0));
   if (own >= bound) {
     constexpr int kAhead = 4;
     for (int row = 0; row < rows; row += kAhead) {
@@ -459,18 +476,18 @@ __device__ __forceinline__ int choose_top(const RowView<T>& r, const Place<kThre
       }
     }
   }
-  if (place.edge() < r.edges && coarse(edge) >= bound) add(number_of(edge), r.edge(place.edge()));
+  if (place.edge() < r.edges && !(edge < least)) add(number_of(edge), r.edge(place.edge()));
   team.sync();
   const int picked = space.count[1];
   if (picked <= z.units()) {
-    for (int i = team.tid; i < picked * each; i += kThreads) {
-      const int v = first(space.picked[i / each]) + i % each * kThreads;
+    for (int i = team.tid; i < picked << log_each; i += kThreads) {
+      const int v = first(space.picked[i >> log_each]) + (i & (each - 1)) * kThreads;
       if (v >= r.vectors) continue;
       A x[E];
       unpack<T>(load_vector(r, v), x);
 #pragma unroll
       for (int c = 0; c < E; ++c)
-        if (coarse(x[c]) >= bound) add(number_of(x[c]), r.element(v) + c);
+        if (!(x[c] < least)) add(number_of(x[c]), r.element(v) + c);
     }
   }
   meanwhile();
