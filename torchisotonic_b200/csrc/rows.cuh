@@ -316,7 +316,8 @@ struct StagedTiles {
   }
   __device__ __forceinline__ void read(int j, uint4 (&q)[kBatch]) const {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) q[i] = at(j)[i * kThreads];
+    for (int i = 0; i < kBatch; ++i)  // (from at(j) the policy's kernel needs a register more, and spills)
+      q[i] = stages[static_cast<unsigned>(j) % kStages * kTile + i * kThreads + tid];
   }
   __device__ __forceinline__ void read_cut(uint4 (&q)[kBatch]) const {
     read(whole, q);
@@ -348,8 +349,9 @@ struct TokenWeights {
   const void* weight;
   int kind;
 
-  __device__ __forceinline__ A at(int64_t r) const {
-    const int64_t mark = marks[r * stride];  // both loads in flight together
+  __device__ __forceinline__ A at(int64_t r) const { return of(marks[r * stride], r); }
+  // (token r's mark may still be on its way: both loads are in flight together)
+  __device__ __forceinline__ A of(int64_t mark, int64_t r) const {
     A w = A(1);
     if (kind == kByteWeight) {
       w = static_cast<const uint8_t*>(weight)[r] ? A(1) : A(0);
