@@ -67,6 +67,7 @@ struct Settled {
   double log_each;  // its logarithm
   double whole;     // their sum with the rest's
   double p;         // of an exp(z), z from the largest logit of the list: its probability
+  double part;      // kWide: of an exp(z), z from the largest logit of this warp's entries: from the list's
   double log_p;     // of a z: its logarithm
   double mean;      // sum P f
   double factor;    // of the rest's gradient
@@ -74,11 +75,20 @@ struct Settled {
 
 constexpr int kListWarps = kMostListed / 32;
 
+// The forward divergence's gradient has the differences p_v sum Q - q_v and P_rest sum Q - Q_rest, small
+// beside their terms where the student is near its teacher: with the terms in float, rows that agree to
+// 0.01 lose two digits of it. So float32 logits have them in double (4096 x 32000, lists of 128: 245 us
+// for 239; 4096 x 131072, 64: 920 for 905). Logits of 16 bits have them in float: their own steps and the
+// gradient's rounding are larger (in double 156 us for 149, and 8192 x 131072 935 for 900).
+template <typename T>
+constexpr bool kWide = sizeof(T) == 4;
+
 // Shared memory of the kThreads threads that work on a row. An entry is handed to the thread that
 // reads and writes its token's element (its owner): each thread has a chain of its entries.
 template <typename A, int kThreads>
 struct ListSpace {
   double *q, *log_q;     // the teacher's probabilities
+  double* e;             // kWide, forward: in log_q's place the student's exp(z), z as in the warp's sums
   double* share;         // the row's share of the loss, over t
   ListSums<A>* sums;     // of each warp that has entries
   Settled* settled;
@@ -98,7 +108,7 @@ struct ListSpace {
   __device__ ListSpace(void* at, int top) {
     const int n = entries(top);
     q = static_cast<double*>(at);
-    log_q = q + n;
+    e = log_q = q + n;
     share = log_q + n;
     sums = reinterpret_cast<ListSums<A>*>(share + 2);
     settled = reinterpret_cast<Settled*>(sums + kListWarps);
@@ -244,6 +254,7 @@ __device__ __forceinline__ void read_list(const DistillArgs<A>& p, int64_t r, co
     sums.far += p.kind == TISO_DISTILL_REVERSE ? product(e, z - log_q) : product(q, log_q - z);
     sums.e += e;
     ++sums.tokens;
+    if (kWide<T> && p.kind == TISO_DISTILL_FORWARD) space.e[i] = e;
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
@@ -313,19 +324,59 @@ struct Student {
   }
 };
 
+// The same in double (kWide), by a warp: each exponential by a lane of its own, one quotient. own: the part
+// of the list of this warp's entries. factor: (P_rest sum Q - Q_rest) / rest.s.
+struct WideStudent {
+  double list_p, part, factor;
+
+  template <typename A, int kThreads>
+  __device__ __forceinline__ WideStudent(const Teacher& teacher, const Part<A>& rest, A most,
+                                         const ListSpace<A, kThreads>& space, int top, int own,
+                                         double inv_temp) {
+    const int lane = threadIdx.x & 31, parts = warps_of<kThreads>(top);
+    const ListSums<A>& sums = space.sums[lane < parts ? lane : 0];
+    const double base = base_of(most), d = (static_cast<double>(base_of(rest.m)) - base) * inv_temp;
+    const double z = (static_cast<double>(base_of(sums.most)) - base) * inv_temp;
+    const double e = exp(lane < kListWarps ? z : -fabs(d));
+    // (a part that is hidden has no maximum)
+    double list_e = lane >= parts || sums.e == 0 ? 0.0 : e * sums.e;
+#pragma unroll
+    for (int i = kListWarps / 2; i; i /= 2) list_e += __shfl_xor_sync(0xffffffffu, list_e, i);
+    list_e = __shfl_sync(0xffffffffu, list_e, 0);
+    part = __shfl_sync(0xffffffffu, sums.e == 0 ? 0.0 : e, own % kListWarps);
+    const double less = __shfl_sync(0xffffffffu, e, kListWarps);
+    const double rest_s = rest.s;
+    const double of_rest = rest_s == 0 ? 0.0 : d < 0 && list_e != 0 ? less : 1.0;
+    const double of_list = list_e == 0 ? 0.0 : d > 0 && rest_s != 0 ? less : 1.0;
+    const double rest_e = of_rest * rest_s, s = rest_e + of_list * list_e;
+    const double one = rest_s == 0 ? 1.0 : rest_s, r = 1 / (s * one);
+    list_p = of_list * one * r;
+    factor = rest_s == 0 ? 0.0 : (teacher.whole * rest_e - teacher.rest_q * s) * r;
+  }
+};
+
 // The first steps after a row's sum, by every warp: what a gradient of the forward divergence is made
 // of; without a logarithm, and in double only what cancels.
-template <typename A, int kThreads>
+template <typename T, typename A, int kThreads>
 __device__ __forceinline__ Settled settle(const DistillArgs<A>& p, const ListSpace<A, kThreads>& space,
                                           const WholeList<A>& list, const Part<A>& rest, int vocab,
-                                          A k) {
+                                          const Place<kThreads>& place, double inv_temp, A k) {
   const Teacher teacher(list.q, list.tokens, vocab, p.kind, p.drop);
-  const Student<A> student(rest, list.most, list.e, k);
   Settled row{};
   row.c = *space.share;
-  if (*space.bad || student.s == A(0)) row.c = nan_of(0.0);
   row.each = p.drop ? (list.q > 0 ? 1 / list.q : list.q) : 1.0;  // nothing to compare with: 0
   row.whole = teacher.whole;
+  if constexpr (kWide<T>) {
+    if (*space.bad || (rest.s == A(0) && list.e == A(0))) row.c = nan_of(0.0);
+    if (p.kind != TISO_DISTILL_FORWARD) return row;
+    const WideStudent student(teacher, rest, list.most, space, p.top, place.tid / 32, inv_temp);
+    row.p = student.list_p;
+    row.part = student.part;
+    row.factor = row.c * student.factor;
+    return row;
+  }
+  const Student<A> student(rest, list.most, list.e, k);
+  if (*space.bad || student.s == A(0)) row.c = nan_of(0.0);
   row.p = student.list_p;
   // p_v (f - sum P f) = p_v whole - q_v
   const A factor = static_cast<A>(teacher.whole) * student.rest_p - static_cast<A>(teacher.rest_q);
@@ -418,7 +469,7 @@ __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
 }
 
 // The gradients of the list's tokens, by the threads of their entries.
-template <int kThreads, typename A>
+template <typename T, int kThreads, typename A>
 __device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t r,
                                                const Place<kThreads>& place, double inv_temp, A k,
                                                const Settled& row, A most,
@@ -430,7 +481,15 @@ __device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t 
       const A z = space.logit[lead] - base_of(most);
       const double q = space.q[lead] * row.each;
       if (p.kind == TISO_DISTILL_FORWARD) {
-        value = static_cast<A>(row.c * (scaled_exp(z, k) * row.p * row.whole - q));
+        double e;
+        if constexpr (!kWide<T>) {
+          e = scaled_exp(z, k);
+        } else if (kThreads == 32 || lead / 32 == place.tid / 32) {
+          e = space.e[lead] * row.part;
+        } else {  // listed again, first among another warp's entries
+          e = exp((static_cast<double>(space.logit[lead]) - static_cast<double>(base_of(most))) * inv_temp);
+        }
+        value = static_cast<A>(row.c * (e * row.p * row.whole - q));
       } else {
         const double log_p =
             (static_cast<double>(space.logit[lead]) - static_cast<double>(base_of(most))) * inv_temp +
@@ -650,7 +709,7 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   }
   const WholeList<A> list(space, p.top, k);
   // every warp takes the few steps to the rest's factor by itself, where they need no logarithm
-  Settled row = settle(p, space, list, rest, a.vocab, k);
+  Settled row = settle<T>(p, space, list, rest, a.vocab, place, inv_temp, k);
   const auto write_results = [&](double d) {
     write_row(p, r, rest, d, row.factor);
     finish(d);
@@ -665,7 +724,7 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
     row = *space.settled;
     if (place.first()) write_results(d);
   }
-  if (grad || p.listed) list_gradients(p, r, place, inv_temp, k, row, list.most, space);
+  if (grad || p.listed) list_gradients<T>(p, r, place, inv_temp, k, row, list.most, space);
   if (p.kind == TISO_DISTILL_FORWARD && place.tid >= kThreads - 32 && place.cta == 0) {
     // by the last warp: the first ones have the list
     Settled all = row;
