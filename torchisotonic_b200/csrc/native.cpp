@@ -67,6 +67,18 @@ const Tensor* tensor_in(py::handle h) {
   return THPVariable_Check(h.ptr()) ? &THPVariable_Unpack(h.ptr()) : nullptr;
 }
 
+// The capture that the current stream is in, 0 for none.
+int64_t capture_of(const Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const auto stream = c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();  // the launch says what is wrong
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
+
 // Whether a tensor needs no conversion: of this type, contiguous, and where and of the sizes that go
 // with the others.
 bool ready(const Tensor* t, ScalarType type, at::IntArrayRef sizes, at::Device device) {
@@ -438,12 +450,30 @@ Tensor policy_grad(const Tensor& x, const Tensor& targets, double temperature, c
   return grad;
 }
 
+// A gradient that was written with its loss is kept for the backward, which gives it away the first time
+// (and rewrites it unless the upstream gradient is the expected one). Only a backward of the same capture, or
+// both outside of any, may have it: a captured backward is replayed, and would leave it as its reader
+// left it; a captured forward is replayed over it.
+void keep_ready(AutogradContext* ctx, const Tensor& grad) {
+  ctx->saved_data["grad"] = grad;
+  ctx->saved_data["capture"] = capture_of(grad);
+}
+// It, or undefined.
+Tensor take_ready(AutogradContext* ctx) {
+  const auto at = ctx->saved_data.find("grad");
+  if (at == ctx->saved_data.end()) return Tensor();
+  Tensor grad = at->second.toTensor();
+  if (capture_of(grad) != ctx->saved_data["capture"].toInt()) return Tensor();
+  ctx->saved_data.erase(at);
+  return grad;
+}
+
 struct Policy : torch::autograd::Function<Policy> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const PolicySettings& s) {
     PolicyResult r = policy(x, s, true);
     ctx->save_for_backward({x, s.targets, r.kept});
     ctx->saved_data["temperature"] = s.temperature;
-    ctx->saved_data["grad"] = r.grad;
+    keep_ready(ctx, r.grad);
     variable_list out = parts(r.out);
     out.push_back(r.logps);
     ctx->mark_non_differentiable({out[1], out[2], out[3]});
@@ -454,14 +484,7 @@ struct Policy : torch::autograd::Function<Policy> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    // the gradient for an upstream gradient of 1, written with the loss, is given away the first
-    // time (the kernel rewrites it unless upstream is 1); later calls write a new one
-    Tensor ready;
-    const auto at = ctx->saved_data.find("grad");
-    if (at != ctx->saved_data.end()) {
-      ready = at->second.toTensor();
-      ctx->saved_data.erase(at);
-    }
+    const Tensor ready = take_ready(ctx);
     Tensor grad;
     {
       const at::NoGradGuard no_grad;
@@ -690,7 +713,7 @@ struct Distill : torch::autograd::Function<Distill> {
     ctx->saved_data["temperature"] = s.temperature;
     ctx->saved_data["ignore_index"] = s.ignore_index;
     ctx->saved_data["upstream"] = s.upstream;
-    ctx->saved_data["grad"] = r.grad;
+    keep_ready(ctx, r.grad);
     ctx->mark_non_differentiable({r.divergence});
     ctx->set_materialize_grads(false);
     return {r.loss, r.divergence};
@@ -699,13 +722,7 @@ struct Distill : torch::autograd::Function<Distill> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    // as of the policy loss: the gradient written with the loss is given away the first time
-    Tensor ready;
-    const auto at = ctx->saved_data.find("grad");
-    if (at != ctx->saved_data.end()) {
-      ready = at->second.toTensor();
-      ctx->saved_data.erase(at);
-    }
+    const Tensor ready = take_ready(ctx);
     return {once(distill_grad(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(),
                               ctx->saved_data["ignore_index"].toInt(), saved[2],
                               ctx->saved_data["upstream"].toDouble(), grads[0], ready)),
