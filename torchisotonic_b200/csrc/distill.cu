@@ -67,7 +67,6 @@ struct Settled {
   double log_each;  // its logarithm
   double whole;     // their sum with the rest's
   double p;         // of an exp(z), z from the largest logit of the list: its probability
-  double part;      // kWide: of an exp(z), z from the largest logit of this warp's entries: from the list's
   double log_p;     // of a z: its logarithm
   double mean;      // sum P f
   double factor;    // of the rest's gradient
@@ -356,32 +355,39 @@ struct WideStudent {
 };
 
 // The first steps after a row's sum, by every warp: what a gradient of the forward divergence is made
-// of; without a logarithm, and in double only what cancels.
+// of; without a logarithm, and in double only what cancels. part (kWide): what takes this warp's entries'
+// exponentials from their largest logit to the list's.
 template <typename T, typename A, int kThreads>
 __device__ __forceinline__ Settled settle(const DistillArgs<A>& p, const ListSpace<A, kThreads>& space,
                                           const WholeList<A>& list, const Part<A>& rest, int vocab,
-                                          const Place<kThreads>& place, double inv_temp, A k) {
+                                          const Place<kThreads>& place, double inv_temp, A k,
+                                          double& part) {
   const Teacher teacher(list.q, list.tokens, vocab, p.kind, p.drop);
-  Settled row{};
-  row.c = *space.share;
-  row.each = p.drop ? (list.q > 0 ? 1 / list.q : list.q) : 1.0;  // nothing to compare with: 0
-  row.whole = teacher.whole;
+  const auto settled = [&](bool nothing) {
+    Settled row{};
+    row.c = *space.share;
+    if (*space.bad || nothing) row.c = nan_of(0.0);
+    row.each = p.drop ? (list.q > 0 ? 1 / list.q : list.q) : 1.0;  // nothing to compare with: 0
+    row.whole = teacher.whole;
+    return row;
+  };
+  // p_v (f - sum P f) = p_v whole - q_v
   if constexpr (kWide<T>) {
-    if (*space.bad || (rest.s == A(0) && list.e == A(0))) row.c = nan_of(0.0);
+    Settled row = settled(rest.s == A(0) && list.e == A(0));
     if (p.kind != TISO_DISTILL_FORWARD) return row;
     const WideStudent student(teacher, rest, list.most, space, p.top, place.tid / 32, inv_temp);
     row.p = student.list_p;
-    row.part = student.part;
+    part = student.part;
     row.factor = row.c * student.factor;
     return row;
+  } else {
+    const Student<A> student(rest, list.most, list.e, k);
+    Settled row = settled(student.s == A(0));
+    row.p = student.list_p;
+    const A factor = static_cast<A>(teacher.whole) * student.rest_p - static_cast<A>(teacher.rest_q);
+    row.factor = static_cast<A>(row.c) * (rest.s == A(0) ? A(0) : factor / rest.s);
+    return row;
   }
-  const Student<A> student(rest, list.most, list.e, k);
-  if (*space.bad || student.s == A(0)) row.c = nan_of(0.0);
-  row.p = student.list_p;
-  // p_v (f - sum P f) = p_v whole - q_v
-  const A factor = static_cast<A>(teacher.whole) * student.rest_p - static_cast<A>(teacher.rest_q);
-  row.factor = static_cast<A>(row.c) * (rest.s == A(0) ? A(0) : factor / rest.s);
-  return row;
 }
 
 // The steps to the divergence, by a warp, in double (it is small beside its terms where the student is
@@ -472,7 +478,7 @@ __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
 template <typename T, int kThreads, typename A>
 __device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t r,
                                                const Place<kThreads>& place, double inv_temp, A k,
-                                               const Settled& row, A most,
+                                               const Settled& row, double part, A most,
                                                const ListSpace<A, kThreads>& space) {
   for (int i = place.tid; i < p.top; i += kThreads) {
     const int lead = space.lead[i];
@@ -485,7 +491,7 @@ __device__ __forceinline__ void list_gradients(const DistillArgs<A>& p, int64_t 
         if constexpr (!kWide<T>) {
           e = scaled_exp(z, k);
         } else if (kThreads == 32 || lead / 32 == place.tid / 32) {
-          e = space.e[lead] * row.part;
+          e = space.e[lead] * part;
         } else {  // listed again, first among another warp's entries
           e = exp((static_cast<double>(space.logit[lead]) - static_cast<double>(base_of(most))) * inv_temp);
         }
@@ -709,7 +715,8 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
   }
   const WholeList<A> list(space, p.top, k);
   // every warp takes the few steps to the rest's factor by itself, where they need no logarithm
-  Settled row = settle<T>(p, space, list, rest, a.vocab, place, inv_temp, k);
+  double part = 1;
+  Settled row = settle<T>(p, space, list, rest, a.vocab, place, inv_temp, k, part);
   const auto write_results = [&](double d) {
     write_row(p, r, rest, d, row.factor);
     finish(d);
@@ -724,7 +731,7 @@ __device__ __forceinline__ void distill_row(const Rows& a, const DistillArgs<A>&
     row = *space.settled;
     if (place.first()) write_results(d);
   }
-  if (grad || p.listed) list_gradients<T>(p, r, place, inv_temp, k, row, list.most, space);
+  if (grad || p.listed) list_gradients<T>(p, r, place, inv_temp, k, row, part, list.most, space);
   if (p.kind == TISO_DISTILL_FORWARD && place.tid >= kThreads - 32 && place.cta == 0) {
     // by the last warp: the first ones have the list
     Settled all = row;
