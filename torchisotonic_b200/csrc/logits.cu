@@ -146,6 +146,16 @@ struct TokenInput {
   }
 };
 
+// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest;
+// for |d| < kFar).
+__device__ __forceinline__ float exp_as(float, double d) {
+  const float hi = static_cast<float>(d);
+  const float lo = static_cast<double>(hi) == d ? 0.0f : static_cast<float>(d - hi);
+  const float e = expf(hi);
+  return __fmaf_rn(e, lo, e);
+}
+__device__ __forceinline__ double exp_as(double, double d) { return exp(d); }
+
 // exp(d) / s and exp(d) s, s a row's sum (up to 2^30). Beyond e^+-60 float has no room for them, nor
 // for exp(d) on the way: a token that the old policy all but excluded has a ratio of any size, which
 // the clip then cuts.

@@ -78,16 +78,6 @@ __device__ __forceinline__ float scaled_exp(float d, float k) {
 }
 __device__ __forceinline__ double scaled_exp(double d, double k) { return exp(__dmul_rn(d, k)); }
 
-// exp of a double to the accumulation type's precision (in float: of its float, times 1 + the rest;
-// for |d| < kFar).
-__device__ __forceinline__ float exp_as(float, double d) {
-  const float hi = static_cast<float>(d);
-  const float lo = static_cast<double>(hi) == d ? 0.0f : static_cast<float>(d - hi);
-  const float e = expf(hi);
-  return __fmaf_rn(e, lo, e);
-}
-__device__ __forceinline__ double exp_as(double, double d) { return exp(d); }
-
 // max(a, b) with a NaN ignored: the NaN reaches the sum through its own exponential.
 __device__ __forceinline__ float max_acc(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double max_acc(double a, double b) { return fmax(a, b); }

@@ -170,9 +170,8 @@ struct Ranked<float> {
   __device__ __forceinline__ Ranked(float value, int at)
       : key(static_cast<uint64_t>(ordered(value)) << 32 | (0xffffffffu - static_cast<unsigned>(at))) {}
   __device__ __forceinline__ bool before(const Ranked& o) const { return key > o.key; }
-  __device__ __forceinline__ uint32_t number() const { return static_cast<uint32_t>(key >> 32); }
   __device__ __forceinline__ float value() const {
-    const uint32_t b = number();
+    const uint32_t b = static_cast<uint32_t>(key >> 32);
     return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
   }
   __device__ __forceinline__ int at() const {
@@ -188,7 +187,6 @@ struct Ranked<double> {
   __device__ __forceinline__ bool before(const Ranked& o) const {
     return key > o.key || (key == o.key && place < o.place);
   }
-  __device__ __forceinline__ uint64_t number() const { return key; }
   __device__ __forceinline__ double value() const {
     return __longlong_as_double(
         static_cast<long long>(key >> 63 ? key & 0x7fffffffffffffffULL : ~key));
@@ -370,7 +368,7 @@ __device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kTh
   // puts down the places of the numbers that are among the `top` largest of n
   const auto choose = [&](int n, const auto& key, const auto& at, int* places, int* count) {
     Cut<A> cut{0, 0xffffffffu};
-    if (n > top) cut = find_cut<4, kThreads, A>(team, n, top, key, at, space.histogram);
+    if (n > top) cut = find_cut<kThreads, A>(team, n, top, key, at, space.histogram);
     for (int i = team.tid; i < n; i += kThreads)
       if (cut.takes(key(i), at(i))) places[atomicAdd(count, 1)] = static_cast<int>(at(i));
     team.sync();
@@ -414,7 +412,7 @@ __device__ __noinline__ int choose_by_groups(const RowView<T> r, const Place<kTh
   };
   Cut<A> cut{0, 0xffffffffu};
   if (n > top)
-    cut = find_cut<4, kThreads, A>(
+    cut = find_cut<kThreads, A>(
         team, n, top, [&](int i) { return ordered(number(i)); },
         [&](int i) { return static_cast<uint32_t>(element(i)); }, space.histogram);
   team.sync();

@@ -96,8 +96,8 @@ __device__ __forceinline__ Digit find_digit(const Team<kThreads>& team, int n, i
   return r;
 }
 
-// The cut that takes k of n > k numbers: key(i) and place(i) < 2^(8 kPlaceBytes), different for each.
-template <int kPlaceBytes, int kThreads, typename A, typename F, typename G>
+// The cut that takes k of n > k numbers: key(i), and place(i), different for each.
+template <int kThreads, typename A, typename F, typename G>
 __device__ __forceinline__ Cut<A> find_cut(const Team<kThreads>& team, int n, int k, const F& key,
                                            const G& place, unsigned* histogram) {
   using U = KeyOf<A>;
@@ -118,7 +118,7 @@ __device__ __forceinline__ Cut<A> find_cut(const Team<kThreads>& team, int n, in
   }
   // equal numbers: the first `need` places, by the digits of their complement
   uint32_t low = 0, low_mask = 0;
-  for (int shift = 8 * kPlaceBytes - 8; shift >= 0; shift -= 8) {
+  for (int shift = 24; shift >= 0; shift -= 8) {
     const Digit d = find_digit<kThreads>(
         team, n, need,
         [&](int i) {
@@ -131,9 +131,7 @@ __device__ __forceinline__ Cut<A> find_cut(const Team<kThreads>& team, int n, in
     need -= d.above;
     if (need == d.inside) break;
   }
-  // complements from `low` on (their upper bytes, the same for all, are ones)
-  const uint32_t upper = kPlaceBytes == 4 ? 0u : ~((1u << (8 * kPlaceBytes % 32)) - 1u);
-  return {found, ~(low | upper)};
+  return {found, ~low};  // complements from `low` on
 }
 
 }  // namespace tiso
