@@ -323,9 +323,10 @@ __device__ __forceinline__ unsigned bound_of_warp(const uint16_t* unit_max, int 
   return bound;
 }
 
-// Up to so many alternatives a warp alone takes its bound from its lanes: 200000 x 2048 bf16, 1 and 20
-// of them, 256 and 518 us so, 472 and 552 us by bisection over the units; 32: 2211 and 826.
-constexpr int kMostByLanes = 16;
+// Up to so many alternatives a warp alone takes its bound from its lanes. 200000 x 2048 bf16, 16, 20, 24 and 28
+// of them: 343, 391, 454 and 531 us so, 470, 483, 491 and 503 by bisection over the units; 50000 x 8192, 20 and 24:
+// 257 and 290, 262 and 272.
+constexpr int kMostByLanes = 20;
 
 // How many of each warp's lanes are to reach the bound, over the warps whose lanes all have a vector;
 // 0 where these are too few to give one.
