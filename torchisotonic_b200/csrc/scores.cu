@@ -328,6 +328,11 @@ __device__ __forceinline__ unsigned bound_of_warp(const uint16_t* unit_max, int 
 // 257 and 290, 262 and 272.
 constexpr int kMostByLanes = 20;
 
+// For more alternatives than this a warp keeps the maximum of each vector of a short row, else that of a
+// lane's batches: 200000 x 2048 bf16, 1, 5, 10 and 16 alternatives 288, 306, 325 and 343 us by vectors, 261,
+// 280, 322 and 372 by batches; 200000 x 777 float32 247, 272, 287 and 300, 230, 253, 288 and 329.
+constexpr int kMostByBatches = 8;
+
 // How many of each warp's lanes are to reach the bound, over the warps whose lanes all have a vector;
 // 0 where these are too few to give one.
 template <int kThreads, typename T>
@@ -838,7 +843,7 @@ TopSizes top_sizes(int top, int64_t vectors, int threads, int ctas) {
   const int64_t share = (tiles + ctas - 1) / ctas;
   const bool whole = share * tile > 1024 && share * tile / 32 >= 2 * top;
   const int64_t groups = whole ? share * tile / 32 : share * tile;
-  const bool fine = threads == 32 && share * kBatch <= kMostUnits;
+  const bool fine = threads == 32 && top > kMostByBatches && share * kBatch <= kMostUnits;
   return {top, static_cast<int>(share), static_cast<int>(groups), whole, fine};
 }
 
