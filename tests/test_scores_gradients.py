@@ -78,8 +78,8 @@ def scores_gradient(x, y, g, h, t):
     vocab = x.shape[-1]
     u, e = units(x.dtype, vocab)
     used = (y != IGNORE)[..., None]
-    z = torch.where(used, x, torch.zeros_like(x)).double() / t
-    z = z - z.amax(-1, keepdim=True)
+    z = torch.where(used, x, torch.zeros_like(x)).double()
+    z = (z - z.amax(-1, keepdim=True)) / t
     s = z.exp().sum(-1, keepdim=True)
     p = z.exp() / s
     size = torch.where(p > 0, z, 0.0).abs()
@@ -155,8 +155,8 @@ def distill_gradient(x, ids, logps, kind, rest, mix, w, t, upstream):
     there = ids != IGNORE
     w = torch.ones(len(x), device="cuda", dtype=torch.float64) if w is None else w.reshape(-1).double()
     w = w * there[:, 0]
-    z = torch.where((w != 0)[:, None], x, torch.zeros_like(x)).double() / t
-    z = z - z.amax(1, keepdim=True)
+    z = torch.where((w != 0)[:, None], x, torch.zeros_like(x)).double()
+    z = (z - z.amax(1, keepdim=True)) / t
     lp = torch.log_softmax(z, 1)
     p = lp.exp()
     row, col = there.nonzero(as_tuple=True)
@@ -170,7 +170,7 @@ def distill_gradient(x, ids, logps, kind, rest, mix, w, t, upstream):
     q_rest = torch.where(listed.all(1, keepdim=True), 0.0, q_rest)
     if rest == "drop":
         q, q_rest = q / q.sum(1, keepdim=True), torch.zeros_like(q_rest)
-    of_rest = torch.where(p_rest > 0, (lp - lp_rest).exp(), 0.0)  # of a token of the rest, within it
+    of_rest = torch.where(lp_rest > -math.inf, (lp - lp_rest).exp(), 0.0)  # of a token of the rest, within it
     relative = e + (8 + 3 * z.abs()) * u
     slack = (ids.shape[1] + 4) * 2.0**-52
     if kind == "forward":
@@ -340,3 +340,30 @@ def test_infinite_results(vocab: int, dtype: torch.dtype) -> None:
     got = ti.distillation_loss(x, ids, logps, kind="reverse")
     assert (got.divergence == math.inf).all() and got.loss == math.inf
     assert ti.distillation_loss(x, ids, logps, kind="jensen").divergence.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("vocab", [40, 2500, 40007])
+def test_lists_at_the_lowest_value(vocab: int, dtype: torch.dtype) -> None:
+    # a student that hides the listed tokens with its type's lowest value: their probability is 0, and as where it is
+    # -inf only the others count; and one that hides all but one, or has the largest value outside the list
+    least = torch.finfo(dtype).min
+    x = (normal((4, vocab), 1) * 3).to(dtype)
+    ids, logps = near_lists(x, 6)
+    rows = torch.arange(4, device="cuda")[:, None]
+    x[rows[1:], ids[1:]] = least
+    x[2] = least
+    x[2, ids[2, 0].item() - 1] = 0
+    x[3, (ids[3] + 1) % vocab] = -least
+    hidden = x.clone()
+    hidden[1:][hidden[1:] == least] = -math.inf
+    hidden[3][hidden[3] != -least] = -math.inf
+    for kind, rest in (("reverse", "bucket"), ("jensen", "bucket"), ("jensen", "drop")):
+        got, want = [], []
+        for z, out in ((x, got), (hidden, want)):
+            leaf = z.detach().requires_grad_()
+            loss = ti.distillation_loss(leaf, ids, logps, kind=kind, rest=rest)
+            out += [loss.loss.detach(), loss.divergence, *torch.autograd.grad(loss.loss, leaf)]
+        for a, b in zip(got, want):
+            assert b.isfinite().all() and torch.equal(a, b)

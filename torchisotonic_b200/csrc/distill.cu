@@ -452,7 +452,8 @@ __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
   }
   if (p.kind == TISO_DISTILL_REVERSE) {
     const double rest_f = rest_log_p - rest_log_q;
-    d = row.mean = of_list / s * (far + e * row.log_p) + product(rest_p, rest_f);
+    // (where the list has no probability log_p may be as far as the type's lowest value)
+    d = row.mean = product(of_list / s, far + e * row.log_p) + product(rest_p, rest_f);
     factor = product(rest_p, rest_f - row.mean);
   } else {
     double mean = 0, cross = 0;
