@@ -21,7 +21,9 @@ namespace tiso {
 namespace {
 
 constexpr int kMostListed = 128;
-constexpr int kSmThreads = 1280;  // resident at 48 registers a thread
+// Resident at 48 registers a thread, which spill: 48 bytes of stores and 88 of loads for 16 bits, 104 and 112
+// in float32. (A warp to a row, at 64: 40 and 80, 64 and 148.)
+constexpr int kSmThreads = 1280;
 // the teacher's rest where it is divided by: a list's float log-probabilities say no less
 constexpr double kLeastRest = 1.0 / (1 << 24);
 

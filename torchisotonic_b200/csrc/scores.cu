@@ -734,7 +734,9 @@ __device__ __forceinline__ void scores_row(const Rows& a, const ScoresArgs<A>& p
   }
 }
 
-constexpr int kSmThreads = 1280;  // resident at 48 registers a thread
+// Resident at 48 registers a thread; with alternatives 8 bytes are spilled for 16 bits, 36 in float32 (stores;
+// float64, with twice the registers, nothing; by groups 64 in float32).
+constexpr int kSmThreads = 1280;
 
 template <typename T, typename A, int kThreads, bool kTop>
 __global__ void __launch_bounds__(kThreads, kSmThreads / kThreads / (sizeof(T) == 8 ? 2 : 1))

@@ -257,7 +257,8 @@ def policy_loss(
     infinite; a factor of 0 (the advantage, ``kl_coef``) leaves its term out also there.
 
     The gradient is written with the loss, for an upstream gradient of exactly 1; any other one
-    (``loss / n``, a scaled loss) takes another pass over the logits in the backward.
+    (``loss / n``, a scaled loss) takes another pass over the logits in the backward, and so does a
+    backward that is captured in a CUDA graph without its forward.
 
     Returns ``PolicyLoss(loss, logps, kl, clip_fraction)``: the loss, differentiable (once) in
     ``logits`` alone; the tokens' log-probabilities (0 where left out); the weighted means of
@@ -346,7 +347,8 @@ def distillation_loss(
 
     The gradient is written with the loss, for an upstream gradient of exactly ``upstream`` (give a
     loss scale, or 1 / the number of micro-batches); any other one takes another pass over the
-    logits in the backward.
+    logits in the backward, and so does a backward that is captured in a CUDA graph without its
+    forward.
 
     Returns ``DistillationLoss(loss, divergence)``: the loss, differentiable (once) in ``logits``
     alone, and every token's ``D`` [...]. float32 (float64 for float64 logits).
