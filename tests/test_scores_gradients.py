@@ -367,3 +367,23 @@ def test_lists_at_the_lowest_value(vocab: int, dtype: torch.dtype) -> None:
             out += [loss.loss.detach(), loss.divergence, *torch.autograd.grad(loss.loss, leaf)]
         for a, b in zip(got, want):
             assert b.isfinite().all() and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("vocab", [40, 2500, 40007])
+def test_nothing_to_compare_with_and_not_finite(vocab: int, dtype: torch.dtype) -> None:
+    # a renormalised list of probability 0 leaves 0; of a row that is not finite NaN, as any other list
+    x = (normal((5, vocab), 1) * 3).to(dtype)
+    ids, logps = near_lists(x, 5)
+    logps[:4] = -math.inf
+    x[1, vocab - 1] = math.nan
+    x[2] = -math.inf
+    x[3, ids[3, 0]] = math.inf
+    bad = torch.tensor([False, True, True, True, False], device="cuda")
+    for kind in ("forward", "jensen"):
+        leaf = x.detach().requires_grad_()
+        got = ti.distillation_loss(leaf, ids, logps, kind=kind, rest="drop")
+        assert torch.equal(got.divergence.isnan(), bad) and got.divergence[0] == 0
+        (gx,) = torch.autograd.grad(got.loss, leaf)
+        assert gx[bad].isnan().all() and (gx[0] == 0).all() and gx[4].isfinite().all()

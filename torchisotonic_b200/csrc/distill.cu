@@ -442,9 +442,9 @@ __device__ __forceinline__ double settle_logs(const DistillArgs<A>& p,
   row.log_each = p.drop ? -of_lane(logarithm, 3) : 0.0;
   row.log_p = list_z - log_s;
   double d, factor = 0;
-  if (p.drop && list.q == 0) {  // nothing to compare with
-    row.c *= 0;
-    row.factor *= 0;
+  if (p.drop && list.q == 0) {  // nothing to compare with: 0, or NaN where the row's sum is
+    row.c *= 0 * s;
+    row.factor = row.c;
     return row.c;
   }
   if (p.kind == TISO_DISTILL_FORWARD) {
